@@ -417,6 +417,93 @@ int jq_mask_encode(const uint8_t *mask, int32_t n, int32_t d, int32_t k_max, int
 int jq_ids_to_mask(const int32_t *ids, const int32_t *counts, int64_t rows, int32_t k_max, const int64_t *idx,
                    int32_t batch, int32_t d, uint8_t *out, void *stream);
 
+/* ---- a policy's memory over the plies of a game ------------------------------
+ * Operators of a policy that plays these games: linear attention with a decay for
+ * each head, rotary positions with several axes, layer norm, with their backward
+ * passes. No counterpart in the reference's environment. Element types are
+ * JQ_F32 and JQ_BF16; sums, statistics and states are kept in float32. Pointers
+ * are device addresses, aligned to their element's size; elements of the last
+ * dimension are adjacent. Launched on the current device; no call allocates,
+ * keeps device memory or synchronises. */
+#define JQ_F32 0
+#define JQ_BF16 1
+#define JQ_ATTENTION_MAX_DIM 128   /* largest key_dim and value_dim */
+#define JQ_ROTARY_MAX_AXES 4
+
+/* A (batch, plies, heads, dim) tensor: strides in elements; data NULL: absent. */
+typedef struct jq_rows {
+    void *data;
+    int64_t batch, ply, head;
+} jq_rows;
+
+/* Linear attention over segments of plies. For each game b and head h, with
+ * lambda = exp(log_decay[h]) and the state S (key_dim, value_dim):
+ *   S_t   = (starts[b][t] ? 0 : lambda * S_{t-1}) + k_t v_t^T
+ *   out_t = scale * q_t S_t                              for t < lengths[b]
+ * Plies from lengths[b] on are not read, and their out, dq, dk and dv are 0; the
+ * final state is the one after the last ply that is read. */
+typedef struct jq_attention {
+    int32_t dtype;                     /* JQ_F32 or JQ_BF16: q, k, v, out, d_out, dq, dk, dv */
+    int32_t batch, plies, heads, key_dim, value_dim;
+    float scale;
+    const float *log_decay;            /* float32 (heads), at most 0 */
+    const uint8_t *starts;             /* (batch, plies), nonzero where a game starts; NULL: nowhere */
+    int64_t starts_batch, starts_ply;  /* strides of starts */
+    const int32_t *lengths;            /* (batch), clamped to [0, plies]; NULL: plies */
+    const float *initial_state;        /* float32 (batch, heads, key_dim, value_dim); NULL: zeros */
+    float *final_state;                /* the same shape; NULL: not written */
+    jq_rows q, k, v, out;              /* out: forward only */
+    /* backward: gradients of out and of the final state go in (d_final NULL: zeros),
+     * those of q, k, v and of the initial state come out (dq, dk and dv, and
+     * d_initial: NULL where not wanted; dk and dv go together) */
+    jq_rows d_out, dq, dk, dv;
+    const float *d_final;
+    float *d_initial;
+    void *workspace;                   /* jq_attention_workspace bytes, 16-byte aligned; NULL if it says 0 */
+    int64_t workspace_bytes;
+} jq_attention;
+/* Bytes of workspace that the forward or (backward != 0) backward pass takes. */
+int jq_attention_workspace(const jq_attention *a, int32_t backward, int64_t *bytes);
+int jq_attention_forward(const jq_attention *a, void *stream);
+int jq_attention_backward(const jq_attention *a, void *stream);
+/* One new ply of each of batch games: q, k, v and out as above with their ply
+ * strides unused, state (float32, (state_rows, heads, key_dim, value_dim), 16-byte
+ * aligned) updated in place. rows (int64, batch; NULL: row b) names each game's
+ * state; a game whose row is outside [0, state_rows) is left out: its out is 0.
+ * Two games with one row race. starts (uint8, batch) may be NULL. */
+int jq_attention_step(int32_t dtype, int32_t batch, int32_t heads, int32_t key_dim, int32_t value_dim, float scale,
+                      const float *log_decay, const jq_rows *q, const jq_rows *k, const jq_rows *v,
+                      const jq_rows *out, float *state, int64_t state_rows, const int64_t *rows,
+                      const uint8_t *starts, void *stream);
+
+/* Rotary positions: pair p of a head turns by positions[axis(p)] * frequencies[p]
+ * radians, (a, b) -> (a cos - b sin, b cos + a sin), or the other way round where
+ * inverse is nonzero (the backward pass). The pairs are (p, pairs + p), or
+ * (2p, 2p + 1) where interleaved is nonzero; section_ends[i] is one past the last
+ * pair that turns with axis i. Elements past 2 * pairs are copied. x and out:
+ * (n0, n1, heads, dim); positions: int32 or (positions64 != 0) int64 (n0, n1,
+ * axes), strides in elements, axes adjacent. */
+int jq_rotary(int32_t dtype, int64_t n0, int64_t n1, int32_t heads, int32_t dim, int32_t pairs, const jq_rows *x,
+              const jq_rows *out, const void *positions, int32_t positions64, int64_t positions_n0,
+              int64_t positions_n1, int32_t axes, const int32_t *section_ends, const float *frequencies,
+              int32_t interleaved, int32_t inverse, void *stream);
+
+/* Layer norm of rows of width elements: out = (x - mean) * rstd * weight + bias,
+ * rstd = 1 / sqrt(variance + eps). weight and bias: (width) of weight_dtype, NULL:
+ * ones and zeros. mean and rstd: float32 (rows), written for the backward pass;
+ * NULL: not written. Strides are between rows, in elements. */
+int jq_layer_norm_forward(int32_t dtype, int32_t weight_dtype, int64_t rows, int32_t width, const void *x,
+                          int64_t x_stride, const void *weight, const void *bias, float eps, void *out,
+                          int64_t out_stride, float *mean, float *rstd, void *stream);
+/* Gradients: dx (rows, width), dweight and dbias (width, of weight_dtype); each may
+ * be NULL. dweight and dbias are summed over the rows in a fixed order; they take
+ * workspace_bytes >= jq_layer_norm_workspace of float32 workspace. */
+int jq_layer_norm_workspace(int64_t rows, int32_t width, int64_t *bytes);
+int jq_layer_norm_backward(int32_t dtype, int32_t weight_dtype, int64_t rows, int32_t width, const void *x,
+                           int64_t x_stride, const void *weight, const float *mean, const float *rstd,
+                           const void *d_out, int64_t d_out_stride, void *dx, int64_t dx_stride, void *dweight,
+                           void *dbias, void *workspace, int64_t workspace_bytes, void *stream);
+
 /* Synchronise `stream`. */
 int jq_sync(void *stream);
 

@@ -16,6 +16,9 @@ JQ_E_ARG, JQ_E_STATE, JQ_E_HIP, JQ_E_OOM, JQ_E_CAPACITY = -1, -2, -3, -4, -5
 SAMPLE_UNIFORM, SAMPLE_LOGITS = 0, 1
 OBS_F32, OBS_BF16, OBS_U8 = 0, 1, 2
 ACT_WORLD, ACT_CANONICAL = 0, 1
+F32, BF16 = 0, 1
+ATTENTION_MAX_DIM = 128
+ROTARY_MAX_AXES = 4
 NUM_CELLS = 289
 NUM_ON_BOARD = 129
 NUM_PIDS = 120
@@ -50,8 +53,26 @@ _EXPORTS = [
     "jq_finalize_import_masked", "jq_rehash", "jq_validate_lineup",
     "jq_sync", "jq_step_host", "jq_legal_dense_host", "jq_env_flags_host", "jq_history_create", "jq_history_destroy", "jq_history_bytes", "jq_history_snapshot",
     "jq_history_reconstruct", "jq_history_reconstruct_bf16", "jq_history_reconstruct_noalloc", "jq_mask_count", "jq_mask_to_ids", "jq_mask_encode", "jq_ids_to_mask", "jq_upload_beliefs",
-    "jq_clear_beliefs",
+    "jq_clear_beliefs", "jq_attention_workspace", "jq_attention_forward", "jq_attention_backward", "jq_attention_step",
+    "jq_rotary", "jq_layer_norm_forward", "jq_layer_norm_workspace", "jq_layer_norm_backward",
 ]
+
+
+class Rows(C.Structure):
+    """jq_rows: a (batch, plies, heads, dim) tensor, strides in elements."""
+    _fields_ = [("data", C.c_void_p), ("batch", C.c_int64), ("ply", C.c_int64), ("head", C.c_int64)]
+
+
+class Attention(C.Structure):
+    """jq_attention."""
+    _fields_ = [("dtype", C.c_int32), ("batch", C.c_int32), ("plies", C.c_int32), ("heads", C.c_int32),
+                ("key_dim", C.c_int32), ("value_dim", C.c_int32), ("scale", C.c_float), ("log_decay", C.c_void_p),
+                ("starts", C.c_void_p), ("starts_batch", C.c_int64), ("starts_ply", C.c_int64),
+                ("lengths", C.c_void_p), ("initial_state", C.c_void_p), ("final_state", C.c_void_p),
+                ("q", Rows), ("k", Rows), ("v", Rows), ("out", Rows),
+                ("d_out", Rows), ("dq", Rows), ("dk", Rows), ("dv", Rows),
+                ("d_final", C.c_void_p), ("d_initial", C.c_void_p),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64)]
 
 
 class JunqiError(RuntimeError):
@@ -78,6 +99,7 @@ def _load() -> C.CDLL:
 def bind(L: C.CDLL) -> C.CDLL:
     """Declare the C-ABI signatures of include/junqi_amd.h on a loaded library."""
     P, I32, I64, U64 = C.c_void_p, C.c_int32, C.c_int64, C.c_uint64
+    F32T, R = C.c_float, C.POINTER(Rows)
     sig = {
         "jq_last_error": ([], C.c_char_p), "jq_version": ([], C.c_char_p),
         "jq_create": ([C.POINTER(P), I32, I32, I32, I32], C.c_int),
@@ -119,6 +141,14 @@ def bind(L: C.CDLL) -> C.CDLL:
         "jq_mask_encode": ([P, I32, I32, I32, P, P, P, P, P, P], C.c_int),
         "jq_ids_to_mask": ([P, P, I64, I32, P, I32, I32, P, P], C.c_int),
         "jq_upload_beliefs": ([P, P, I32, P], C.c_int), "jq_clear_beliefs": ([P], C.c_int),
+        "jq_attention_workspace": ([C.POINTER(Attention), I32, C.POINTER(I64)], C.c_int),
+        "jq_attention_forward": ([C.POINTER(Attention), P], C.c_int),
+        "jq_attention_backward": ([C.POINTER(Attention), P], C.c_int),
+        "jq_attention_step": ([I32, I32, I32, I32, I32, F32T, P, R, R, R, R, P, I64, P, P, P], C.c_int),
+        "jq_rotary": ([I32, I64, I64, I32, I32, I32, R, R, P, I32, I64, I64, I32, C.POINTER(I32), P, I32, I32, P], C.c_int),
+        "jq_layer_norm_forward": ([I32, I32, I64, I32, P, I64, P, P, F32T, P, I64, P, P, P], C.c_int),
+        "jq_layer_norm_workspace": ([I64, I32, C.POINTER(I64)], C.c_int),
+        "jq_layer_norm_backward": ([I32, I32, I64, I32, P, I64, P, P, P, P, I64, P, I64, P, P, P, I64, P], C.c_int),
     }
     for name, (args, res) in sig.items():
         fn = getattr(L, name)

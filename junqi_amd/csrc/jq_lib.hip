@@ -14,6 +14,7 @@
 
 #include "junqi_amd.h"
 #include "jq_device.h"
+#include "jq_error.h"
 #include "jq_kernels.h"
 #include "jq_obs.h"
 #include "jq_history.h"
@@ -65,7 +66,9 @@ namespace {
 
 thread_local std::string g_err;
 
-int fail(int code, const char *fmt, ...)
+}  // namespace
+
+int jq::fail(int code, const char *fmt, ...)
 {
     char buf[512];
     va_list ap;
@@ -75,6 +78,15 @@ int fail(int code, const char *fmt, ...)
     g_err = buf;
     return code;
 }
+
+int jq::launch_check(const char *what)
+{
+    const hipError_t err = hipGetLastError();
+    if (err != hipSuccess) return fail(JQ_E_HIP, "%s launch: %s", what, hipGetErrorString(err));
+    return JQ_OK;
+}
+
+namespace {
 
 #define HIP_TRY(expr)                                                                      \
     do {                                                                                   \
@@ -357,13 +369,6 @@ int check_env(jq_env *e)
 {
     if (!e) return fail(JQ_E_ARG, "null handle");
     if (hipSetDevice(e->device) != hipSuccess) return fail(JQ_E_HIP, "hipSetDevice(%d) failed", e->device);
-    return JQ_OK;
-}
-
-int launch_check(const char *what)
-{
-    const hipError_t err = hipGetLastError();
-    if (err != hipSuccess) return fail(JQ_E_HIP, "%s launch: %s", what, hipGetErrorString(err));
     return JQ_OK;
 }
 

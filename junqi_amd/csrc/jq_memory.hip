@@ -1,0 +1,312 @@
+// C entry points of the operators of a policy's memory over plies: linear
+// attention, rotary positions, layer norm. Declarations and contracts live in
+// include/junqi_amd.h.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <climits>
+
+#include "junqi_amd.h"
+#include "jq_error.h"
+#include "jq_memory.h"
+#include "jq_attention.h"
+#include "jq_rotary.h"
+#include "jq_norm.h"
+
+using namespace jq;
+
+namespace {
+
+hipStream_t strm(void *s) { return reinterpret_cast<hipStream_t>(s); }
+
+int check_dtype(int32_t dtype)
+{
+    if (dtype != JQ_F32 && dtype != JQ_BF16) return fail(JQ_E_ARG, "element type %d is neither JQ_F32 nor JQ_BF16", dtype);
+    return JQ_OK;
+}
+
+size_t elem_bytes(int32_t dtype) { return dtype == JQ_F32 ? 4 : 2; }
+
+bool aligned(const void *p, size_t to) { return (uintptr_t)p % to == 0; }
+
+int check_rows(const jq_rows &r, int32_t dtype, const char *name)
+{
+    if (!r.data) return fail(JQ_E_ARG, "null %s", name);
+    if (!aligned(r.data, elem_bytes(dtype))) return fail(JQ_E_ARG, "%s must be aligned to its element size", name);
+    return JQ_OK;
+}
+
+#define TRY(expr)                  \
+    do {                           \
+        const int rc_ = (expr);    \
+        if (rc_) return rc_;       \
+    } while (0)
+
+int check_dims(int32_t batch, int32_t heads, int32_t dk, int32_t dv)
+{
+    if (batch < 0 || heads <= 0) return fail(JQ_E_ARG, "bad shapes (batch %d, heads %d)", batch, heads);
+    if (dk <= 0 || dv <= 0 || dk > JQ_ATTENTION_MAX_DIM || dv > JQ_ATTENTION_MAX_DIM)
+        return fail(JQ_E_ARG, "key_dim %d and value_dim %d must be in [1, %d]", dk, dv, JQ_ATTENTION_MAX_DIM);
+    if ((int64_t)batch * heads > INT_MAX) return fail(JQ_E_ARG, "batch * heads %lld is too large", (long long)batch * heads);
+    return JQ_OK;
+}
+
+int check_attention(const jq_attention *a)
+{
+    if (!a) return fail(JQ_E_ARG, "null arguments");
+    TRY(check_dtype(a->dtype));
+    TRY(check_dims(a->batch, a->heads, a->key_dim, a->value_dim));
+    if (a->plies < 0 || a->plies > INT_MAX - 1024) return fail(JQ_E_ARG, "plies %d out of range", a->plies);
+    return JQ_OK;
+}
+
+int check_attention_inputs(const jq_attention *a)
+{
+    if (!a->log_decay) return fail(JQ_E_ARG, "null log_decay");
+    if (a->plies == 0) return JQ_OK;
+    TRY(check_rows(a->q, a->dtype, "q"));
+    TRY(check_rows(a->k, a->dtype, "k"));
+    return check_rows(a->v, a->dtype, "v");
+}
+
+ScanArgs scan_args(const jq_attention *a)
+{
+    ScanArgs s{};
+    s.batch = a->batch;
+    s.plies = a->plies;
+    s.heads = a->heads;
+    s.log_decay = a->log_decay;
+    s.starts = a->starts;
+    s.starts_batch = a->starts_batch;
+    s.starts_ply = a->starts_ply;
+    s.lengths = a->lengths;
+    s.in_scale = s.out_scale = 1.f;
+    return s;
+}
+
+template <class T>
+int launch_scan(const ScanArgs &s, hipStream_t stream)
+{
+    const dim3 grid(s.batch * s.heads), block(128);
+    if (s.kd <= 32) hipLaunchKernelGGL((k_attention_scan<T, 32>), grid, block, 0, stream, s);
+    else if (s.kd <= 64) hipLaunchKernelGGL((k_attention_scan<T, 64>), grid, block, 0, stream, s);
+    else hipLaunchKernelGGL((k_attention_scan<T, 128>), grid, block, 0, stream, s);
+    return launch_check("k_attention_scan");
+}
+
+int scan(int32_t dtype, const ScanArgs &s, hipStream_t stream)
+{
+    return dtype == JQ_F32 ? launch_scan<float>(s, stream) : launch_scan<bf16>(s, stream);
+}
+
+template <class T, class W>
+int norm_backward(int64_t rows, int32_t width, const void *x, int64_t x_stride, const void *weight, const float *mean,
+                  const float *rstd, const void *d_out, int64_t d_stride, void *dx, int64_t dx_stride, void *dweight,
+                  void *dbias, float *part, hipStream_t stream)
+{
+    const T *xt = static_cast<const T *>(x), *dt = static_cast<const T *>(d_out);
+    if (dx && rows) {
+        hipLaunchKernelGGL((k_norm_dx<T, W>), dim3(rows), dim3(64), 0, stream, xt, x_stride, width,
+                           static_cast<const W *>(weight), mean, rstd, dt, d_stride, static_cast<T *>(dx), dx_stride);
+        TRY(launch_check("k_norm_dx"));
+    }
+    if (!dweight && !dbias) return JQ_OK;
+    const int blocks = (width + 63) / 64, parts = (int)std::min<int64_t>(NORM_PARTS, rows);
+    if (parts) {
+        hipLaunchKernelGGL((k_norm_dw<T>), dim3(blocks, parts), dim3(64), 0, stream, xt, x_stride, rows, width, mean,
+                           rstd, dt, d_stride, part);
+        TRY(launch_check("k_norm_dw"));
+    }
+    hipLaunchKernelGGL((k_norm_join<W>), dim3(blocks), dim3(64), 0, stream, part, parts, width,
+                       static_cast<W *>(dweight), static_cast<W *>(dbias));
+    return launch_check("k_norm_join");
+}
+
+template <class T, class W>
+int norm_forward(int64_t rows, int32_t width, const void *x, int64_t x_stride, const void *weight, const void *bias,
+                 float eps, void *out, int64_t out_stride, float *mean, float *rstd, hipStream_t stream)
+{
+    hipLaunchKernelGGL((k_norm_forward<T, W>), dim3(rows), dim3(64), 0, stream, static_cast<const T *>(x), x_stride,
+                       width, static_cast<const W *>(weight), static_cast<const W *>(bias), eps,
+                       static_cast<T *>(out), out_stride, mean, rstd);
+    return launch_check("k_norm_forward");
+}
+
+int check_norm(int32_t dtype, int32_t weight_dtype, int64_t rows, int32_t width)
+{
+    TRY(check_dtype(dtype));
+    if (weight_dtype != JQ_F32 && weight_dtype != dtype)
+        return fail(JQ_E_ARG, "weights are float32 or of the rows' type");
+    if (rows < 0 || rows > INT_MAX) return fail(JQ_E_ARG, "rows %lld out of range", (long long)rows);
+    if (width <= 0) return fail(JQ_E_ARG, "width %d must be positive", width);
+    return JQ_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int jq_attention_workspace(const jq_attention *a, int32_t backward, int64_t *bytes)
+{
+    TRY(check_attention(a));
+    if (!bytes) return fail(JQ_E_ARG, "null output");
+    *bytes = 0;
+    return JQ_OK;
+}
+
+int jq_attention_forward(const jq_attention *a, void *stream)
+{
+    TRY(check_attention(a));
+    if (a->batch == 0) return JQ_OK;
+    TRY(check_attention_inputs(a));
+    if (a->plies) TRY(check_rows(a->out, a->dtype, "out"));
+    ScanArgs s = scan_args(a);
+    s.q = a->q, s.k = a->k, s.v = a->v, s.o = a->out;
+    s.kd = a->key_dim, s.vd = a->value_dim;
+    s.s_in = a->initial_state, s.s_out = a->final_state, s.s_row = a->value_dim, s.s_col = 1;
+    s.out_scale = a->scale;
+    return scan(a->dtype, s, strm(stream));
+}
+
+int jq_attention_backward(const jq_attention *a, void *stream)
+{
+    TRY(check_attention(a));
+    if (a->batch == 0) return JQ_OK;
+    TRY(check_attention_inputs(a));
+    if (a->plies) TRY(check_rows(a->d_out, a->dtype, "d_out"));
+    if (!a->dk.data != !a->dv.data) return fail(JQ_E_ARG, "dk and dv go together");
+    if (a->d_initial && !a->dk.data && a->plies) return fail(JQ_E_ARG, "d_initial comes with dk and dv");
+    if (a->dq.data) {
+        TRY(check_rows(a->dq, a->dtype, "dq"));
+        ScanArgs s = scan_args(a);
+        s.q = a->d_out, s.k = a->v, s.v = a->k, s.o = a->dq;
+        s.kd = a->value_dim, s.vd = a->key_dim;
+        s.s_in = a->initial_state, s.s_row = 1, s.s_col = a->value_dim;
+        s.out_scale = a->scale;
+        TRY(scan(a->dtype, s, strm(stream)));
+    }
+    if (a->dk.data || a->d_initial) {
+        if (a->plies) {
+            TRY(check_rows(a->dk, a->dtype, "dk"));
+            TRY(check_rows(a->dv, a->dtype, "dv"));
+        }
+        ScanArgs s = scan_args(a);
+        s.reverse = true;
+        s.in_scale = a->scale;
+        s.q = a->k, s.k = a->q, s.v = a->d_out, s.o = a->dv;
+        s.kd = a->key_dim, s.vd = a->value_dim;
+        s.s_in = a->d_final, s.s_out = a->d_initial, s.s_row = a->value_dim, s.s_col = 1;
+        TRY(scan(a->dtype, s, strm(stream)));
+        s.q = a->v, s.k = a->d_out, s.v = a->q, s.o = a->dk;
+        s.kd = a->value_dim, s.vd = a->key_dim;
+        s.s_out = nullptr, s.s_row = 1, s.s_col = a->value_dim;
+        TRY(scan(a->dtype, s, strm(stream)));
+    }
+    return JQ_OK;
+}
+
+int jq_attention_step(int32_t dtype, int32_t batch, int32_t heads, int32_t key_dim, int32_t value_dim, float scale,
+                      const float *log_decay, const jq_rows *q, const jq_rows *k, const jq_rows *v,
+                      const jq_rows *out, float *state, int64_t state_rows, const int64_t *rows,
+                      const uint8_t *starts, void *stream)
+{
+    TRY(check_dtype(dtype));
+    TRY(check_dims(batch, heads, key_dim, value_dim));
+    if (state_rows < 0) return fail(JQ_E_ARG, "negative state_rows");
+    if (batch == 0) return JQ_OK;
+    if (!log_decay || !q || !k || !v || !out) return fail(JQ_E_ARG, "null device pointer");
+    TRY(check_rows(*q, dtype, "q"));
+    TRY(check_rows(*k, dtype, "k"));
+    TRY(check_rows(*v, dtype, "v"));
+    TRY(check_rows(*out, dtype, "out"));
+    if (state_rows && !state) return fail(JQ_E_ARG, "null state");
+    if (!aligned(state, 16)) return fail(JQ_E_ARG, "state must be 16-byte aligned");
+    const StepArgs a{*q, *k, *v, *out, heads, key_dim, value_dim, scale, log_decay, state, state_rows, rows, starts};
+    const dim3 grid(batch * heads), block(128);
+    if (dtype == JQ_F32) hipLaunchKernelGGL(k_attention_step<float>, grid, block, 0, strm(stream), a);
+    else hipLaunchKernelGGL(k_attention_step<bf16>, grid, block, 0, strm(stream), a);
+    return launch_check("k_attention_step");
+}
+
+int jq_rotary(int32_t dtype, int64_t n0, int64_t n1, int32_t heads, int32_t dim, int32_t pairs, const jq_rows *x,
+              const jq_rows *out, const void *positions, int32_t positions64, int64_t positions_n0,
+              int64_t positions_n1, int32_t axes, const int32_t *section_ends, const float *frequencies,
+              int32_t interleaved, int32_t inverse, void *stream)
+{
+    TRY(check_dtype(dtype));
+    if (n0 < 0 || n1 < 0 || heads < 0 || dim <= 0 || pairs < 0 || 2 * (int64_t)pairs > dim)
+        return fail(JQ_E_ARG, "bad shapes (%lld x %lld tokens, heads %d, dim %d, pairs %d)", (long long)n0, (long long)n1,
+                    heads, dim, pairs);
+    if (axes < 1 || axes > JQ_ROTARY_MAX_AXES) return fail(JQ_E_ARG, "axes %d not in [1, %d]", axes, JQ_ROTARY_MAX_AXES);
+    if (!section_ends) return fail(JQ_E_ARG, "null section_ends");
+    for (int i = 0; i < axes; ++i)
+        if (section_ends[i] < (i ? section_ends[i - 1] : 0))
+            return fail(JQ_E_ARG, "section ends must not fall: %d at axis %d", section_ends[i], i);
+    if (section_ends[axes - 1] != pairs)
+        return fail(JQ_E_ARG, "the sections hold %d pairs, not %d", section_ends[axes - 1], pairs);
+    if (n0 == 0 || n1 == 0 || heads == 0) return JQ_OK;
+    if (n0 > INT_MAX / n1) return fail(JQ_E_ARG, "%lld x %lld tokens are too many", (long long)n0, (long long)n1);
+    if (!x || !out || (pairs && (!positions || !frequencies))) return fail(JQ_E_ARG, "null device pointer");
+    TRY(check_rows(*x, dtype, "x"));
+    TRY(check_rows(*out, dtype, "out"));
+    if (!aligned(positions, positions64 ? 8 : 4)) return fail(JQ_E_ARG, "positions must be aligned to their element size");
+    RotaryArgs a{*x, *out, n1, heads, dim, pairs, axes, positions, positions_n0, positions_n1, {}, frequencies,
+                 positions64 != 0, interleaved != 0, inverse != 0};
+    std::copy(section_ends, section_ends + axes, a.ends);
+    if (dtype == JQ_F32) hipLaunchKernelGGL(k_rotary<float>, dim3(n0 * n1), dim3(64), 0, strm(stream), a);
+    else hipLaunchKernelGGL(k_rotary<bf16>, dim3(n0 * n1), dim3(64), 0, strm(stream), a);
+    return launch_check("k_rotary");
+}
+
+int jq_layer_norm_forward(int32_t dtype, int32_t weight_dtype, int64_t rows, int32_t width, const void *x,
+                          int64_t x_stride, const void *weight, const void *bias, float eps, void *out,
+                          int64_t out_stride, float *mean, float *rstd, void *stream)
+{
+    TRY(check_norm(dtype, weight_dtype, rows, width));
+    if (rows == 0) return JQ_OK;
+    if (!x || !out) return fail(JQ_E_ARG, "null device pointer");
+    if (!aligned(x, elem_bytes(dtype)) || !aligned(out, elem_bytes(dtype)))
+        return fail(JQ_E_ARG, "rows must be aligned to their element size");
+    if (dtype == JQ_F32)
+        return norm_forward<float, float>(rows, width, x, x_stride, weight, bias, eps, out, out_stride, mean, rstd, strm(stream));
+    if (weight_dtype == JQ_F32)
+        return norm_forward<bf16, float>(rows, width, x, x_stride, weight, bias, eps, out, out_stride, mean, rstd, strm(stream));
+    return norm_forward<bf16, bf16>(rows, width, x, x_stride, weight, bias, eps, out, out_stride, mean, rstd, strm(stream));
+}
+
+int jq_layer_norm_workspace(int64_t rows, int32_t width, int64_t *bytes)
+{
+    TRY(check_norm(JQ_F32, JQ_F32, rows, width));
+    if (!bytes) return fail(JQ_E_ARG, "null output");
+    *bytes = std::min<int64_t>(NORM_PARTS, rows) * 2 * width * (int64_t)sizeof(float);
+    return JQ_OK;
+}
+
+int jq_layer_norm_backward(int32_t dtype, int32_t weight_dtype, int64_t rows, int32_t width, const void *x,
+                           int64_t x_stride, const void *weight, const float *mean, const float *rstd,
+                           const void *d_out, int64_t d_out_stride, void *dx, int64_t dx_stride, void *dweight,
+                           void *dbias, void *workspace, int64_t workspace_bytes, void *stream)
+{
+    TRY(check_norm(dtype, weight_dtype, rows, width));
+    if (rows && (!x || !mean || !rstd || !d_out)) return fail(JQ_E_ARG, "null device pointer");
+    if (!aligned(x, elem_bytes(dtype)) || !aligned(d_out, elem_bytes(dtype)) || !aligned(dx, elem_bytes(dtype)))
+        return fail(JQ_E_ARG, "rows must be aligned to their element size");
+    if (dweight || dbias) {
+        int64_t need = 0;
+        TRY(jq_layer_norm_workspace(rows, width, &need));
+        if (workspace_bytes < need || (need && !workspace))
+            return fail(JQ_E_ARG, "workspace of %lld bytes, %lld are needed", (long long)workspace_bytes, (long long)need);
+        if (!aligned(workspace, 4)) return fail(JQ_E_ARG, "workspace must be 4-byte aligned");
+    }
+    float *part = static_cast<float *>(workspace);
+    if (dtype == JQ_F32)
+        return norm_backward<float, float>(rows, width, x, x_stride, weight, mean, rstd, d_out, d_out_stride, dx,
+                                           dx_stride, dweight, dbias, part, strm(stream));
+    if (weight_dtype == JQ_F32)
+        return norm_backward<bf16, float>(rows, width, x, x_stride, weight, mean, rstd, d_out, d_out_stride, dx,
+                                          dx_stride, dweight, dbias, part, strm(stream));
+    return norm_backward<bf16, bf16>(rows, width, x, x_stride, weight, mean, rstd, d_out, d_out_stride, dx, dx_stride,
+                                     dweight, dbias, part, strm(stream));
+}
+
+}  // extern "C"
