@@ -20,6 +20,18 @@ template <class T> __device__ __forceinline__ T *row_at(const jq_rows &r, int64_
     return static_cast<T *>(r.data) + b * r.batch + t * r.ply + h * r.head;
 }
 
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
+
+// 16 bytes of T.
+template <class T> struct Vec;
+template <> struct Vec<float> { typedef f32x4 type; static constexpr int N = 4; };
+template <> struct Vec<bf16> { typedef bf16x8 type; static constexpr int N = 8; };
+
 // Sum over the wave, in every lane.
 __device__ __forceinline__ float wave_total(float x)
 {

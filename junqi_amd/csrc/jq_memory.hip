@@ -69,6 +69,74 @@ int check_attention_inputs(const jq_attention *a)
     return check_rows(a->v, a->dtype, "v");
 }
 
+// Whether a pass may take r's rows as whole aligned vectors of `bytes` through a
+// buffer descriptor of `plies` of them: no two rows share bytes, and they span less
+// than 2 GiB.
+bool whole_vectors(const jq_rows &r, int dim, size_t elem, size_t bytes, int plies)
+{
+    const int64_t n = (int64_t)(bytes / elem);
+    return aligned(r.data, bytes) && dim % n == 0 && r.batch % n == 0 && r.ply % n == 0 && r.head % n == 0 &&
+           r.ply >= dim && r.ply < ((int64_t)1 << 31) / (int64_t)elem / (plies + 1);
+}
+
+template <class T, int D, bool REV, bool FAST>
+int launch_pass(const ScanArgs &s, hipStream_t stream)
+{
+    const int heads = s.batch * s.heads;
+    if (s.segments > 1) {
+        hipLaunchKernelGGL((k_attention_pass<T, D, REV, FAST, false>), dim3(heads, s.segments - 1), dim3(4 * D), 0, stream, s);
+        TRY(launch_check("k_attention_pass (states)"));
+        hipLaunchKernelGGL(k_attention_join<REV>, dim3(heads, (s.kd * s.vd + 255) / 256), dim3(256), 0, stream, s);
+        TRY(launch_check("k_attention_join"));
+    }
+    hipLaunchKernelGGL((k_attention_pass<T, D, REV, FAST, true>), dim3(heads, s.segments), dim3(4 * D), 0, stream, s);
+    return launch_check("k_attention_pass");
+}
+
+template <class T, int D>
+int scan_width(const ScanArgs &s, hipStream_t stream)
+{
+    const bool fast = whole_vectors(s.q, s.kd, sizeof(T), 16, Mma<T>::CH) && whole_vectors(s.k, s.kd, sizeof(T), 16, Mma<T>::CH) &&
+                      whole_vectors(s.v, s.vd, sizeof(T), 16, Mma<T>::CH) &&
+                      whole_vectors(s.o, s.vd, sizeof(T), 4 * sizeof(T), Mma<T>::CH);
+    if (s.reverse) return fast ? launch_pass<T, D, true, true>(s, stream) : launch_pass<T, D, true, false>(s, stream);
+    return fast ? launch_pass<T, D, false, true>(s, stream) : launch_pass<T, D, false, false>(s, stream);
+}
+
+template <class T>
+int scan_as(const ScanArgs &s, hipStream_t stream)
+{
+    const int d = std::max(s.kd, s.vd);
+    return d <= 32 ? scan_width<T, 32>(s, stream) : d <= 64 ? scan_width<T, 64>(s, stream) : scan_width<T, 128>(s, stream);
+}
+
+int scan(int32_t dtype, const ScanArgs &s, hipStream_t stream)
+{
+    return dtype == JQ_F32 ? scan_as<float>(s, stream) : scan_as<bf16>(s, stream);
+}
+
+// How a call's plies are split: few games and heads leave the card idle unless
+// parts of a long axis run side by side.
+constexpr int SPLIT_BLOCKS = 1024, SPLIT_MIN_CHUNKS = 4;
+struct Split { int segments, seg_plies; };
+Split split_of(const jq_attention *a)
+{
+    const int ch = a->dtype == JQ_F32 ? Mma<float>::CH : Mma<bf16>::CH;
+    const int64_t heads = std::max<int64_t>(1, (int64_t)a->batch * a->heads), chunks = ((int64_t)a->plies + ch - 1) / ch;
+    const int64_t want = std::min(SPLIT_BLOCKS / heads, chunks / SPLIT_MIN_CHUNKS);
+    if (want < 2) return {1, (int)std::max<int64_t>(chunks, 1) * ch};
+    const int64_t each = (chunks + want - 1) / want;
+    return {(int)((chunks + each - 1) / each), (int)each * ch};
+}
+
+int64_t split_bytes(const jq_attention *a)
+{
+    const Split s = split_of(a);
+    if (s.segments < 2) return 0;
+    const int64_t n = (int64_t)a->batch * a->heads * s.segments;
+    return n * ((int64_t)a->key_dim * a->value_dim + 1) * (int64_t)sizeof(float);
+}
+
 ScanArgs scan_args(const jq_attention *a)
 {
     ScanArgs s{};
@@ -81,22 +149,21 @@ ScanArgs scan_args(const jq_attention *a)
     s.starts_ply = a->starts_ply;
     s.lengths = a->lengths;
     s.in_scale = s.out_scale = 1.f;
+    const Split split = split_of(a);
+    s.segments = split.segments;
+    s.seg_plies = split.seg_plies;
+    s.seg_states = static_cast<float *>(a->workspace);
+    s.seg_carry = s.seg_states ? s.seg_states + (int64_t)a->batch * a->heads * split.segments * a->key_dim * a->value_dim : nullptr;
     return s;
 }
 
-template <class T>
-int launch_scan(const ScanArgs &s, hipStream_t stream)
+int check_workspace(const jq_attention *a)
 {
-    const dim3 grid(s.batch * s.heads), block(128);
-    if (s.kd <= 32) hipLaunchKernelGGL((k_attention_scan<T, 32>), grid, block, 0, stream, s);
-    else if (s.kd <= 64) hipLaunchKernelGGL((k_attention_scan<T, 64>), grid, block, 0, stream, s);
-    else hipLaunchKernelGGL((k_attention_scan<T, 128>), grid, block, 0, stream, s);
-    return launch_check("k_attention_scan");
-}
-
-int scan(int32_t dtype, const ScanArgs &s, hipStream_t stream)
-{
-    return dtype == JQ_F32 ? launch_scan<float>(s, stream) : launch_scan<bf16>(s, stream);
+    const int64_t need = split_bytes(a);
+    if (a->workspace_bytes < need || (need && !a->workspace))
+        return fail(JQ_E_ARG, "workspace of %lld bytes, %lld are needed", (long long)a->workspace_bytes, (long long)need);
+    if (!aligned(a->workspace, 16)) return fail(JQ_E_ARG, "workspace must be 16-byte aligned");
+    return JQ_OK;
 }
 
 template <class T, class W>
@@ -150,7 +217,7 @@ int jq_attention_workspace(const jq_attention *a, int32_t backward, int64_t *byt
 {
     TRY(check_attention(a));
     if (!bytes) return fail(JQ_E_ARG, "null output");
-    *bytes = 0;
+    *bytes = split_bytes(a);
     return JQ_OK;
 }
 
@@ -160,6 +227,7 @@ int jq_attention_forward(const jq_attention *a, void *stream)
     if (a->batch == 0) return JQ_OK;
     TRY(check_attention_inputs(a));
     if (a->plies) TRY(check_rows(a->out, a->dtype, "out"));
+    TRY(check_workspace(a));
     ScanArgs s = scan_args(a);
     s.q = a->q, s.k = a->k, s.v = a->v, s.o = a->out;
     s.kd = a->key_dim, s.vd = a->value_dim;
@@ -174,6 +242,7 @@ int jq_attention_backward(const jq_attention *a, void *stream)
     if (a->batch == 0) return JQ_OK;
     TRY(check_attention_inputs(a));
     if (a->plies) TRY(check_rows(a->d_out, a->dtype, "d_out"));
+    TRY(check_workspace(a));
     if (!a->dk.data != !a->dv.data) return fail(JQ_E_ARG, "dk and dv go together");
     if (a->d_initial && !a->dk.data && a->plies) return fail(JQ_E_ARG, "d_initial comes with dk and dv");
     if (a->dq.data) {
