@@ -429,6 +429,7 @@ int jq_ids_to_mask(const int32_t *ids, const int32_t *counts, int64_t rows, int3
 #define JQ_BF16 1
 #define JQ_ATTENTION_MAX_DIM 128   /* largest key_dim and value_dim */
 #define JQ_ROTARY_MAX_AXES 4
+#define JQ_ROTARY_MAX_PAIRS 4096
 
 /* A (batch, plies, heads, dim) tensor: strides in elements; data NULL: absent. */
 typedef struct jq_rows {

@@ -19,6 +19,7 @@ ACT_WORLD, ACT_CANONICAL = 0, 1
 F32, BF16 = 0, 1
 ATTENTION_MAX_DIM = 128
 ROTARY_MAX_AXES = 4
+ROTARY_MAX_PAIRS = 4096
 NUM_CELLS = 289
 NUM_ON_BOARD = 129
 NUM_PIDS = 120

@@ -35,22 +35,24 @@ struct ScanArgs {
 // A product takes two fragments: lane l holds row (or column) l % 16 and, with
 // g = l / 16, the depths that its e-th elements stand for. The result has column
 // l % 16 and rows 4g .. 4g + 3 in lane l. Depths may be taken in any order that
-// both fragments share: `row` and `col` take them as they lie, `row_s` in the
-// order in which a result's rows lie in its lanes, so that a state goes from
-// result to operand without leaving its registers.
+// both fragments share. `deep`, `col` and the split state take them in the order in
+// which a result's rows lie in its lanes (depth), so that a state goes from result
+// to operand without leaving its registers; `row` takes them as they lie.
 template <class T> struct Mma;
 
 template <> struct Mma<bf16> {
     typedef bf16x8 Frag;
     static constexpr int CH = 64;   // plies of a chunk
     static constexpr int KB = 32;   // depth of a fragment
-    static constexpr int PARTS = 3; // terms that hold a float
     static __device__ __forceinline__ f32x4 mul(Frag a, Frag b, f32x4 c)
     {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
     }
+    static __device__ __forceinline__ int depth(int g, int e) { return 16 * (e >> 2) + 4 * g + (e & 3); }
+    // where depths d .. d + 3, d % 4 == 0, of a row stored for `row` lie, for `row` to give them in `depth`'s order
+    static __device__ __forceinline__ int place(int d) { return (d & ~31) + 2 * (d & 15) + ((d & 16) >> 2); }
     static __device__ __forceinline__ Frag row(const bf16 *p, int g) { return *reinterpret_cast<const Frag *>(p + 8 * g); }
-    static __device__ __forceinline__ Frag row_s(const bf16 *p, int g)
+    static __device__ __forceinline__ Frag deep(const bf16 *p, int g)
     {
         const bf16x4 x = *reinterpret_cast<const bf16x4 *>(p + 4 * g), y = *reinterpret_cast<const bf16x4 *>(p + 16 + 4 * g);
         return Frag{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
@@ -60,43 +62,78 @@ template <> struct Mma<bf16> {
     static __device__ __forceinline__ Frag col(const bf16 *p, int ld, int l)
     {
         typedef short s16x4 __attribute__((ext_vector_type(4)));
-        typedef __attribute__((address_space(3))) s16x4 *lds_ptr;
-        const bf16 *at = p + (8 * (l >> 4) + ((l & 15) >> 2)) * ld + 4 * (l & 3);
-        const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)at);
-        const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(at + 4 * ld));
         typedef short s16x8 __attribute__((ext_vector_type(8)));
+        typedef __attribute__((address_space(3))) s16x4 *lds_ptr;
+        const bf16 *at = p + (l >> 2) * ld + 4 * (l & 3);
+        const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)at);
+        const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(at + 16 * ld));
         return __builtin_bit_cast(Frag, s16x8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]});
     }
-    static __device__ __forceinline__ int depth(int g, int e) { return 8 * g + e; }
+    // x as a sum of N terms: 8 bits each
+    template <int N> static __device__ __forceinline__ void split(const float (&x)[8], Frag (&part)[N])
+    {
+        // (-1, 0) and (0, -1) from registers: as an operand's inline constant, -1 lands in the other half
+        uint32_t first = 0x0000BF80u, second = 0xBF800000u;
+        asm("" : "+s"(first), "+s"(second));
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+            float a = x[e], b = x[e + 1];
+#pragma unroll
+            for (int u = 0; u < N; ++u) {
+                const bf16x2 h{(bf16)a, (bf16)b};
+                part[u][e] = h[0];
+                part[u][e + 1] = h[1];
+                if (u + 1 < N) {   // what is left: exact
+                    a = __builtin_amdgcn_fdot2_f32_bf16(h, __builtin_bit_cast(bf16x2, first), a, false);
+                    b = __builtin_amdgcn_fdot2_f32_bf16(h, __builtin_bit_cast(bf16x2, second), b, false);
+                }
+            }
+        }
+    }
 };
 
 template <> struct Mma<float> {
     typedef f32x4 Frag;
     static constexpr int CH = 32;
     static constexpr int KB = 16;
-    static constexpr int PARTS = 1;
     static __device__ __forceinline__ f32x4 mul(Frag a, Frag b, f32x4 c)
     {
 #pragma unroll
         for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], c, 0, 0, 0);
         return c;
     }
+    static __device__ __forceinline__ int depth(int g, int e) { return 4 * g + e; }
+    static __device__ __forceinline__ int place(int d) { return d; }
     static __device__ __forceinline__ Frag row(const float *p, int g) { return *reinterpret_cast<const Frag *>(p + 4 * g); }
-    static __device__ __forceinline__ Frag row_s(const float *p, int g) { return row(p, g); }
+    static __device__ __forceinline__ Frag deep(const float *p, int g) { return row(p, g); }
     static __device__ __forceinline__ Frag col(const float *p, int ld, int l)
     {
         const float *at = p + 4 * (l >> 4) * ld + (l & 15);
         return Frag{at[0], at[ld], at[2 * ld], at[3 * ld]};
     }
-    static __device__ __forceinline__ int depth(int g, int e) { return 4 * g + e; }
+    template <int N> static __device__ __forceinline__ void split(const float (&x)[4], Frag (&part)[N])
+    {
+        part[0] = Frag{x[0], x[1], x[2], x[3]};
+    }
 };
 
-// lambda^d from log2 lambda (lambda^0 is 1 for lambda = 0 too).
-__device__ __forceinline__ float power(float log2_lam, int d) { return d ? __builtin_amdgcn_exp2f(log2_lam * d) : 1.f; }
+// Terms that a float32 operand is split into. In bfloat16, three hold all of a
+// float32: sums that come out in float32. Two hold 16 bits: operands of sums that
+// are rounded to bfloat16.
+template <class T, int N> constexpr int PARTS = sizeof(T) == 2 ? N : 1;
+
+// log2 lambda, and lambda^d from it: lambda = 0 has a logarithm whose products with
+// whole numbers are finite, so that lambda^0 is 1.
+__device__ __forceinline__ float log2_lambda(float log_decay)
+{
+    const float x = log_decay * 1.44269504088896340736f;
+    return x < -1e30f ? -1e30f : x;
+}
+__device__ __forceinline__ float power(float log2_lam, float d) { return __builtin_amdgcn_exp2f(log2_lam * d); }
 
 // What the plies of a chunk need to know of it, made once for each chunk.
 template <int CH>
-struct Marks {
+struct alignas(16) Marks {
     float sees[CH];    // lambda's power from the chunk's begin (REV: end) to the ply; -1: it sees nothing from there
     float leaves[CH];  // lambda's power from the ply to the chunk's end (REV: begin) times in_scale; 0: nothing is left
     int game[CH];      // games that start in the chunk up to the ply
@@ -113,14 +150,14 @@ struct Chunk {
     using Frag = typename M::Frag;
     static constexpr int CH = M::CH, KB = M::KB, NT = CH / 16, WAVES = D / 16, THREADS = 64 * WAVES;
     static constexpr int LD = D + Vec<T>::N, PLD = CH + Vec<T>::N;   // 16 bytes of padding turn the rows over the banks
-    static constexpr int FE = M::KB / 4;                             // elements of a fragment
+    static constexpr int FE = KB / 4;                                // elements of a fragment
 
     f32x4 s[D / 16];   // state (16t + 4g + r, 16w + l % 16)
     float g2;          // log2 lambda
     int w, l, lc, g;
 
     __device__ __forceinline__ Chunk(float log_decay)
-        : g2(log_decay * 1.44269504088896340736f), w(threadIdx.x >> 6), l(threadIdx.x & 63), lc(l & 15), g(l >> 4)
+        : g2(log2_lambda(log_decay)), w(threadIdx.x >> 6), l(threadIdx.x & 63), lc(l & 15), g(l >> 4)
     {
     }
 
@@ -171,7 +208,7 @@ struct Chunk {
     // tiles on the diagonal and on one side of it, shared out over the waves.
     __device__ __forceinline__ void scores(const T *q, const T *k, T *p, const Marks<CH> &mk, float scale) const
     {
-        const bool starts = mk.starts;
+        const bool starts = __builtin_amdgcn_readfirstlane(mk.starts);
         for (int m = w; m < NT * (NT + 1) / 2; m += WAVES) {
             const int a = m < 1 ? 0 : m < 3 ? 1 : m < 6 ? 2 : 3, b = m - a * (a + 1) / 2;
             const int it = REV ? b : a, jt = REV ? a : b;
@@ -180,13 +217,18 @@ struct Chunk {
             for (int c = 0; c < D; c += KB)
                 acc = M::mul(M::row(k + (16 * jt + lc) * LD + c, g), M::row(q + (16 * it + lc) * LD + c, g), acc);
             const int i = 16 * it + lc, j0 = 16 * jt + 4 * g;
+            const float d0 = (float)(REV ? j0 - i : i - j0);
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const int d = REV ? j0 + r - i : i - j0 - r;
-                const bool seen = d >= 0 && (!starts || mk.game[i] == mk.game[j0 + r]);
-                acc[r] = seen ? acc[r] * (scale * power(g2, d)) : 0.f;
+                const float d = REV ? d0 + r : d0 - r;
+                acc[r] = d >= 0.f ? acc[r] * (scale * power(g2, d)) : 0.f;
             }
-            store4(p + i * PLD + j0, acc);
+            if (starts) {
+                const int game = mk.game[i];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) acc[r] = game == mk.game[j0 + r] ? acc[r] : 0.f;
+            }
+            store4(p + i * PLD + M::place(j0), acc);
         }
     }
 
@@ -204,13 +246,17 @@ struct Chunk {
         for (int it = 0; it < NT; ++it) o[it] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int c = 0; c < D / KB; ++c) {
-            Frag hi, lo;
-            state_frag(c, hi, lo);
+            constexpr int N = PARTS<T, 2>;
+            Frag part[N];
+            float x[FE];
+#pragma unroll
+            for (int e = 0; e < FE; ++e) x[e] = s[(c * KB + 4 * e) / 16][e & 3];
+            M::template split<N>(x, part);
 #pragma unroll
             for (int it = 0; it < NT; ++it) {
-                const Frag x = M::row_s(q + (16 * it + lc) * LD + c * KB, g);
-                o[it] = M::mul(hi, x, o[it]);
-                if constexpr (sizeof(T) == 2) o[it] = M::mul(lo, x, o[it]);
+                const Frag y = M::deep(q + (16 * it + lc) * LD + c * KB, g);
+#pragma unroll
+                for (int u = 0; u < N; ++u) o[it] = M::mul(part[u], y, o[it]);
             }
         }
 #pragma unroll
@@ -220,17 +266,6 @@ struct Chunk {
             for (int r = 0; r < 4; ++r) o[it][r] = f >= 0.f ? o[it][r] * (f * scale) : 0.f;
         }
     }
-
-    __device__ __forceinline__ void state_frag(int c, bf16x8 &hi, bf16x8 &lo) const
-    {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const float x = s[2 * c + (e >> 2)][e & 3];
-            hi[e] = (bf16)x;
-            lo[e] = (bf16)(x - (float)hi[e]);
-        }
-    }
-    __device__ __forceinline__ void state_frag(int c, f32x4 &hi, f32x4 &) const { hi = s[c]; }
 
     // o += P v (OUT), and the state after the chunk.
     template <bool OUT>
@@ -254,27 +289,18 @@ struct Chunk {
                 if (!OUT || (REV ? c * KB + KB <= 16 * it : c * KB >= 16 * it + 16)) continue;   // nothing to see there
                 o[it] = M::mul(x, M::row(p + (16 * it + lc) * PLD + c * KB, g), o[it]);
             }
-            Frag part[M::PARTS];
-            weigh(x, mk.leaves + c * KB, part);
+            // the plies' values times what is left of them after the chunk
+            constexpr int N = PARTS<T, 3>;
+            Frag part[N];
+            float left[FE];
+#pragma unroll
+            for (int e = 0; e < FE; ++e) left[e] = (float)x[e] * mk.leaves[c * KB + M::depth(g, e)];
+            M::template split<N>(left, part);
 #pragma unroll
             for (int t = 0; t < D / 16; ++t) {
                 const Frag y = M::col(k + c * KB * LD + 16 * t, LD, l);
 #pragma unroll
-                for (int u = 0; u < M::PARTS; ++u) s[t] = M::mul(y, part[u], s[t]);
-            }
-        }
-    }
-
-    // Plies' values times what is left of them after the chunk, as terms that hold a float.
-    __device__ __forceinline__ void weigh(Frag x, const float *leaves, Frag (&part)[M::PARTS]) const
-    {
-#pragma unroll
-        for (int e = 0; e < FE; ++e) {
-            float y = (float)x[e] * leaves[M::depth(g, e)];
-#pragma unroll
-            for (int u = 0; u < M::PARTS; ++u) {
-                part[u][e] = from_float<T>(y);
-                y -= (float)part[u][e];
+                for (int u = 0; u < N; ++u) s[t] = M::mul(y, part[u], s[t]);
             }
         }
     }
@@ -418,7 +444,7 @@ struct Plies {
 // their way. OUT: the plies' outputs, from the state before the segment; else only
 // the state that the segment's own plies leave, for the states before the others.
 template <class T, int D, bool REV, bool FAST, bool OUT>
-__global__ __launch_bounds__(4 * D, 4) void k_attention_pass(ScanArgs a)
+__global__ __launch_bounds__(4 * D, D == 32 ? 3 : 4) void k_attention_pass(ScanArgs a)
 {
     using C = Chunk<T, D, REV>;
     using P = Plies<T, D, FAST>;
@@ -528,7 +554,8 @@ struct StepArgs {
     const uint8_t *starts;
 };
 
-// One ply of every game: one block per game and head, one thread per column.
+// One ply of every game, for value dims that are not whole vectors: one block per
+// game and head, one thread per column.
 template <class T>
 __global__ __launch_bounds__(128) void k_attention_step(StepArgs a)
 {
@@ -551,6 +578,62 @@ __global__ __launch_bounds__(128) void k_attention_step(StepArgs a)
         sum += (float)q[i] * x;
     }
     o[c] = from_float<T>(a.scale * sum);
+}
+
+// The same with a wave for each game and head. L lanes hold a row's columns, four
+// each; the 64 / L groups of lanes take a part of the rows each, STEP_ROWS at a time
+// with all their loads on their way, and their sums are joined by shuffles: no
+// barriers, the state is read and written once.
+constexpr int STEP_ROWS = 16, STEP_WAVES = 4;
+template <class T, int L>
+__global__ __launch_bounds__(64 * STEP_WAVES) void k_attention_step_wave(StepArgs a, int count)
+{
+    const int at = blockIdx.x * STEP_WAVES + (threadIdx.x >> 6);
+    if (at >= count) return;
+    const int b = at / a.heads, h = at % a.heads, l = threadIdx.x & 63, c = 4 * (l % L), g = l / L;
+    const bool on = c < a.dv;
+    const int64_t row = a.rows ? a.rows[b] : b;
+    const bool live = row >= 0 && row < a.state_rows;
+    f32x4 sum{0.f, 0.f, 0.f, 0.f};
+    if (live && on) {
+        float *s = a.state + (row * a.heads + h) * a.dk * a.dv + c;
+        const T *q = row_at<const T>(a.q, b, 0, h), *k = row_at<const T>(a.k, b, 0, h), *vp = row_at<const T>(a.v, b, 0, h) + c;
+        const f32x4 v{(float)vp[0], (float)vp[1], (float)vp[2], (float)vp[3]};
+        const float lam = expf(a.log_decay[h]);
+        const bool start = a.starts && a.starts[b];
+        const int each = (a.dk + 64 / L - 1) / (64 / L), end = min(a.dk, (g + 1) * each);
+        for (int i0 = g * each; i0 < end; i0 += STEP_ROWS) {
+            f32x4 x[STEP_ROWS];
+            float qs[STEP_ROWS], ks[STEP_ROWS];
+#pragma unroll
+            for (int i = 0; i < STEP_ROWS; ++i) {
+                const int r = min(i0 + i, end - 1);
+                x[i] = *reinterpret_cast<const f32x4 *>(s + r * a.dv);
+                qs[i] = (float)q[r];
+                ks[i] = (float)k[r];
+            }
+#pragma unroll
+            for (int i = 0; i < STEP_ROWS; ++i) {
+                if (i0 + i >= end) break;
+                f32x4 y;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    y[e] = fmaf(ks[i], v[e], start ? 0.f : lam * x[i][e]);
+                    sum[e] = fmaf(qs[i], y[e], sum[e]);
+                }
+                *reinterpret_cast<f32x4 *>(s + (i0 + i) * a.dv) = y;
+            }
+        }
+    }
+#pragma unroll
+    for (int o = L; o < 64; o <<= 1)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum[e] += __shfl_xor(sum[e], o);
+    if (g == 0 && on) {
+        T *o = row_at<T>(a.o, b, 0, h) + c;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = from_float<T>(live ? a.scale * sum[e] : 0.f);
+    }
 }
 
 }  // namespace jq

@@ -5,6 +5,7 @@
 
 #include <algorithm>
 #include <climits>
+#include <type_traits>
 
 #include "junqi_amd.h"
 #include "jq_error.h"
@@ -47,7 +48,8 @@ int check_dims(int32_t batch, int32_t heads, int32_t dk, int32_t dv)
     if (batch < 0 || heads <= 0) return fail(JQ_E_ARG, "bad shapes (batch %d, heads %d)", batch, heads);
     if (dk <= 0 || dv <= 0 || dk > JQ_ATTENTION_MAX_DIM || dv > JQ_ATTENTION_MAX_DIM)
         return fail(JQ_E_ARG, "key_dim %d and value_dim %d must be in [1, %d]", dk, dv, JQ_ATTENTION_MAX_DIM);
-    if ((int64_t)batch * heads > INT_MAX) return fail(JQ_E_ARG, "batch * heads %lld is too large", (long long)batch * heads);
+    if ((int64_t)batch * heads >= 1 << 23)   // a launch holds fewer than 2^32 threads
+        return fail(JQ_E_ARG, "batch * heads %lld is too large", (long long)batch * heads);
     return JQ_OK;
 }
 
@@ -166,36 +168,109 @@ int check_workspace(const jq_attention *a)
     return JQ_OK;
 }
 
-template <class T, class W>
-int norm_backward(int64_t rows, int32_t width, const void *x, int64_t x_stride, const void *weight, const float *mean,
-                  const float *rstd, const void *d_out, int64_t d_stride, void *dx, int64_t dx_stride, void *dweight,
-                  void *dbias, float *part, hipStream_t stream)
+template <class T>
+void step(const StepArgs &a, int count, hipStream_t stream)
 {
-    const T *xt = static_cast<const T *>(x), *dt = static_cast<const T *>(d_out);
-    if (dx && rows) {
-        hipLaunchKernelGGL((k_norm_dx<T, W>), dim3(rows), dim3(64), 0, stream, xt, x_stride, width,
-                           static_cast<const W *>(weight), mean, rstd, dt, d_stride, static_cast<T *>(dx), dx_stride);
-        TRY(launch_check("k_norm_dx"));
+    const dim3 grid((count + STEP_WAVES - 1) / STEP_WAVES), block(64 * STEP_WAVES);
+    if (a.dv % 4) hipLaunchKernelGGL(k_attention_step<T>, dim3(count), dim3(128), 0, stream, a);
+    else if (a.dv <= 16) hipLaunchKernelGGL((k_attention_step_wave<T, 4>), grid, block, 0, stream, a, count);
+    else if (a.dv <= 32) hipLaunchKernelGGL((k_attention_step_wave<T, 8>), grid, block, 0, stream, a, count);
+    else if (a.dv <= 64) hipLaunchKernelGGL((k_attention_step_wave<T, 16>), grid, block, 0, stream, a, count);
+    else hipLaunchKernelGGL((k_attention_step_wave<T, 32>), grid, block, 0, stream, a, count);
+}
+
+// Blocks for that much work: kernels over rows and tokens take the rest a grid's
+// stride on (a launch holds fewer than 2^32 threads).
+int grid_of(int64_t blocks) { return (int)std::min<int64_t>(blocks, 1 << 20); }
+
+template <class T, int N, bool INTERLEAVED>
+int launch_rotary(const RotaryArgs &a, int64_t all, hipStream_t stream)
+{
+    // about four items a thread, the tables within their share of LDS
+    const int items = std::max(1, a.dim / N * a.heads);
+    const int tokens = std::max(1, std::min(1024 / items, ROTARY_TABLE / std::max(1, a.pairs)));
+    hipLaunchKernelGGL((k_rotary<T, N, INTERLEAVED>), dim3(grid_of((all + tokens - 1) / tokens)), dim3(256),
+                       2 * sizeof(float) * tokens * a.pairs, stream, a, all, tokens);
+    return launch_check("k_rotary");
+}
+
+template <class T>
+int rotary(const RotaryArgs &a, int64_t all, hipStream_t stream)
+{
+    // whole vectors where the pairs are made of them, else pair by pair
+    constexpr int N = Vec<T>::N;
+    if (a.interleaved)
+        return 2 * a.pairs % N == 0 ? launch_rotary<T, N, true>(a, all, stream) : launch_rotary<T, 2, true>(a, all, stream);
+    return a.pairs % N == 0 ? launch_rotary<T, N, false>(a, all, stream) : launch_rotary<T, 1, false>(a, all, stream);
+}
+
+// f(group, vectors a lane) for the narrowest group that holds a row in registers;
+// false for a row that is wider than that.
+template <class T, class F>
+bool norm_shape(int width, F &&f)
+{
+    const int vectors = (width + Vec<T>::N - 1) / Vec<T>::N;
+    using std::integral_constant;
+    if (vectors <= 4) f(integral_constant<int, 4>(), integral_constant<int, 1>());
+    else if (vectors <= 8) f(integral_constant<int, 8>(), integral_constant<int, 1>());
+    else if (vectors <= 16) f(integral_constant<int, 16>(), integral_constant<int, 1>());
+    else if (vectors <= 32) f(integral_constant<int, 32>(), integral_constant<int, 1>());
+    else if (vectors <= 64) f(integral_constant<int, 64>(), integral_constant<int, 1>());
+    else if (vectors <= 128) f(integral_constant<int, 64>(), integral_constant<int, 2>());
+    else if (vectors <= 256) f(integral_constant<int, 256>(), integral_constant<int, 1>());
+    else if (vectors <= 512) f(integral_constant<int, 256>(), integral_constant<int, 2>());
+    else if (vectors <= 1024) f(integral_constant<int, 256>(), integral_constant<int, 4>());
+    else if (vectors <= 2048) f(integral_constant<int, 1024>(), integral_constant<int, 2>());
+    else return false;
+    return true;
+}
+
+// Blocks of the backward pass, each with its own sums of the weights' gradients:
+// four blocks a CU, and four rows a group at least, so that the sums' traffic stays
+// below the rows'.
+constexpr int NORM_BLOCKS = 1024, NORM_ROWS = 4;
+
+template <class T>
+int norm_parts(int64_t rows, int32_t width)
+{
+    int64_t parts = std::min<int64_t>((rows + NORM_ROWS - 1) / NORM_ROWS, NORM_BLOCKS);
+    norm_shape<T>(width, [&](auto g, auto nv) {
+        const int64_t each = (int64_t)NORM_ROWS * NormRow<T, g(), nv()>::GROUPS;
+        parts = std::min<int64_t>((rows + each - 1) / each, NORM_BLOCKS);
+    });
+    return (int)parts;
+}
+
+template <class T, class W>
+int norm_backward(NormArgs a, void *dweight, void *dbias, hipStream_t stream)
+{
+    const bool sums = dweight || dbias;
+    if (!sums) a.part = nullptr;
+    const int parts = norm_parts<T>(a.rows, a.width);
+    if (a.rows && (a.o || sums)) {
+        const bool fits = norm_shape<T>(a.width, [&](auto g, auto nv) {
+            hipLaunchKernelGGL((k_norm_backward<T, W, g(), nv()>), dim3(parts), dim3(NormRow<T, g(), nv()>::BLOCK), 0,
+                               stream, a);
+        });
+        if (!fits && a.o) hipLaunchKernelGGL((k_norm_dx_wide<T, W>), dim3(grid_of(a.rows)), dim3(1024), 0, stream, a);
+        if (!fits && sums) hipLaunchKernelGGL((k_norm_dw_wide<T>), dim3((a.width + 255) / 256, parts), dim3(256), 0, stream, a);
+        TRY(launch_check("k_norm_backward"));
     }
-    if (!dweight && !dbias) return JQ_OK;
-    const int blocks = (width + 63) / 64, parts = (int)std::min<int64_t>(NORM_PARTS, rows);
-    if (parts) {
-        hipLaunchKernelGGL((k_norm_dw<T>), dim3(blocks, parts), dim3(64), 0, stream, xt, x_stride, rows, width, mean,
-                           rstd, dt, d_stride, part);
-        TRY(launch_check("k_norm_dw"));
-    }
-    hipLaunchKernelGGL((k_norm_join<W>), dim3(blocks), dim3(64), 0, stream, part, parts, width,
+    if (!sums) return JQ_OK;
+    hipLaunchKernelGGL((k_norm_join<W>), dim3((a.width + 15) / 16, 2), dim3(256), 0, stream, a.part, parts, a.width,
                        static_cast<W *>(dweight), static_cast<W *>(dbias));
     return launch_check("k_norm_join");
 }
 
 template <class T, class W>
-int norm_forward(int64_t rows, int32_t width, const void *x, int64_t x_stride, const void *weight, const void *bias,
-                 float eps, void *out, int64_t out_stride, float *mean, float *rstd, hipStream_t stream)
+int norm_forward(const NormArgs &a, hipStream_t stream)
 {
-    hipLaunchKernelGGL((k_norm_forward<T, W>), dim3(rows), dim3(64), 0, stream, static_cast<const T *>(x), x_stride,
-                       width, static_cast<const W *>(weight), static_cast<const W *>(bias), eps,
-                       static_cast<T *>(out), out_stride, mean, rstd);
+    const bool fits = norm_shape<T>(a.width, [&](auto g, auto nv) {
+        using R = NormRow<T, g(), nv()>;
+        hipLaunchKernelGGL((k_norm_forward<T, W, g(), nv()>), dim3(grid_of((a.rows + R::GROUPS - 1) / R::GROUPS)),
+                           dim3(R::BLOCK), 0, stream, a);
+    });
+    if (!fits) hipLaunchKernelGGL((k_norm_forward_wide<T, W>), dim3(grid_of(a.rows)), dim3(1024), 0, stream, a);
     return launch_check("k_norm_forward");
 }
 
@@ -291,9 +366,8 @@ int jq_attention_step(int32_t dtype, int32_t batch, int32_t heads, int32_t key_d
     if (state_rows && !state) return fail(JQ_E_ARG, "null state");
     if (!aligned(state, 16)) return fail(JQ_E_ARG, "state must be 16-byte aligned");
     const StepArgs a{*q, *k, *v, *out, heads, key_dim, value_dim, scale, log_decay, state, state_rows, rows, starts};
-    const dim3 grid(batch * heads), block(128);
-    if (dtype == JQ_F32) hipLaunchKernelGGL(k_attention_step<float>, grid, block, 0, strm(stream), a);
-    else hipLaunchKernelGGL(k_attention_step<bf16>, grid, block, 0, strm(stream), a);
+    if (dtype == JQ_F32) step<float>(a, batch * heads, strm(stream));
+    else step<bf16>(a, batch * heads, strm(stream));
     return launch_check("k_attention_step");
 }
 
@@ -306,6 +380,8 @@ int jq_rotary(int32_t dtype, int64_t n0, int64_t n1, int32_t heads, int32_t dim,
     if (n0 < 0 || n1 < 0 || heads < 0 || dim <= 0 || pairs < 0 || 2 * (int64_t)pairs > dim)
         return fail(JQ_E_ARG, "bad shapes (%lld x %lld tokens, heads %d, dim %d, pairs %d)", (long long)n0, (long long)n1,
                     heads, dim, pairs);
+    if (pairs > JQ_ROTARY_MAX_PAIRS || (int64_t)heads * dim > INT_MAX)
+        return fail(JQ_E_ARG, "%d pairs (at most %d) and %d heads of %d elements are too many", pairs, JQ_ROTARY_MAX_PAIRS, heads, dim);
     if (axes < 1 || axes > JQ_ROTARY_MAX_AXES) return fail(JQ_E_ARG, "axes %d not in [1, %d]", axes, JQ_ROTARY_MAX_AXES);
     if (!section_ends) return fail(JQ_E_ARG, "null section_ends");
     for (int i = 0; i < axes; ++i)
@@ -322,9 +398,7 @@ int jq_rotary(int32_t dtype, int64_t n0, int64_t n1, int32_t heads, int32_t dim,
     RotaryArgs a{*x, *out, n1, heads, dim, pairs, axes, positions, positions_n0, positions_n1, {}, frequencies,
                  positions64 != 0, interleaved != 0, inverse != 0};
     std::copy(section_ends, section_ends + axes, a.ends);
-    if (dtype == JQ_F32) hipLaunchKernelGGL(k_rotary<float>, dim3(n0 * n1), dim3(64), 0, strm(stream), a);
-    else hipLaunchKernelGGL(k_rotary<bf16>, dim3(n0 * n1), dim3(64), 0, strm(stream), a);
-    return launch_check("k_rotary");
+    return dtype == JQ_F32 ? rotary<float>(a, n0 * n1, strm(stream)) : rotary<bf16>(a, n0 * n1, strm(stream));
 }
 
 int jq_layer_norm_forward(int32_t dtype, int32_t weight_dtype, int64_t rows, int32_t width, const void *x,
@@ -336,18 +410,16 @@ int jq_layer_norm_forward(int32_t dtype, int32_t weight_dtype, int64_t rows, int
     if (!x || !out) return fail(JQ_E_ARG, "null device pointer");
     if (!aligned(x, elem_bytes(dtype)) || !aligned(out, elem_bytes(dtype)))
         return fail(JQ_E_ARG, "rows must be aligned to their element size");
-    if (dtype == JQ_F32)
-        return norm_forward<float, float>(rows, width, x, x_stride, weight, bias, eps, out, out_stride, mean, rstd, strm(stream));
-    if (weight_dtype == JQ_F32)
-        return norm_forward<bf16, float>(rows, width, x, x_stride, weight, bias, eps, out, out_stride, mean, rstd, strm(stream));
-    return norm_forward<bf16, bf16>(rows, width, x, x_stride, weight, bias, eps, out, out_stride, mean, rstd, strm(stream));
+    const NormArgs a{x, weight, bias, nullptr, out, x_stride, out_stride, 0, rows, width, eps, mean, rstd, nullptr};
+    if (dtype == JQ_F32) return norm_forward<float, float>(a, strm(stream));
+    return weight_dtype == JQ_F32 ? norm_forward<bf16, float>(a, strm(stream)) : norm_forward<bf16, bf16>(a, strm(stream));
 }
 
 int jq_layer_norm_workspace(int64_t rows, int32_t width, int64_t *bytes)
 {
     TRY(check_norm(JQ_F32, JQ_F32, rows, width));
     if (!bytes) return fail(JQ_E_ARG, "null output");
-    *bytes = std::min<int64_t>(NORM_PARTS, rows) * 2 * width * (int64_t)sizeof(float);
+    *bytes = (int64_t)std::max(norm_parts<float>(rows, width), norm_parts<bf16>(rows, width)) * 2 * width * (int64_t)sizeof(float);
     return JQ_OK;
 }
 
@@ -367,15 +439,11 @@ int jq_layer_norm_backward(int32_t dtype, int32_t weight_dtype, int64_t rows, in
             return fail(JQ_E_ARG, "workspace of %lld bytes, %lld are needed", (long long)workspace_bytes, (long long)need);
         if (!aligned(workspace, 4)) return fail(JQ_E_ARG, "workspace must be 4-byte aligned");
     }
-    float *part = static_cast<float *>(workspace);
-    if (dtype == JQ_F32)
-        return norm_backward<float, float>(rows, width, x, x_stride, weight, mean, rstd, d_out, d_out_stride, dx,
-                                           dx_stride, dweight, dbias, part, strm(stream));
-    if (weight_dtype == JQ_F32)
-        return norm_backward<bf16, float>(rows, width, x, x_stride, weight, mean, rstd, d_out, d_out_stride, dx,
-                                          dx_stride, dweight, dbias, part, strm(stream));
-    return norm_backward<bf16, bf16>(rows, width, x, x_stride, weight, mean, rstd, d_out, d_out_stride, dx, dx_stride,
-                                     dweight, dbias, part, strm(stream));
+    const NormArgs a{x, weight, nullptr, d_out, dx, x_stride, dx_stride, d_out_stride, rows, width, 0.f,
+                     const_cast<float *>(mean), const_cast<float *>(rstd), static_cast<float *>(workspace)};
+    if (dtype == JQ_F32) return norm_backward<float, float>(a, dweight, dbias, strm(stream));
+    return weight_dtype == JQ_F32 ? norm_backward<bf16, float>(a, dweight, dbias, strm(stream))
+                                  : norm_backward<bf16, bf16>(a, dweight, dbias, strm(stream));
 }
 
 }  // extern "C"

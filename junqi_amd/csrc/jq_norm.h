@@ -4,89 +4,306 @@
 
 namespace jq {
 
-// One wave per row: the mean, then the squares of what is off it, then the result.
-template <class T, class W>
-__global__ __launch_bounds__(64) void k_norm_forward(const T *__restrict__ x, int64_t x_stride, int width,
-                                                     const W *__restrict__ w, const W *__restrict__ bias, float eps,
-                                                     T *__restrict__ o, int64_t o_stride, float *mean_out,
-                                                     float *rstd_out)
+// Rows are walked in vectors of 16 bytes by groups of G lanes: lane i of a group has
+// vectors i, i + G, ... (NV of them), so a row stays in registers between its
+// statistics and its result and is read once. Up to a wave's 64 lanes a group is
+// part of a wave and a block has several; G = 256 and 1024 are a block each.
+constexpr int norm_block(int group) { return group > 256 ? group : 256; }
+
+template <class T, int G, int NV>
+struct NormRow {
+    static constexpr int N = Vec<T>::N, BLOCK = norm_block(G), GROUPS = BLOCK / G;
+    float x[NV * N];
+
+    __device__ __forceinline__ static int lane() { return threadIdx.x % G; }
+
+    // f(first element, index in x, count) for this lane's vectors
+    template <class F>
+    __device__ __forceinline__ static void each(int width, F &&f)
+    {
+#pragma unroll
+        for (int u = 0; u < NV; ++u) {
+            const int c = (lane() + u * G) * N;
+            if (c < width) f(c, u * N, min(N, width - c));
+        }
+    }
+
+    __device__ __forceinline__ void load(const T *row, int width)
+    {
+#pragma unroll
+        for (int i = 0; i < NV * N; ++i) x[i] = 0.f;
+        each(width, [&](int c, int i, int n) { load_vec(row + c, n, x + i); });
+    }
+
+    // n elements (all of a vector but at the row's end) at any element alignment
+    __device__ __forceinline__ static void load_vec(const T *p, int n, float *x)
+    {
+        if (n == N) {
+            typedef typename Vec<T>::type V __attribute__((aligned(sizeof(T))));
+            const V v = *reinterpret_cast<const V *>(p);
+#pragma unroll
+            for (int e = 0; e < N; ++e) x[e] = (float)v[e];
+        } else
+#pragma unroll
+            for (int e = 0; e < N; ++e)
+                if (e < n) x[e] = (float)p[e];
+    }
+    __device__ __forceinline__ static void store_vec(T *p, int n, const float *x)
+    {
+        if (n == N) {
+            typedef typename Vec<T>::type V __attribute__((aligned(sizeof(T))));
+            V v;
+#pragma unroll
+            for (int e = 0; e < N; ++e) v[e] = from_float<T>(x[e]);
+            *reinterpret_cast<V *>(p) = v;
+        } else
+#pragma unroll
+            for (int e = 0; e < N; ++e)
+                if (e < n) p[e] = from_float<T>(x[e]);
+    }
+
+    // the group's sums of a and b, in every lane; red: 2 * BLOCK / 64 floats of LDS
+    __device__ __forceinline__ static void sum(float &a, float &b, float *red)
+    {
+#pragma unroll
+        for (int o = min(G, 64) / 2; o; o >>= 1) {
+            a += __shfl_xor(a, o);
+            b += __shfl_xor(b, o);
+        }
+        if constexpr (G > 64) {
+            constexpr int W = G / 64;
+            __syncthreads();
+            if (threadIdx.x % 64 == 0) {
+                red[threadIdx.x / 64] = a;
+                red[W + threadIdx.x / 64] = b;
+            }
+            __syncthreads();
+            a = b = 0.f;
+#pragma unroll
+            for (int i = 0; i < W; ++i) {
+                a += red[i];
+                b += red[W + i];
+            }
+        }
+    }
+};
+
+struct NormArgs {
+    const void *x, *w, *bias, *d;   // d: gradient of the result (backward)
+    void *o;                        // result, or gradient of x
+    int64_t x_stride, o_stride, d_stride, rows;
+    int width;
+    float eps, *mean, *rstd, *part;
+};
+
+// out = (x - mean) rstd w + bias. The variance is that of the differences, so an
+// offset far from 0 costs no digits.
+template <class T, class W, int G, int NV>
+__global__ __launch_bounds__(norm_block(G)) void k_norm_forward(NormArgs a)
 {
-    const int64_t r = blockIdx.x;
-    x += r * x_stride;
-    o += r * o_stride;
-    float sum = 0.f, sq = 0.f;
-    for (int c = threadIdx.x; c < width; c += 64) sum += (float)x[c];
-    const float mean = wave_total(sum) / width;
-    for (int c = threadIdx.x; c < width; c += 64) sq += ((float)x[c] - mean) * ((float)x[c] - mean);
-    const float rstd = rsqrtf(wave_total(sq) / width + eps);
-    for (int c = threadIdx.x; c < width; c += 64)
-        o[c] = from_float<T>(((float)x[c] - mean) * rstd * (w ? (float)w[c] : 1.f) + (bias ? (float)bias[c] : 0.f));
-    if (threadIdx.x == 0) {
-        if (mean_out) mean_out[r] = mean;
-        if (rstd_out) rstd_out[r] = rstd;
+    using R = NormRow<T, G, NV>;
+    __shared__ float red[2 * R::BLOCK / 64];
+    const W *w = static_cast<const W *>(a.w), *bias = static_cast<const W *>(a.bias);
+    for (int64_t r = (int64_t)blockIdx.x * R::GROUPS + threadIdx.x / G; r < a.rows; r += (int64_t)gridDim.x * R::GROUPS) {
+        R row;
+        row.load(static_cast<const T *>(a.x) + r * a.x_stride, a.width);
+        float s = 0.f, q = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV * R::N; ++i) s += row.x[i];
+        R::sum(s, q, red);
+        const float mean = s / a.width;
+        q = 0.f;
+        R::each(a.width, [&](int, int i, int n) {
+#pragma unroll
+            for (int e = 0; e < R::N; ++e) {
+                row.x[i + e] -= mean;
+                if (e < n) q = fmaf(row.x[i + e], row.x[i + e], q);
+            }
+        });
+        R::sum(q, s, red);
+        const float rstd = 1.f / sqrtf(q / a.width + a.eps);
+        T *o = static_cast<T *>(a.o) + r * a.o_stride;
+        R::each(a.width, [&](int c, int i, int n) {
+            float y[R::N];
+#pragma unroll
+            for (int e = 0; e < R::N; ++e) y[e] = row.x[i + e] * rstd;
+            if (w)
+#pragma unroll
+                for (int e = 0; e < R::N; ++e) y[e] *= e < n ? (float)w[c + e] : 0.f;
+            if (bias)
+#pragma unroll
+                for (int e = 0; e < R::N; ++e) y[e] += e < n ? (float)bias[c + e] : 0.f;
+            R::store_vec(o + c, n, y);
+        });
+        if (R::lane() == 0) {
+            if (a.mean) a.mean[r] = mean;
+            if (a.rstd) a.rstd[r] = rstd;
+        }
     }
 }
 
-// dx = rstd (g - mean(g) - xhat mean(g xhat)), g = d_out w. One wave per row.
-template <class T, class W>
-__global__ __launch_bounds__(64) void k_norm_dx(const T *__restrict__ x, int64_t x_stride, int width,
-                                                const W *__restrict__ w, const float *__restrict__ mean,
-                                                const float *__restrict__ rstd, const T *__restrict__ d,
-                                                int64_t d_stride, T *__restrict__ dx, int64_t dx_stride)
+// dx = rstd (g - mean(g) - xhat mean(g xhat)), g = d w, and this block's part of
+// dw = sum d xhat and db = sum d: its groups go over rows a grid's stride apart with
+// the sums of their columns in registers, and join them in order at the end.
+// part[block][0][c]: dw, [1]: db.
+template <class T, class W, int G, int NV>
+__global__ __launch_bounds__(norm_block(G)) void k_norm_backward(NormArgs a)
 {
-    const int64_t r = blockIdx.x;
-    x += r * x_stride;
-    d += r * d_stride;
-    dx += r * dx_stride;
-    const float m = mean[r], rs = rstd[r];
-    float g1 = 0.f, g2 = 0.f;
-    for (int c = threadIdx.x; c < width; c += 64) {
-        const float g = (float)d[c] * (w ? (float)w[c] : 1.f);
-        g1 += g;
-        g2 += g * (((float)x[c] - m) * rs);
+    using R = NormRow<T, G, NV>;
+    constexpr int N = R::N;
+    __shared__ float red[2 * R::BLOCK / 64];
+    __shared__ float join[R::GROUPS > 1 ? R::BLOCK * N : 1];
+    const W *w = static_cast<const W *>(a.w);
+    float dw[NV * N] = {}, db[NV * N] = {}, weight[NV * N];
+#pragma unroll
+    for (int i = 0; i < NV * N; ++i) weight[i] = 1.f;
+    if (w)
+        R::each(a.width, [&](int c, int i, int n) {
+#pragma unroll
+            for (int e = 0; e < N; ++e)
+                if (e < n) weight[i + e] = (float)w[c + e];
+        });
+    for (int64_t r = (int64_t)blockIdx.x * R::GROUPS + threadIdx.x / G; r < a.rows; r += (int64_t)gridDim.x * R::GROUPS) {
+        R row, d;
+        row.load(static_cast<const T *>(a.x) + r * a.x_stride, a.width);
+        d.load(static_cast<const T *>(a.d) + r * a.d_stride, a.width);
+        const float mean = a.mean[r], rstd = a.rstd[r];
+        float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV * N; ++i) {   // past the row's end d is 0
+            row.x[i] = (row.x[i] - mean) * rstd;
+            db[i] += d.x[i];
+            dw[i] = fmaf(d.x[i], row.x[i], dw[i]);
+            d.x[i] *= weight[i];
+            s1 += d.x[i];
+            s2 = fmaf(d.x[i], row.x[i], s2);
+        }
+        if (a.o) {
+            R::sum(s1, s2, red);
+            s1 /= a.width;
+            s2 /= a.width;
+            T *o = static_cast<T *>(a.o) + r * a.o_stride;
+            R::each(a.width, [&](int c, int i, int n) {
+                float y[N];
+#pragma unroll
+                for (int e = 0; e < N; ++e) y[e] = rstd * (d.x[i + e] - s1 - row.x[i + e] * s2);
+                R::store_vec(o + c, n, y);
+            });
+        }
     }
-    g1 = wave_total(g1) / width;
-    g2 = wave_total(g2) / width;
-    for (int c = threadIdx.x; c < width; c += 64) {
-        const float g = (float)d[c] * (w ? (float)w[c] : 1.f);
-        dx[c] = from_float<T>(rs * (g - g1 - ((float)x[c] - m) * rs * g2));
+    if (!a.part) return;
+    float *part = a.part + (int64_t)blockIdx.x * 2 * a.width;
+#pragma unroll
+    for (int which = 0; which < 2; ++which)
+#pragma unroll
+        for (int u = 0; u < NV; ++u) {
+            float y[N];
+#pragma unroll
+            for (int e = 0; e < N; ++e) y[e] = which ? db[u * N + e] : dw[u * N + e];
+            if constexpr (R::GROUPS > 1) {
+                __syncthreads();
+#pragma unroll
+                for (int e = 0; e < N; ++e) join[threadIdx.x * N + e] = y[e];
+                __syncthreads();
+                if (threadIdx.x >= G) continue;
+                for (int g = 1; g < R::GROUPS; ++g)
+#pragma unroll
+                    for (int e = 0; e < N; ++e) y[e] += join[(g * G + threadIdx.x) * N + e];
+            }
+            const int c = (R::lane() + u * G) * N;
+#pragma unroll
+            for (int e = 0; e < N; ++e)
+                if (c + e < a.width) part[which * a.width + c + e] = y[e];
+        }
+}
+
+// Rows wider than a block's registers: read again for each step of the same sums.
+template <class T, class W>
+__global__ __launch_bounds__(1024) void k_norm_forward_wide(NormArgs a)
+{
+    using R = NormRow<T, 1024, 1>;
+    __shared__ float red[32];
+    for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
+        const T *x = static_cast<const T *>(a.x) + r * a.x_stride;
+        const W *w = static_cast<const W *>(a.w), *bias = static_cast<const W *>(a.bias);
+        float s = 0.f, q = 0.f;
+        for (int c = threadIdx.x; c < a.width; c += 1024) s += (float)x[c];
+        R::sum(s, q, red);
+        const float mean = s / a.width;
+        q = 0.f;
+        for (int c = threadIdx.x; c < a.width; c += 1024) q = fmaf((float)x[c] - mean, (float)x[c] - mean, q);
+        R::sum(q, s, red);
+        const float rstd = 1.f / sqrtf(q / a.width + a.eps);
+        T *o = static_cast<T *>(a.o) + r * a.o_stride;
+        for (int c = threadIdx.x; c < a.width; c += 1024)
+            o[c] = from_float<T>(((float)x[c] - mean) * rstd * (w ? (float)w[c] : 1.f) + (bias ? (float)bias[c] : 0.f));
+        if (threadIdx.x == 0) {
+            if (a.mean) a.mean[r] = mean;
+            if (a.rstd) a.rstd[r] = rstd;
+        }
     }
 }
 
-constexpr int NORM_PARTS = 512;   // row ranges that are summed apart
+template <class T, class W>
+__global__ __launch_bounds__(1024) void k_norm_dx_wide(NormArgs a)
+{
+    using R = NormRow<T, 1024, 1>;
+    __shared__ float red[32];
+    for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
+        const T *x = static_cast<const T *>(a.x) + r * a.x_stride, *d = static_cast<const T *>(a.d) + r * a.d_stride;
+        const W *w = static_cast<const W *>(a.w);
+        const float mean = a.mean[r], rstd = a.rstd[r];
+        float s1 = 0.f, s2 = 0.f;
+        for (int c = threadIdx.x; c < a.width; c += 1024) {
+            const float g = (float)d[c] * (w ? (float)w[c] : 1.f);
+            s1 += g;
+            s2 = fmaf(g, ((float)x[c] - mean) * rstd, s2);
+        }
+        R::sum(s1, s2, red);
+        s1 /= a.width;
+        s2 /= a.width;
+        T *o = static_cast<T *>(a.o) + r * a.o_stride;
+        for (int c = threadIdx.x; c < a.width; c += 1024)
+            o[c] = from_float<T>(rstd * ((float)d[c] * (w ? (float)w[c] : 1.f) - s1 - ((float)x[c] - mean) * rstd * s2));
+    }
+}
 
-// Sums of one range of rows for 64 columns: part[y][0][c] of d_out xhat, [1] of d_out.
+// part as in k_norm_backward: blockIdx.y's range of rows, 256 columns a block.
 template <class T>
-__global__ __launch_bounds__(64) void k_norm_dw(const T *__restrict__ x, int64_t x_stride, int64_t rows, int width,
-                                                const float *__restrict__ mean, const float *__restrict__ rstd,
-                                                const T *__restrict__ d, int64_t d_stride, float *__restrict__ part)
+__global__ __launch_bounds__(256) void k_norm_dw_wide(NormArgs a)
 {
-    const int c = blockIdx.x * 64 + threadIdx.x;
-    if (c >= width) return;
+    const int c = blockIdx.x * 256 + threadIdx.x;
+    if (c >= a.width) return;
+    const T *x = static_cast<const T *>(a.x) + c, *d = static_cast<const T *>(a.d) + c;
     float sw = 0.f, sb = 0.f;
-    for (int64_t r = rows * blockIdx.y / gridDim.y; r < rows * (blockIdx.y + 1) / gridDim.y; ++r) {
-        const float g = (float)d[r * d_stride + c];
-        sw += g * (((float)x[r * x_stride + c] - mean[r]) * rstd[r]);
+    for (int64_t r = a.rows * blockIdx.y / gridDim.y; r < a.rows * (blockIdx.y + 1) / gridDim.y; ++r) {
+        const float g = (float)d[r * a.d_stride];
+        sw = fmaf(g, ((float)x[r * a.x_stride] - a.mean[r]) * a.rstd[r], sw);
         sb += g;
     }
-    part[(int64_t)(2 * blockIdx.y) * width + c] = sw;
-    part[(int64_t)(2 * blockIdx.y + 1) * width + c] = sb;
+    a.part[(int64_t)(2 * blockIdx.y) * a.width + c] = sw;
+    a.part[(int64_t)(2 * blockIdx.y + 1) * a.width + c] = sb;
 }
 
-// The ranges' sums joined in order.
+// The blocks' sums joined: 16 columns of dw (blockIdx.y 0) or db a block, each by 16
+// threads that take every 16th part and are joined in order.
 template <class W>
-__global__ __launch_bounds__(64) void k_norm_join(const float *__restrict__ part, int parts, int width,
-                                                  W *__restrict__ dw, W *__restrict__ db)
+__global__ __launch_bounds__(256) void k_norm_join(const float *__restrict__ part, int parts, int width,
+                                                   W *__restrict__ dw, W *__restrict__ db)
 {
-    const int c = blockIdx.x * 64 + threadIdx.x;
-    if (c >= width) return;
-    float sw = 0.f, sb = 0.f;
-    for (int y = 0; y < parts; ++y) {
-        sw += part[(int64_t)(2 * y) * width + c];
-        sb += part[(int64_t)(2 * y + 1) * width + c];
-    }
-    if (dw) dw[c] = from_float<W>(sw);
-    if (db) db[c] = from_float<W>(sb);
+    W *out = blockIdx.y ? db : dw;
+    if (!out) return;
+    __shared__ float sum[16][16];
+    const int i = threadIdx.x % 16, j = threadIdx.x / 16, c = blockIdx.x * 16 + i;
+    float s = 0.f;
+    if (c < width)
+#pragma unroll 8
+        for (int y = j; y < parts; y += 16) s += part[(2 * (int64_t)y + blockIdx.y) * width + c];
+    sum[j][i] = s;
+    __syncthreads();
+    if (j || c >= width) return;
+    for (int y = 1; y < 16; ++y) s += sum[y][i];
+    out[c] = from_float<W>(s);
 }
 
 }  // namespace jq

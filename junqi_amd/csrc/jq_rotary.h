@@ -23,32 +23,71 @@ __device__ __forceinline__ void turn_of(int64_t position, float frequency, float
     sincospif((float)(half - 2.0 * rint(0.5 * half)), &s, &c);
 }
 
-// One block per token: a pair's angle is computed once for all heads.
-template <class T>
-__global__ __launch_bounds__(64) void k_rotary(RotaryArgs a)
+// A block takes `tokens` tokens at a time: first the cosines and sines of their
+// pairs, once for all heads, into LDS; then the heads' elements, N at a time at any
+// element alignment. Work item (token, head, i): i below `turns` turns N elements
+// (two parts of N where pairs are apart), the others copy.
+constexpr int ROTARY_TABLE = 2048;   // pairs of a block's tokens at most (unless one token has more)
+template <class T, int N, bool INTERLEAVED>
+__global__ __launch_bounds__(256) void k_rotary(RotaryArgs a, int64_t all, int tokens)
 {
-    const int64_t b = blockIdx.x / a.n1, t = blockIdx.x % a.n1;
-    const int64_t at = b * a.p0 + t * a.p1;
-    for (int p = threadIdx.x; p < a.pairs; p += 64) {
-        int axis = 0;
-        while (p >= a.ends[axis]) ++axis;
-        const int64_t pos = a.positions64 ? static_cast<const int64_t *>(a.positions)[at + axis]
-                                          : static_cast<const int32_t *>(a.positions)[at + axis];
-        float c, s;
-        turn_of(pos, a.frequencies[p], c, s);
-        if (a.inverse) s = -s;
-        const int i = a.interleaved ? 2 * p : p, j = a.interleaved ? 2 * p + 1 : a.pairs + p;
-        for (int h = 0; h < a.heads; ++h) {
-            const T *x = row_at<const T>(a.x, b, t, h);
-            T *o = row_at<T>(a.o, b, t, h);
-            const float u = (float)x[i], v = (float)x[j];
-            o[i] = from_float<T>(u * c - v * s);
-            o[j] = from_float<T>(v * c + u * s);
+    typedef T V __attribute__((ext_vector_type(N), aligned(sizeof(T))));
+    extern __shared__ float table[];   // cos of (token, pair), then sin
+    float *cs = table, *sn = table + tokens * a.pairs;
+    const int turns = INTERLEAVED ? 2 * a.pairs / N : a.pairs / N, rest = a.dim - 2 * a.pairs;
+    const bool whole = rest % N == 0;   // the rest is copied in vectors too, or by element
+    const int items = turns + (whole ? rest / N : rest);
+    for (int64_t t0 = (int64_t)blockIdx.x * tokens; t0 < all; t0 += (int64_t)gridDim.x * tokens) {
+        const int n = (int)min((int64_t)tokens, all - t0);
+        __syncthreads();
+        for (int x = threadIdx.x; x < n * a.pairs; x += 256) {
+            const int token = x / a.pairs, p = x % a.pairs;
+            const int64_t at = (t0 + token) / a.n1 * a.p0 + (t0 + token) % a.n1 * a.p1;
+            int axis = 0;
+            while (p >= a.ends[axis]) ++axis;
+            const int64_t pos = a.positions64 ? static_cast<const int64_t *>(a.positions)[at + axis]
+                                              : static_cast<const int32_t *>(a.positions)[at + axis];
+            float c, s;
+            turn_of(pos, a.frequencies[p], c, s);
+            cs[x] = c;
+            sn[x] = a.inverse ? -s : s;
+        }
+        __syncthreads();
+        for (int x = threadIdx.x; x < n * a.heads * items; x += 256) {
+            const int i = x % items, head = x / items % a.heads, token = x / items / a.heads;
+            const int64_t b = (t0 + token) / a.n1, t = (t0 + token) % a.n1;
+            const T *in = row_at<const T>(a.x, b, t, head);
+            T *out = row_at<T>(a.o, b, t, head);
+            if (i >= turns) {
+                const int at = 2 * a.pairs + (i - turns) * (whole ? N : 1);
+                if (whole) *reinterpret_cast<V *>(out + at) = *reinterpret_cast<const V *>(in + at);
+                else out[at] = in[at];
+            } else if constexpr (INTERLEAVED) {
+                const V u = *reinterpret_cast<const V *>(in + i * N);
+                V y;
+#pragma unroll
+                for (int e = 0; e < N; e += 2) {
+                    const int p = token * a.pairs + (i * N + e) / 2;
+                    const float c = cs[p], s = sn[p], u0 = (float)u[e], u1 = (float)u[e + 1];
+                    y[e] = from_float<T>(u0 * c - u1 * s);
+                    y[e + 1] = from_float<T>(u1 * c + u0 * s);
+                }
+                *reinterpret_cast<V *>(out + i * N) = y;
+            } else {
+                const V u = *reinterpret_cast<const V *>(in + i * N), v = *reinterpret_cast<const V *>(in + a.pairs + i * N);
+                V y, z;
+#pragma unroll
+                for (int e = 0; e < N; ++e) {
+                    const int p = token * a.pairs + i * N + e;
+                    const float c = cs[p], s = sn[p], u0 = (float)u[e], u1 = (float)v[e];
+                    y[e] = from_float<T>(u0 * c - u1 * s);
+                    z[e] = from_float<T>(u1 * c + u0 * s);
+                }
+                *reinterpret_cast<V *>(out + i * N) = y;
+                *reinterpret_cast<V *>(out + a.pairs + i * N) = z;
+            }
         }
     }
-    for (int h = 0; h < a.heads; ++h)
-        for (int i = 2 * a.pairs + threadIdx.x; i < a.dim; i += 64)
-            row_at<T>(a.o, b, t, h)[i] = row_at<const T>(a.x, b, t, h)[i];
 }
 
 }  // namespace jq

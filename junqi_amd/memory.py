@@ -322,8 +322,8 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, frequencies: torch.Tensor, 
     axes, pairs, d = len(sections), sum(sections), x.shape[-1]
     if not 1 <= axes <= L.ROTARY_MAX_AXES or min(sections) < 0:
         raise ValueError(f"sections must be 1 to {L.ROTARY_MAX_AXES} counts of pairs, got {sections}")
-    if not 0 < 2 * pairs <= d:
-        raise ValueError(f"{pairs} pairs do not fit heads of {d} elements")
+    if not 0 < 2 * pairs <= d or pairs > L.ROTARY_MAX_PAIRS:
+        raise ValueError(f"{pairs} pairs do not fit heads of {d} elements (at most {L.ROTARY_MAX_PAIRS} pairs)")
     _check("positions", positions, (*x.shape[:-2], axes), (torch.int32, torch.int64), x)
     _check("frequencies", frequencies, (pairs,), (torch.float32,), x)
     if frequencies.requires_grad and torch.is_grad_enabled():
