@@ -229,6 +229,7 @@ bool norm_shape(int width, F &&f)
 // four blocks a CU, and four rows a group at least, so that the sums' traffic stays
 // below the rows'.
 constexpr int NORM_BLOCKS = 1024, NORM_ROWS = 4;
+constexpr int NORM_FORWARD_THREADS = 2048 * 256;   // of the forward pass: all that a card's CUs hold
 
 template <class T>
 int norm_parts(int64_t rows, int32_t width)
@@ -267,7 +268,7 @@ int norm_forward(const NormArgs &a, hipStream_t stream)
 {
     const bool fits = norm_shape<T>(a.width, [&](auto g, auto nv) {
         using R = NormRow<T, g(), nv()>;
-        hipLaunchKernelGGL((k_norm_forward<T, W, g(), nv()>), dim3(grid_of((a.rows + R::GROUPS - 1) / R::GROUPS)),
+        hipLaunchKernelGGL((k_norm_forward<T, W, g(), nv()>), dim3(std::min<int64_t>((a.rows + R::GROUPS - 1) / R::GROUPS, NORM_FORWARD_THREADS / R::BLOCK)),
                            dim3(R::BLOCK), 0, stream, a);
     });
     if (!fits) hipLaunchKernelGGL((k_norm_forward_wide<T, W>), dim3(grid_of(a.rows)), dim3(1024), 0, stream, a);

@@ -32,21 +32,38 @@ struct NormRow {
     {
 #pragma unroll
         for (int i = 0; i < NV * N; ++i) x[i] = 0.f;
-        each(width, [&](int c, int i, int n) { load_vec(row + c, n, x + i); });
+        each(width, [&](int c, int i, int n) { load_vec(row + c, n, x + i, 0.f); });
+    }
+
+    // x = this lane's columns of p (weights), or `other` without p and past the row's end
+    template <class W>
+    __device__ __forceinline__ static void columns(const W *p, int width, float other, float (&x)[NV * N])
+    {
+#pragma unroll
+        for (int i = 0; i < NV * N; ++i) x[i] = other;
+        if (p) each(width, [&](int c, int i, int n) { load_vec(p + c, n, x + i, other); });
     }
 
     // n elements (all of a vector but at the row's end) at any element alignment
-    __device__ __forceinline__ static void load_vec(const T *p, int n, float *x)
+    template <class U>
+    __device__ __forceinline__ static void load_vec(const U *p, int n, float *x, float other)
     {
+        constexpr int M = Vec<U>::N < N ? Vec<U>::N : N;
+        typedef U V __attribute__((ext_vector_type(M), aligned(sizeof(U))));
         if (n == N) {
-            typedef typename Vec<T>::type V __attribute__((aligned(sizeof(T))));
-            const V v = *reinterpret_cast<const V *>(p);
 #pragma unroll
-            for (int e = 0; e < N; ++e) x[e] = (float)v[e];
-        } else
+            for (int i = 0; i < N; i += M) {
+                const V v = *reinterpret_cast<const V *>(p + i);
 #pragma unroll
-            for (int e = 0; e < N; ++e)
-                if (e < n) x[e] = (float)p[e];
+                for (int e = 0; e < M; ++e) x[i + e] = (float)v[e];
+            }
+        } else {   // without a branch for each element: their loads go out together
+            U v[N];
+#pragma unroll
+            for (int e = 0; e < N; ++e) v[e] = p[e < n ? e : n - 1];
+#pragma unroll
+            for (int e = 0; e < N; ++e) x[e] = e < n ? (float)v[e] : other;
+        }
     }
     __device__ __forceinline__ static void store_vec(T *p, int n, const float *x)
     {
@@ -97,25 +114,35 @@ struct NormArgs {
 };
 
 // out = (x - mean) rstd w + bias. The variance is that of the differences, so an
-// offset far from 0 costs no digits.
+// offset far from 0 costs no digits. Groups go over rows a grid's stride apart, with
+// weight and bias in registers and the next row on its way.
 template <class T, class W, int G, int NV>
 __global__ __launch_bounds__(norm_block(G)) void k_norm_forward(NormArgs a)
 {
     using R = NormRow<T, G, NV>;
+    constexpr int N = R::N;
     __shared__ float red[2 * R::BLOCK / 64];
+    const int64_t step = (int64_t)gridDim.x * R::GROUPS;
+    int64_t r = (int64_t)blockIdx.x * R::GROUPS + threadIdx.x / G;
+    if (r >= a.rows) return;   // groups of more than a wave are blocks: none waits for it
+    R row, next;
+    row.load(static_cast<const T *>(a.x) + r * a.x_stride, a.width);
     const W *w = static_cast<const W *>(a.w), *bias = static_cast<const W *>(a.bias);
-    for (int64_t r = (int64_t)blockIdx.x * R::GROUPS + threadIdx.x / G; r < a.rows; r += (int64_t)gridDim.x * R::GROUPS) {
-        R row;
-        row.load(static_cast<const T *>(a.x) + r * a.x_stride, a.width);
+    float weight[NV * N], offset[NV * N];
+    R::columns(w, a.width, 1.f, weight);
+    R::columns(bias, a.width, 0.f, offset);
+    for (;;) {
+        const int64_t then = r + step;
+        if (then < a.rows) next.load(static_cast<const T *>(a.x) + then * a.x_stride, a.width);
         float s = 0.f, q = 0.f;
 #pragma unroll
-        for (int i = 0; i < NV * R::N; ++i) s += row.x[i];
+        for (int i = 0; i < NV * N; ++i) s += row.x[i];
         R::sum(s, q, red);
         const float mean = s / a.width;
         q = 0.f;
         R::each(a.width, [&](int, int i, int n) {
 #pragma unroll
-            for (int e = 0; e < R::N; ++e) {
+            for (int e = 0; e < N; ++e) {
                 row.x[i + e] -= mean;
                 if (e < n) q = fmaf(row.x[i + e], row.x[i + e], q);
             }
@@ -124,21 +151,18 @@ __global__ __launch_bounds__(norm_block(G)) void k_norm_forward(NormArgs a)
         const float rstd = 1.f / sqrtf(q / a.width + a.eps);
         T *o = static_cast<T *>(a.o) + r * a.o_stride;
         R::each(a.width, [&](int c, int i, int n) {
-            float y[R::N];
+            float y[N];
 #pragma unroll
-            for (int e = 0; e < R::N; ++e) y[e] = row.x[i + e] * rstd;
-            if (w)
-#pragma unroll
-                for (int e = 0; e < R::N; ++e) y[e] *= e < n ? (float)w[c + e] : 0.f;
-            if (bias)
-#pragma unroll
-                for (int e = 0; e < R::N; ++e) y[e] += e < n ? (float)bias[c + e] : 0.f;
+            for (int e = 0; e < N; ++e) y[e] = row.x[i + e] * rstd * weight[i + e] + offset[i + e];
             R::store_vec(o + c, n, y);
         });
         if (R::lane() == 0) {
             if (a.mean) a.mean[r] = mean;
             if (a.rstd) a.rstd[r] = rstd;
         }
+        if (then >= a.rows) break;
+        row = next;
+        r = then;
     }
 }
 
@@ -155,14 +179,7 @@ __global__ __launch_bounds__(norm_block(G)) void k_norm_backward(NormArgs a)
     __shared__ float join[R::GROUPS > 1 ? R::BLOCK * N : 1];
     const W *w = static_cast<const W *>(a.w);
     float dw[NV * N] = {}, db[NV * N] = {}, weight[NV * N];
-#pragma unroll
-    for (int i = 0; i < NV * N; ++i) weight[i] = 1.f;
-    if (w)
-        R::each(a.width, [&](int c, int i, int n) {
-#pragma unroll
-            for (int e = 0; e < N; ++e)
-                if (e < n) weight[i + e] = (float)w[c + e];
-        });
+    R::columns(w, a.width, 1.f, weight);
     for (int64_t r = (int64_t)blockIdx.x * R::GROUPS + threadIdx.x / G; r < a.rows; r += (int64_t)gridDim.x * R::GROUPS) {
         R row, d;
         row.load(static_cast<const T *>(a.x) + r * a.x_stride, a.width);

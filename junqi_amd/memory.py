@@ -15,6 +15,7 @@ do not synchronise. Wrong arguments raise ValueError.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 
 import torch
@@ -26,25 +27,28 @@ from ._lib import check, lib
 _DTYPES = {torch.float32: L.F32, torch.bfloat16: L.BF16}
 
 
+_same_device = contextlib.nullcontext()
+
+
 def _on(t: torch.Tensor):
-    """The device of `t` made current: the kernels launch there."""
-    return torch.cuda.device(t.device)
+    """The device of `t` made current, where it is not: the kernels launch there."""
+    return _same_device if t.get_device() == torch._C._cuda_getDevice() else torch.cuda.device(t.device)
 
 
 def _stream(t: torch.Tensor) -> int:
-    return torch.cuda.current_stream(t.device).cuda_stream
+    """torch.cuda.current_stream(t.device).cuda_stream without the Stream object: a
+    tenth of its 3 us, which counts in a call of 15."""
+    return torch._C._cuda_getCurrentRawStream(t.get_device())
 
 
 def _ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
 
-def _rows(t: torch.Tensor | None) -> L.Rows:
+def _rows(t: torch.Tensor) -> L.Rows:
     """A (batch, plies, heads, dim) tensor with adjacent elements for the C calls."""
-    if t is None:
-        return L.Rows()
-    s = t.stride()
-    return L.Rows(t.data_ptr(), s[0], s[1], s[2])
+    b, p, h, _ = t.stride()
+    return L.Rows(t.data_ptr(), b, p, h)
 
 
 def _adjacent(t: torch.Tensor) -> torch.Tensor:
@@ -61,7 +65,7 @@ def _like(t: torch.Tensor) -> torch.Tensor:
 def _check_rows(name: str, t: torch.Tensor, like: torch.Tensor | None = None) -> None:
     if not isinstance(t, torch.Tensor):
         raise ValueError(f"{name} must be a tensor, got {type(t).__name__}")
-    if t.device.type != "cuda":
+    if not t.is_cuda:
         raise ValueError(f"{name} must be a CUDA tensor")
     if t.dtype not in _DTYPES:
         raise ValueError(f"{name} must be float32 or bfloat16, got {t.dtype}")
@@ -75,7 +79,7 @@ def _check(name: str, t: torch.Tensor, shape: tuple[int, ...], dtypes: tuple[tor
         raise ValueError(f"{name} must be a tensor, got {type(t).__name__}")
     if t.device != like.device:
         raise ValueError(f"{name} must be on {like.device}, got {t.device}")
-    if tuple(t.shape) != shape:
+    if t.shape != shape:
         raise ValueError(f"{name} must have shape {shape}, got {tuple(t.shape)}")
     if t.dtype not in dtypes:
         raise ValueError(f"{name} must be {' or '.join(str(d).removeprefix('torch.') for d in dtypes)}, got {t.dtype}")
@@ -156,7 +160,11 @@ class _Attention(torch.autograd.Function):
             d_initial = torch.empty_like(initial)
         if d_final is not None:
             d_final = d_final.contiguous()
-        a.d_out, a.dq, a.dk, a.dv = _rows(d_out), _rows(dq), _rows(dk), _rows(dv)
+        a.d_out = _rows(d_out)
+        if dq is not None:
+            a.dq = _rows(dq)
+        if dk is not None:
+            a.dk, a.dv = _rows(dk), _rows(dv)
         a.d_final, a.d_initial = _ptr(d_final), _ptr(d_initial)
         with _on(q):
             work = _workspace(a, True, q)   # noqa: F841
