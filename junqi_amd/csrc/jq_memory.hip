@@ -190,7 +190,7 @@ int launch_rotary(const RotaryArgs &a, int64_t all, hipStream_t stream)
     const int items = std::max(1, a.dim / N * a.heads);
     const int tokens = std::max(1, std::min(1024 / items, ROTARY_TABLE / std::max(1, a.pairs)));
     hipLaunchKernelGGL((k_rotary<T, N, INTERLEAVED>), dim3(grid_of((all + tokens - 1) / tokens)), dim3(256),
-                       2 * sizeof(float) * tokens * a.pairs, stream, a, all, tokens);
+                       tokens * (2 * sizeof(int64_t) + 2 * sizeof(float) * a.pairs), stream, a, all, tokens);
     return launch_check("k_rotary");
 }
 

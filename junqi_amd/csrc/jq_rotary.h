@@ -32,17 +32,27 @@ template <class T, int N, bool INTERLEAVED>
 __global__ __launch_bounds__(256) void k_rotary(RotaryArgs a, int64_t all, int tokens)
 {
     typedef T V __attribute__((ext_vector_type(N), aligned(sizeof(T))));
-    extern __shared__ float table[];   // cos of (token, pair), then sin
-    float *cs = table, *sn = table + tokens * a.pairs;
+    extern __shared__ __align__(8) char lds[];   // offsets of each token's rows; cos of (token, pair), then sin
+    int64_t *in_at = reinterpret_cast<int64_t *>(lds), *out_at = in_at + tokens;
+    float *cs = reinterpret_cast<float *>(out_at + tokens), *sn = cs + tokens * a.pairs;
     const int turns = INTERLEAVED ? 2 * a.pairs / N : a.pairs / N, rest = a.dim - 2 * a.pairs;
     const bool whole = rest % N == 0;   // the rest is copied in vectors too, or by element
     const int items = turns + (whole ? rest / N : rest);
+    // this thread's first item, and the way to its next, 256 on
+    const unsigned per = items, heads = a.heads, x0 = threadIdx.x;
+    const unsigned i0 = x0 % per, h0 = x0 / per % heads, k0 = x0 / per / heads;
+    const unsigned di = 256 % per, dh = 256 / per % heads, dk = 256 / per / heads;
     for (int64_t t0 = (int64_t)blockIdx.x * tokens; t0 < all; t0 += (int64_t)gridDim.x * tokens) {
         const int n = (int)min((int64_t)tokens, all - t0);
         __syncthreads();
+        for (int token = threadIdx.x; token < n; token += 256) {
+            const int64_t b = (t0 + token) / a.n1, t = (t0 + token) % a.n1;
+            in_at[token] = b * a.x.batch + t * a.x.ply;
+            out_at[token] = b * a.o.batch + t * a.o.ply;
+        }
         for (int x = threadIdx.x; x < n * a.pairs; x += 256) {
-            const int token = x / a.pairs, p = x % a.pairs;
-            const int64_t at = (t0 + token) / a.n1 * a.p0 + (t0 + token) % a.n1 * a.p1;
+            const int token = (unsigned)x / (unsigned)a.pairs, p = x - token * a.pairs;
+            const int64_t b = a.n1 == all ? 0 : (t0 + token) / a.n1, at = b * a.p0 + (t0 + token - b * a.n1) * a.p1;
             int axis = 0;
             while (p >= a.ends[axis]) ++axis;
             const int64_t pos = a.positions64 ? static_cast<const int64_t *>(a.positions)[at + axis]
@@ -53,22 +63,29 @@ __global__ __launch_bounds__(256) void k_rotary(RotaryArgs a, int64_t all, int t
             sn[x] = a.inverse ? -s : s;
         }
         __syncthreads();
-        for (int x = threadIdx.x; x < n * a.heads * items; x += 256) {
-            const int i = x % items, head = x / items % a.heads, token = x / items / a.heads;
-            const int64_t b = (t0 + token) / a.n1, t = (t0 + token) % a.n1;
-            const T *in = row_at<const T>(a.x, b, t, head);
-            T *out = row_at<T>(a.o, b, t, head);
+        for (unsigned at = i0, head = h0, token = k0; token < (unsigned)n;) {
+            const int i = at;
+            const T *in = static_cast<const T *>(a.x.data) + in_at[token] + head * a.x.head;
+            T *out = static_cast<T *>(a.o.data) + out_at[token] + head * a.o.head;
+            const float *c0 = cs + token * a.pairs, *s0 = sn + token * a.pairs;
+            at += di;
+            const bool over = at >= per;
+            at -= over ? per : 0;
+            head += dh + over;
+            const bool past = head >= heads;
+            head -= past ? heads : 0;
+            token += dk + past;
             if (i >= turns) {
-                const int at = 2 * a.pairs + (i - turns) * (whole ? N : 1);
-                if (whole) *reinterpret_cast<V *>(out + at) = *reinterpret_cast<const V *>(in + at);
-                else out[at] = in[at];
+                const int c = 2 * a.pairs + (i - turns) * (whole ? N : 1);
+                if (whole) *reinterpret_cast<V *>(out + c) = *reinterpret_cast<const V *>(in + c);
+                else out[c] = in[c];
             } else if constexpr (INTERLEAVED) {
                 const V u = *reinterpret_cast<const V *>(in + i * N);
                 V y;
 #pragma unroll
                 for (int e = 0; e < N; e += 2) {
-                    const int p = token * a.pairs + (i * N + e) / 2;
-                    const float c = cs[p], s = sn[p], u0 = (float)u[e], u1 = (float)u[e + 1];
+                    const int p = (i * N + e) / 2;
+                    const float c = c0[p], s = s0[p], u0 = (float)u[e], u1 = (float)u[e + 1];
                     y[e] = from_float<T>(u0 * c - u1 * s);
                     y[e + 1] = from_float<T>(u1 * c + u0 * s);
                 }
@@ -78,8 +95,8 @@ __global__ __launch_bounds__(256) void k_rotary(RotaryArgs a, int64_t all, int t
                 V y, z;
 #pragma unroll
                 for (int e = 0; e < N; ++e) {
-                    const int p = token * a.pairs + i * N + e;
-                    const float c = cs[p], s = sn[p], u0 = (float)u[e], u1 = (float)v[e];
+                    const int p = i * N + e;
+                    const float c = c0[p], s = s0[p], u0 = (float)u[e], u1 = (float)v[e];
                     y[e] = from_float<T>(u0 * c - u1 * s);
                     z[e] = from_float<T>(u1 * c + u0 * s);
                 }
