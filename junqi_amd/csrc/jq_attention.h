@@ -23,7 +23,6 @@ struct ScanArgs {
     float *s_out;
     int s_row, s_col;
     float in_scale, out_scale;
-    bool reverse;
     // a long axis is split into segments of seg_plies (whole chunks) that run side by
     // side: seg_states[(b, h)][g] (kd, vd) is the state before segment g, seg_carry
     // what a segment leaves of it
@@ -157,7 +156,7 @@ struct Chunk {
     int w, l, lc, g;
 
     __device__ __forceinline__ Chunk(float log_decay)
-        : g2(log2_lambda(log_decay)), w(threadIdx.x >> 6), l(threadIdx.x & 63), lc(l & 15), g(l >> 4)
+        : g2(log2_lambda(log_decay)), w(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)), l(threadIdx.x & 63), lc(l & 15), g(l >> 4)
     {
     }
 
@@ -204,31 +203,36 @@ struct Chunk {
         }
     }
 
-    // P[i][j] = scale lambda^|i - j| q_i.k_j for the plies j that i sees, else 0; the
-    // tiles on the diagonal and on one side of it, shared out over the waves.
-    __device__ __forceinline__ void scores(const T *q, const T *k, T *p, const Marks<CH> &mk, float scale) const
+    // p[i][j] = scale lambda^|i - j| q_i.k_j for the plies j that i sees, else 0, of N
+    // pairs q, k; the tiles on the diagonal and on one side of it, shared out over the
+    // waves.
+    template <int N>
+    __device__ __forceinline__ void scores(const T *const (&q)[N], const T *const (&k)[N], T *const (&p)[N],
+                                           const Marks<CH> &mk, float scale) const
     {
         const bool starts = __builtin_amdgcn_readfirstlane(mk.starts);
         for (int m = w; m < NT * (NT + 1) / 2; m += WAVES) {
             const int a = m < 1 ? 0 : m < 3 ? 1 : m < 6 ? 2 : 3, b = m - a * (a + 1) / 2;
-            const int it = REV ? b : a, jt = REV ? a : b;
-            f32x4 acc{0.f, 0.f, 0.f, 0.f};
+            const int it = REV ? b : a, jt = REV ? a : b, i = 16 * it + lc, j0 = 16 * jt + 4 * g;
+            f32x4 acc[N];
+#pragma unroll
+            for (int u = 0; u < N; ++u) acc[u] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int c = 0; c < D; c += KB)
-                acc = M::mul(M::row(k + (16 * jt + lc) * LD + c, g), M::row(q + (16 * it + lc) * LD + c, g), acc);
-            const int i = 16 * it + lc, j0 = 16 * jt + 4 * g;
+#pragma unroll
+                for (int u = 0; u < N; ++u)
+                    acc[u] = M::mul(M::row(k[u] + (16 * jt + lc) * LD + c, g), M::row(q[u] + i * LD + c, g), acc[u]);
             const float d0 = (float)(REV ? j0 - i : i - j0);
+            const int game = starts ? mk.game[i] : 0;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const float d = REV ? d0 + r : d0 - r;
-                acc[r] = d >= 0.f ? acc[r] * (scale * power(g2, d)) : 0.f;
-            }
-            if (starts) {
-                const int game = mk.game[i];
+                const float d = REV ? d0 + r : d0 - r, f = scale * power(g2, d);
+                const bool seen = d >= 0.f && (!starts || game == mk.game[j0 + r]);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) acc[r] = game == mk.game[j0 + r] ? acc[r] : 0.f;
+                for (int u = 0; u < N; ++u) acc[u][r] = seen ? acc[u][r] * f : 0.f;
             }
-            store4(p + i * PLD + M::place(j0), acc);
+#pragma unroll
+            for (int u = 0; u < N; ++u) store4(p[u] + i * PLD + M::place(j0), acc[u]);
         }
     }
 
@@ -259,27 +263,24 @@ struct Chunk {
                 for (int u = 0; u < N; ++u) o[it] = M::mul(part[u], y, o[it]);
             }
         }
-#pragma unroll
-        for (int it = 0; it < NT; ++it) {
-            const float f = mk.sees[16 * it + lc];
-#pragma unroll
-            for (int r = 0; r < 4; ++r) o[it][r] = f >= 0.f ? o[it][r] * (f * scale) : 0.f;
-        }
+        seen(mk, scale, o);
     }
 
-    // o += P v (OUT), and the state after the chunk.
-    template <bool OUT>
+    // o += P v (OUT), and the state after the chunk (STATE).
+    template <bool OUT, bool STATE>
     __device__ __forceinline__ void apply(const T *k, const T *v, const T *p, const Marks<CH> &mk, f32x4 (&o)[NT])
     {
-        const float carry = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, mk.carry)));
-        if (carry >= 0.f) {
+        if constexpr (STATE) {
+            const float carry = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, mk.carry)));
+            if (carry >= 0.f) {
 #pragma unroll
-            for (int t = 0; t < D / 16; ++t)
+                for (int t = 0; t < D / 16; ++t)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) s[t][r] *= carry;
-        } else {
+                    for (int r = 0; r < 4; ++r) s[t][r] *= carry;
+            } else {
 #pragma unroll
-            for (int t = 0; t < D / 16; ++t) s[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+                for (int t = 0; t < D / 16; ++t) s[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+            }
         }
 #pragma unroll
         for (int c = 0; c < CH / KB; ++c) {
@@ -289,28 +290,82 @@ struct Chunk {
                 if (!OUT || (REV ? c * KB + KB <= 16 * it : c * KB >= 16 * it + 16)) continue;   // nothing to see there
                 o[it] = M::mul(x, M::row(p + (16 * it + lc) * PLD + c * KB, g), o[it]);
             }
-            // the plies' values times what is left of them after the chunk
-            constexpr int N = PARTS<T, 3>;
-            Frag part[N];
-            float left[FE];
+            if constexpr (STATE) {
+                // the plies' values times what is left of them after the chunk
+                constexpr int N = PARTS<T, 3>;
+                Frag part[N];
+                float left[FE];
 #pragma unroll
-            for (int e = 0; e < FE; ++e) left[e] = (float)x[e] * mk.leaves[c * KB + M::depth(g, e)];
-            M::template split<N>(left, part);
+                for (int e = 0; e < FE; ++e) left[e] = (float)x[e] * mk.leaves[c * KB + M::depth(g, e)];
+                M::template split<N>(left, part);
 #pragma unroll
-            for (int t = 0; t < D / 16; ++t) {
-                const Frag y = M::col(k + c * KB * LD + 16 * t, LD, l);
+                for (int t = 0; t < D / 16; ++t) {
+                    const Frag y = M::col(k + c * KB * LD + 16 * t, LD, l);
 #pragma unroll
-                for (int u = 0; u < N; ++u) s[t] = M::mul(y, part[u], s[t]);
+                    for (int u = 0; u < N; ++u) s[t] = M::mul(y, part[u], s[t]);
+                }
             }
+        }
+    }
+
+    // ---- the state turned over, for the pass that needs both of its sides: as terms in
+    // LDS, turned[u][c][i] for element (i, c)
+    static constexpr int TURNED = PARTS<T, 2>;
+    __device__ __forceinline__ void turn(T *turned) const
+    {
+#pragma unroll
+        for (int t = 0; t < D / 16; ++t) {
+            f32x4 x = s[t];
+#pragma unroll
+            for (int u = 0; u < TURNED; ++u) {
+                T *at = turned + (u * D + 16 * w + lc) * LD + 16 * t + 4 * g;
+                store4(at, x);
+                if (u + 1 < TURNED)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) x[r] -= (float)from_float<T>(x[r]);
+            }
+        }
+    }
+
+    // like inter, for the turned state: rows of o are this wave's columns of its other side
+    __device__ __forceinline__ void inter_turned(const T *turned, const T *q, const Marks<CH> &mk, float scale,
+                                                 f32x4 (&o)[NT]) const
+    {
+#pragma unroll
+        for (int it = 0; it < NT; ++it) o[it] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < D / KB; ++c) {
+            Frag part[TURNED];
+#pragma unroll
+            for (int u = 0; u < TURNED; ++u) part[u] = M::col(turned + (u * D + c * KB) * LD + 16 * w, LD, l);
+#pragma unroll
+            for (int it = 0; it < NT; ++it) {
+                const Frag y = M::deep(q + (16 * it + lc) * LD + c * KB, g);
+#pragma unroll
+                for (int u = 0; u < TURNED; ++u) o[it] = M::mul(part[u], y, o[it]);
+            }
+        }
+        seen(mk, scale, o);
+    }
+
+    // o times what is left of the state at its plies
+    __device__ __forceinline__ void seen(const Marks<CH> &mk, float scale, f32x4 (&o)[NT]) const
+    {
+#pragma unroll
+        for (int it = 0; it < NT; ++it) {
+            const float f = mk.sees[16 * it + lc];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) o[it][r] = f >= 0.f ? o[it][r] * (f * scale) : 0.f;
         }
     }
 
     // The chunk ply by ply, for tiles with infinities or NaN: a product with 0 in
     // their place is not 0, and a ply must get nothing of those it does not see.
-    // put(i, x): x = this wave's value column l % 16 of ply i.
-    template <class F>
+    // put(i, x): x = this wave's value column l % 16 of ply i. each(i, t, r, y): y = the
+    // state's element (16t + 4g + r, 16w + l % 16) that ply i sees.
+    template <class F, class E>
     __device__ __forceinline__ void singly(const T *q, const T *k, const T *v, const Marks<CH> &mk, float in_scale,
-                                           float out_scale, F &&put)
+                                           float out_scale, F &&put, E &&each)
     {
         const float lam = power(g2, 1);
         for (int m = 0; m < mk.n; ++m) {
@@ -327,6 +382,7 @@ struct Chunk {
                     if (!REV) y = start ? 0.f : lam * y;
                     y += (float)k[i * LD + c] * x;
                     o += (float)q[i * LD + c] * y;
+                    each(i, t, r, y);
                     if (REV) y = start ? 0.f : lam * y;
                     s[t][r] = y;
                 }
@@ -498,17 +554,17 @@ __global__ __launch_bounds__(4 * D, D == 32 ? 3 : 4) void k_attention_pass(ScanA
             ch.singly(OUT ? qs : ks, ks, vs, mk, a.in_scale, a.out_scale, [&](int i, float x) {
                 const int c = 16 * ch.w + ch.lc;
                 if (OUT && ch.g == 0 && c < a.vd) o.base[(t0 + i) * o.ply + c] = from_float<T>(x);
-            });
+            }, [](int, int, int, float) {});
         } else if constexpr (OUT) {
             f32x4 acc[NT];
-            ch.scores(qs, ks, ps, mk, a.in_scale * a.out_scale);
+            ch.template scores<1>({qs}, {ks}, {ps}, mk, a.in_scale * a.out_scale);
             ch.inter(qs, mk, a.out_scale, acc);
             __syncthreads();
-            ch.template apply<true>(ks, vs, ps, mk, acc);
+            ch.template apply<true, true>(ks, vs, ps, mk, acc);
             o.put(t0, n, ch.lc, 16 * ch.w + 4 * ch.g, acc);
         } else {
             f32x4 none[NT];
-            ch.template apply<false>(ks, vs, nullptr, mk, none);
+            ch.template apply<false, true>(ks, vs, nullptr, mk, none);
         }
         __syncthreads();
     }
@@ -520,6 +576,113 @@ __global__ __launch_bounds__(4 * D, D == 32 ? 3 : 4) void k_attention_pass(ScanA
         if (threadIdx.x == 0)
             a.seg_carry[(int64_t)blockIdx.x * a.segments + seg] = any_start ? -1.f : power(ch.g2, max(end - s0, 0));
     }
+}
+
+// The gradients of k and v over one segment of one game and head, in reverse, from
+// one reading of q, k, v and d_out. With R the gradient of the state after a ply,
+//   dv_j = R^T k_j and dk_j = R v_j   where R = scale sum_{i >= j} lambda^(i - j) q_i d_i^T + ...
+// are two passes with one state: dv is the pass (k, q, d_out), whose state stays in
+// registers; dk is (v, d_out, q) on its transpose, which the waves leave for each
+// other in LDS, as terms. Both share the plies' weights.
+struct GradArgs {
+    ScanArgs scan;       // q: k, k: q, v: d_out, o: dv
+    jq_rows values, dk;  // v and the gradient of k
+};
+template <class T, int D> constexpr int kv_lds()
+{
+    using C = Chunk<T, D, true>;
+    return (4 * C::CH * C::LD + 2 * C::CH * C::PLD + C::TURNED * D * C::LD) * (int)sizeof(T);
+}
+template <class T, int D, bool FAST>
+__global__ __launch_bounds__(4 * D, 2) void k_attention_kv(GradArgs ga)
+{
+    using C = Chunk<T, D, true>;
+    using P = Plies<T, D, FAST>;
+    using V = typename P::V;
+    constexpr int CH = C::CH, LD = C::LD, NT = C::NT, PLD = C::PLD;
+    const ScanArgs &a = ga.scan;
+    extern __shared__ __align__(16) char dynamic[];
+    T *ks = reinterpret_cast<T *>(dynamic), *qs = ks + CH * LD, *ds = qs + CH * LD, *vs = ds + CH * LD;
+    T *p1 = vs + CH * LD, *p2 = p1 + CH * PLD, *turned = p2 + CH * PLD;
+    __shared__ Marks<CH> mk;
+    __shared__ int bad[2];
+    const int b = blockIdx.x / a.heads, h = blockIdx.x % a.heads, seg = blockIdx.y;
+    const int len = a.lengths ? min(max(a.lengths[b], 0), a.plies) : a.plies;
+    const int s0 = seg * a.seg_plies, s1 = a.plies - s0 > a.seg_plies ? s0 + a.seg_plies : a.plies, end = min(s1, len);
+    const int chunks = end > s0 ? (end - s0 + CH - 1) / CH : 0;
+    C ch(a.log_decay[h]);
+    const int64_t size = (int64_t)a.kd * a.vd;
+    if (a.segments > 1) ch.load_state(a.seg_states + ((int64_t)blockIdx.x * a.segments + seg) * size, a.kd, a.vd, a.vd, 1);
+    else ch.load_state(a.s_in ? a.s_in + blockIdx.x * size : nullptr, a.kd, a.vd, a.vd, 1);
+    const P k(a.q, b, h, a.kd), q(a.k, b, h, a.kd), d(a.v, b, h, a.vd), v(ga.values, b, h, a.vd);
+    const P dv(a.o, b, h, a.vd), dk(ga.dk, b, h, a.kd);
+    const uint8_t *starts = a.starts ? a.starts + b * a.starts_batch : nullptr;
+    for (int x = threadIdx.x; x < 2 * CH * PLD; x += C::THREADS) p1[x] = T(0.f);   // tiles beside the diagonal stay 0
+    ch.turn(turned);
+    if (threadIdx.x < 2) bad[threadIdx.x] = 0;
+    __syncthreads();
+
+    V kt[2], qt[2], dt[2], vt[2];
+    bool start = false;
+    const auto begin = [&](int m) { return s0 + (chunks - 1 - m) * CH; };
+    const auto fetch = [&](int m) {
+        const int t0 = begin(m), n = min(CH, end - t0);
+        k.load(t0, n, kt);
+        q.load(t0, n, qt);
+        d.load(t0, n, dt);
+        v.load(t0, n, vt);
+        start = starts && ch.l < n && starts[(t0 + ch.l) * a.starts_ply];
+    };
+    if (chunks) fetch(0);
+    for (int m = 0; m < chunks; ++m) {
+        const int t0 = begin(m), n = min(CH, end - t0);
+        if (ch.w == 0) ch.mark(mk, start, n, a.in_scale);
+        P::stage(ks, kt);
+        P::stage(qs, qt);
+        P::stage(ds, dt);
+        P::stage(vs, vt);
+        const float sum = probe(dt[1], probe(dt[0], probe(qt[1], probe(qt[0], 0.f))));
+        if (sum != sum) bad[m & 1] = 1;
+        __syncthreads();
+        if (m + 1 < chunks) fetch(m + 1);
+        if (threadIdx.x == 0) bad[(m + 1) & 1] = 0;
+        if (bad[m & 1]) {
+            float *red = reinterpret_cast<float *>(p1);   // [wave][D], for the sums over all columns
+            static_assert(C::WAVES * D * sizeof(float) <= CH * PLD * sizeof(T));
+            ch.singly(ks, qs, ds, mk, a.in_scale, 1.f, [&](int i, float x) {
+                const int c = 16 * ch.w + ch.lc;
+                if (ch.g == 0 && c < a.vd) dv.base[(t0 + i) * dv.ply + c] = from_float<T>(x);
+                __syncthreads();
+                if (threadIdx.x < a.kd) {
+                    float y = 0.f;
+                    for (int u = 0; u < C::WAVES; ++u) y += red[u * D + threadIdx.x];
+                    dk.base[(t0 + i) * dk.ply + threadIdx.x] = from_float<T>(y);
+                }
+                __syncthreads();
+            }, [&](int i, int t, int r, float y) {
+                y *= (float)vs[i * LD + 16 * ch.w + ch.lc];
+#pragma unroll
+                for (int o = 8; o; o >>= 1) y += __shfl_xor(y, o);
+                if (ch.lc == 0) red[ch.w * D + 16 * t + 4 * ch.g + r] = y;
+            });
+            for (int x = threadIdx.x; x < CH * PLD; x += C::THREADS) p1[x] = T(0.f);
+        } else {
+            f32x4 o1[NT], o2[NT];
+            ch.template scores<2>({ks, vs}, {qs, ds}, {p1, p2}, mk, a.in_scale);
+            ch.inter(ks, mk, 1.f, o1);
+            ch.inter_turned(turned, vs, mk, 1.f, o2);
+            __syncthreads();
+            ch.template apply<true, true>(qs, ds, p1, mk, o1);
+            ch.template apply<true, false>(nullptr, qs, p2, mk, o2);
+            dv.put(t0, n, ch.lc, 16 * ch.w + 4 * ch.g, o1);
+            dk.put(t0, n, ch.lc, 16 * ch.w + 4 * ch.g, o2);
+        }
+        ch.turn(turned);
+        __syncthreads();
+    }
+    dv.clear(max(s0, len), s1);
+    dk.clear(max(s0, len), s1);
+    if (a.s_out && seg == 0) ch.store_state(a.s_out + blockIdx.x * size, a.kd, a.vd, a.vd, 1);
 }
 
 // What the segments leave, in their order: seg_states[g] becomes the state before

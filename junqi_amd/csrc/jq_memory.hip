@@ -5,7 +5,9 @@
 
 #include <algorithm>
 #include <climits>
+#include <initializer_list>
 #include <type_traits>
+#include <utility>
 
 #include "junqi_amd.h"
 #include "jq_error.h"
@@ -81,40 +83,85 @@ bool whole_vectors(const jq_rows &r, int dim, size_t elem, size_t bytes, int pli
            r.ply >= dim && r.ply < ((int64_t)1 << 31) / (int64_t)elem / (plies + 1);
 }
 
+// The states before the segments of a split axis.
 template <class T, int D, bool REV, bool FAST>
-int launch_pass(const ScanArgs &s, hipStream_t stream)
+int launch_states(const ScanArgs &s, hipStream_t stream)
 {
     const int heads = s.batch * s.heads;
-    if (s.segments > 1) {
-        hipLaunchKernelGGL((k_attention_pass<T, D, REV, FAST, false>), dim3(heads, s.segments - 1), dim3(4 * D), 0, stream, s);
-        TRY(launch_check("k_attention_pass (states)"));
-        hipLaunchKernelGGL(k_attention_join<REV>, dim3(heads, (s.kd * s.vd + 255) / 256), dim3(256), 0, stream, s);
-        TRY(launch_check("k_attention_join"));
-    }
-    hipLaunchKernelGGL((k_attention_pass<T, D, REV, FAST, true>), dim3(heads, s.segments), dim3(4 * D), 0, stream, s);
+    if (s.segments < 2) return JQ_OK;
+    hipLaunchKernelGGL((k_attention_pass<T, D, REV, FAST, false>), dim3(heads, s.segments - 1), dim3(4 * D), 0, stream, s);
+    TRY(launch_check("k_attention_pass (states)"));
+    hipLaunchKernelGGL(k_attention_join<REV>, dim3(heads, (s.kd * s.vd + 255) / 256), dim3(256), 0, stream, s);
+    return launch_check("k_attention_join");
+}
+
+template <class T, int D, bool FAST>
+int launch_forward(const ScanArgs &s, hipStream_t stream)
+{
+    TRY((launch_states<T, D, false, FAST>(s, stream)));
+    const int heads = s.batch * s.heads;
+    hipLaunchKernelGGL((k_attention_pass<T, D, false, FAST, true>), dim3(heads, s.segments), dim3(4 * D), 0, stream, s);
     return launch_check("k_attention_pass");
+}
+
+template <class T, int D, bool FAST>
+int launch_kv(const GradArgs &g, hipStream_t stream)
+{
+    TRY((launch_states<T, D, true, FAST>(g.scan, stream)));
+    const auto kernel = k_attention_kv<T, D, FAST>;
+    if (kv_lds<T, D>() > 48 * 1024 &&
+        hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kv_lds<T, D>()) != hipSuccess)
+        return fail(JQ_E_HIP, "k_attention_kv: %d bytes of LDS are refused", kv_lds<T, D>());
+    hipLaunchKernelGGL(kernel, dim3(g.scan.batch * g.scan.heads, g.scan.segments), dim3(4 * D), (kv_lds<T, D>()), stream, g);
+    return launch_check("k_attention_kv");
+}
+
+// Whether a pass may take all of these as whole vectors.
+template <class T>
+bool all_whole(std::initializer_list<std::pair<const jq_rows *, int>> rows, size_t bytes)
+{
+    for (const auto &r : rows)
+        if (!whole_vectors(*r.first, r.second, sizeof(T), bytes, Mma<T>::CH)) return false;
+    return true;
 }
 
 template <class T, int D>
 int scan_width(const ScanArgs &s, hipStream_t stream)
 {
-    const bool fast = whole_vectors(s.q, s.kd, sizeof(T), 16, Mma<T>::CH) && whole_vectors(s.k, s.kd, sizeof(T), 16, Mma<T>::CH) &&
-                      whole_vectors(s.v, s.vd, sizeof(T), 16, Mma<T>::CH) &&
-                      whole_vectors(s.o, s.vd, sizeof(T), 4 * sizeof(T), Mma<T>::CH);
-    if (s.reverse) return fast ? launch_pass<T, D, true, true>(s, stream) : launch_pass<T, D, true, false>(s, stream);
-    return fast ? launch_pass<T, D, false, true>(s, stream) : launch_pass<T, D, false, false>(s, stream);
+    const bool fast = all_whole<T>({{&s.q, s.kd}, {&s.k, s.kd}, {&s.v, s.vd}}, 16) && all_whole<T>({{&s.o, s.vd}}, 4 * sizeof(T));
+    return fast ? launch_forward<T, D, true>(s, stream) : launch_forward<T, D, false>(s, stream);
 }
 
+template <class T, int D>
+int kv_width(const GradArgs &g, hipStream_t stream)
+{
+    const ScanArgs &s = g.scan;
+    const bool fast = all_whole<T>({{&s.q, s.kd}, {&s.k, s.kd}, {&s.v, s.vd}, {&g.values, s.vd}}, 16) &&
+                      all_whole<T>({{&s.o, s.vd}, {&g.dk, s.kd}}, 4 * sizeof(T));
+    return fast ? launch_kv<T, D, true>(g, stream) : launch_kv<T, D, false>(g, stream);
+}
+
+// The pass forward in time for its wider dim.
 template <class T>
 int scan_as(const ScanArgs &s, hipStream_t stream)
 {
     const int d = std::max(s.kd, s.vd);
     return d <= 32 ? scan_width<T, 32>(s, stream) : d <= 64 ? scan_width<T, 64>(s, stream) : scan_width<T, 128>(s, stream);
 }
-
 int scan(int32_t dtype, const ScanArgs &s, hipStream_t stream)
 {
     return dtype == JQ_F32 ? scan_as<float>(s, stream) : scan_as<bf16>(s, stream);
+}
+
+template <class T>
+int scan_kv_as(const GradArgs &g, hipStream_t stream)
+{
+    const int d = std::max(g.scan.kd, g.scan.vd);
+    return d <= 32 ? kv_width<T, 32>(g, stream) : d <= 64 ? kv_width<T, 64>(g, stream) : kv_width<T, 128>(g, stream);
+}
+int scan_kv(int32_t dtype, const GradArgs &g, hipStream_t stream)
+{
+    return dtype == JQ_F32 ? scan_kv_as<float>(g, stream) : scan_kv_as<bf16>(g, stream);
 }
 
 // How a call's plies are split: few games and heads leave the card idle unless
@@ -335,17 +382,13 @@ int jq_attention_backward(const jq_attention *a, void *stream)
             TRY(check_rows(a->dk, a->dtype, "dk"));
             TRY(check_rows(a->dv, a->dtype, "dv"));
         }
-        ScanArgs s = scan_args(a);
-        s.reverse = true;
+        GradArgs g{scan_args(a), a->v, a->dk};
+        ScanArgs &s = g.scan;
         s.in_scale = a->scale;
         s.q = a->k, s.k = a->q, s.v = a->d_out, s.o = a->dv;
         s.kd = a->key_dim, s.vd = a->value_dim;
         s.s_in = a->d_final, s.s_out = a->d_initial, s.s_row = a->value_dim, s.s_col = 1;
-        TRY(scan(a->dtype, s, strm(stream)));
-        s.q = a->v, s.k = a->d_out, s.v = a->q, s.o = a->dk;
-        s.kd = a->value_dim, s.vd = a->key_dim;
-        s.s_out = nullptr, s.s_row = 1, s.s_col = a->value_dim;
-        TRY(scan(a->dtype, s, strm(stream)));
+        TRY(scan_kv(a->dtype, g, strm(stream)));
     }
     return JQ_OK;
 }
