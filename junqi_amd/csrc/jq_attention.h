@@ -12,6 +12,12 @@ namespace jq {
 // All passes are this one with the tensors in other places:
 //   out: q, k, v forward           dq: d_out, v, k forward, on the transposed state
 //   dv:  k, q, d_out in reverse    dk: v, d_out, q in reverse, on the transposed state
+//
+// A chunk of plies a .. a + n at a time, with P_ij = lambda^(i - j) q_i.k_j for the
+// plies j <= i that i sees (in reverse: j >= i, lambda^(j - i)):
+//   o_i = out_scale (in_scale sum_j P_ij v_j + lambda^(i - a + 1) q_i S)
+//   S  <- lambda^n S + in_scale sum_j lambda^(a + n - 1 - j) k_j v_j^T
+// with the state's term left out where a game starts in between.
 struct ScanArgs {
     jq_rows q, k, v, o;
     int batch, plies, heads, kd, vd;   // kd: dim of q and k, vd: dim of v and o
@@ -34,24 +40,21 @@ struct ScanArgs {
 // A product takes two fragments: lane l holds row (or column) l % 16 and, with
 // g = l / 16, the depths that its e-th elements stand for. The result has column
 // l % 16 and rows 4g .. 4g + 3 in lane l. Depths may be taken in any order that
-// both fragments share. `deep`, `col` and the split state take them in the order in
-// which a result's rows lie in its lanes (depth), so that a state goes from result
-// to operand without leaving its registers; `row` takes them as they lie.
+// both fragments share; here it is the order in which a result's rows lie in its
+// lanes (depth), so that the state and P go from result to operand without leaving
+// their registers.
 template <class T> struct Mma;
 
 template <> struct Mma<bf16> {
     typedef bf16x8 Frag;
-    static constexpr int CH = 64;   // plies of a chunk
     static constexpr int KB = 32;   // depth of a fragment
     static __device__ __forceinline__ f32x4 mul(Frag a, Frag b, f32x4 c)
     {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
     }
     static __device__ __forceinline__ int depth(int g, int e) { return 16 * (e >> 2) + 4 * g + (e & 3); }
-    // where depths d .. d + 3, d % 4 == 0, of a row stored for `row` lie, for `row` to give them in `depth`'s order
-    static __device__ __forceinline__ int place(int d) { return (d & ~31) + 2 * (d & 15) + ((d & 16) >> 2); }
-    static __device__ __forceinline__ Frag row(const bf16 *p, int g) { return *reinterpret_cast<const Frag *>(p + 8 * g); }
-    static __device__ __forceinline__ Frag deep(const bf16 *p, int g)
+    // depths = elements p[0 .. KB) of this lane's row
+    static __device__ __forceinline__ Frag row(const bf16 *p, int g)
     {
         const bf16x4 x = *reinterpret_cast<const bf16x4 *>(p + 4 * g), y = *reinterpret_cast<const bf16x4 *>(p + 16 + 4 * g);
         return Frag{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
@@ -93,7 +96,6 @@ template <> struct Mma<bf16> {
 
 template <> struct Mma<float> {
     typedef f32x4 Frag;
-    static constexpr int CH = 32;
     static constexpr int KB = 16;
     static __device__ __forceinline__ f32x4 mul(Frag a, Frag b, f32x4 c)
     {
@@ -102,9 +104,7 @@ template <> struct Mma<float> {
         return c;
     }
     static __device__ __forceinline__ int depth(int g, int e) { return 4 * g + e; }
-    static __device__ __forceinline__ int place(int d) { return d; }
     static __device__ __forceinline__ Frag row(const float *p, int g) { return *reinterpret_cast<const Frag *>(p + 4 * g); }
-    static __device__ __forceinline__ Frag deep(const float *p, int g) { return row(p, g); }
     static __device__ __forceinline__ Frag col(const float *p, int ld, int l)
     {
         const float *at = p + 4 * (l >> 4) * ld + (l & 15);
@@ -128,267 +128,287 @@ __device__ __forceinline__ float log2_lambda(float log_decay)
     const float x = log_decay * 1.44269504088896340736f;
     return x < -1e30f ? -1e30f : x;
 }
-__device__ __forceinline__ float power(float log2_lam, float d) { return __builtin_amdgcn_exp2f(log2_lam * d); }
+__device__ __forceinline__ float power(float log2_lam, int d) { return __builtin_amdgcn_exp2f(log2_lam * (float)d); }
 
-// What the plies of a chunk need to know of it, made once for each chunk.
-template <int CH>
-struct alignas(16) Marks {
-    float sees[CH];    // lambda's power from the chunk's begin (REV: end) to the ply; -1: it sees nothing from there
-    float leaves[CH];  // lambda's power from the ply to the chunk's end (REV: begin) times in_scale; 0: nothing is left
-    int game[CH];      // games that start in the chunk up to the ply
-    float carry;       // lambda's power over the chunk; -1: a game starts in it
-    int n;             // plies
-    bool starts;       // a game starts in it
+// Four elements of a result in T.
+__device__ __forceinline__ void store4(bf16 *p, f32x4 x)
+{
+    *reinterpret_cast<bf16x4 *>(p) = bf16x4{(bf16)x[0], (bf16)x[1], (bf16)x[2], (bf16)x[3]};
+}
+__device__ __forceinline__ void store4(float *p, f32x4 x) { *reinterpret_cast<f32x4 *>(p) = x; }
+
+// The games of a chunk of n plies: bit i of `starts` where one starts at ply i. The
+// same in all lanes.
+struct Games {
+    uint32_t starts;
+    int n;
+    static __device__ __forceinline__ uint32_t upto(int i) { return (2u << i) - 1; }   // plies 0 .. i
+    __device__ __forceinline__ bool from_begin(int i) const { return i < n && !(starts & upto(i)); }   // i sees the begin
+    __device__ __forceinline__ bool to_end(int i) const { return i < n && !(starts & ~upto(i)); }      // the end sees i
+    __device__ __forceinline__ bool same(int i, int j) const { return !(starts & upto(i) & ~upto(j)); }   // j <= i
 };
 
-// One chunk of a pass for D columns: D / 16 waves, each with 16 columns of the
-// value-side and of the state.
+// A wave's part of a pass for heads of D elements: the state's columns c0 .. c0 + CW
+// in registers, and all that has those columns. One wave takes a whole head up to
+// D = 64, so that nothing waits for another wave; for D = 128 the state's registers
+// go over four, which each compute P for themselves. Chunks have the depth of one
+// fragment: P, as it comes out of its product, is the next product's operand.
+constexpr int pass_waves(int dim) { return dim / 32; }
 template <class T, int D, bool REV>
 struct Chunk {
     using M = Mma<T>;
     using Frag = typename M::Frag;
-    static constexpr int CH = M::CH, KB = M::KB, NT = CH / 16, WAVES = D / 16, THREADS = 64 * WAVES;
-    static constexpr int LD = D + Vec<T>::N, PLD = CH + Vec<T>::N;   // 16 bytes of padding turn the rows over the banks
-    static constexpr int FE = KB / 4;                                // elements of a fragment
+    static constexpr int WAVES = pass_waves(D), CW = D / WAVES;
+    static constexpr int KB = M::KB, CH = KB, NT = CH / 16, KT = D / 16, CT = CW / 16, FE = KB / 4;
+    static constexpr int LD = D + Vec<T>::N;   // 16 bytes of padding turn a tile's rows over the banks
 
-    f32x4 s[D / 16];   // state (16t + 4g + r, 16w + l % 16)
+    f32x4 s[KT][CT];   // state (16t + 4g + r, c0 + 16c + l % 16)
     float g2;          // log2 lambda
-    int w, l, lc, g;
+    float in_scale, out_scale;
+    int l, lc, g, c0;
+    // of a whole chunk in which no game starts: lambda's powers with their scales, for
+    // P's tiles u tiles beside the diagonal (0 where a ply is not seen), for what a ply
+    // sees of the state before, and for what is left of it after
+    f32x4 apart[NT];
+    float sees[NT], left[FE];
 
-    __device__ __forceinline__ Chunk(float log_decay)
-        : g2(log2_lambda(log_decay)), w(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)), l(threadIdx.x & 63), lc(l & 15), g(l >> 4)
+    __device__ __forceinline__ Chunk(float log_decay, float in_scale_, float out_scale_, int wave)
+        : g2(log2_lambda(log_decay)), in_scale(in_scale_), out_scale(out_scale_), l(threadIdx.x & 63), lc(l & 15), g(l >> 4), c0(wave * CW)
     {
+#pragma unroll
+        for (int u = 0; u < NT; ++u)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int d = 16 * u + (REV ? 4 * g + r - lc : lc - 4 * g - r);
+                apart[u][r] = d >= 0 ? in_scale * out_scale * power(g2, d) : 0.f;
+            }
+        const Games gm{0, CH};
+        reach(gm, lc, g, sees, left);
     }
 
-    // f(register t, r of the state, its offset) for this lane's part of a (rows, cols) state
+    // what the plies of a chunk see of the state before it, and what is left of them after
+    __device__ __forceinline__ void reach(const Games &gm, int lc, int g, float (&see)[NT], float (&leave)[FE]) const
+    {
+#pragma unroll
+        for (int it = 0; it < NT; ++it) {
+            const int i = 16 * it + lc;
+            const float f = out_scale * power(g2, REV ? gm.n - 1 - i : i + 1);
+            see[it] = (REV ? gm.to_end(i) : gm.from_begin(i)) ? f : 0.f;
+        }
+#pragma unroll
+        for (int e = 0; e < FE; ++e) {
+            const int j = M::depth(g, e);
+            const float f = in_scale * power(g2, REV ? j + 1 : gm.n - 1 - j);
+            leave[e] = (REV ? gm.from_begin(j) : gm.to_end(j)) ? f : 0.f;
+        }
+    }
+
+    // f(t, c, r, offset) for this lane's part of a (rows, cols) state
     template <class F>
     __device__ __forceinline__ void each(int rows, int cols, int s_row, int s_col, F &&f)
     {
-        int i0 = 4 * g, c = 16 * w + lc;
-        asm("" : "+v"(i0), "+v"(c));   // the offsets are made where they are used, not kept over the pass
-        const int at = i0 * s_row + c * s_col;
-        if (c >= cols) rows = 0;
+        int i0 = 4 * g, j0 = c0 + lc;
+        asm("" : "+v"(i0), "+v"(j0));   // the offsets are made where they are used, not kept over the pass
 #pragma unroll
-        for (int t = 0; t < D / 16; ++t)
+        for (int c = 0; c < CT; ++c)
+            if (j0 + 16 * c < cols)
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-                if (i0 + 16 * t + r < rows) f(t, r, at + (16 * t + r) * s_row);
+                for (int t = 0; t < KT; ++t)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (i0 + 16 * t + r < rows) f(t, c, r, (i0 + 16 * t + r) * s_row + (j0 + 16 * c) * s_col);
     }
     __device__ __forceinline__ void load_state(const float *p, int rows, int cols, int s_row, int s_col)
     {
 #pragma unroll
-        for (int t = 0; t < D / 16; ++t) s[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-        if (p) each(rows, cols, s_row, s_col, [&](int t, int r, int at) { s[t][r] = p[at]; });
+        for (int t = 0; t < KT; ++t)
+#pragma unroll
+            for (int c = 0; c < CT; ++c) s[t][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (p) each(rows, cols, s_row, s_col, [&](int t, int c, int r, int at) { s[t][c][r] = p[at]; });
     }
     __device__ __forceinline__ void store_state(float *p, int rows, int cols, int s_row, int s_col)
     {
-        each(rows, cols, s_row, s_col, [&](int t, int r, int at) { p[at] = s[t][r]; });
+        each(rows, cols, s_row, s_col, [&](int t, int c, int r, int at) { p[at] = s[t][c][r]; });
     }
 
-    // Lane i: ply i of a chunk of n plies, `start` where a game starts there. One wave.
-    __device__ __forceinline__ void mark(Marks<CH> &mk, bool start, int n, float in_scale) const
+    // o[c][it] (rows: value columns c0 + 16c .., column: ply 16it + l % 16) = the
+    // chunk's outputs (OUT), and the state after it, from its tiles in LDS.
+    template <bool OUT>
+    __device__ __forceinline__ void run(const T *q, const T *k, const T *v, const Games &gm, f32x4 (&o)[CT][NT])
     {
-        const uint64_t mask = __ballot(start);
-        const int i = l, game = __popcll(mask & ((2ull << i) - 1)), games = __popcll(mask);
-        if (i < CH) {
-            const bool from = game == 0, to = game == games;   // sees the begin; is seen from the end
-            mk.sees[i] = i < n && (REV ? to : from) ? power(g2, REV ? n - 1 - i : i + 1) : -1.f;
-            mk.leaves[i] = i < n && (REV ? from : to) ? in_scale * power(g2, REV ? i + 1 : n - 1 - i) : 0.f;
-            mk.game[i] = game;
+        float see[NT], leave[FE];
+#pragma unroll
+        for (int it = 0; it < NT; ++it) see[it] = sees[it];
+#pragma unroll
+        for (int e = 0; e < FE; ++e) leave[e] = left[e];
+        const bool whole = !gm.starts && gm.n == CH;
+        if (!whole) {
+            int lc_ = lc, g_ = g;
+            asm volatile("" : "+v"(lc_), "+v"(g_));   // made here, not kept over the pass for chunks that are few
+            reach(gm, lc_, g_, see, leave);
         }
-        if (i == 0) {
-            mk.carry = games ? -1.f : power(g2, n);
-            mk.n = n;
-            mk.starts = games != 0;
-        }
-    }
-
-    // p[i][j] = scale lambda^|i - j| q_i.k_j for the plies j that i sees, else 0, of N
-    // pairs q, k; the tiles on the diagonal and on one side of it, shared out over the
-    // waves.
-    template <int N>
-    __device__ __forceinline__ void scores(const T *const (&q)[N], const T *const (&k)[N], T *const (&p)[N],
-                                           const Marks<CH> &mk, float scale) const
-    {
-        const bool starts = __builtin_amdgcn_readfirstlane(mk.starts);
-        for (int m = w; m < NT * (NT + 1) / 2; m += WAVES) {
-            const int a = m < 1 ? 0 : m < 3 ? 1 : m < 6 ? 2 : 3, b = m - a * (a + 1) / 2;
-            const int it = REV ? b : a, jt = REV ? a : b, i = 16 * it + lc, j0 = 16 * jt + 4 * g;
-            f32x4 acc[N];
+        Frag p[NT];
+        if constexpr (OUT) {
+            Frag x[NT][D / KB];
 #pragma unroll
-            for (int u = 0; u < N; ++u) acc[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int it = 0; it < NT; ++it)
 #pragma unroll
-            for (int c = 0; c < D; c += KB)
+                for (int c = 0; c < D / KB; ++c) x[it][c] = M::row(q + (16 * it + lc) * LD + c * KB, g);
+            scores(x, k, gm, p);
+            // what the state before the chunk answers
 #pragma unroll
-                for (int u = 0; u < N; ++u)
-                    acc[u] = M::mul(M::row(k[u] + (16 * jt + lc) * LD + c, g), M::row(q[u] + i * LD + c, g), acc[u]);
-            const float d0 = (float)(REV ? j0 - i : i - j0);
-            const int game = starts ? mk.game[i] : 0;
+            for (int c = 0; c < CT; ++c)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const float d = REV ? d0 + r : d0 - r, f = scale * power(g2, d);
-                const bool seen = d >= 0.f && (!starts || game == mk.game[j0 + r]);
+                for (int it = 0; it < NT; ++it) o[c][it] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int u = 0; u < N; ++u) acc[u][r] = seen ? acc[u][r] * f : 0.f;
-            }
+            for (int d = 0; d < D / KB; ++d)
 #pragma unroll
-            for (int u = 0; u < N; ++u) store4(p[u] + i * PLD + M::place(j0), acc[u]);
-        }
-    }
-
-    static __device__ __forceinline__ void store4(bf16 *p, f32x4 x)
-    {
-        *reinterpret_cast<bf16x4 *>(p) = bf16x4{(bf16)x[0], (bf16)x[1], (bf16)x[2], (bf16)x[3]};
-    }
-    static __device__ __forceinline__ void store4(float *p, f32x4 x) { *reinterpret_cast<f32x4 *>(p) = x; }
-
-    // o[it] (columns i = 16it + l % 16, rows: this wave's value columns) = what the
-    // state before the chunk answers to q_i.
-    __device__ __forceinline__ void inter(const T *q, const Marks<CH> &mk, float scale, f32x4 (&o)[NT]) const
-    {
+                for (int c = 0; c < CT; ++c) {
+                    constexpr int N = PARTS<T, 2>;
+                    Frag part[N];
+                    float y[FE];
 #pragma unroll
-        for (int it = 0; it < NT; ++it) o[it] = f32x4{0.f, 0.f, 0.f, 0.f};
+                    for (int e = 0; e < FE; ++e) y[e] = s[(d * KB + 4 * e) / 16][c][e & 3];
+                    M::template split<N>(y, part);
 #pragma unroll
-        for (int c = 0; c < D / KB; ++c) {
-            constexpr int N = PARTS<T, 2>;
-            Frag part[N];
-            float x[FE];
+                    for (int it = 0; it < NT; ++it)
 #pragma unroll
-            for (int e = 0; e < FE; ++e) x[e] = s[(c * KB + 4 * e) / 16][e & 3];
-            M::template split<N>(x, part);
+                        for (int u = 0; u < N; ++u) o[c][it] = M::mul(part[u], x[it][d], o[c][it]);
+                }
+            if (!whole) {   // a state that is not seen may hold NaN
+                int lc_ = lc;
+                asm volatile("" : "+v"(lc_));
 #pragma unroll
-            for (int it = 0; it < NT; ++it) {
-                const Frag y = M::deep(q + (16 * it + lc) * LD + c * KB, g);
+                for (int it = 0; it < NT; ++it) {
+                    const bool on = REV ? gm.to_end(16 * it + lc_) : gm.from_begin(16 * it + lc_);
 #pragma unroll
-                for (int u = 0; u < N; ++u) o[it] = M::mul(part[u], y, o[it]);
-            }
-        }
-        seen(mk, scale, o);
-    }
-
-    // o += P v (OUT), and the state after the chunk (STATE).
-    template <bool OUT, bool STATE>
-    __device__ __forceinline__ void apply(const T *k, const T *v, const T *p, const Marks<CH> &mk, f32x4 (&o)[NT])
-    {
-        if constexpr (STATE) {
-            const float carry = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, mk.carry)));
-            if (carry >= 0.f) {
+                    for (int c = 0; c < CT; ++c)
 #pragma unroll
-                for (int t = 0; t < D / 16; ++t)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) s[t][r] *= carry;
-            } else {
-#pragma unroll
-                for (int t = 0; t < D / 16; ++t) s[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-            }
-        }
-#pragma unroll
-        for (int c = 0; c < CH / KB; ++c) {
-            const Frag x = M::col(v + c * KB * LD + 16 * w, LD, l);
-#pragma unroll
-            for (int it = 0; it < NT; ++it) {
-                if (!OUT || (REV ? c * KB + KB <= 16 * it : c * KB >= 16 * it + 16)) continue;   // nothing to see there
-                o[it] = M::mul(x, M::row(p + (16 * it + lc) * PLD + c * KB, g), o[it]);
-            }
-            if constexpr (STATE) {
-                // the plies' values times what is left of them after the chunk
-                constexpr int N = PARTS<T, 3>;
-                Frag part[N];
-                float left[FE];
-#pragma unroll
-                for (int e = 0; e < FE; ++e) left[e] = (float)x[e] * mk.leaves[c * KB + M::depth(g, e)];
-                M::template split<N>(left, part);
-#pragma unroll
-                for (int t = 0; t < D / 16; ++t) {
-                    const Frag y = M::col(k + c * KB * LD + 16 * t, LD, l);
-#pragma unroll
-                    for (int u = 0; u < N; ++u) s[t] = M::mul(y, part[u], s[t]);
+                        for (int r = 0; r < 4; ++r) o[c][it][r] = on ? o[c][it][r] : 0.f;
                 }
             }
+#pragma unroll
+            for (int c = 0; c < CT; ++c)
+#pragma unroll
+                for (int it = 0; it < NT; ++it)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) o[c][it][r] *= see[it];
         }
-    }
-
-    // ---- the state turned over, for the pass that needs both of its sides: as terms in
-    // LDS, turned[u][c][i] for element (i, c)
-    static constexpr int TURNED = PARTS<T, 2>;
-    __device__ __forceinline__ void turn(T *turned) const
-    {
+        if (gm.starts) {   // nothing is left of the state
 #pragma unroll
-        for (int t = 0; t < D / 16; ++t) {
-            f32x4 x = s[t];
+            for (int t = 0; t < KT; ++t)
 #pragma unroll
-            for (int u = 0; u < TURNED; ++u) {
-                T *at = turned + (u * D + 16 * w + lc) * LD + 16 * t + 4 * g;
-                store4(at, x);
-                if (u + 1 < TURNED)
+                for (int c = 0; c < CT; ++c) s[t][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+        } else {
+            const float carry = power(g2, gm.n);
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) x[r] -= (float)from_float<T>(x[r]);
+            for (int t = 0; t < KT; ++t)
+#pragma unroll
+                for (int c = 0; c < CT; ++c)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) s[t][c][r] *= carry;
+        }
+#pragma unroll
+        for (int c = 0; c < CT; ++c) {
+            const Frag x = M::col(v + c0 + 16 * c, LD, l);
+            if constexpr (OUT)
+#pragma unroll
+                for (int it = 0; it < NT; ++it) o[c][it] = M::mul(x, p[it], o[c][it]);
+            constexpr int N = PARTS<T, 3>;
+            Frag part[N];
+            float y[FE];
+#pragma unroll
+            for (int e = 0; e < FE; ++e) y[e] = (float)x[e] * leave[e];
+            M::template split<N>(y, part);
+#pragma unroll
+            for (int t = 0; t < KT; ++t) {
+                const Frag z = M::col(k + 16 * t, LD, l);
+#pragma unroll
+                for (int u = 0; u < N; ++u) s[t][c] = M::mul(z, part[u], s[t][c]);
             }
         }
     }
 
-    // like inter, for the turned state: rows of o are this wave's columns of its other side
-    __device__ __forceinline__ void inter_turned(const T *turned, const T *q, const Marks<CH> &mk, float scale,
-                                                 f32x4 (&o)[NT]) const
+    // p[it] = P's columns i = 16it + l % 16 as an operand over the plies j, times the scales.
+    __device__ __forceinline__ void scores(const Frag (&x)[NT][D / KB], const T *k, const Games &gm, Frag (&p)[NT]) const
     {
+        f32x4 acc[NT][NT];   // [it][jt]
 #pragma unroll
-        for (int it = 0; it < NT; ++it) o[it] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int jt = 0; jt < NT; ++jt) {
 #pragma unroll
-        for (int c = 0; c < D / KB; ++c) {
-            Frag part[TURNED];
+            for (int it = 0; it < NT; ++it) acc[it][jt] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int u = 0; u < TURNED; ++u) part[u] = M::col(turned + (u * D + c * KB) * LD + 16 * w, LD, l);
+            for (int c = 0; c < D / KB; ++c) {
+                const Frag y = M::row(k + (16 * jt + lc) * LD + c * KB, g);
 #pragma unroll
-            for (int it = 0; it < NT; ++it) {
-                const Frag y = M::deep(q + (16 * it + lc) * LD + c * KB, g);
-#pragma unroll
-                for (int u = 0; u < TURNED; ++u) o[it] = M::mul(part[u], y, o[it]);
+                for (int it = 0; it < NT; ++it)
+                    if (REV ? jt >= it : jt <= it) acc[it][jt] = M::mul(y, x[it][c], acc[it][jt]);
             }
         }
-        seen(mk, scale, o);
-    }
-
-    // o times what is left of the state at its plies
-    __device__ __forceinline__ void seen(const Marks<CH> &mk, float scale, f32x4 (&o)[NT]) const
-    {
+        // a ply that is not seen leaves 0, whatever its product is
 #pragma unroll
-        for (int it = 0; it < NT; ++it) {
-            const float f = mk.sees[16 * it + lc];
+        for (int it = 0; it < NT; ++it)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) o[it][r] = f >= 0.f ? o[it][r] * (f * scale) : 0.f;
+            for (int jt = 0; jt < NT; ++jt)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int u = REV ? jt - it : it - jt;
+                    float y = 0.f;
+                    if (u >= 0) {
+                        y = acc[it][jt][r] * apart[u < 0 ? 0 : u][r];
+                        if (u == 0) y = (REV ? 4 * g + r >= lc : lc >= 4 * g + r) ? y : 0.f;
+                    }
+                    acc[it][jt][r] = y;
+                }
+        if (gm.starts) {
+            int lc_ = lc, g_ = g;
+            asm volatile("" : "+v"(lc_), "+v"(g_));
+#pragma unroll
+            for (int it = 0; it < NT; ++it)
+#pragma unroll
+                for (int jt = 0; jt < NT; ++jt)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const int i = 16 * it + lc_, j = 16 * jt + 4 * g_ + r;
+                        acc[it][jt][r] = (REV ? gm.same(j, i) : gm.same(i, j)) ? acc[it][jt][r] : 0.f;
+                    }
         }
+#pragma unroll
+        for (int it = 0; it < NT; ++it)
+#pragma unroll
+            for (int e = 0; e < FE; ++e) p[it][e] = from_float<T>(acc[it][e >> 2][e & 3]);
     }
 
     // The chunk ply by ply, for tiles with infinities or NaN: a product with 0 in
     // their place is not 0, and a ply must get nothing of those it does not see.
-    // put(i, x): x = this wave's value column l % 16 of ply i. each(i, t, r, y): y = the
-    // state's element (16t + 4g + r, 16w + l % 16) that ply i sees.
-    template <class F, class E>
-    __device__ __forceinline__ void singly(const T *q, const T *k, const T *v, const Marks<CH> &mk, float in_scale,
-                                           float out_scale, F &&put, E &&each)
+    // put(i, c, x): x = value column c0 + 16c + l % 16 of ply i.
+    template <class F>
+    __device__ __forceinline__ void singly(const T *q, const T *k, const T *v, const Games &gm, F &&put)
     {
         const float lam = power(g2, 1);
-        for (int m = 0; m < mk.n; ++m) {
-            const int i = REV ? mk.n - 1 - m : m;
-            const bool start = mk.game[i] != (i ? mk.game[i - 1] : 0);
-            const float x = in_scale * (float)v[i * LD + 16 * w + lc];
-            float o = 0.f;
+        for (int m = 0; m < gm.n; ++m) {
+            const int i = REV ? gm.n - 1 - m : m;
+            const bool start = (gm.starts >> i) & 1;
 #pragma unroll
-            for (int t = 0; t < D / 16; ++t)
+            for (int c = 0; c < CT; ++c) {
+                const float x = in_scale * (float)v[i * LD + c0 + 16 * c + lc];
+                float o = 0.f;
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int c = 16 * t + 4 * g + r;
-                    float y = s[t][r];
-                    if (!REV) y = start ? 0.f : lam * y;
-                    y += (float)k[i * LD + c] * x;
-                    o += (float)q[i * LD + c] * y;
-                    each(i, t, r, y);
-                    if (REV) y = start ? 0.f : lam * y;
-                    s[t][r] = y;
-                }
-            o += __shfl_xor(o, 16);
-            o += __shfl_xor(o, 32);
-            put(i, out_scale * o);
+                for (int t = 0; t < KT; ++t)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const int at = i * LD + 16 * t + 4 * g + r;
+                        float y = s[t][c][r];
+                        if (!REV) y = start ? 0.f : lam * y;
+                        y += (float)k[at] * x;
+                        o += (float)q[at] * y;
+                        if (REV) y = start ? 0.f : lam * y;
+                        s[t][c][r] = y;
+                    }
+                o += __shfl_xor(o, 16);
+                o += __shfl_xor(o, 32);
+                put(i, c, out_scale * o);
+            }
         }
     }
 };
@@ -397,9 +417,8 @@ struct Chunk {
 __device__ __forceinline__ float probe(bf16x8 x, float sum)
 {
 #pragma unroll
-    for (int i = 0; i < 8; i += 2) {
+    for (int i = 0; i < 8; i += 2)
         sum = __builtin_amdgcn_fdot2_f32_bf16(bf16x2{x[i], x[i + 1]}, bf16x2{bf16(0.f), bf16(0.f)}, sum, false);
-    }
     return sum;
 }
 __device__ __forceinline__ float probe(f32x4 x, float sum)
@@ -409,15 +428,29 @@ __device__ __forceinline__ float probe(f32x4 x, float sum)
     return sum;
 }
 
-// Rows of one game and head that a block reads or writes, a chunk of plies at a
-// time. FAST: through a buffer descriptor of the chunk's plies, whose bounds give
-// zeros for (and drop) rows past the chunk's end without a branch; rows are whole
-// aligned 16-byte vectors and a chunk spans less than 2 GiB (the host's check).
-// Otherwise element by element.
-template <class T, int D, bool FAST>
+// Waves of a block that share its tiles wait for each other; a wave alone only keeps
+// its own order.
+template <int WAVES>
+__device__ __forceinline__ void meet()
+{
+    if constexpr (WAVES > 1) __syncthreads();
+    else {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
+// Rows of one game and head that a block of THREADS reads or writes, a chunk of
+// plies at a time. FAST: through a buffer descriptor of the chunk's plies, whose
+// bounds give zeros for (and drop) rows past the chunk's end without a branch; rows
+// are whole aligned 16-byte vectors and a chunk spans less than 2 GiB (the host's
+// check). Otherwise element by element.
+template <class T, int D, int THREADS, bool FAST>
 struct Plies {
     using V = typename Vec<T>::type;
-    static constexpr int N = Vec<T>::N, PER_ROW = D / N, CH = Mma<T>::CH;
+    static constexpr int N = Vec<T>::N, PER_ROW = D / N, CH = Mma<T>::KB, LD = D + N;
+    static constexpr int NV = CH * PER_ROW / THREADS, ROWS = THREADS / PER_ROW;   // vectors of a thread, ROWS rows apart
+    static_assert(NV * ROWS == CH, "a tile is NV vectors a thread");
     T *base;
     int64_t ply;
     int dim;
@@ -428,261 +461,262 @@ struct Plies {
     {
         return __builtin_amdgcn_make_buffer_rsrc(base + t0 * ply, 0, (int)(((n - 1) * ply + dim) * sizeof(T)), 0x00020000);
     }
-
-    // this thread's two vectors of the tile of plies t0 .. t0 + n, CH / 2 rows apart; zeros elsewhere
-    __device__ __forceinline__ void load(int t0, int n, V (&x)[2]) const
+    // byte offset of this thread's first vector in a chunk; past any bound where it is beside the row
+    __device__ __forceinline__ int first() const
     {
         const int row = threadIdx.x / PER_ROW, c = threadIdx.x % PER_ROW * N;
+        return c < dim ? (row * (int)ply + c) * (int)sizeof(T) : INT32_MIN;
+    }
+    __device__ __forceinline__ int step() const { return threadIdx.x % PER_ROW * N < dim ? ROWS * (int)ply * (int)sizeof(T) : 0; }
+
+    // this thread's vectors of the tile of plies t0 .. t0 + n; zeros elsewhere
+    __device__ __forceinline__ void load(int t0, int n, V (&x)[NV]) const
+    {
         if constexpr (FAST) {
             const __amdgpu_buffer_rsrc_t r = chunk(t0, n);
-            const int step = (int)ply * (int)sizeof(T);
-            const int at = c < dim ? row * step + c * (int)sizeof(T) : INT32_MIN;   // past any bound
-            x[0] = __builtin_bit_cast(V, __builtin_amdgcn_raw_buffer_load_b128(r, at, 0, 0));
-            x[1] = __builtin_bit_cast(V, __builtin_amdgcn_raw_buffer_load_b128(r, c < dim ? at + CH / 2 * step : INT32_MIN, 0, 0));
-        } else {
+            int at = first();
+            const int by = step();
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const int i = row + u * (CH / 2);
+            for (int u = 0; u < NV; ++u, at += by)
+                x[u] = __builtin_bit_cast(V, __builtin_amdgcn_raw_buffer_load_b128(r, at, 0, 0));
+        } else {
+            const int row = threadIdx.x / PER_ROW, c = threadIdx.x % PER_ROW * N;
+#pragma unroll
+            for (int u = 0; u < NV; ++u) {
                 x[u] = V{};
 #pragma unroll
                 for (int e = 0; e < N; ++e)
-                    if (i < n && c + e < dim) x[u][e] = base[(t0 + i) * ply + c + e];
+                    if (row + u * ROWS < n && c + e < dim) x[u][e] = base[(t0 + row + u * ROWS) * ply + c + e];
             }
         }
     }
-
-    // rows 16 it + l % 16, columns c .. c + 3 of the chunk, from a product's result
-    template <int NT>
-    __device__ __forceinline__ void put(int t0, int n, int lc, int c, const f32x4 (&x)[NT]) const
+    // a tile in LDS out to plies t0 .. t0 + n
+    __device__ __forceinline__ void store(int t0, int n, const T *lds) const
     {
+        const T *p = lds + threadIdx.x / PER_ROW * LD + threadIdx.x % PER_ROW * N;
         if constexpr (FAST) {
             const __amdgpu_buffer_rsrc_t r = chunk(t0, n);
-            const int step = (int)ply * (int)sizeof(T);
-            int at = c < dim ? lc * step + c * (int)sizeof(T) : INT32_MIN;
+            int at = first();
+            const int by = step();
 #pragma unroll
-            for (int it = 0; it < NT; ++it) {
-                if constexpr (sizeof(T) == 2) {
-                    const bf16x4 y{(bf16)x[it][0], (bf16)x[it][1], (bf16)x[it][2], (bf16)x[it][3]};
-                    __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, y), r, at, 0, 0);
-                } else {
-                    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, x[it]), r, at, 0, 0);
-                }
-                at = c < dim ? at + 16 * step : at;
-            }
+            for (int u = 0; u < NV; ++u, at += by)
+                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, *reinterpret_cast<const V *>(p + u * ROWS * LD)), r, at, 0, 0);
         } else {
+            const int row = threadIdx.x / PER_ROW, c = threadIdx.x % PER_ROW * N;
 #pragma unroll
-            for (int it = 0; it < NT; ++it)
+            for (int u = 0; u < NV; ++u)
 #pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    if (16 * it + lc < n && c + r < dim)
-                        base[(t0 + 16 * it + lc) * ply + c + r] = from_float<T>(x[it][r]);
+                for (int e = 0; e < N; ++e)
+                    if (row + u * ROWS < n && c + e < dim) base[(t0 + row + u * ROWS) * ply + c + e] = p[u * ROWS * LD + e];
         }
     }
-
     // zeros from ply t0 to t1
     __device__ __forceinline__ void clear(int t0, int t1) const
     {
-        for (int t = t0 + (int)(threadIdx.x >> 6); t < t1; t += D / 16)
+        for (int t = t0 + (int)(threadIdx.x >> 6); t < t1; t += THREADS / 64)
             for (int c = threadIdx.x & 63; c < dim; c += 64) base[t * ply + c] = from_float<T>(0.f);
     }
-
-    // a thread's two vectors of a tile into LDS
-    static __device__ __forceinline__ void stage(T *lds, const V (&x)[2])
+    // a thread's vectors of a tile into LDS
+    static __device__ __forceinline__ void stage(T *lds, const V (&x)[NV])
     {
-        T *p = lds + threadIdx.x / PER_ROW * (D + N) + threadIdx.x % PER_ROW * N;
-        *reinterpret_cast<V *>(p) = x[0];
-        *reinterpret_cast<V *>(p + CH / 2 * (D + N)) = x[1];
+        T *p = lds + threadIdx.x / PER_ROW * LD + threadIdx.x % PER_ROW * N;
+#pragma unroll
+        for (int u = 0; u < NV; ++u) *reinterpret_cast<V *>(p + u * ROWS * LD) = x[u];
+    }
+    static __device__ __forceinline__ float probe_all(const V (&x)[NV], float sum)
+    {
+#pragma unroll
+        for (int u = 0; u < NV; ++u) sum = probe(x[u], sum);
+        return sum;
+    }
+};
+
+// The plies of one segment of one game and head.
+struct Segment {
+    int b, h, seg, s0, s1, end, chunks;   // s0 .. s1 of all plies, s0 .. end of the game's
+    __device__ __forceinline__ Segment(const ScanArgs &a, int seg_, int ch) : b(blockIdx.x / a.heads), h(blockIdx.x % a.heads), seg(seg_)
+    {
+        const int len = a.lengths ? min(max(a.lengths[b], 0), a.plies) : a.plies;
+        s0 = seg * a.seg_plies;
+        s1 = a.plies - s0 > a.seg_plies ? s0 + a.seg_plies : a.plies;
+        end = max(s0, min(s1, len));
+        chunks = (end - s0 + ch - 1) / ch;
     }
 };
 
 // A pass over one segment of one game and head by one block: chunks in turn, the
-// state in registers. While a chunk is worked on, the next one's tiles are on
-// their way. OUT: the plies' outputs, from the state before the segment; else only
-// the state that the segment's own plies leave, for the states before the others.
+// state in registers. While a chunk is worked on, the next one's rows are on their
+// way. OUT: the plies' outputs, from the state before the segment; else only the
+// state that the segment's own plies leave, for the states before the others.
 template <class T, int D, bool REV, bool FAST, bool OUT>
-__global__ __launch_bounds__(4 * D, D == 32 ? 3 : 4) void k_attention_pass(ScanArgs a)
+__global__ __launch_bounds__(64 * pass_waves(D), 2) void k_attention_pass(ScanArgs a)
 {
     using C = Chunk<T, D, REV>;
-    using P = Plies<T, D, FAST>;
+    constexpr int CH = C::CH, LD = C::LD, WAVES = C::WAVES;
+    using P = Plies<T, D, 64 * WAVES, FAST>;
     using V = typename P::V;
-    constexpr int CH = C::CH, LD = C::LD, NT = C::NT;
-    __shared__ __align__(16) T qs[OUT ? CH * LD : 1], ks[CH * LD], vs[CH * LD], ps[OUT ? CH * C::PLD : 1];
-    __shared__ Marks<CH> mk;
+    __shared__ __align__(16) T qs[OUT ? CH * LD : 1], ks[CH * LD], vs[CH * LD];
     __shared__ int bad[2];
-    const int b = blockIdx.x / a.heads, h = blockIdx.x % a.heads;
-    const int seg = blockIdx.y + (!OUT && REV ? 1 : 0);   // the last segment's own state goes nowhere
-    const int len = a.lengths ? min(max(a.lengths[b], 0), a.plies) : a.plies;
-    const int s0 = seg * a.seg_plies, s1 = a.plies - s0 > a.seg_plies ? s0 + a.seg_plies : a.plies, end = min(s1, len);
-    const int chunks = end > s0 ? (end - s0 + CH - 1) / CH : 0;
-    C ch(a.log_decay[h]);
+    const Segment sg(a, blockIdx.y + (!OUT && REV ? 1 : 0), CH);   // the last segment's own state goes nowhere
+    C ch(a.log_decay[sg.h], a.in_scale, a.out_scale, WAVES > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0);
     const int64_t size = (int64_t)a.kd * a.vd;
-    float *slot = a.seg_states + ((int64_t)blockIdx.x * a.segments + seg) * size;
+    float *slot = a.seg_states + ((int64_t)blockIdx.x * a.segments + sg.seg) * size;
     if (!OUT) ch.load_state(nullptr, 0, 0, 0, 0);
     else if (a.segments > 1) ch.load_state(slot, a.kd, a.vd, a.vd, 1);
     else ch.load_state(a.s_in ? a.s_in + blockIdx.x * size : nullptr, a.kd, a.vd, a.s_row, a.s_col);
-    const P q(a.q, b, h, a.kd), k(a.k, b, h, a.kd), v(a.v, b, h, a.vd), o(a.o, b, h, a.vd);
-    const uint8_t *starts = a.starts ? a.starts + b * a.starts_batch : nullptr;
-    if (OUT)
-        for (int x = threadIdx.x; x < CH * C::PLD; x += C::THREADS) ps[x] = T(0.f);   // tiles beside the diagonal stay 0
-    if (threadIdx.x < 2) bad[threadIdx.x] = 0;
-    __syncthreads();
+    const P q(a.q, sg.b, sg.h, a.kd), k(a.k, sg.b, sg.h, a.kd), v(a.v, sg.b, sg.h, a.vd), o(a.o, sg.b, sg.h, a.vd);
+    const uint8_t *starts = a.starts ? a.starts + sg.b * a.starts_batch : nullptr;
+    if (WAVES > 1) {
+        if (threadIdx.x < 2) bad[threadIdx.x] = 0;
+        meet<WAVES>();
+    }
 
-    V qt[2], kt[2], vt[2];
+    V qt[P::NV], kt[P::NV], vt[P::NV];
     bool start = false, any_start = false;
-    const auto begin = [&](int m) { return s0 + (REV ? chunks - 1 - m : m) * CH; };
+    const auto begin = [&](int m) { return sg.s0 + (REV ? sg.chunks - 1 - m : m) * CH; };
     const auto fetch = [&](int m) {
-        const int t0 = begin(m), n = min(CH, end - t0);
+        const int t0 = begin(m), n = min(CH, sg.end - t0);
+        start = starts && ch.l < n && starts[(t0 + ch.l) * a.starts_ply];
         if (OUT) q.load(t0, n, qt);
         k.load(t0, n, kt);
         v.load(t0, n, vt);
-        start = starts && ch.l < n && starts[(t0 + ch.l) * a.starts_ply];
     };
-    if (chunks) fetch(0);
-    for (int m = 0; m < chunks; ++m) {
-        const int t0 = begin(m), n = min(CH, end - t0);
-        if (ch.w == 0) ch.mark(mk, start, n, a.in_scale);
-        if (!OUT) any_start |= __ballot(start) != 0;
+    if (sg.chunks) fetch(0);
+    for (int m = 0; m < sg.chunks; ++m) {
+        const int t0 = begin(m);
+        const Games gm{(uint32_t)__ballot(start), min(CH, sg.end - t0)};
+        any_start |= gm.starts != 0;
         if (OUT) P::stage(qs, qt);
         P::stage(ks, kt);
         P::stage(vs, vt);
-        const float sum = probe(vt[1], probe(vt[0], probe(kt[1], probe(kt[0], 0.f))));
-        if (sum != sum) bad[m & 1] = 1;
-        __syncthreads();
-        if (m + 1 < chunks) fetch(m + 1);
-        if (threadIdx.x == 0) bad[(m + 1) & 1] = 0;
-        if (bad[m & 1]) {
-            ch.singly(OUT ? qs : ks, ks, vs, mk, a.in_scale, a.out_scale, [&](int i, float x) {
-                const int c = 16 * ch.w + ch.lc;
-                if (OUT && ch.g == 0 && c < a.vd) o.base[(t0 + i) * o.ply + c] = from_float<T>(x);
-            }, [](int, int, int, float) {});
-        } else if constexpr (OUT) {
-            f32x4 acc[NT];
-            ch.template scores<1>({qs}, {ks}, {ps}, mk, a.in_scale * a.out_scale);
-            ch.inter(qs, mk, a.out_scale, acc);
-            __syncthreads();
-            ch.template apply<true, true>(ks, vs, ps, mk, acc);
-            o.put(t0, n, ch.lc, 16 * ch.w + 4 * ch.g, acc);
-        } else {
-            f32x4 none[NT];
-            ch.template apply<false, true>(ks, vs, nullptr, mk, none);
+        const float sum = P::probe_all(kt, P::probe_all(vt, 0.f));
+        bool singly = __ballot(sum != sum) != 0;
+        if (WAVES > 1 && singly) bad[m & 1] = 1;
+        meet<WAVES>();
+        if (WAVES > 1) {
+            singly = bad[m & 1];
+            if (threadIdx.x == 0) bad[(m + 1) & 1] = 0;
         }
-        __syncthreads();
+        if (m + 1 < sg.chunks) fetch(m + 1);
+        f32x4 acc[C::CT][C::NT];
+        if (singly) {
+            meet<WAVES>();   // bad is read
+            ch.singly(OUT ? qs : ks, ks, vs, gm, [&](int i, int c, float x) {
+                const int j = ch.c0 + 16 * c + ch.lc;
+                if (OUT && ch.g == 0 && j < a.vd) o.base[(t0 + i) * o.ply + j] = from_float<T>(x);
+            });
+            meet<WAVES>();
+        } else {
+            ch.template run<OUT>(qs, ks, vs, gm, acc);
+            meet<WAVES>();
+            if constexpr (OUT) {   // out through LDS, a row's bytes together
+#pragma unroll
+                for (int c = 0; c < C::CT; ++c)
+#pragma unroll
+                    for (int it = 0; it < C::NT; ++it)
+                        store4(qs + (16 * it + ch.lc) * LD + ch.c0 + 16 * c + 4 * ch.g, acc[c][it]);
+                meet<WAVES>();
+                o.store(t0, gm.n, qs);   // the elements that this thread's next rows replace
+            }
+        }
     }
     if constexpr (OUT) {
-        o.clear(max(s0, len), s1);
-        if (a.s_out && seg == (REV ? 0 : a.segments - 1)) ch.store_state(a.s_out + blockIdx.x * size, a.kd, a.vd, a.s_row, a.s_col);
+        o.clear(sg.end, sg.s1);
+        if (a.s_out && sg.seg == (REV ? 0 : a.segments - 1))
+            ch.store_state(a.s_out + blockIdx.x * size, a.kd, a.vd, a.s_row, a.s_col);
     } else {
         ch.store_state(slot, a.kd, a.vd, a.vd, 1);
         if (threadIdx.x == 0)
-            a.seg_carry[(int64_t)blockIdx.x * a.segments + seg] = any_start ? -1.f : power(ch.g2, max(end - s0, 0));
+            a.seg_carry[(int64_t)blockIdx.x * a.segments + sg.seg] = any_start ? -1.f : power(ch.g2, sg.end - sg.s0);
     }
 }
 
 // The gradients of k and v over one segment of one game and head, in reverse, from
-// one reading of q, k, v and d_out. With R the gradient of the state after a ply,
-//   dv_j = R^T k_j and dk_j = R v_j   where R = scale sum_{i >= j} lambda^(i - j) q_i d_i^T + ...
-// are two passes with one state: dv is the pass (k, q, d_out), whose state stays in
-// registers; dk is (v, d_out, q) on its transpose, which the waves leave for each
-// other in LDS, as terms. Both share the plies' weights.
+// one reading of q, k, v and d_out: two passes side by side on the same tiles, dv
+// (k, q, d_out) by one half of the block's waves and dk (v, d_out, q), on the
+// transposed state, by the other.
 struct GradArgs {
     ScanArgs scan;       // q: k, k: q, v: d_out, o: dv
     jq_rows values, dk;  // v and the gradient of k
 };
-template <class T, int D> constexpr int kv_lds()
-{
-    using C = Chunk<T, D, true>;
-    return (4 * C::CH * C::LD + 2 * C::CH * C::PLD + C::TURNED * D * C::LD) * (int)sizeof(T);
-}
 template <class T, int D, bool FAST>
-__global__ __launch_bounds__(4 * D, 2) void k_attention_kv(GradArgs ga)
+__global__ __launch_bounds__(128 * pass_waves(D), 2) void k_attention_kv(GradArgs ga)
 {
     using C = Chunk<T, D, true>;
-    using P = Plies<T, D, FAST>;
+    constexpr int CH = C::CH, LD = C::LD, WAVES = 2 * C::WAVES;
+    using P = Plies<T, D, 64 * WAVES, FAST>;
     using V = typename P::V;
-    constexpr int CH = C::CH, LD = C::LD, NT = C::NT, PLD = C::PLD;
     const ScanArgs &a = ga.scan;
-    extern __shared__ __align__(16) char dynamic[];
-    T *ks = reinterpret_cast<T *>(dynamic), *qs = ks + CH * LD, *ds = qs + CH * LD, *vs = ds + CH * LD;
-    T *p1 = vs + CH * LD, *p2 = p1 + CH * PLD, *turned = p2 + CH * PLD;
-    __shared__ Marks<CH> mk;
+    __shared__ __align__(16) T ks[CH * LD], qs[CH * LD], ds[CH * LD], vs[CH * LD];
     __shared__ int bad[2];
-    const int b = blockIdx.x / a.heads, h = blockIdx.x % a.heads, seg = blockIdx.y;
-    const int len = a.lengths ? min(max(a.lengths[b], 0), a.plies) : a.plies;
-    const int s0 = seg * a.seg_plies, s1 = a.plies - s0 > a.seg_plies ? s0 + a.seg_plies : a.plies, end = min(s1, len);
-    const int chunks = end > s0 ? (end - s0 + CH - 1) / CH : 0;
-    C ch(a.log_decay[h]);
+    const Segment sg(a, blockIdx.y, CH);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const bool second = wave >= C::WAVES;   // dk
+    C ch(a.log_decay[sg.h], a.in_scale, 1.f, wave % C::WAVES);
     const int64_t size = (int64_t)a.kd * a.vd;
-    if (a.segments > 1) ch.load_state(a.seg_states + ((int64_t)blockIdx.x * a.segments + seg) * size, a.kd, a.vd, a.vd, 1);
-    else ch.load_state(a.s_in ? a.s_in + blockIdx.x * size : nullptr, a.kd, a.vd, a.vd, 1);
-    const P k(a.q, b, h, a.kd), q(a.k, b, h, a.kd), d(a.v, b, h, a.vd), v(ga.values, b, h, a.vd);
-    const P dv(a.o, b, h, a.vd), dk(ga.dk, b, h, a.kd);
-    const uint8_t *starts = a.starts ? a.starts + b * a.starts_batch : nullptr;
-    for (int x = threadIdx.x; x < 2 * CH * PLD; x += C::THREADS) p1[x] = T(0.f);   // tiles beside the diagonal stay 0
-    ch.turn(turned);
+    const float *init = a.segments > 1 ? a.seg_states + ((int64_t)blockIdx.x * a.segments + sg.seg) * size
+                                       : a.s_in ? a.s_in + blockIdx.x * size : nullptr;
+    if (second) ch.load_state(init, a.vd, a.kd, 1, a.vd);
+    else ch.load_state(init, a.kd, a.vd, a.vd, 1);
+    const P k(a.q, sg.b, sg.h, a.kd), q(a.k, sg.b, sg.h, a.kd), d(a.v, sg.b, sg.h, a.vd), v(ga.values, sg.b, sg.h, a.vd);
+    const P dv(a.o, sg.b, sg.h, a.vd), dk(ga.dk, sg.b, sg.h, a.kd);
+    const uint8_t *starts = a.starts ? a.starts + sg.b * a.starts_batch : nullptr;
     if (threadIdx.x < 2) bad[threadIdx.x] = 0;
     __syncthreads();
 
-    V kt[2], qt[2], dt[2], vt[2];
+    V kt[P::NV], qt[P::NV], dt[P::NV], vt[P::NV];
     bool start = false;
-    const auto begin = [&](int m) { return s0 + (chunks - 1 - m) * CH; };
+    const auto begin = [&](int m) { return sg.s0 + (sg.chunks - 1 - m) * CH; };
     const auto fetch = [&](int m) {
-        const int t0 = begin(m), n = min(CH, end - t0);
+        const int t0 = begin(m), n = min(CH, sg.end - t0);
+        start = starts && ch.l < n && starts[(t0 + ch.l) * a.starts_ply];
         k.load(t0, n, kt);
         q.load(t0, n, qt);
         d.load(t0, n, dt);
         v.load(t0, n, vt);
-        start = starts && ch.l < n && starts[(t0 + ch.l) * a.starts_ply];
     };
-    if (chunks) fetch(0);
-    for (int m = 0; m < chunks; ++m) {
-        const int t0 = begin(m), n = min(CH, end - t0);
-        if (ch.w == 0) ch.mark(mk, start, n, a.in_scale);
+    if (sg.chunks) fetch(0);
+    for (int m = 0; m < sg.chunks; ++m) {
+        const int t0 = begin(m);
+        const Games gm{(uint32_t)__ballot(start), min(CH, sg.end - t0)};
         P::stage(ks, kt);
         P::stage(qs, qt);
         P::stage(ds, dt);
         P::stage(vs, vt);
-        const float sum = probe(dt[1], probe(dt[0], probe(qt[1], probe(qt[0], 0.f))));
-        if (sum != sum) bad[m & 1] = 1;
+        const float sum = P::probe_all(qt, P::probe_all(dt, 0.f));
+        if (__ballot(sum != sum)) bad[m & 1] = 1;
         __syncthreads();
-        if (m + 1 < chunks) fetch(m + 1);
+        const bool singly = bad[m & 1];
         if (threadIdx.x == 0) bad[(m + 1) & 1] = 0;
-        if (bad[m & 1]) {
-            float *red = reinterpret_cast<float *>(p1);   // [wave][D], for the sums over all columns
-            static_assert(C::WAVES * D * sizeof(float) <= CH * PLD * sizeof(T));
-            ch.singly(ks, qs, ds, mk, a.in_scale, 1.f, [&](int i, float x) {
-                const int c = 16 * ch.w + ch.lc;
-                if (ch.g == 0 && c < a.vd) dv.base[(t0 + i) * dv.ply + c] = from_float<T>(x);
-                __syncthreads();
-                if (threadIdx.x < a.kd) {
-                    float y = 0.f;
-                    for (int u = 0; u < C::WAVES; ++u) y += red[u * D + threadIdx.x];
-                    dk.base[(t0 + i) * dk.ply + threadIdx.x] = from_float<T>(y);
-                }
-                __syncthreads();
-            }, [&](int i, int t, int r, float y) {
-                y *= (float)vs[i * LD + 16 * ch.w + ch.lc];
-#pragma unroll
-                for (int o = 8; o; o >>= 1) y += __shfl_xor(y, o);
-                if (ch.lc == 0) red[ch.w * D + 16 * t + 4 * ch.g + r] = y;
+        if (m + 1 < sg.chunks) fetch(m + 1);
+        const T *x = second ? vs : ks, *y = second ? ds : qs, *z = second ? qs : ds;
+        f32x4 acc[C::CT][C::NT];
+        if (singly) {
+            T *out = second ? dk.base : dv.base;
+            const int64_t ply = second ? dk.ply : dv.ply;
+            const int dim = second ? a.kd : a.vd;
+            ch.singly(x, y, z, gm, [&](int i, int c, float value) {
+                const int j = ch.c0 + 16 * c + ch.lc;
+                if (ch.g == 0 && j < dim) out[(t0 + i) * ply + j] = from_float<T>(value);
             });
-            for (int x = threadIdx.x; x < CH * PLD; x += C::THREADS) p1[x] = T(0.f);
-        } else {
-            f32x4 o1[NT], o2[NT];
-            ch.template scores<2>({ks, vs}, {qs, ds}, {p1, p2}, mk, a.in_scale);
-            ch.inter(ks, mk, 1.f, o1);
-            ch.inter_turned(turned, vs, mk, 1.f, o2);
             __syncthreads();
-            ch.template apply<true, true>(qs, ds, p1, mk, o1);
-            ch.template apply<true, false>(nullptr, qs, p2, mk, o2);
-            dv.put(t0, n, ch.lc, 16 * ch.w + 4 * ch.g, o1);
-            dk.put(t0, n, ch.lc, 16 * ch.w + 4 * ch.g, o2);
+        } else {
+            ch.template run<true>(x, y, z, gm, acc);
+            __syncthreads();
+            T *to = second ? ks : vs;   // the tiles that this thread's next rows replace
+#pragma unroll
+            for (int c = 0; c < C::CT; ++c)
+#pragma unroll
+                for (int it = 0; it < C::NT; ++it)
+                    store4(to + (16 * it + ch.lc) * LD + ch.c0 + 16 * c + 4 * ch.g, acc[c][it]);
+            __syncthreads();
+            dv.store(t0, gm.n, vs);
+            dk.store(t0, gm.n, ks);
         }
-        ch.turn(turned);
-        __syncthreads();
     }
-    dv.clear(max(s0, len), s1);
-    dk.clear(max(s0, len), s1);
-    if (a.s_out && seg == 0) ch.store_state(a.s_out + blockIdx.x * size, a.kd, a.vd, a.vd, 1);
+    dv.clear(sg.end, sg.s1);
+    dk.clear(sg.end, sg.s1);
+    if (a.s_out && sg.seg == 0 && !second) ch.store_state(a.s_out + blockIdx.x * size, a.kd, a.vd, a.vd, 1);
 }
 
 // What the segments leave, in their order: seg_states[g] becomes the state before

@@ -89,7 +89,7 @@ int launch_states(const ScanArgs &s, hipStream_t stream)
 {
     const int heads = s.batch * s.heads;
     if (s.segments < 2) return JQ_OK;
-    hipLaunchKernelGGL((k_attention_pass<T, D, REV, FAST, false>), dim3(heads, s.segments - 1), dim3(4 * D), 0, stream, s);
+    hipLaunchKernelGGL((k_attention_pass<T, D, REV, FAST, false>), dim3(heads, s.segments - 1), dim3(64 * pass_waves(D)), 0, stream, s);
     TRY(launch_check("k_attention_pass (states)"));
     hipLaunchKernelGGL(k_attention_join<REV>, dim3(heads, (s.kd * s.vd + 255) / 256), dim3(256), 0, stream, s);
     return launch_check("k_attention_join");
@@ -100,7 +100,7 @@ int launch_forward(const ScanArgs &s, hipStream_t stream)
 {
     TRY((launch_states<T, D, false, FAST>(s, stream)));
     const int heads = s.batch * s.heads;
-    hipLaunchKernelGGL((k_attention_pass<T, D, false, FAST, true>), dim3(heads, s.segments), dim3(4 * D), 0, stream, s);
+    hipLaunchKernelGGL((k_attention_pass<T, D, false, FAST, true>), dim3(heads, s.segments), dim3(64 * pass_waves(D)), 0, stream, s);
     return launch_check("k_attention_pass");
 }
 
@@ -108,11 +108,8 @@ template <class T, int D, bool FAST>
 int launch_kv(const GradArgs &g, hipStream_t stream)
 {
     TRY((launch_states<T, D, true, FAST>(g.scan, stream)));
-    const auto kernel = k_attention_kv<T, D, FAST>;
-    if (kv_lds<T, D>() > 48 * 1024 &&
-        hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kv_lds<T, D>()) != hipSuccess)
-        return fail(JQ_E_HIP, "k_attention_kv: %d bytes of LDS are refused", kv_lds<T, D>());
-    hipLaunchKernelGGL(kernel, dim3(g.scan.batch * g.scan.heads, g.scan.segments), dim3(4 * D), (kv_lds<T, D>()), stream, g);
+    hipLaunchKernelGGL((k_attention_kv<T, D, FAST>), dim3(g.scan.batch * g.scan.heads, g.scan.segments),
+                       dim3(128 * pass_waves(D)), 0, stream, g);
     return launch_check("k_attention_kv");
 }
 
@@ -121,14 +118,14 @@ template <class T>
 bool all_whole(std::initializer_list<std::pair<const jq_rows *, int>> rows, size_t bytes)
 {
     for (const auto &r : rows)
-        if (!whole_vectors(*r.first, r.second, sizeof(T), bytes, Mma<T>::CH)) return false;
+        if (!whole_vectors(*r.first, r.second, sizeof(T), bytes, Mma<T>::KB)) return false;
     return true;
 }
 
 template <class T, int D>
 int scan_width(const ScanArgs &s, hipStream_t stream)
 {
-    const bool fast = all_whole<T>({{&s.q, s.kd}, {&s.k, s.kd}, {&s.v, s.vd}}, 16) && all_whole<T>({{&s.o, s.vd}}, 4 * sizeof(T));
+    const bool fast = all_whole<T>({{&s.q, s.kd}, {&s.k, s.kd}, {&s.v, s.vd}}, 16) && all_whole<T>({{&s.o, s.vd}}, 16);
     return fast ? launch_forward<T, D, true>(s, stream) : launch_forward<T, D, false>(s, stream);
 }
 
@@ -137,7 +134,7 @@ int kv_width(const GradArgs &g, hipStream_t stream)
 {
     const ScanArgs &s = g.scan;
     const bool fast = all_whole<T>({{&s.q, s.kd}, {&s.k, s.kd}, {&s.v, s.vd}, {&g.values, s.vd}}, 16) &&
-                      all_whole<T>({{&s.o, s.vd}, {&g.dk, s.kd}}, 4 * sizeof(T));
+                      all_whole<T>({{&s.o, s.vd}, {&g.dk, s.kd}}, 16);
     return fast ? launch_kv<T, D, true>(g, stream) : launch_kv<T, D, false>(g, stream);
 }
 
@@ -170,7 +167,7 @@ constexpr int SPLIT_BLOCKS = 1024, SPLIT_MIN_CHUNKS = 4;
 struct Split { int segments, seg_plies; };
 Split split_of(const jq_attention *a)
 {
-    const int ch = a->dtype == JQ_F32 ? Mma<float>::CH : Mma<bf16>::CH;
+    const int ch = a->dtype == JQ_F32 ? Mma<float>::KB : Mma<bf16>::KB;
     const int64_t heads = std::max<int64_t>(1, (int64_t)a->batch * a->heads), chunks = ((int64_t)a->plies + ch - 1) / ch;
     const int64_t want = std::min(SPLIT_BLOCKS / heads, chunks / SPLIT_MIN_CHUNKS);
     if (want < 2) return {1, (int)std::max<int64_t>(chunks, 1) * ch};
