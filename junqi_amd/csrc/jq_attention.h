@@ -34,6 +34,7 @@ struct ScanArgs {
     // what a segment leaves of it
     int segments, seg_plies;
     float *seg_states, *seg_carry;
+    int seg_row, seg_col;              // strides of a seg_states' element
 };
 
 // ---- products of 16 x 16 tiles -------------------------------------------------
@@ -153,7 +154,7 @@ struct Games {
 // D = 64, so that nothing waits for another wave; for D = 128 the state's registers
 // go over four, which each compute P for themselves. Chunks have the depth of one
 // fragment: P, as it comes out of its product, is the next product's operand.
-constexpr int pass_waves(int dim) { return dim / 32; }
+constexpr int pass_waves(int dim) { return dim == 128 ? 8 : dim / 32; }
 template <class T, int D, bool REV>
 struct Chunk {
     using M = Mma<T>;
@@ -249,19 +250,27 @@ struct Chunk {
         }
         Frag p[NT];
         if constexpr (OUT) {
-            Frag x[NT][D / KB];
+            // P's products, and what the state before the chunk answers, a depth of q at a time
+            f32x4 acc[NT][NT];   // [it][jt]
 #pragma unroll
-            for (int it = 0; it < NT; ++it)
+            for (int it = 0; it < NT; ++it) {
 #pragma unroll
-                for (int c = 0; c < D / KB; ++c) x[it][c] = M::row(q + (16 * it + lc) * LD + c * KB, g);
-            scores(x, k, gm, p);
-            // what the state before the chunk answers
+                for (int jt = 0; jt < NT; ++jt) acc[it][jt] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int c = 0; c < CT; ++c)
+                for (int c = 0; c < CT; ++c) o[c][it] = f32x4{0.f, 0.f, 0.f, 0.f};
+            }
 #pragma unroll
-                for (int it = 0; it < NT; ++it) o[c][it] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int d = 0; d < D / KB; ++d) {
+                Frag x[NT];
 #pragma unroll
-            for (int d = 0; d < D / KB; ++d)
+                for (int it = 0; it < NT; ++it) x[it] = M::row(q + (16 * it + lc) * LD + d * KB, g);
+#pragma unroll
+                for (int jt = 0; jt < NT; ++jt) {
+                    const Frag y = M::row(k + (16 * jt + lc) * LD + d * KB, g);
+#pragma unroll
+                    for (int it = 0; it < NT; ++it)
+                        if (REV ? jt >= it : jt <= it) acc[it][jt] = M::mul(y, x[it], acc[it][jt]);
+                }
 #pragma unroll
                 for (int c = 0; c < CT; ++c) {
                     constexpr int N = PARTS<T, 2>;
@@ -271,10 +280,12 @@ struct Chunk {
                     for (int e = 0; e < FE; ++e) y[e] = s[(d * KB + 4 * e) / 16][c][e & 3];
                     M::template split<N>(y, part);
 #pragma unroll
-                    for (int it = 0; it < NT; ++it)
+                    for (int u = 0; u < N; ++u)   // no product waits for the one just before it
 #pragma unroll
-                        for (int u = 0; u < N; ++u) o[c][it] = M::mul(part[u], x[it][d], o[c][it]);
+                        for (int it = 0; it < NT; ++it) o[c][it] = M::mul(part[u], x[it], o[c][it]);
                 }
+            }
+            weigh(acc, gm, p);
             if (!whole) {   // a state that is not seen may hold NaN
                 int lc_ = lc;
                 asm volatile("" : "+v"(lc_));
@@ -308,43 +319,37 @@ struct Chunk {
 #pragma unroll
                     for (int r = 0; r < 4; ++r) s[t][c][r] *= carry;
         }
+        Frag x[CT], part[CT][PARTS<T, 3>];
 #pragma unroll
         for (int c = 0; c < CT; ++c) {
-            const Frag x = M::col(v + c0 + 16 * c, LD, l);
-            if constexpr (OUT)
-#pragma unroll
-                for (int it = 0; it < NT; ++it) o[c][it] = M::mul(x, p[it], o[c][it]);
-            constexpr int N = PARTS<T, 3>;
-            Frag part[N];
+            x[c] = M::col(v + c0 + 16 * c, LD, l);
             float y[FE];
 #pragma unroll
-            for (int e = 0; e < FE; ++e) y[e] = (float)x[e] * leave[e];
-            M::template split<N>(y, part);
-#pragma unroll
-            for (int t = 0; t < KT; ++t) {
-                const Frag z = M::col(k + 16 * t, LD, l);
-#pragma unroll
-                for (int u = 0; u < N; ++u) s[t][c] = M::mul(z, part[u], s[t][c]);
-            }
+            for (int e = 0; e < FE; ++e) y[e] = (float)x[c][e] * leave[e];
+            M::template split<PARTS<T, 3>>(y, part[c]);
         }
+#pragma unroll
+        for (int t = 0; t < KT; t += 2) {
+            const Frag z0 = M::col(k + 16 * t, LD, l), z1 = M::col(k + 16 * t + 16, LD, l);
+#pragma unroll
+            for (int u = 0; u < PARTS<T, 3>; ++u)
+#pragma unroll
+                for (int c = 0; c < CT; ++c) {
+                    s[t][c] = M::mul(z0, part[c][u], s[t][c]);
+                    s[t + 1][c] = M::mul(z1, part[c][u], s[t + 1][c]);
+                }
+        }
+        if constexpr (OUT)
+#pragma unroll
+            for (int it = 0; it < NT; ++it)
+#pragma unroll
+                for (int c = 0; c < CT; ++c) o[c][it] = M::mul(x[c], p[it], o[c][it]);
     }
 
-    // p[it] = P's columns i = 16it + l % 16 as an operand over the plies j, times the scales.
-    __device__ __forceinline__ void scores(const Frag (&x)[NT][D / KB], const T *k, const Games &gm, Frag (&p)[NT]) const
+    // p[it] = P's columns i = 16it + l % 16 as an operand over the plies j, times the
+    // scales, from its products.
+    __device__ __forceinline__ void weigh(f32x4 (&acc)[NT][NT], const Games &gm, Frag (&p)[NT]) const
     {
-        f32x4 acc[NT][NT];   // [it][jt]
-#pragma unroll
-        for (int jt = 0; jt < NT; ++jt) {
-#pragma unroll
-            for (int it = 0; it < NT; ++it) acc[it][jt] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int c = 0; c < D / KB; ++c) {
-                const Frag y = M::row(k + (16 * jt + lc) * LD + c * KB, g);
-#pragma unroll
-                for (int it = 0; it < NT; ++it)
-                    if (REV ? jt >= it : jt <= it) acc[it][jt] = M::mul(y, x[it][c], acc[it][jt]);
-            }
-        }
         // a ply that is not seen leaves 0, whatever its product is
 #pragma unroll
         for (int it = 0; it < NT; ++it)
@@ -451,9 +456,12 @@ struct Plies {
     static constexpr int N = Vec<T>::N, PER_ROW = D / N, CH = Mma<T>::KB, LD = D + N;
     static constexpr int NV = CH * PER_ROW / THREADS, ROWS = THREADS / PER_ROW;   // vectors of a thread, ROWS rows apart
     static_assert(NV * ROWS == CH, "a tile is NV vectors a thread");
+    static constexpr int STREAM = 2;   // non-temporal: each row passes once (1,024 x 256 plies forward 178 -> 168 us, backward's 304 -> 296)
     T *base;
     int64_t ply;
     int dim;
+
+    static __device__ __forceinline__ int me() { return threadIdx.x % THREADS; }   // a block's halves read different tiles
 
     __device__ __forceinline__ Plies(const jq_rows &r, int b, int h, int dim_) : base(row_at<T>(r, b, 0, h)), ply(r.ply), dim(dim_) {}
 
@@ -464,10 +472,10 @@ struct Plies {
     // byte offset of this thread's first vector in a chunk; past any bound where it is beside the row
     __device__ __forceinline__ int first() const
     {
-        const int row = threadIdx.x / PER_ROW, c = threadIdx.x % PER_ROW * N;
+        const int row = me() / PER_ROW, c = me() % PER_ROW * N;
         return c < dim ? (row * (int)ply + c) * (int)sizeof(T) : INT32_MIN;
     }
-    __device__ __forceinline__ int step() const { return threadIdx.x % PER_ROW * N < dim ? ROWS * (int)ply * (int)sizeof(T) : 0; }
+    __device__ __forceinline__ int step() const { return me() % PER_ROW * N < dim ? ROWS * (int)ply * (int)sizeof(T) : 0; }
 
     // this thread's vectors of the tile of plies t0 .. t0 + n; zeros elsewhere
     __device__ __forceinline__ void load(int t0, int n, V (&x)[NV]) const
@@ -478,9 +486,9 @@ struct Plies {
             const int by = step();
 #pragma unroll
             for (int u = 0; u < NV; ++u, at += by)
-                x[u] = __builtin_bit_cast(V, __builtin_amdgcn_raw_buffer_load_b128(r, at, 0, 0));
+                x[u] = __builtin_bit_cast(V, __builtin_amdgcn_raw_buffer_load_b128(r, at, 0, STREAM));
         } else {
-            const int row = threadIdx.x / PER_ROW, c = threadIdx.x % PER_ROW * N;
+            const int row = me() / PER_ROW, c = me() % PER_ROW * N;
 #pragma unroll
             for (int u = 0; u < NV; ++u) {
                 x[u] = V{};
@@ -493,16 +501,17 @@ struct Plies {
     // a tile in LDS out to plies t0 .. t0 + n
     __device__ __forceinline__ void store(int t0, int n, const T *lds) const
     {
-        const T *p = lds + threadIdx.x / PER_ROW * LD + threadIdx.x % PER_ROW * N;
+        const T *p = lds + me() / PER_ROW * LD + me() % PER_ROW * N;
         if constexpr (FAST) {
             const __amdgpu_buffer_rsrc_t r = chunk(t0, n);
             int at = first();
             const int by = step();
 #pragma unroll
             for (int u = 0; u < NV; ++u, at += by)
-                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, *reinterpret_cast<const V *>(p + u * ROWS * LD)), r, at, 0, 0);
+                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, *reinterpret_cast<const V *>(p + u * ROWS * LD)), r, at, 0,
+                                                       STREAM);
         } else {
-            const int row = threadIdx.x / PER_ROW, c = threadIdx.x % PER_ROW * N;
+            const int row = me() / PER_ROW, c = me() % PER_ROW * N;
 #pragma unroll
             for (int u = 0; u < NV; ++u)
 #pragma unroll
@@ -513,13 +522,13 @@ struct Plies {
     // zeros from ply t0 to t1
     __device__ __forceinline__ void clear(int t0, int t1) const
     {
-        for (int t = t0 + (int)(threadIdx.x >> 6); t < t1; t += THREADS / 64)
-            for (int c = threadIdx.x & 63; c < dim; c += 64) base[t * ply + c] = from_float<T>(0.f);
+        for (int t = t0 + me() / 64; t < t1; t += THREADS / 64)
+            for (int c = me() % 64; c < dim; c += 64) base[t * ply + c] = from_float<T>(0.f);
     }
     // a thread's vectors of a tile into LDS
     static __device__ __forceinline__ void stage(T *lds, const V (&x)[NV])
     {
-        T *p = lds + threadIdx.x / PER_ROW * LD + threadIdx.x % PER_ROW * N;
+        T *p = lds + me() / PER_ROW * LD + me() % PER_ROW * N;
 #pragma unroll
         for (int u = 0; u < NV; ++u) *reinterpret_cast<V *>(p + u * ROWS * LD) = x[u];
     }
@@ -562,7 +571,7 @@ __global__ __launch_bounds__(64 * pass_waves(D), 2) void k_attention_pass(ScanAr
     const int64_t size = (int64_t)a.kd * a.vd;
     float *slot = a.seg_states + ((int64_t)blockIdx.x * a.segments + sg.seg) * size;
     if (!OUT) ch.load_state(nullptr, 0, 0, 0, 0);
-    else if (a.segments > 1) ch.load_state(slot, a.kd, a.vd, a.vd, 1);
+    else if (a.segments > 1) ch.load_state(slot, a.kd, a.vd, a.seg_row, a.seg_col);
     else ch.load_state(a.s_in ? a.s_in + blockIdx.x * size : nullptr, a.kd, a.vd, a.s_row, a.s_col);
     const P q(a.q, sg.b, sg.h, a.kd), k(a.k, sg.b, sg.h, a.kd), v(a.v, sg.b, sg.h, a.vd), o(a.o, sg.b, sg.h, a.vd);
     const uint8_t *starts = a.starts ? a.starts + sg.b * a.starts_batch : nullptr;

@@ -95,12 +95,11 @@ int launch_states(const ScanArgs &s, hipStream_t stream)
     return launch_check("k_attention_join");
 }
 
-template <class T, int D, bool FAST>
-int launch_forward(const ScanArgs &s, hipStream_t stream)
+template <class T, int D, bool REV, bool FAST>
+int launch_pass(const ScanArgs &s, hipStream_t stream)
 {
-    TRY((launch_states<T, D, false, FAST>(s, stream)));
-    const int heads = s.batch * s.heads;
-    hipLaunchKernelGGL((k_attention_pass<T, D, false, FAST, true>), dim3(heads, s.segments), dim3(64 * pass_waves(D)), 0, stream, s);
+    hipLaunchKernelGGL((k_attention_pass<T, D, REV, FAST, true>), dim3(s.batch * s.heads, s.segments),
+                       dim3(64 * pass_waves(D)), 0, stream, s);
     return launch_check("k_attention_pass");
 }
 
@@ -108,9 +107,20 @@ template <class T, int D, bool FAST>
 int launch_kv(const GradArgs &g, hipStream_t stream)
 {
     TRY((launch_states<T, D, true, FAST>(g.scan, stream)));
-    hipLaunchKernelGGL((k_attention_kv<T, D, FAST>), dim3(g.scan.batch * g.scan.heads, g.scan.segments),
-                       dim3(128 * pass_waves(D)), 0, stream, g);
-    return launch_check("k_attention_kv");
+    if constexpr (D == 128) {
+        // both passes' waves in one block would have half the registers that they need
+        TRY((launch_pass<T, D, true, FAST>(g.scan, stream)));
+        ScanArgs s = g.scan;
+        s.q = g.values, s.k = g.scan.v, s.v = g.scan.k, s.o = g.dk;
+        s.kd = g.scan.vd, s.vd = g.scan.kd;
+        s.s_row = 1, s.s_col = s.kd, s.s_out = nullptr;
+        s.seg_row = 1, s.seg_col = s.kd;
+        return launch_pass<T, D, true, FAST>(s, stream);
+    } else {
+        hipLaunchKernelGGL((k_attention_kv<T, D, FAST>), dim3(g.scan.batch * g.scan.heads, g.scan.segments),
+                           dim3(128 * pass_waves(D)), 0, stream, g);
+        return launch_check("k_attention_kv");
+    }
 }
 
 // Whether a pass may take all of these as whole vectors.
@@ -126,7 +136,12 @@ template <class T, int D>
 int scan_width(const ScanArgs &s, hipStream_t stream)
 {
     const bool fast = all_whole<T>({{&s.q, s.kd}, {&s.k, s.kd}, {&s.v, s.vd}}, 16) && all_whole<T>({{&s.o, s.vd}}, 16);
-    return fast ? launch_forward<T, D, true>(s, stream) : launch_forward<T, D, false>(s, stream);
+    if (fast) {
+        TRY((launch_states<T, D, false, true>(s, stream)));
+        return launch_pass<T, D, false, true>(s, stream);
+    }
+    TRY((launch_states<T, D, false, false>(s, stream)));
+    return launch_pass<T, D, false, false>(s, stream);
 }
 
 template <class T, int D>
@@ -162,14 +177,18 @@ int scan_kv(int32_t dtype, const GradArgs &g, hipStream_t stream)
 }
 
 // How a call's plies are split: few games and heads leave the card idle unless
-// parts of a long axis run side by side.
-constexpr int SPLIT_BLOCKS = 1024, SPLIT_MIN_CHUNKS = 4;
+// parts of a long axis run side by side, at the price of reading k and v twice and of
+// the states between. As many segments as make SPLIT_WAVES waves: 2 x 65,537 plies of
+// 8 heads of 128 in 2,048 / 4,096 / 8,192 / 16,384 waves 692 / 678 / 708 / 755 us of
+// kernels, unsplit 13,900.
+constexpr int SPLIT_WAVES = 4096, SPLIT_MIN_CHUNKS = 4;
 struct Split { int segments, seg_plies; };
 Split split_of(const jq_attention *a)
 {
-    const int ch = a->dtype == JQ_F32 ? Mma<float>::KB : Mma<bf16>::KB;
+    const int ch = a->dtype == JQ_F32 ? Mma<float>::KB : Mma<bf16>::KB, dim = std::max(a->key_dim, a->value_dim);
+    const int waves = pass_waves(dim <= 32 ? 32 : dim <= 64 ? 64 : 128);
     const int64_t heads = std::max<int64_t>(1, (int64_t)a->batch * a->heads), chunks = ((int64_t)a->plies + ch - 1) / ch;
-    const int64_t want = std::min(SPLIT_BLOCKS / heads, chunks / SPLIT_MIN_CHUNKS);
+    const int64_t want = std::min(SPLIT_WAVES / (heads * waves), chunks / SPLIT_MIN_CHUNKS);
     if (want < 2) return {1, (int)std::max<int64_t>(chunks, 1) * ch};
     const int64_t each = (chunks + want - 1) / want;
     return {(int)((chunks + each - 1) / each), (int)each * ch};
@@ -195,6 +214,7 @@ ScanArgs scan_args(const jq_attention *a)
     s.starts_ply = a->starts_ply;
     s.lengths = a->lengths;
     s.in_scale = s.out_scale = 1.f;
+    s.seg_col = 1;
     const Split split = split_of(a);
     s.segments = split.segments;
     s.seg_plies = split.seg_plies;
@@ -353,6 +373,7 @@ int jq_attention_forward(const jq_attention *a, void *stream)
     s.kd = a->key_dim, s.vd = a->value_dim;
     s.s_in = a->initial_state, s.s_out = a->final_state, s.s_row = a->value_dim, s.s_col = 1;
     s.out_scale = a->scale;
+    s.seg_row = s.vd;
     return scan(a->dtype, s, strm(stream));
 }
 
@@ -371,6 +392,7 @@ int jq_attention_backward(const jq_attention *a, void *stream)
         s.q = a->d_out, s.k = a->v, s.v = a->k, s.o = a->dq;
         s.kd = a->value_dim, s.vd = a->key_dim;
         s.s_in = a->initial_state, s.s_row = 1, s.s_col = a->value_dim;
+        s.seg_row = s.vd;
         s.out_scale = a->scale;
         TRY(scan(a->dtype, s, strm(stream)));
     }
@@ -385,6 +407,7 @@ int jq_attention_backward(const jq_attention *a, void *stream)
         s.q = a->k, s.k = a->q, s.v = a->d_out, s.o = a->dv;
         s.kd = a->key_dim, s.vd = a->value_dim;
         s.s_in = a->d_final, s.s_out = a->d_initial, s.s_row = a->value_dim, s.s_col = 1;
+        s.seg_row = s.vd;
         TRY(scan_kv(a->dtype, g, strm(stream)));
     }
     return JQ_OK;
