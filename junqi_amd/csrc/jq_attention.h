@@ -35,6 +35,7 @@ struct ScanArgs {
     int segments, seg_plies;
     float *seg_states, *seg_carry;
     int seg_row, seg_col;              // strides of a seg_states' element
+    bool stream;                       // the rows go past the caches
 };
 
 // ---- products of 16 x 16 tiles -------------------------------------------------
@@ -456,14 +457,17 @@ struct Plies {
     static constexpr int N = Vec<T>::N, PER_ROW = D / N, CH = Mma<T>::KB, LD = D + N;
     static constexpr int NV = CH * PER_ROW / THREADS, ROWS = THREADS / PER_ROW;   // vectors of a thread, ROWS rows apart
     static_assert(NV * ROWS == CH, "a tile is NV vectors a thread");
-    static constexpr int STREAM = 2;   // non-temporal: each row passes once (1,024 x 256 plies forward 178 -> 168 us, backward's 304 -> 296)
     T *base;
     int64_t ply;
     int dim;
+    bool stream;   // past the caches
 
     static __device__ __forceinline__ int me() { return threadIdx.x % THREADS; }   // a block's halves read different tiles
 
-    __device__ __forceinline__ Plies(const jq_rows &r, int b, int h, int dim_) : base(row_at<T>(r, b, 0, h)), ply(r.ply), dim(dim_) {}
+    __device__ __forceinline__ Plies(const jq_rows &r, int b, int h, int dim_, bool stream_)
+        : base(row_at<T>(r, b, 0, h)), ply(r.ply), dim(dim_), stream(stream_)
+    {
+    }
 
     __device__ __forceinline__ __amdgpu_buffer_rsrc_t chunk(int t0, int n) const
     {
@@ -484,9 +488,14 @@ struct Plies {
             const __amdgpu_buffer_rsrc_t r = chunk(t0, n);
             int at = first();
             const int by = step();
+            if (stream)
 #pragma unroll
-            for (int u = 0; u < NV; ++u, at += by)
-                x[u] = __builtin_bit_cast(V, __builtin_amdgcn_raw_buffer_load_b128(r, at, 0, STREAM));
+                for (int u = 0; u < NV; ++u, at += by)
+                    x[u] = __builtin_bit_cast(V, __builtin_amdgcn_raw_buffer_load_b128(r, at, 0, 2));
+            else
+#pragma unroll
+                for (int u = 0; u < NV; ++u, at += by)
+                    x[u] = __builtin_bit_cast(V, __builtin_amdgcn_raw_buffer_load_b128(r, at, 0, 0));
         } else {
             const int row = me() / PER_ROW, c = me() % PER_ROW * N;
 #pragma unroll
@@ -506,10 +515,17 @@ struct Plies {
             const __amdgpu_buffer_rsrc_t r = chunk(t0, n);
             int at = first();
             const int by = step();
+            V y[NV];
 #pragma unroll
-            for (int u = 0; u < NV; ++u, at += by)
-                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, *reinterpret_cast<const V *>(p + u * ROWS * LD)), r, at, 0,
-                                                       STREAM);
+            for (int u = 0; u < NV; ++u) y[u] = *reinterpret_cast<const V *>(p + u * ROWS * LD);
+            if (stream)
+#pragma unroll
+                for (int u = 0; u < NV; ++u, at += by)
+                    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, y[u]), r, at, 0, 2);
+            else
+#pragma unroll
+                for (int u = 0; u < NV; ++u, at += by)
+                    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, y[u]), r, at, 0, 0);
         } else {
             const int row = me() / PER_ROW, c = me() % PER_ROW * N;
 #pragma unroll
@@ -573,7 +589,7 @@ __global__ __launch_bounds__(64 * pass_waves(D), 2) void k_attention_pass(ScanAr
     if (!OUT) ch.load_state(nullptr, 0, 0, 0, 0);
     else if (a.segments > 1) ch.load_state(slot, a.kd, a.vd, a.seg_row, a.seg_col);
     else ch.load_state(a.s_in ? a.s_in + blockIdx.x * size : nullptr, a.kd, a.vd, a.s_row, a.s_col);
-    const P q(a.q, sg.b, sg.h, a.kd), k(a.k, sg.b, sg.h, a.kd), v(a.v, sg.b, sg.h, a.vd), o(a.o, sg.b, sg.h, a.vd);
+    const P q(a.q, sg.b, sg.h, a.kd, a.stream), k(a.k, sg.b, sg.h, a.kd, a.stream), v(a.v, sg.b, sg.h, a.vd, a.stream), o(a.o, sg.b, sg.h, a.vd, a.stream);
     const uint8_t *starts = a.starts ? a.starts + sg.b * a.starts_batch : nullptr;
     if (WAVES > 1) {
         if (threadIdx.x < 2) bad[threadIdx.x] = 0;
@@ -667,8 +683,8 @@ __global__ __launch_bounds__(128 * pass_waves(D), 2) void k_attention_kv(GradArg
                                        : a.s_in ? a.s_in + blockIdx.x * size : nullptr;
     if (second) ch.load_state(init, a.vd, a.kd, 1, a.vd);
     else ch.load_state(init, a.kd, a.vd, a.vd, 1);
-    const P k(a.q, sg.b, sg.h, a.kd), q(a.k, sg.b, sg.h, a.kd), d(a.v, sg.b, sg.h, a.vd), v(ga.values, sg.b, sg.h, a.vd);
-    const P dv(a.o, sg.b, sg.h, a.vd), dk(ga.dk, sg.b, sg.h, a.kd);
+    const P k(a.q, sg.b, sg.h, a.kd, a.stream), q(a.k, sg.b, sg.h, a.kd, a.stream), d(a.v, sg.b, sg.h, a.vd, a.stream), v(ga.values, sg.b, sg.h, a.vd, a.stream);
+    const P dv(a.o, sg.b, sg.h, a.vd, a.stream), dk(ga.dk, sg.b, sg.h, a.kd, a.stream);
     const uint8_t *starts = a.starts ? a.starts + sg.b * a.starts_batch : nullptr;
     if (threadIdx.x < 2) bad[threadIdx.x] = 0;
     __syncthreads();
@@ -791,7 +807,7 @@ __global__ __launch_bounds__(128) void k_attention_step(StepArgs a)
 // with all their loads on their way, and their sums are joined by shuffles: no
 // barriers, the state is read and written once.
 constexpr int STEP_ROWS = 16, STEP_WAVES = 4;
-template <class T, int L>
+template <class T, int L, bool STREAM>
 __global__ __launch_bounds__(64 * STEP_WAVES) void k_attention_step_wave(StepArgs a, int count)
 {
     const int at = blockIdx.x * STEP_WAVES + (threadIdx.x >> 6);
@@ -814,7 +830,8 @@ __global__ __launch_bounds__(64 * STEP_WAVES) void k_attention_step_wave(StepArg
 #pragma unroll
             for (int i = 0; i < STEP_ROWS; ++i) {
                 const int r = min(i0 + i, end - 1);
-                x[i] = *reinterpret_cast<const f32x4 *>(s + r * a.dv);
+                const f32x4 *at = reinterpret_cast<const f32x4 *>(s + r * a.dv);
+                x[i] = STREAM ? __builtin_nontemporal_load(at) : *at;
                 qs[i] = (float)q[r];
                 ks[i] = (float)k[r];
             }
@@ -827,7 +844,9 @@ __global__ __launch_bounds__(64 * STEP_WAVES) void k_attention_step_wave(StepArg
                     y[e] = fmaf(ks[i], v[e], start ? 0.f : lam * x[i][e]);
                     sum[e] = fmaf(qs[i], y[e], sum[e]);
                 }
-                *reinterpret_cast<f32x4 *>(s + (i0 + i) * a.dv) = y;
+                f32x4 *at = reinterpret_cast<f32x4 *>(s + (i0 + i) * a.dv);
+                if (STREAM) __builtin_nontemporal_store(y, at);
+                else *at = y;
             }
         }
     }

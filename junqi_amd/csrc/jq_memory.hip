@@ -22,6 +22,14 @@ namespace {
 
 hipStream_t strm(void *s) { return reinterpret_cast<hipStream_t>(s); }
 
+// Calls over more bytes than that go past the caches, which would not hold them to
+// their next use; what smaller ones touch is found there. One ply, 4 heads of 64 x 64
+// in bfloat16, through the caches / past them: 1,024 games (67 MB of states) 24.5 /
+// 26.0 us, 4,096 (268 MB) 83.8 / 95.8, 8,192 (537 MB) 211 / 190, 32,768 846 / 749
+// (5.7 TB/s). Segments of 256 plies, 4 heads of 64, forward, the same rows again: 512
+// games (268 MB) 56 / 64 us, 1,024 135 / 126.
+constexpr int64_t STREAM_BYTES = 400ll << 20;
+
 int check_dtype(int32_t dtype)
 {
     if (dtype != JQ_F32 && dtype != JQ_BF16) return fail(JQ_E_ARG, "element type %d is neither JQ_F32 nor JQ_BF16", dtype);
@@ -178,18 +186,20 @@ int scan_kv(int32_t dtype, const GradArgs &g, hipStream_t stream)
 
 // How a call's plies are split: few games and heads leave the card idle unless
 // parts of a long axis run side by side, at the price of reading k and v twice and of
-// the states between. As many segments as make SPLIT_WAVES waves: 2 x 65,537 plies of
-// 8 heads of 128 in 2,048 / 4,096 / 8,192 / 16,384 waves 692 / 678 / 708 / 755 us of
-// kernels, unsplit 13,900.
-constexpr int SPLIT_WAVES = 4096, SPLIT_MIN_CHUNKS = 4;
+// the states between. Below SPLIT_BELOW waves, and from four segments of
+// SPLIT_MIN_CHUNKS chunks on. Forward in bfloat16, split / in one piece: 32 games of
+// 1,024 plies and 4 heads of 64 (256 waves) 38 / 60 us, 64 games (512) 69 / 61, 128
+// games 111 / 86; 32 games of 256 plies 22 / 18; 2 x 65,537 plies of 8 heads of 128 in
+// 2,048 / 4,096 / 8,192 / 16,384 waves 692 / 678 / 708 / 755 us of kernels.
+constexpr int SPLIT_WAVES = 4096, SPLIT_BELOW = 512, SPLIT_MIN_CHUNKS = 4;
 struct Split { int segments, seg_plies; };
 Split split_of(const jq_attention *a)
 {
     const int ch = a->dtype == JQ_F32 ? Mma<float>::KB : Mma<bf16>::KB, dim = std::max(a->key_dim, a->value_dim);
-    const int waves = pass_waves(dim <= 32 ? 32 : dim <= 64 ? 64 : 128);
-    const int64_t heads = std::max<int64_t>(1, (int64_t)a->batch * a->heads), chunks = ((int64_t)a->plies + ch - 1) / ch;
-    const int64_t want = std::min(SPLIT_WAVES / (heads * waves), chunks / SPLIT_MIN_CHUNKS);
-    if (want < 2) return {1, (int)std::max<int64_t>(chunks, 1) * ch};
+    const int64_t waves = std::max<int64_t>(1, (int64_t)a->batch * a->heads) * pass_waves(dim <= 32 ? 32 : dim <= 64 ? 64 : 128);
+    const int64_t chunks = ((int64_t)a->plies + ch - 1) / ch;
+    const int64_t want = waves < SPLIT_BELOW ? std::min(SPLIT_WAVES / waves, chunks / SPLIT_MIN_CHUNKS) : 1;
+    if (want < 4) return {1, (int)std::max<int64_t>(chunks, 1) * ch};
     const int64_t each = (chunks + want - 1) / want;
     return {(int)((chunks + each - 1) / each), (int)each * ch};
 }
@@ -215,6 +225,7 @@ ScanArgs scan_args(const jq_attention *a)
     s.lengths = a->lengths;
     s.in_scale = s.out_scale = 1.f;
     s.seg_col = 1;
+    s.stream = (int64_t)a->batch * a->plies * a->heads * (a->key_dim + a->value_dim) * 2 * (int64_t)elem_bytes(a->dtype) > STREAM_BYTES;
     const Split split = split_of(a);
     s.segments = split.segments;
     s.seg_plies = split.seg_plies;
@@ -232,15 +243,23 @@ int check_workspace(const jq_attention *a)
     return JQ_OK;
 }
 
+template <class T, bool STREAM>
+void step_waves(const StepArgs &a, int count, hipStream_t stream)
+{
+    const dim3 grid((count + STEP_WAVES - 1) / STEP_WAVES), block(64 * STEP_WAVES);
+    if (a.dv <= 16) hipLaunchKernelGGL((k_attention_step_wave<T, 4, STREAM>), grid, block, 0, stream, a, count);
+    else if (a.dv <= 32) hipLaunchKernelGGL((k_attention_step_wave<T, 8, STREAM>), grid, block, 0, stream, a, count);
+    else if (a.dv <= 64) hipLaunchKernelGGL((k_attention_step_wave<T, 16, STREAM>), grid, block, 0, stream, a, count);
+    else hipLaunchKernelGGL((k_attention_step_wave<T, 32, STREAM>), grid, block, 0, stream, a, count);
+}
+
 template <class T>
 void step(const StepArgs &a, int count, hipStream_t stream)
 {
-    const dim3 grid((count + STEP_WAVES - 1) / STEP_WAVES), block(64 * STEP_WAVES);
+    const int64_t bytes = (int64_t)count * a.dk * a.dv * (int64_t)sizeof(float);
     if (a.dv % 4) hipLaunchKernelGGL(k_attention_step<T>, dim3(count), dim3(128), 0, stream, a);
-    else if (a.dv <= 16) hipLaunchKernelGGL((k_attention_step_wave<T, 4>), grid, block, 0, stream, a, count);
-    else if (a.dv <= 32) hipLaunchKernelGGL((k_attention_step_wave<T, 8>), grid, block, 0, stream, a, count);
-    else if (a.dv <= 64) hipLaunchKernelGGL((k_attention_step_wave<T, 16>), grid, block, 0, stream, a, count);
-    else hipLaunchKernelGGL((k_attention_step_wave<T, 32>), grid, block, 0, stream, a, count);
+    else if (bytes > STREAM_BYTES) step_waves<T, true>(a, count, stream);
+    else step_waves<T, false>(a, count, stream);
 }
 
 // Blocks for that much work: kernels over rows and tokens take the rest a grid's
