@@ -424,7 +424,7 @@ int jq_ids_to_mask(const int32_t *ids, const int32_t *counts, int64_t rows, int3
  * JQ_F32 and JQ_BF16; sums, statistics and states are kept in float32. Pointers
  * are device addresses, aligned to their element's size; elements of the last
  * dimension are adjacent. Launched on the current device; no call allocates,
- * keeps device memory or synchronises. */
+ * keeps device memory or synchronises. batch * heads stays below 2^23. */
 #define JQ_F32 0
 #define JQ_BF16 1
 #define JQ_ATTENTION_MAX_DIM 128   /* largest key_dim and value_dim */
@@ -468,8 +468,8 @@ int jq_attention_workspace(const jq_attention *a, int32_t backward, int64_t *byt
 int jq_attention_forward(const jq_attention *a, void *stream);
 int jq_attention_backward(const jq_attention *a, void *stream);
 /* One new ply of each of batch games: q, k, v and out as above with their ply
- * strides unused, state (float32, (state_rows, heads, key_dim, value_dim), 16-byte
- * aligned) updated in place. rows (int64, batch; NULL: row b) names each game's
+ * strides unused, state (float32, (state_rows, heads, key_dim, value_dim), best
+ * 16-byte aligned) updated in place. rows (int64, batch; NULL: row b) names each game's
  * state; a game whose row is outside [0, state_rows) is left out: its out is 0.
  * Two games with one row race. starts (uint8, batch) may be NULL. */
 int jq_attention_step(int32_t dtype, int32_t batch, int32_t heads, int32_t key_dim, int32_t value_dim, float scale,

@@ -7,7 +7,10 @@ namespace jq {
 // Rows are walked in vectors of 16 bytes by groups of G lanes: lane i of a group has
 // vectors i, i + G, ... (NV of them), so a row stays in registers between its
 // statistics and its result and is read once. Up to a wave's 64 lanes a group is
-// part of a wave and a block has several; G = 256 and 1024 are a block each.
+// part of a wave and a block has several; G = 256 and 1024 are a block each. Bound by
+// the rows' traffic: 262,144 rows of 256 in bfloat16 forward (268 MB) 62 us, backward
+// (403 MB) 93 us, 4.3 TB/s both; a wave per row that reads it three times and a
+// column's sums apart took 722 us in all, 158 now.
 constexpr int norm_block(int group) { return group > 256 ? group : 256; }
 
 template <class T, int G, int NV>

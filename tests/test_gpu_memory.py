@@ -377,6 +377,20 @@ def test_step_discards_a_bad_state(memory):
     assert out[1].isnan().all() and state[1].isnan().all()
 
 
+def test_step_of_an_unaligned_state(memory):
+    """A state whose first element is not at a 16-byte boundary, and one that is."""
+    x = _inputs(23, 4, 1, 1, 8, 8, F32, "none", "none")
+    store = torch.randn(4 * 64 + 1, generator=torch.Generator().manual_seed(1)).cuda()
+    odd, even = store[1:].view(4, 1, 8, 8), store[1:].clone().view(4, 1, 8, 8)
+    args = [x[n][:, 0] for n in ("q", "k", "v")] + [x["log_decay"]]
+    want = _define(*(_cpu(t[:, None]) for t in args[:3]), _cpu(x["log_decay"]), None, None, _cpu(even), 8 ** -0.5)
+    mag = _define(*(_cpu(t[:, None]).abs() for t in args[:3]), _cpu(x["log_decay"]), None, None, _cpu(even).abs(), 8 ** -0.5)
+    for s in (odd, even):
+        out = memory.linear_attention_step(*args, s)
+        _close("out", out, want[0][:, 0], mag[0][:, 0] * 16 * EPS)
+        _close("state", s, want[1], mag[1] * 8 * EPS)
+
+
 def test_step_of_nothing(memory):
     z = torch.empty(0, 2, 8, device="cuda")
     out = memory.linear_attention_step(z, z, z, torch.zeros(2, device="cuda"), torch.empty(0, 2, 8, 8, device="cuda"))

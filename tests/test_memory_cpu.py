@@ -62,7 +62,7 @@ def test_step_arguments(jl):
     r = jl.Rows(64, 8, 0, 8)
     ok = dict(dtype=jl.F32, batch=2, heads=1, dk=8, dv=8, scale=1.0, ld=64, q=r, k=r, v=r, out=r, state=64, n=2, rows=None, st=None)
     for over in ({"dtype": 5}, {"batch": -1}, {"heads": 0}, {"dk": 129}, {"dv": 0}, {"ld": None}, {"q": jl.Rows()}, {"n": -1},
-                 {"state": None}, {"state": 68}, {"out": jl.Rows(65)}):
+                 {"state": None}, {"state": 66}, {"out": jl.Rows(65)}):
         assert jl.lib.jq_attention_step(*{**ok, **over}.values(), None) == jl.JQ_E_ARG, over
 
 
