@@ -313,8 +313,8 @@ bool norm_shape(int width, F &&f)
 // below the rows'.
 constexpr int NORM_BLOCKS = 1024, NORM_ROWS = 4;
 // Threads of the forward pass: all that the card's CUs hold, so that a block goes over
-// many rows (262,144 rows of 256 in bfloat16 62 us; a block for every eight rows, with
-// weight and bias read again for each, 244).
+// many rows (262,144 rows of 256 in bfloat16: a block for every eight rows, with weight
+// and bias read again for each, took 244 us where this took 62, 49 since).
 constexpr int NORM_FORWARD_THREADS = 2048 * 256;
 
 template <class T>

@@ -8,9 +8,10 @@ namespace jq {
 // vectors i, i + G, ... (NV of them), so a row stays in registers between its
 // statistics and its result and is read once. Up to a wave's 64 lanes a group is
 // part of a wave and a block has several; G = 256 and 1024 are a block each. Bound by
-// the rows' traffic: 262,144 rows of 256 in bfloat16 forward (268 MB) 62 us, backward
-// (403 MB) 93 us, 4.3 TB/s both; a wave per row that reads it three times and a
-// column's sums apart took 722 us in all, 158 now.
+// the rows' traffic: 262,144 rows of 256 in bfloat16 forward (268 MB) 49 us, 5.5 TB/s,
+// backward (403 MB) 80 us, 5.0 TB/s, where a plain copy reaches 6.0. A wave per row that
+// reads it three times and a column's sums apart took 722 us in all, 136 now; sums by
+// shuffles through LDS, and rows turned to float32 as they come, 62 and 93.
 constexpr int norm_block(int group) { return group > 256 ? group : 256; }
 
 template <class T, int G, int NV>
@@ -31,11 +32,29 @@ struct NormRow {
         }
     }
 
-    __device__ __forceinline__ void load(const T *row, int width)
+    // this lane's vectors of a row as they lie in memory, and x from them: a row on its
+    // way is not waited for before it is taken
+    typedef typename Vec<T>::type Raw;
+    __device__ __forceinline__ static void fetch(const T *row, int width, Raw (&raw)[NV])
+    {
+        typedef Raw At __attribute__((aligned(sizeof(T))));   // any element alignment
+#pragma unroll
+        for (int u = 0; u < NV; ++u) raw[u] = Raw{};
+        each(width, [&](int c, int i, int n) {
+            const T *p = row + c;
+            if (n == N) raw[i / N] = *reinterpret_cast<const At *>(p);
+            else
+#pragma unroll
+                for (int e = 0; e < N; ++e) {   // without a branch for each element: their loads go out together
+                    const T y = p[e < n ? e : n - 1];
+                    raw[i / N][e] = e < n ? y : T(0.f);
+                }
+        });
+    }
+    __device__ __forceinline__ void take(const Raw (&raw)[NV])
     {
 #pragma unroll
-        for (int i = 0; i < NV * N; ++i) x[i] = 0.f;
-        each(width, [&](int c, int i, int n) { load_vec(row + c, n, x + i, 0.f); });
+        for (int i = 0; i < NV * N; ++i) x[i] = (float)raw[i / N][i % N];
     }
 
     // x = this lane's columns of p (weights), or `other` without p and past the row's end
@@ -85,11 +104,8 @@ struct NormRow {
     // the group's sums of a and b, in every lane; red: 2 * BLOCK / 64 floats of LDS
     __device__ __forceinline__ static void sum(float &a, float &b, float *red)
     {
-#pragma unroll
-        for (int o = min(G, 64) / 2; o; o >>= 1) {
-            a += __shfl_xor(a, o);
-            b += __shfl_xor(b, o);
-        }
+        a = group_total<(G < 64 ? G : 64)>(a);
+        b = group_total<(G < 64 ? G : 64)>(b);
         if constexpr (G > 64) {
             constexpr int W = G / 64;
             __syncthreads();
@@ -128,15 +144,17 @@ __global__ __launch_bounds__(norm_block(G)) void k_norm_forward(NormArgs a)
     const int64_t step = (int64_t)gridDim.x * R::GROUPS;
     int64_t r = (int64_t)blockIdx.x * R::GROUPS + threadIdx.x / G;
     if (r >= a.rows) return;   // groups of more than a wave are blocks: none waits for it
-    R row, next;
-    row.load(static_cast<const T *>(a.x) + r * a.x_stride, a.width);
+    R row;
+    typename R::Raw next[NV];
+    R::fetch(static_cast<const T *>(a.x) + r * a.x_stride, a.width, next);
     const W *w = static_cast<const W *>(a.w), *bias = static_cast<const W *>(a.bias);
     float weight[NV * N], offset[NV * N];
     R::columns(w, a.width, 1.f, weight);
     R::columns(bias, a.width, 0.f, offset);
     for (;;) {
         const int64_t then = r + step;
-        if (then < a.rows) next.load(static_cast<const T *>(a.x) + then * a.x_stride, a.width);
+        row.take(next);
+        if (then < a.rows) R::fetch(static_cast<const T *>(a.x) + then * a.x_stride, a.width, next);
         float s = 0.f, q = 0.f;
 #pragma unroll
         for (int i = 0; i < NV * N; ++i) s += row.x[i];
@@ -164,7 +182,6 @@ __global__ __launch_bounds__(norm_block(G)) void k_norm_forward(NormArgs a)
             if (a.rstd) a.rstd[r] = rstd;
         }
         if (then >= a.rows) break;
-        row = next;
         r = then;
     }
 }
@@ -183,11 +200,25 @@ __global__ __launch_bounds__(norm_block(G)) void k_norm_backward(NormArgs a)
     const W *w = static_cast<const W *>(a.w);
     float dw[NV * N] = {}, db[NV * N] = {}, weight[NV * N];
     R::columns(w, a.width, 1.f, weight);
-    for (int64_t r = (int64_t)blockIdx.x * R::GROUPS + threadIdx.x / G; r < a.rows; r += (int64_t)gridDim.x * R::GROUPS) {
-        R row, d;
-        row.load(static_cast<const T *>(a.x) + r * a.x_stride, a.width);
-        d.load(static_cast<const T *>(a.d) + r * a.d_stride, a.width);
-        const float mean = a.mean[r], rstd = a.rstd[r];
+    constexpr bool AHEAD = NV == 1;   // the next row is on its way: wider rows have no registers left for it
+    const int64_t step = (int64_t)gridDim.x * R::GROUPS;
+    R row, d;
+    typename R::Raw next[NV], next_d[NV];
+    float next_mean, next_rstd;
+    const auto fetch = [&](int64_t r) {
+        R::fetch(static_cast<const T *>(a.x) + r * a.x_stride, a.width, next);
+        R::fetch(static_cast<const T *>(a.d) + r * a.d_stride, a.width, next_d);
+        next_mean = a.mean[r];
+        next_rstd = a.rstd[r];
+    };
+    const int64_t first = (int64_t)blockIdx.x * R::GROUPS + threadIdx.x / G;
+    if (AHEAD && first < a.rows) fetch(first);
+    for (int64_t r = first; r < a.rows; r += step) {
+        if (!AHEAD) fetch(r);
+        row.take(next);
+        d.take(next_d);
+        const float mean = next_mean, rstd = next_rstd;
+        if (AHEAD && r + step < a.rows) fetch(r + step);
         float s1 = 0.f, s2 = 0.f;
 #pragma unroll
         for (int i = 0; i < NV * N; ++i) {   // past the row's end d is 0
@@ -226,6 +257,7 @@ __global__ __launch_bounds__(norm_block(G)) void k_norm_backward(NormArgs a)
                 for (int e = 0; e < N; ++e) join[threadIdx.x * N + e] = y[e];
                 __syncthreads();
                 if (threadIdx.x >= G) continue;
+#pragma unroll (R::GROUPS > 8 ? 8 : 1)   // all at once would take the registers of waves that the rows need
                 for (int g = 1; g < R::GROUPS; ++g)
 #pragma unroll
                     for (int e = 0; e < N; ++e) y[e] += join[(g * G + threadIdx.x) * N + e];
