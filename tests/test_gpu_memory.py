@@ -548,6 +548,22 @@ def test_norm(memory, dtype, wdtype, lead, width):
         assert torch.equal(memory.layer_norm(x, w, b), out)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows,width", [(2500, 2001), (5, 3001), (6, 12001), (4100, 129), (700, 500)])
+def test_norm_widths(memory, dtype, rows, width):
+    """Rows held by every shape of a block, ends inside a vector; more rows than groups."""
+    g = torch.Generator().manual_seed(width)
+    x = (torch.randn(rows, width, generator=g) * 2 + 0.7).to(dtype).cuda().requires_grad_()
+    w = (1 + torch.randn(width, generator=g) * 0.2).cuda().requires_grad_()
+    b = (torch.randn(width, generator=g) * 0.2).cuda().requires_grad_()
+    d = torch.randn(rows, width, generator=g).to(dtype).cuda()
+    out = memory.layer_norm(x, w, b)
+    want = _normed(x, w, b, 1e-5, d)
+    bounds = _norm_bounds(x, w, b, 1e-5, d)
+    for i, (name, got) in enumerate(zip(("out", "dx", "dweight", "dbias"), (out, *torch.autograd.grad(out, (x, w, b), d)))):
+        _close(name, got, want[i], bounds[i])
+
+
 def test_norm_forms(memory):
     """Without weight or bias; row views; rows that are all the same; large offsets."""
     g = torch.Generator().manual_seed(3)
