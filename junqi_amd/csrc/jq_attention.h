@@ -786,52 +786,32 @@ struct StepArgs {
     const uint8_t *starts;
 };
 
-// One ply of every game, for states that are not whole aligned vectors: one block
-// per game and head, one thread per column.
-template <class T>
-__global__ __launch_bounds__(128) void k_attention_step(StepArgs a)
-{
-    const int b = blockIdx.x / a.heads, h = blockIdx.x % a.heads, c = threadIdx.x;
-    if (c >= a.dv) return;
-    T *o = row_at<T>(a.o, b, 0, h);
-    const int64_t row = a.rows ? a.rows[b] : b;
-    if (row < 0 || row >= a.state_rows) {
-        o[c] = from_float<T>(0.f);
-        return;
-    }
-    float *s = a.state + (row * a.heads + h) * a.dk * a.dv;
-    const T *q = row_at<const T>(a.q, b, 0, h), *k = row_at<const T>(a.k, b, 0, h);
-    const float v = (float)row_at<const T>(a.v, b, 0, h)[c], lam = expf(a.log_decay[h]);
-    const bool start = a.starts && a.starts[b];
-    float sum = 0.f;
-    for (int i = 0; i < a.dk; ++i) {
-        const float x = (start ? 0.f : lam * s[i * a.dv + c]) + (float)k[i] * v;
-        s[i * a.dv + c] = x;
-        sum += (float)q[i] * x;
-    }
-    o[c] = from_float<T>(a.scale * sum);
-}
-
-// The same with a wave for each game and head. L lanes hold a row's columns, four
-// each; the 64 / L groups of lanes take a part of the rows each, STEP_ROWS at a time
+// One ply of every game, a wave for each game and head. L lanes hold a row's columns,
+// four each (ODD: rows that are not whole vectors, the last lane with what is left);
+// the 64 / L groups of lanes take a part of the rows each, STEP_ROWS at a time
 // with all their loads on their way, and their sums are joined by shuffles: no
 // barriers, the state is read and written once. Bound by that: 32,768 games of 4 heads
-// of 64 x 64 (4.36 GB) in 744 us, 5.9 TB/s (one thread per column: 1,858).
+// of 64 x 64 (4.36 GB) in 744 us, 5.9 TB/s (one thread per column: 1,858);
+// 4,693 games of 4 heads of 50 x 50 in float32 (390 MB) in 66 us (284).
 constexpr int STEP_ROWS = 16, STEP_WAVES = 4;
-template <class T, int L, bool STREAM>
+template <class T, int L, bool STREAM, bool ODD>
 __global__ __launch_bounds__(64 * STEP_WAVES) void k_attention_step_wave(StepArgs a, int count)
 {
+    typedef f32x4 At __attribute__((aligned(4)));   // states lie at any alignment of their elements
     const int at = blockIdx.x * STEP_WAVES + (threadIdx.x >> 6);
     if (at >= count) return;
     const int b = at / a.heads, h = at % a.heads, l = threadIdx.x & 63, c = 4 * (l % L), g = l / L;
     const bool on = c < a.dv;
+    const int n = ODD ? min(4, a.dv - c) : 4;   // columns of this lane
     const int64_t row = a.rows ? a.rows[b] : b;
     const bool live = row >= 0 && row < a.state_rows;
     f32x4 sum{0.f, 0.f, 0.f, 0.f};
     if (live && on) {
         float *s = a.state + (row * a.heads + h) * a.dk * a.dv + c;
         const T *q = row_at<const T>(a.q, b, 0, h), *k = row_at<const T>(a.k, b, 0, h), *vp = row_at<const T>(a.v, b, 0, h) + c;
-        const f32x4 v{(float)vp[0], (float)vp[1], (float)vp[2], (float)vp[3]};
+        f32x4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = (float)vp[min(e, n - 1)];
         const float lam = expf(a.log_decay[h]);
         const bool start = a.starts && a.starts[b];
         const int each = (a.dk + 64 / L - 1) / (64 / L), end = min(a.dk, (g + 1) * each);
@@ -841,8 +821,11 @@ __global__ __launch_bounds__(64 * STEP_WAVES) void k_attention_step_wave(StepArg
 #pragma unroll
             for (int i = 0; i < STEP_ROWS; ++i) {
                 const int r = min(i0 + i, end - 1);
-                const f32x4 *at = reinterpret_cast<const f32x4 *>(s + r * a.dv);
-                x[i] = STREAM ? __builtin_nontemporal_load(at) : *at;
+                const float *at = s + r * a.dv;
+                if (n == 4) x[i] = STREAM ? __builtin_nontemporal_load(reinterpret_cast<const At *>(at)) : *reinterpret_cast<const At *>(at);
+                else
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[i][e] = at[min(e, n - 1)];
                 qs[i] = (float)q[r];
                 ks[i] = (float)k[r];
             }
@@ -855,9 +838,14 @@ __global__ __launch_bounds__(64 * STEP_WAVES) void k_attention_step_wave(StepArg
                     y[e] = fmaf(ks[i], v[e], start ? 0.f : lam * x[i][e]);
                     sum[e] = fmaf(qs[i], y[e], sum[e]);
                 }
-                f32x4 *at = reinterpret_cast<f32x4 *>(s + (i0 + i) * a.dv);
-                if (STREAM) __builtin_nontemporal_store(y, at);
-                else *at = y;
+                float *at = s + (i0 + i) * a.dv;
+                if (n < 4)
+#pragma unroll
+                    for (int e = 0; e < 3; ++e) {
+                        if (e < n) at[e] = y[e];
+                    }
+                else if (STREAM) __builtin_nontemporal_store(y, reinterpret_cast<At *>(at));
+                else *reinterpret_cast<At *>(at) = y;
             }
         }
     }
@@ -868,7 +856,8 @@ __global__ __launch_bounds__(64 * STEP_WAVES) void k_attention_step_wave(StepArg
     if (g == 0 && on) {
         T *o = row_at<T>(a.o, b, 0, h) + c;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = from_float<T>(live ? a.scale * sum[e] : 0.f);
+        for (int e = 0; e < 4; ++e)
+            if (e < n) o[e] = from_float<T>(live ? a.scale * sum[e] : 0.f);
     }
 }
 

@@ -200,6 +200,7 @@ __global__ __launch_bounds__(norm_block(G)) void k_norm_backward(NormArgs a)
     const W *w = static_cast<const W *>(a.w);
     float dw[NV * N] = {}, db[NV * N] = {}, weight[NV * N];
     R::columns(w, a.width, 1.f, weight);
+    constexpr int JOIN = R::GROUPS > 8 ? 8 : 1;   // groups joined at once: all would take the registers of waves that the rows need
     constexpr bool AHEAD = NV == 1;   // the next row is on its way: wider rows have no registers left for it
     const int64_t step = (int64_t)gridDim.x * R::GROUPS;
     R row, d;
@@ -257,7 +258,7 @@ __global__ __launch_bounds__(norm_block(G)) void k_norm_backward(NormArgs a)
                 for (int e = 0; e < N; ++e) join[threadIdx.x * N + e] = y[e];
                 __syncthreads();
                 if (threadIdx.x >= G) continue;
-#pragma unroll (R::GROUPS > 8 ? 8 : 1)   // all at once would take the registers of waves that the rows need
+#pragma unroll JOIN
                 for (int g = 1; g < R::GROUPS; ++g)
 #pragma unroll
                     for (int e = 0; e < N; ++e) y[e] += join[(g * G + threadIdx.x) * N + e];

@@ -353,6 +353,32 @@ def test_step(memory, shape, dtype):
         _close("state", got_state, expect, off)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("games,key_dim,value_dim", [(9, 5, 2), (9, 17, 3), (9, 64, 5), (9, 7, 17), (9, 33, 35), (9, 50, 50), (9, 128, 67),
+                                                     (9, 127, 127), (22000, 50, 50)])   # the last: more than the caches hold
+def test_step_of_odd_dims(memory, dtype, games, key_dim, value_dim):
+    """Rows of a state that end inside a vector, and the elements beside the states untouched."""
+    g = torch.Generator("cuda").manual_seed(value_dim)
+    size = games * 2 * key_dim * value_dim
+    store = torch.randn(size + 2, device="cuda", generator=g)
+    state = store[1:-1].view(games, 2, key_dim, value_dim)
+    before = store.clone()
+    q, k = (torch.randn(games, 2, key_dim, device="cuda", generator=g).to(dtype) for _ in range(2))
+    v = torch.randn(games, 2, value_dim, device="cuda", generator=g).to(dtype)
+    decay = torch.tensor([-0.2, -0.01], device="cuda")
+    out = memory.linear_attention_step(q, k, v, decay, state)
+    assert store[0] == before[0] and store[-1] == before[-1]
+    old, lam = before[1:-1].view_as(state).double(), decay.double().exp()[:, None, None]
+    kv = k.double()[..., :, None] * v.double()[..., None, :]
+    want = lam * old + kv
+    assert ((state.double() - want).abs() <= (lam * old.abs() + kv.abs()) * 8 * EPS).all()
+    scale = key_dim ** -0.5
+    answer = (q.double()[..., None] * want).sum(-2) * scale
+    mag = (q.double().abs()[..., None] * (lam * old.abs() + kv.abs())).sum(-2) * scale
+    bound = mag * (key_dim + 8) * EPS + (0 if dtype == F32 else answer.abs() * 2.0 ** -8)
+    assert ((out.double() - answer).abs() <= bound).all()
+
+
 def test_step_follows_the_segments(memory):
     """Plies one by one, from a zero state, answer what the whole segment does."""
     x = _inputs(20, 5, 40, 2, 48, 64, F32, "some", "none", False)
