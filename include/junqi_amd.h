@@ -469,7 +469,7 @@ int jq_attention_forward(const jq_attention *a, void *stream);
 int jq_attention_backward(const jq_attention *a, void *stream);
 /* One new ply of each of batch games: q, k, v and out as above with their ply
  * strides unused, state (float32, (state_rows, heads, key_dim, value_dim), best
- * 4-byte aligned) updated in place. rows (int64, batch; NULL: row b) names each game's
+ * 16-byte aligned) updated in place. rows (int64, batch; NULL: row b) names each game's
  * state; a game whose row is outside [0, state_rows) is left out: its out is 0.
  * Two games with one row race. starts (uint8, batch) may be NULL. */
 int jq_attention_step(int32_t dtype, int32_t batch, int32_t heads, int32_t key_dim, int32_t value_dim, float scale,
