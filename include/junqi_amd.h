@@ -421,7 +421,8 @@ int jq_ids_to_mask(const int32_t *ids, const int32_t *counts, int64_t rows, int3
  * Operators of a policy that plays these games: linear attention with a decay for
  * each head, rotary positions with several axes, layer norm, with their backward
  * passes. No counterpart in the reference's environment. Element types are
- * JQ_F32 and JQ_BF16; sums, statistics and states are kept in float32. Pointers
+ * JQ_F32 and JQ_BF16; sums, statistics and states are kept in float32 (operands in
+ * float32 of sums that are rounded to bfloat16 are taken with 16 bits). Pointers
  * are device addresses, aligned to their element's size; elements of the last
  * dimension are adjacent. Launched on the current device; no call allocates,
  * keeps device memory or synchronises. batch * heads stays below 2^23. */

@@ -119,8 +119,12 @@ template <> struct Mma<float> {
 };
 
 // Terms that a float32 operand is split into. In bfloat16, three hold all of a
-// float32: sums that come out in float32. Two hold 16 bits: operands of sums that
-// are rounded to bfloat16.
+// float32: sums that come out in float32, the states. Two hold 16 bits: operands (P,
+// and the state where it is read) of sums that are rounded to bfloat16, 8 bits. Against
+// the definition in 64 bits these outputs are off by 1.66e-3 in the mean, as much as
+// its own rounding to bfloat16, with two terms and with three, which take 8 % longer
+// (training 1,024 x 256 plies 559 -> 599 us, two records of 65,537 plies 540 -> 594).
+// One term for P is as fast as two, and off by 1.8e-3 to 2.4e-3.
 template <class T, int N> constexpr int PARTS = sizeof(T) == 2 ? N : 1;
 
 // log2 lambda, and lambda^d from it: lambda = 0 has a logarithm whose products with
@@ -257,7 +261,7 @@ struct Chunk {
             asm volatile("" : "+v"(lc_), "+v"(g_));   // made here, not kept over the pass for chunks that are few
             reach(gm, lc_, g_, see, leave);
         }
-        Frag p[NT];
+        Frag p[NT][PARTS<T, 2>];
         if constexpr (OUT) {
             // P's products, and what the state before the chunk answers, a depth of q at a time
             f32x4 acc[NT][NT];   // [it][jt]
@@ -350,14 +354,16 @@ struct Chunk {
         }
         if constexpr (OUT)
 #pragma unroll
-            for (int it = 0; it < NT; ++it)
+            for (int u = 0; u < PARTS<T, 2>; ++u)
 #pragma unroll
-                for (int c = 0; c < CT; ++c) o[c][it] = M::mul(x[c], p[it], o[c][it]);
+                for (int it = 0; it < NT; ++it)
+#pragma unroll
+                    for (int c = 0; c < CT; ++c) o[c][it] = M::mul(x[c], p[it][u], o[c][it]);
     }
 
     // p[it] = P's columns i = 16it + l % 16 as an operand over the plies j, times the
     // scales, from its products.
-    __device__ __forceinline__ void weigh(f32x4 (&acc)[NT][NT], const Games &gm, Frag (&p)[NT]) const
+    __device__ __forceinline__ void weigh(f32x4 (&acc)[NT][NT], const Games &gm, Frag (&p)[NT][PARTS<T, 2>]) const
     {
         // a ply that is not seen leaves 0, whatever its product is
 #pragma unroll
@@ -388,9 +394,12 @@ struct Chunk {
                     }
         }
 #pragma unroll
-        for (int it = 0; it < NT; ++it)
+        for (int it = 0; it < NT; ++it) {
+            float y[FE];
 #pragma unroll
-            for (int e = 0; e < FE; ++e) p[it][e] = from_float<T>(acc[it][e >> 2][e & 3]);
+            for (int e = 0; e < FE; ++e) y[e] = acc[it][e >> 2][e & 3];
+            M::template split<PARTS<T, 2>>(y, p[it]);
+        }
     }
 
     // The chunk ply by ply, for tiles with infinities or NaN: a product with 0 in

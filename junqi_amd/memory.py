@@ -9,8 +9,10 @@ learns it from rollout segments, in which games end and start anew, and
 `linear_attention_step` carries it along with the environment's games.
 
 Tensors must be on the GPU (there is no host path), in float32 or bfloat16;
-sums, statistics and states are float32. Calls run on torch's current stream and
-do not synchronise. Wrong arguments raise ValueError.
+sums, statistics and states are float32. Where linear attention's bfloat16 results
+are products with float32 operands (a state, the weights of the plies), these are
+taken with 16 bits, so that the result's own rounding is what it is off by. Calls run
+on torch's current stream and do not synchronise. Wrong arguments raise ValueError.
 """
 
 from __future__ import annotations
