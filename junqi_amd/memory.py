@@ -22,6 +22,7 @@ import ctypes as C
 
 import torch
 from torch.autograd.function import once_differentiable
+from torch.autograd.graph import increment_version
 
 from . import _lib as L
 from ._lib import check, lib
@@ -275,6 +276,7 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log
         check(lib.jq_attention_step(_DTYPES[q.dtype], b, h, dk, dv, dk ** -0.5 if scale is None else float(scale),
                                     log_decay.data_ptr(), r[0], r[1], r[2], r[3], state.data_ptr(), state.shape[0],
                                     _ptr(rows), _ptr(starts), _stream(q)))
+    increment_version((state, out))   # autograd: what saved them may not use them any more
     return out
 
 
