@@ -21,6 +21,7 @@ import contextlib
 import ctypes as C
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 from torch.autograd.graph import increment_version
 
@@ -63,6 +64,13 @@ def _like(t: torch.Tensor) -> torch.Tensor:
     """A new tensor of t's shape and, where it can be kept, t's order of dimensions."""
     out = torch.empty_like(t)
     return out if out.stride(-1) == 1 or t.shape[-1] == 1 else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+
+
+def _differentiated(*tensors: torch.Tensor | None) -> bool:
+    """Whether autograd has to see the call: an input requires a gradient, or may have
+    a forward-mode tangent, which the autograd functions refuse."""
+    return forward_ad._current_level >= 0 or (
+        torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors))
 
 
 def _check_rows(name: str, t: torch.Tensor, like: torch.Tensor | None = None) -> None:
@@ -218,8 +226,7 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
         initial_state = initial_state.contiguous()
     scale = dk ** -0.5 if scale is None else float(scale)
     q, k, v = _adjacent(q), _adjacent(k), _adjacent(v)
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
-                                    or (initial_state is not None and initial_state.requires_grad)):
+    if _differentiated(q, k, v, initial_state):
         out, state = _Attention.apply(q, k, v, log_decay, starts, lengths, initial_state, scale, return_state)
     else:
         out, state = _attention_forward(q, k, v, log_decay, starts, lengths, initial_state, scale, return_state)
@@ -255,6 +262,9 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log
         raise ValueError("state must be contiguous: it is updated in place")
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or state.requires_grad):
         raise ValueError("linear_attention_step has no gradient: use linear_attention, or torch.no_grad()")
+    if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None
+                                              for t in (q, k, v, log_decay, state)):
+        raise ValueError("linear_attention_step has no forward-mode derivative")
     if rows is None:
         if state.shape[0] != b:
             raise ValueError(f"state must have a row for each of {b} games, got {state.shape[0]} (or rows to be given)")
@@ -345,7 +355,7 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, frequencies: torch.Tensor, 
     shape = x.shape
     if x.ndim > 4:
         x, positions = x.reshape(-1, *shape[-2:]), positions.reshape(-1, axes)
-    if x.requires_grad and torch.is_grad_enabled():
+    if _differentiated(x):
         out = _Rotary.apply(x, positions, frequencies, ends, bool(interleaved))
     else:
         out = _rotary_call(x, positions, frequencies, ends, bool(interleaved), False)
@@ -417,8 +427,7 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     weight = None if weight is None else weight.contiguous()
     bias = None if bias is None else bias.contiguous()
     x2 = _adjacent(x).reshape(-1, w)
-    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
-                                    or (bias is not None and bias.requires_grad)):
+    if _differentiated(x, weight, bias):
         out = _Norm.apply(x2, weight, bias, float(eps))
     else:
         out = _norm_forward(x2, weight, bias, float(eps), False)[0]
