@@ -402,11 +402,26 @@ struct Chunk {
         }
     }
 
-    // The chunk ply by ply, for tiles with infinities or NaN: a product with 0 in
-    // their place is not 0, and a ply must get nothing of those it does not see.
+    // whether an element of this wave's part of the state is infinite
+    __device__ __forceinline__ bool infinite() const
+    {
+        float m = 0.f;
+#pragma unroll
+        for (int t = 0; t < KT; ++t)
+#pragma unroll
+            for (int c = 0; c < CT; ++c)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) m = fmaxf(m, fabsf(s[t][c][r]));
+        return __ballot(m == __builtin_inff()) != 0;
+    }
+
+    // The chunk ply by ply as the definition says, for tiles with infinities or NaN (a
+    // product with 0 in their place is not 0, and a ply must get nothing of those it does
+    // not see) and for states with infinities (which are no sum of two terms, and whose
+    // product with a power that has become 0 is not 0).
     // put(i, c, x): x = value column c0 + 16c + l % 16 of ply i.
     template <class F>
-    __device__ __forceinline__ void singly(const T *q, const T *k, const T *v, const Games &gm, F &&put)
+    __device__ __forceinline__ void singly(const T *q, const T *k, const T *v, const Games &gm, int rows, int cols, F &&put)
     {
         const float lam = power(g2, 1);
         for (int m = 0; m < gm.n; ++m) {
@@ -416,6 +431,9 @@ struct Chunk {
             for (int c = 0; c < CT; ++c) {
                 const float x = in_scale * (float)v[i * LD + c0 + 16 * c + lc];
                 float o = 0.f;
+                // beside the state's elements nothing is added: 0 times an infinity is not 0
+                int own = c0 + 16 * c + lc < cols ? rows - 4 * g : 0;
+                asm volatile("" : "+v"(own));   // compared here, the results not kept over the pass: 5 % of its time
 #pragma unroll
                 for (int t = 0; t < KT; ++t)
 #pragma unroll
@@ -423,7 +441,7 @@ struct Chunk {
                         const int at = i * LD + 16 * t + 4 * g + r;
                         float y = s[t][c][r];
                         if (!REV) y = start ? 0.f : lam * y;
-                        y += (float)k[at] * x;
+                        if (16 * t + r < own) y += (float)k[at] * x;
                         o += (float)q[at] * y;
                         if (REV) y = start ? 0.f : lam * y;
                         s[t][c][r] = y;
@@ -565,8 +583,9 @@ struct Plies {
 #pragma unroll
         for (int u = 0; u < NV; ++u) *reinterpret_cast<V *>(p + u * ROWS * LD) = x[u];
     }
-    static __device__ __forceinline__ float probe_all(const V (&x)[NV], float sum)
+    static __device__ __forceinline__ float probe_all(const V (&x)[NV])
     {
+        float sum = 0.f;
 #pragma unroll
         for (int u = 0; u < NV; ++u) sum = probe(x[u], sum);
         return sum;
@@ -610,6 +629,7 @@ __global__ __launch_bounds__(64 * pass_waves(D), 2) void k_attention_pass(ScanAr
     else ch.load_state(a.s_in ? a.s_in + blockIdx.x * size : nullptr, a.kd, a.vd, a.s_row, a.s_col);
     const P q(a.q, sg.b, sg.h, a.kd, a.stream), k(a.k, sg.b, sg.h, a.kd, a.stream), v(a.v, sg.b, sg.h, a.vd, a.stream), o(a.o, sg.b, sg.h, a.vd, a.stream);
     const uint8_t *starts = a.starts ? a.starts + sg.b * a.starts_batch : nullptr;
+    bool wild = ch.infinite();
     if (WAVES > 1) {
         if (threadIdx.x < 2) bad[threadIdx.x] = 0;
         meet<WAVES>();
@@ -633,8 +653,9 @@ __global__ __launch_bounds__(64 * pass_waves(D), 2) void k_attention_pass(ScanAr
         if (OUT) P::stage(qs, qt);
         P::stage(ks, kt);
         P::stage(vs, vt);
-        const float sum = P::probe_all(kt, P::probe_all(vt, 0.f));
-        bool singly = __ballot(sum != sum) != 0;
+        float sum = P::probe_all(kt) + P::probe_all(vt);
+        if (OUT) sum += P::probe_all(qt);
+        bool singly = wild || __ballot(sum != sum) != 0;
         if (WAVES > 1 && singly) bad[m & 1] = 1;
         meet<WAVES>();
         if (WAVES > 1) {
@@ -645,10 +666,11 @@ __global__ __launch_bounds__(64 * pass_waves(D), 2) void k_attention_pass(ScanAr
         f32x4 acc[C::CT][C::NT];
         if (singly) {
             meet<WAVES>();   // bad is read
-            ch.singly(OUT ? qs : ks, ks, vs, gm, [&](int i, int c, float x) {
+            ch.singly(OUT ? qs : ks, ks, vs, gm, a.kd, a.vd, [&](int i, int c, float x) {
                 const int j = ch.c0 + 16 * c + ch.lc;
                 if (OUT && ch.g == 0 && j < a.vd) o.base[(t0 + i) * o.ply + j] = from_float<T>(x);
             });
+            wild = ch.infinite();
             meet<WAVES>();
         } else {
             ch.template run<OUT>(qs, ks, vs, gm, acc);
@@ -709,7 +731,7 @@ __global__ __launch_bounds__(128 * pass_waves(D), 2) void k_attention_kv(GradArg
     __syncthreads();
 
     V kt[P::NV], qt[P::NV], dt[P::NV], vt[P::NV];
-    bool start = false;
+    bool start = false, wild = ch.infinite();
     const auto begin = [&](int m) { return sg.s0 + (sg.chunks - 1 - m) * CH; };
     const auto fetch = [&](int m) {
         const int t0 = begin(m), n = min(CH, sg.end - t0);
@@ -727,8 +749,8 @@ __global__ __launch_bounds__(128 * pass_waves(D), 2) void k_attention_kv(GradArg
         P::stage(qs, qt);
         P::stage(ds, dt);
         P::stage(vs, vt);
-        const float sum = P::probe_all(qt, P::probe_all(dt, 0.f));
-        if (__ballot(sum != sum)) bad[m & 1] = 1;
+        const float sum = (P::probe_all(kt) + P::probe_all(qt)) + (P::probe_all(dt) + P::probe_all(vt));
+        if (wild || __ballot(sum != sum)) bad[m & 1] = 1;
         __syncthreads();
         const bool singly = bad[m & 1];
         if (threadIdx.x == 0) bad[(m + 1) & 1] = 0;
@@ -739,10 +761,11 @@ __global__ __launch_bounds__(128 * pass_waves(D), 2) void k_attention_kv(GradArg
             T *out = second ? dk.base : dv.base;
             const int64_t ply = second ? dk.ply : dv.ply;
             const int dim = second ? a.kd : a.vd;
-            ch.singly(x, y, z, gm, [&](int i, int c, float value) {
+            ch.singly(x, y, z, gm, second ? a.vd : a.kd, dim, [&](int i, int c, float value) {
                 const int j = ch.c0 + 16 * c + ch.lc;
                 if (ch.g == 0 && j < dim) out[(t0 + i) * ply + j] = from_float<T>(value);
             });
+            wild = ch.infinite();
             __syncthreads();
         } else {
             ch.template run<true>(x, y, z, gm, acc);
@@ -774,12 +797,13 @@ __global__ __launch_bounds__(256) void k_attention_join(ScanArgs a)
     float s = a.s_in ? a.s_in[(int64_t)blockIdx.x * size + i * a.s_row + j * a.s_col] : 0.f;
     float *slots = a.seg_states + (int64_t)blockIdx.x * a.segments * size + e;
     const float *carry = a.seg_carry + (int64_t)blockIdx.x * a.segments;
+    const bool fades = power(log2_lambda(a.log_decay[blockIdx.x % a.heads]), 1) > 0.f;   // lambda is not 0, whatever its power has become
 #pragma unroll 4
     for (int m = 0; m < a.segments - 1; ++m) {
         const int g = REV ? a.segments - 1 - m : m;
         const float own = slots[(int64_t)g * size], c = carry[g];
         slots[(int64_t)g * size] = s;
-        s = c >= 0.f ? c * s + own : own;
+        s = c < 0.f ? own : (c == 0.f && fades && fabsf(s) == __builtin_inff() ? s : c * s) + own;
     }
     slots[(int64_t)(REV ? 0 : a.segments - 1) * size] = s;
 }
