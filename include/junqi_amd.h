@@ -425,7 +425,8 @@ int jq_ids_to_mask(const int32_t *ids, const int32_t *counts, int64_t rows, int3
  * float32 of sums that are rounded to bfloat16 are taken with 16 bits). Pointers
  * are device addresses, aligned to their element's size; elements of the last
  * dimension are adjacent. Launched on the current device; no call allocates,
- * keeps device memory or synchronises. batch * heads stays below 2^23. */
+ * keeps device memory or synchronises. batch * heads stays below 2^23, plies and
+ * a norm's width below 2^31 - 1024, rows and tokens below 2^31. */
 #define JQ_F32 0
 #define JQ_BF16 1
 #define JQ_ATTENTION_MAX_DIM 128   /* largest key_dim and value_dim */

@@ -370,7 +370,8 @@ int check_norm(int32_t dtype, int32_t weight_dtype, int64_t rows, int32_t width)
     if (weight_dtype != JQ_F32 && weight_dtype != dtype)
         return fail(JQ_E_ARG, "weights are float32 or of the rows' type");
     if (rows < 0 || rows > INT_MAX) return fail(JQ_E_ARG, "rows %lld out of range", (long long)rows);
-    if (width <= 0) return fail(JQ_E_ARG, "width %d must be positive", width);
+    if (width <= 0 || width > INT_MAX - 1024)   // the kernels walk a row's columns up to 1,024 past its end
+        return fail(JQ_E_ARG, "width %d out of range", width);
     return JQ_OK;
 }
 

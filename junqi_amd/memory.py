@@ -103,11 +103,19 @@ def _check_decay(log_decay: torch.Tensor, heads: int, like: torch.Tensor) -> tor
     return log_decay.contiguous()
 
 
-def _check_dims(key_dim: int, value_dim: int, heads: int) -> None:
+_INT_MAX = 2 ** 31 - 1   # sizes past it would reach the C calls cut off
+_MOST_STEPPED = _INT_MAX - 1024
+
+
+def _check_dims(batch: int, plies: int, heads: int, key_dim: int, value_dim: int) -> None:
     if not (1 <= key_dim <= L.ATTENTION_MAX_DIM and 1 <= value_dim <= L.ATTENTION_MAX_DIM):
         raise ValueError(f"head dims must be in [1, {L.ATTENTION_MAX_DIM}], got {key_dim} for keys and {value_dim} for values")
     if heads < 1:
         raise ValueError("there must be a head")
+    if batch * heads >= 1 << 23 or heads > _INT_MAX:   # heads of no game too
+        raise ValueError(f"{batch} games of {heads} heads are too many")
+    if plies > _MOST_STEPPED:
+        raise ValueError(f"{plies} plies are too many")
 
 
 # ------------------------------------------------------------------ linear attention
@@ -214,7 +222,7 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_deca
                          f"{tuple(q.shape)}, {tuple(k.shape)} and {tuple(v.shape)}")
     b, t, h, dk = q.shape
     dv = v.shape[3]
-    _check_dims(dk, dv, h)
+    _check_dims(b, t, h, dk, dv)
     log_decay = _check_decay(log_decay, h, q)
     if starts is not None:
         _check("starts", starts, (b, t), (torch.bool, torch.uint8), q)
@@ -253,7 +261,7 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log
                          f"{tuple(q.shape)}, {tuple(k.shape)} and {tuple(v.shape)}")
     b, h, dk = q.shape
     dv = v.shape[2]
-    _check_dims(dk, dv, h)
+    _check_dims(b, 1, h, dk, dv)
     log_decay = _check_decay(log_decay, h, q)
     if not isinstance(state, torch.Tensor) or state.ndim != 4:
         raise ValueError("state must be an (R, H, key_dim, value_dim) tensor")
@@ -346,6 +354,8 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, frequencies: torch.Tensor, 
         raise ValueError(f"sections must be 1 to {L.ROTARY_MAX_AXES} counts of pairs, got {sections}")
     if not 0 < 2 * pairs <= d or pairs > L.ROTARY_MAX_PAIRS:
         raise ValueError(f"{pairs} pairs do not fit heads of {d} elements (at most {L.ROTARY_MAX_PAIRS} pairs)")
+    if x.shape[-2] * d > _INT_MAX:
+        raise ValueError(f"{x.shape[-2]} heads of {d} elements are too many")
     _check("positions", positions, (*x.shape[:-2], axes), (torch.int32, torch.int64), x)
     _check("frequencies", frequencies, (pairs,), (torch.float32,), x)
     if frequencies.requires_grad and torch.is_grad_enabled():
@@ -419,6 +429,8 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     if x.ndim < 1 or x.shape[-1] < 1:
         raise ValueError(f"x must be (..., width) with a positive width, got {tuple(x.shape)}")
     w = x.shape[-1]
+    if w > _MOST_STEPPED:
+        raise ValueError(f"rows of {w} elements are too wide")
     for name, t in (("weight", weight), ("bias", bias)):
         if t is not None:
             _check(name, t, (w,), (torch.float32, x.dtype), x)
