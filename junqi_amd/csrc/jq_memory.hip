@@ -184,21 +184,36 @@ int scan_kv(int32_t dtype, const GradArgs &g, hipStream_t stream)
     return dtype == JQ_F32 ? scan_kv_as<float>(g, stream) : scan_kv_as<bf16>(g, stream);
 }
 
-// How a call's plies are split: few games and heads leave the card idle unless
-// parts of a long axis run side by side, at the price of reading k and v twice and of
-// the states between. Below SPLIT_BELOW waves, and from four segments of
-// SPLIT_MIN_CHUNKS chunks on. Forward in bfloat16, split / in one piece: 32 games of
-// 1,024 plies and 4 heads of 64 (256 waves) 38 / 60 us, 64 games (512) 69 / 61, 128
-// games 111 / 86; 32 games of 256 plies 22 / 18; 2 x 65,537 plies of 8 heads of 128 in
-// 2,048 / 4,096 / 8,192 / 16,384 waves 692 / 678 / 708 / 755 us of kernels.
-constexpr int SPLIT_WAVES = 4096, SPLIT_BELOW = 512, SPLIT_MIN_CHUNKS = 4;
+// How a call's plies are split: few games and heads, a block each, leave the card's 256
+// CUs idle unless parts of a long axis run side by side, at the price of reading k and v
+// twice and of the states between. So bfloat16 is split below a block a CU (up to it where
+// a block is one wave), float32, which its products bound, up to two blocks, and both from
+// four segments of SPLIT_MIN_CHUNKS chunks on. Forward, split / in one piece, us:
+//                heads of 128          heads of 64           heads of 32
+//   blocks    1,024    8,192 plies   1,024    8,192        1,024    8,192
+//   bf16  64   60/90   286/694        33/62   120/475
+//        128   90/90   525/696        38/63   209/473       26/47   135/351
+//        256                          71/64   357/474       41/48   329/349
+//        384                          84/87   497/676       59/51   466/381
+//        512                         108/88   622/685       73/51   609/463
+//   f32   64  117/250  705/1,955      48/143  223/1,129
+//        128  200/250 1,376/1,966     77/146  404/1,131     32/91   214/706
+//        256                         121/146  761/1,135     55/91   368/707
+//        512                         206/219 1,535/1,729    89/93   663/713
+//        768                                               125/112  980/804
+// (heads of 128, eight waves each, have no four segments above 128 blocks.) 2 x 65,537
+// plies of 8 heads of 128 in 2,048 / 4,096 / 8,192 / 16,384 waves: 692 / 678 / 708 /
+// 755 us of kernels.
+constexpr int SPLIT_WAVES = 4096, SPLIT_BLOCKS_BF16 = 256, SPLIT_BLOCKS_F32 = 512, SPLIT_MIN_CHUNKS = 4;
 struct Split { int segments, seg_plies; };
 Split split_of(const jq_attention *a)
 {
     const int ch = a->dtype == JQ_F32 ? Mma<float>::KB : Mma<bf16>::KB, dim = std::max(a->key_dim, a->value_dim);
-    const int64_t waves = std::max<int64_t>(1, (int64_t)a->batch * a->heads) * pass_waves(dim <= 32 ? 32 : dim <= 64 ? 64 : 128);
+    const int64_t blocks = std::max<int64_t>(1, (int64_t)a->batch * a->heads);
+    const int64_t waves = blocks * pass_waves(dim <= 32 ? 32 : dim <= 64 ? 64 : 128);
     const int64_t chunks = ((int64_t)a->plies + ch - 1) / ch;
-    const int64_t want = waves < SPLIT_BELOW ? std::min(SPLIT_WAVES / waves, chunks / SPLIT_MIN_CHUNKS) : 1;
+    const int64_t want = blocks <= (a->dtype == JQ_F32 ? SPLIT_BLOCKS_F32 : SPLIT_BLOCKS_BF16 - (dim > 32))
+                             ? std::min(SPLIT_WAVES / waves, chunks / SPLIT_MIN_CHUNKS) : 1;
     if (want < 4) return {1, (int)std::max<int64_t>(chunks, 1) * ch};
     const int64_t each = (chunks + want - 1) / want;
     return {(int)((chunks + each - 1) / each), (int)each * ch};

@@ -54,3 +54,14 @@ def _check(memory, seed, b, t, h, dk, dv, dtype, *, starts=0.02, lengths=None, t
 def test_attention_errors_in_the_mean(memory, shape, dtype):
     print(f"[attention] {shape} {dtype}", flush=True)
     _check(memory, sum(shape), *shape, dtype)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("shape,lengths,starts", [((2, 900, 3, 64, 40), (730, 900), 0.002), ((2, 1100, 2, 128, 72), (1100, 645), 0.002),
+                                                  ((3, 700, 4, 96, 128), (700, 0, 333), 0.0), ((2, 1300, 2, 32, 24), (1, 1299), 0.005),
+                                                  ((8, 560, 8, 128, 128), None, 0.001), ((40, 530, 5, 64, 64), None, 0.001)])
+def test_attention_in_segments(memory, shape, lengths, starts, dtype):
+    """Long axes that are split: heads of every width, keys and values of different dims, games
+    that end inside a segment or before it, states that are carried over several."""
+    print(f"[segments] {shape} {dtype}", flush=True)
+    _check(memory, sum(shape), *shape, dtype, starts=starts, lengths=lengths, time_major=shape[0] == 3)
