@@ -1,10 +1,12 @@
 """A policy with a memory over plies, playing and learning on the GPU.
 
-Each game keeps one state per head. While playing, a ply's token goes through
+The pieces are hidden, so each seat of a game keeps a memory of its own: one state
+per head, in row game * 4 + seat. While playing, a ply's token goes through
 `layer_norm`, `rotary` at (ply, seat) and `linear_attention_step`, which carries the
-states of all games; a game that ends starts anew in place, and so does its memory.
-An update runs the same network over the stored segment with `linear_attention`,
-whose `starts` part the games, and learns from the rewards (REINFORCE).
+acting seats' states along (`rows`); a game that ends starts anew in place, and so do
+its memories. An update runs the same network over the stored segment, each seat's
+plies one after another, with `linear_attention`, whose `starts` part the games and
+whose `lengths` end the seats' plies, and learns from the rewards (REINFORCE).
 
   python examples/memory_policy.py [games] [plies] [updates]
 """
@@ -24,6 +26,7 @@ from junqi_amd import memory  # noqa: E402
 GLOBALS = 28           # of an observation
 ACTIONS = 16641        # canonical action ids
 EATS, KILLED = 2, 4    # events of a ply
+SEATS = 4
 HEADS, DIM = 4, 64
 WIDTH = HEADS * DIM
 
@@ -64,18 +67,47 @@ class MemoryPolicy(nn.Module):
         return self.out(self.norm_out(x + mixed.flatten(-2).to(x.dtype))) @ self.actions
 
     def new_state(self, games: int, device) -> torch.Tensor:
-        return torch.zeros(games, HEADS, DIM, DIM, device=device)
+        return torch.zeros(games * SEATS, HEADS, DIM, DIM, device=device)
 
     @torch.no_grad()
     def play(self, glob, positions, state, starts):
-        """Logits of one ply of every game; `state` moves on in place. (games, ...)"""
+        """Logits of one ply of every game; the acting seats' states move on in place. (games, ...)"""
         x, q, k, v = self._token(glob, positions)
-        return self._logits(x, memory.linear_attention_step(q, k, v, self.log_decay, state, starts=starts))
+        games = torch.arange(len(starts), device=starts.device)
+        state.view(len(starts), SEATS, -1).masked_fill_(starts[:, None, None], 0.0)
+        mixed = memory.linear_attention_step(q, k, v, self.log_decay, state, rows=games * SEATS + positions[:, 1])
+        return self._logits(x, mixed)
 
     def forward(self, glob, positions, state, starts):
-        """Logits of a segment's plies, (games, plies, ...), from the state before it."""
+        """Logits of a segment's plies, (games, plies, ...), from the states before it."""
         x, q, k, v = self._token(glob, positions)
-        return self._logits(x, memory.linear_attention(q, k, v, self.log_decay, starts=starts, initial_state=state))
+        at, lengths, begins = seat_rows(positions[..., 1], starts)
+        rows, most = len(lengths), begins.shape[1]
+
+        def by_seat(t):
+            t = t.flatten(0, 1)
+            return t.new_zeros(rows * most, HEADS, DIM).index_copy(0, at.flatten(), t).view(rows, most, HEADS, DIM)
+        mixed = memory.linear_attention(by_seat(q), by_seat(k), by_seat(v), self.log_decay, starts=begins, lengths=lengths,
+                                        initial_state=state)
+        return self._logits(x, mixed.flatten(0, 1).index_select(0, at.flatten()).view_as(q))
+
+
+def seat_rows(seats, starts):
+    """Where a segment's plies, (games, plies), lie with each seat's one after another: their
+    index in (games * 4, most), how many each row has, and where it begins a new game."""
+    games, plies = seats.shape
+    acts = torch.nn.functional.one_hot(seats.long(), SEATS)                                  # (games, plies, 4)
+    nth = (acts.cumsum(1) - 1).gather(2, seats.long()[..., None]).squeeze(-1)
+    lengths = acts.sum(1).flatten()
+    most = int(lengths.max())
+    row = torch.arange(games, device=seats.device)[:, None] * SEATS + seats.long()
+    at = row * most + nth
+    # games begun before or with each ply: a seat's ply is its first of a game where that is more
+    # than at its ply before (0 before the segment: a game goes on where none has begun since)
+    begun = starts.cumsum(1).flatten()
+    held = torch.zeros(games * SEATS * most, dtype=begun.dtype, device=seats.device).index_copy(0, at.flatten(), begun)
+    held = held.view(-1, most)
+    return at, lengths, held != torch.nn.functional.pad(held[:, :-1], (1, 0))
 
 
 def rollout(policy: MemoryPolicy, r, state: torch.Tensor, began: torch.Tensor, plies: int, seed: int) -> dict:
