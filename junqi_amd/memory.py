@@ -288,6 +288,10 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log
         _check("out", out, (b, h, dv), (q.dtype,), q)
         if dv > 1 and out.stride(2) != 1:
             raise ValueError("the elements of out's last dimension must be adjacent")
+        if (b > 1 and out.stride(0) == 0) or (h > 1 and out.stride(1) == 0):
+            raise ValueError("the rows of out must not share memory")
+        if torch.is_grad_enabled() and out.requires_grad:
+            raise ValueError("out must not require a gradient: what is written to it has none")
     q, k, v = _adjacent(q), _adjacent(k), _adjacent(v)
     r = [L.Rows(x.data_ptr(), x.stride(0), 0, x.stride(1)) for x in (q, k, v, out)]
     with _on(q):
