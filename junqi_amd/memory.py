@@ -368,7 +368,7 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, frequencies: torch.Tensor, 
     positions, frequencies = _adjacent(positions), frequencies.contiguous()
     shape = x.shape
     if x.ndim > 4:
-        x, positions = x.reshape(-1, *shape[-2:]), positions.reshape(-1, axes)
+        x, positions = x.flatten(0, -3), positions.flatten(0, -2)
     if _differentiated(x):
         out = _Rotary.apply(x, positions, frequencies, ends, bool(interleaved))
     else:

@@ -32,3 +32,12 @@ def test_an_output_that_cannot_be_written_is_refused(memory):
     with torch.no_grad():
         memory.linear_attention_step(*ply, decay, state, out=learned)
     assert learned.any()
+
+
+@pytest.mark.parametrize("shape", [(0, 2, 3, 2, 8), (2, 3, 0, 2, 8), (2, 3, 4, 0, 8), (2, 3, 0, 0, 8), (2, 0, 8), (0, 2, 8), (3, 4, 0, 8)])
+def test_rotary_of_nothing(memory, shape):
+    x = torch.empty(shape, device="cuda", requires_grad=True)
+    positions = torch.zeros(*shape[:-2], 2, dtype=torch.int64, device="cuda")
+    out = memory.rotary(x, positions, memory.rotary_frequencies((2, 2), device="cuda"), (2, 2))
+    assert out.shape == shape
+    assert torch.autograd.grad(out, x, torch.empty_like(out))[0].shape == shape
