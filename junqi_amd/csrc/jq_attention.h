@@ -163,10 +163,10 @@ struct Games {
 // way (four waves: 256 registers and spills, 575 us against 504 for the outputs of
 // 2 x 65,537 plies of 8 heads). Chunks of 64 plies, P shared through LDS by four
 // waves of 16 columns each, took 185 us for the outputs of 1,024 x 256 plies of 4 heads
-// of 64 in bfloat16 (160 now), and the gradients of k and v 338 (272): three barriers
-// and twice the LDS traffic a chunk. Of the 160 us, the same loads, stores and
-// barriers without the products take 150, the products without the loads 140: memory
-// and issue are balanced (VALU 46 % busy, MFMA 18 %, LDS 24 %).
+// of 64 in bfloat16 (165 now), and the gradients of k and v 338 (291): three barriers
+// and twice the LDS traffic a chunk. With P of one term, 160 us, the same loads, stores
+// and barriers without the products took 150, the products without the loads 140: memory
+// and issue are balanced (VALU 46 % busy, MFMA 18 %, LDS 22 %).
 constexpr int pass_waves(int dim) { return dim == 128 ? 8 : dim / 32; }
 template <class T, int D, bool REV>
 struct Chunk {
@@ -607,9 +607,9 @@ struct Segment {
 
 // A pass over one segment of one game and head by one block: chunks in turn, the
 // state in registers; every row is read and written once. 670 MB (1,024 x 256 plies of
-// 4 heads of 64 in bfloat16 with their states) in 160 us: 4.2 TB/s, where a plain copy
-// reaches 6.0. Rows of two chunks on their way instead of one: no faster. While a chunk is worked on, the next one's rows are on their
-// way. OUT: the plies' outputs, from the state before the segment; else only the
+// 4 heads of 64 in bfloat16 with their states) in 165 us: 4.1 TB/s, where a plain copy
+// reaches 6.0. While a chunk is worked on, the next one's rows are on their way (of two
+// chunks: no faster). OUT: the plies' outputs, from the state before the segment; else only the
 // state that the segment's own plies leave, for the states before the others.
 template <class T, int D, bool REV, bool FAST, bool OUT>
 __global__ __launch_bounds__(64 * pass_waves(D), 2) void k_attention_pass(ScanArgs a)
@@ -825,7 +825,8 @@ struct StepArgs {
 // with all their loads on their way, and their sums are joined by shuffles: no
 // barriers, the state is read and written once. Bound by that: 32,768 games of 4 heads
 // of 64 x 64 (4.36 GB) in 744 us, 5.9 TB/s (one thread per column: 1,858);
-// 4,693 games of 4 heads of 50 x 50 in float32 (390 MB) in 66 us (284).
+// 4,693 games of 4 heads of 50 x 50 in float32 (188 MB, which the caches hold) in 66 us
+// (284), 60,000 (2.4 GB) in 1,234 us, 3.9 TB/s.
 constexpr int STEP_ROWS = 16, STEP_WAVES = 4;
 template <class T, int L, bool STREAM, bool ODD>
 __global__ __launch_bounds__(64 * STEP_WAVES) void k_attention_step_wave(StepArgs a, int count)

@@ -11,7 +11,10 @@ namespace jq {
 // the rows' traffic: 262,144 rows of 256 in bfloat16 forward (268 MB) 49 us, 5.5 TB/s,
 // backward (403 MB) 80 us, 5.0 TB/s, where a plain copy reaches 6.0. A wave per row that
 // reads it three times and a column's sums apart took 722 us in all, 136 now; sums by
-// shuffles through LDS, and rows turned to float32 as they come, 62 and 93.
+// shuffles through LDS, and rows turned to float32 as they come, 62 and 93. Widths that
+// leave lanes idle, or have a block a row, are slower: 134 MB of bfloat16 rows forward 44 us
+// at widths of 256 and 1,000, 71 at 300, 66 at 1,500; backward 104 and 172 at 256 and 8,000
+// (256 registers: one wave a SIMD), 423 at 12,000 (87 registers spilled).
 constexpr int norm_block(int group) { return group > 256 ? group : 256; }
 
 template <class T, int G, int NV>

@@ -30,7 +30,8 @@ __device__ __forceinline__ void turn_of(int64_t position, float frequency, float
 // traffic: 262,144 tokens of 8 heads of 64 in bfloat16 (537 MB) in 94 us, 5.7 TB/s;
 // with two heads a token the angles count, 528,771 tokens of 2 heads of 56 in float32
 // (478 MB) in 118 us, 4.0 TB/s. A block per token, an angle per pair and thread: 237
-// and 301 us.
+// and 301 us. Pairs apart that are no whole vectors go one at a time: 8 heads of 12 or 20
+// pairs in bfloat16 (537 MB) in 290 us, of 16 or 24 in 97.
 constexpr int ROTARY_TABLE = 2048;   // pairs of a block's tokens at most (unless one token has more)
 template <class T, int N, bool INTERLEAVED>
 __global__ __launch_bounds__(256) void k_rotary(RotaryArgs a, int64_t all, int tokens)
