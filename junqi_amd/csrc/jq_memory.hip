@@ -186,25 +186,28 @@ int scan_kv(int32_t dtype, const GradArgs &g, hipStream_t stream)
 
 // How a call's plies are split: few games and heads, a block each, leave the card's 256
 // CUs idle unless parts of a long axis run side by side, at the price of reading k and v
-// twice and of the states between. So bfloat16 is split below a block a CU (up to it where
-// a block is one wave), float32, which its products bound, up to two blocks, and both from
-// four segments of SPLIT_MIN_CHUNKS chunks on. Forward, split / in one piece, us:
-//                heads of 128          heads of 64           heads of 32
-//   blocks    1,024    8,192 plies   1,024    8,192        1,024    8,192
-//   bf16  64   60/90   286/694        33/62   120/475
-//        128   90/90   525/696        38/63   209/473       26/47   135/351
-//        256                          71/64   357/474       41/48   329/349
-//        384                          84/87   497/676       59/51   466/381
-//        512                         108/88   622/685       73/51   609/463
-//   f32   64  117/250  705/1,955      48/143  223/1,129
-//        128  200/250 1,376/1,966     77/146  404/1,131     32/91   214/706
-//        256                         121/146  761/1,135     55/91   368/707
-//        512                         206/219 1,535/1,729    89/93   663/713
-//        768                                               125/112  980/804
-// (heads of 128, eight waves each, have no four segments above 128 blocks.) 2 x 65,537
-// plies of 8 heads of 128 in 2,048 / 4,096 / 8,192 / 16,384 waves: 692 / 678 / 708 /
-// 755 us of kernels.
-constexpr int SPLIT_WAVES = 4096, SPLIT_BLOCKS_BF16 = 256, SPLIT_BLOCKS_F32 = 512, SPLIT_MIN_CHUNKS = 4;
+// twice, of the states between and of two more launches. Split / in one piece, us:
+//                   forward, plies                     with the gradients
+//   heads      blocks   512     1,024     8,192         512       1,024       8,192
+//   128 bf16     64    40/48    60/90    286/694      165/192    228/360   1,037/2,753
+//                96    59/48    83/90    417/696      213/191    302/360   1,531/2,763
+//               128    62/48    90/90    525/696      226/194    337/361   1,906/2,768
+//   128 f32     128   115/128  200/250 1,376/1,966    431/511    747/1,003 5,156/7,876
+//    64 bf16    128    34/35    38/63    209/473      161/135    156/198     700/1,469
+//               192    37/35    58/64    284/475      160/136    191/198     980/1,470
+//               256    39/35    71/64    357/474      162/136    238/199   1,249/1,474
+//    64 f32     192    59/76    98/147   581/1,131    202/228    334/444   2,009/3,473
+//               256    76/75   121/146   761/1,135    259/230    409/445   2,619/3,490
+//    32 bf16    256    25/26    41/48    329/349      160/130    157/151   1,096/1,094
+//               384    33/28    59/51    466/381      159/129    191/172   1,571/1,320
+//    32 f32     384    39/49    72/92    522/711      164/172    247/333   1,752/2,570
+// So: below 512 waves, 255 heads of 64 and 511 of 32, from four segments of
+// SPLIT_MIN_CHUNKS chunks on; heads of 128, eight waves each, up to 128 of them, of which
+// four segments take SPLIT_WAVES waves, but above 64 only from 32 chunks on. 2 x 65,537
+// plies of 8 heads of 128 in 2,048 / 4,096 / 8,192 / 16,384 waves: 692 / 678 / 708 / 755 us
+// of kernels.
+constexpr int SPLIT_WAVES = 4096, SPLIT_MIN_CHUNKS = 4, SPLIT_LONG_CHUNKS = 32;
+constexpr int split_blocks(int dim, int64_t chunks) { return dim > 64 ? (chunks < SPLIT_LONG_CHUNKS ? 64 : 128) : dim > 32 ? 255 : 511; }
 struct Split { int segments, seg_plies; };
 Split split_of(const jq_attention *a)
 {
@@ -212,8 +215,7 @@ Split split_of(const jq_attention *a)
     const int64_t blocks = std::max<int64_t>(1, (int64_t)a->batch * a->heads);
     const int64_t waves = blocks * pass_waves(dim <= 32 ? 32 : dim <= 64 ? 64 : 128);
     const int64_t chunks = ((int64_t)a->plies + ch - 1) / ch;
-    const int64_t want = blocks <= (a->dtype == JQ_F32 ? SPLIT_BLOCKS_F32 : SPLIT_BLOCKS_BF16 - (dim > 32))
-                             ? std::min(SPLIT_WAVES / waves, chunks / SPLIT_MIN_CHUNKS) : 1;
+    const int64_t want = blocks <= split_blocks(dim, chunks) ? std::min(SPLIT_WAVES / waves, chunks / SPLIT_MIN_CHUNKS) : 1;
     if (want < 4) return {1, (int)std::max<int64_t>(chunks, 1) * ch};
     const int64_t each = (chunks + want - 1) / want;
     return {(int)((chunks + each - 1) / each), (int)each * ch};
