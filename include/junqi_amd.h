@@ -507,6 +507,114 @@ int jq_layer_norm_backward(int32_t dtype, int32_t weight_dtype, int64_t rows, in
                            const void *d_out, int64_t d_out_stride, void *dx, int64_t dx_stride, void *dweight,
                            void *dbias, void *workspace, int64_t workspace_bytes, void *stream);
 
+/* ---- a policy's selective memory -----------------------------------------------
+ * A state space scan whose steps depend on the input, and the short causal
+ * convolution before it, beside the operators above and under the same terms.
+ * plies stay at or below 2^30, channels at or below 2^20. */
+#define JQ_SCAN_MAX_STATES 64
+#define JQ_CONV_MAX_TAPS 8
+
+/* The selective scan over segments of plies. For each game, channel d and state n,
+ * with dt = softplus(delta + delta_bias) (or without the softplus) and h before the
+ * first ply the initial state:
+ *   h_t = exp(dt_t a[d][n]) * (starts[t] ? 0 : h_{t-1}) + dt_t u_t b_t[n]
+ *   y_t = sum over n of c_t[n] h_t + skip[d] u_t;   out_t = y_t * silu(gate_t)
+ * for t < lengths[game]; plies from there on are not read, and their out and
+ * gradients are 0. Channel d has the b and c of group d / (channels / groups). */
+typedef struct jq_scan {
+    int32_t dtype;                     /* JQ_F32 or JQ_BF16: u, delta, gate, b, c, out and their gradients */
+    int32_t batch, plies, channels, states, groups;
+    int32_t softplus;
+    const float *a;                    /* float32 (channels, states) */
+    const float *skip, *delta_bias;    /* float32 (channels); NULL: 0 */
+    const uint8_t *starts;             /* (batch, plies), nonzero where a game starts; NULL: nowhere */
+    int64_t starts_batch, starts_ply;  /* strides of starts */
+    const int32_t *lengths;            /* (batch), clamped to [0, plies]; NULL: plies */
+    const float *initial_state;        /* float32 (batch, channels, states); NULL: zeros */
+    float *final_state;                /* the same shape; NULL: not written */
+    jq_rows u, delta, gate, out;       /* (batch, plies, channels), head unused; gate NULL: none */
+    jq_rows b, c;                      /* (batch, plies, groups, states) */
+    float *saved;                      /* jq_scan_saved bytes: written by a forward pass that a backward pass follows (else NULL) */
+    /* backward: gradients of out and of the final state go in (d_final NULL: zeros), those
+     * of the inputs come out, each NULL where not wanted */
+    jq_rows d_out, du, ddelta, dgate, db, dc;
+    float *da, *dskip, *ddelta_bias;
+    const float *d_final;
+    float *d_initial;
+    void *workspace;                   /* jq_scan_workspace bytes, 4-byte aligned; NULL if it says 0 */
+    int64_t workspace_bytes;
+} jq_scan;
+/* Bytes of workspace that the forward or (backward != 0) backward pass with these outputs takes. */
+int jq_scan_workspace(const jq_scan *a, int32_t backward, int64_t *bytes);
+int jq_scan_saved(const jq_scan *a, int64_t *bytes);
+int jq_scan_forward(const jq_scan *a, void *stream);
+int jq_scan_backward(const jq_scan *a, void *stream);
+/* One new ply (a->plies 1) of each of a->batch games: a's inputs and out; its starts,
+ * lengths, states and saved are unused. state (float32, (state_rows, channels, states))
+ * is updated in place; rows and starts as in jq_attention_step. */
+int jq_scan_step(const jq_scan *a, float *state, int64_t state_rows, const int64_t *rows, const uint8_t *starts, void *stream);
+
+/* A causal convolution over the last taps plies of each channel:
+ *   out_t = bias[d] + sum over j < taps of weight[d][j] x_{t - taps + 1 + j},  then o * sigmoid(o) where silu;
+ * inputs before a game's start are 0, those before the first ply are the initial state's.
+ * Plies from lengths[game] on are not read, and their out and dx are 0; the final state is
+ * the taps - 1 inputs before that ply (0 where they are of an earlier game). */
+typedef struct jq_conv {
+    int32_t dtype, weight_dtype;       /* x, out, states; weight and bias: JQ_F32 or dtype */
+    int32_t batch, plies, channels, taps;
+    int32_t silu;
+    const void *weight, *bias;         /* (channels, taps), (channels); bias NULL: 0 */
+    const uint8_t *starts;             /* as in jq_scan */
+    int64_t starts_batch, starts_ply;
+    const int32_t *lengths;
+    const void *initial_state;         /* (batch, taps - 1, channels); NULL: zeros */
+    void *final_state;                 /* the same shape; NULL: not written */
+    jq_rows x, out;                    /* (batch, plies, channels), head unused */
+    /* backward; each output NULL where not wanted */
+    jq_rows d_out, dx;
+    void *dweight, *dbias;
+    const void *d_final;
+    void *d_initial;
+    void *workspace;                   /* jq_conv_workspace bytes (backward), 4-byte aligned; NULL if it says 0 */
+    int64_t workspace_bytes;
+} jq_conv;
+int jq_conv_workspace(const jq_conv *a, int64_t *bytes);
+int jq_conv_forward(const jq_conv *a, void *stream);
+int jq_conv_backward(const jq_conv *a, void *stream);
+/* One new ply (a->plies 1) of each game: state ((state_rows, taps - 1, channels) of dtype)
+ * is updated in place; rows and starts as in jq_attention_step. */
+int jq_conv_step(const jq_conv *a, void *state, int64_t state_rows, const int64_t *rows, const uint8_t *starts, void *stream);
+
+/* ---- what a policy answers with -------------------------------------------------
+ * Logits of the actions, with count how often the row's recent actions name one:
+ *   x = logit; where count > 0: x = (x > 0 ? x / repetition : x * repetition) - frequency * count - presence;
+ *   out = x + bias where the mask has the action, else -infinity. */
+#define JQ_LOGITS_MASK_WORDS 0   /* (rows, ceil(actions / 32)) uint32, bit j of word i is action 32 i + j */
+#define JQ_LOGITS_MASK_BYTES 1   /* (rows, actions) uint8 */
+typedef struct jq_logits {
+    int32_t dtype;                     /* logits, out and their gradients */
+    int32_t mask_kind;
+    int64_t rows;
+    int32_t actions;
+    int32_t recent_count, recent64;    /* recent: int32 or (recent64 != 0) int64 */
+    const void *logits;
+    int64_t logits_stride;             /* strides between rows, in elements */
+    const float *bias;                 /* float32 (actions); NULL: 0 */
+    const void *mask;                  /* NULL: every action */
+    int64_t mask_stride;
+    const void *recent;                /* (rows, recent_count) ids; those outside [0, actions) are passed over */
+    int64_t recent_stride;
+    const int32_t *recent_lengths;     /* (rows), clamped to [0, recent_count]; NULL: recent_count */
+    float repetition, frequency, presence;
+    const float *repetitions, *frequencies, *presences;   /* float32 (rows): each row's own; NULL: the one above */
+} jq_logits;
+int jq_logits_forward(const jq_logits *a, void *out, int64_t out_stride, void *stream);
+/* Gradients of the logits and of the bias (each NULL where not wanted; d_bias takes
+ * jq_logits_workspace bytes of 4-byte aligned workspace). */
+int jq_logits_workspace(const jq_logits *a, int64_t *bytes);
+int jq_logits_backward(const jq_logits *a, const void *d_out, int64_t d_out_stride, void *d_logits, int64_t d_logits_stride,
+                       float *d_bias, void *workspace, int64_t workspace_bytes, void *stream);
+
 /* Synchronise `stream`. */
 int jq_sync(void *stream);
 

@@ -20,6 +20,10 @@ F32, BF16 = 0, 1
 ATTENTION_MAX_DIM = 128
 ROTARY_MAX_AXES = 4
 ROTARY_MAX_PAIRS = 4096
+SCAN_MAX_STATES = 64
+CONV_MAX_TAPS = 8
+MASK_WORDS_PACKED, MASK_BYTES = 0, 1
+MOST_CHANNELS, MOST_PLIES = 1 << 20, 1 << 30
 NUM_CELLS = 289
 NUM_ON_BOARD = 129
 NUM_PIDS = 120
@@ -56,6 +60,8 @@ _EXPORTS = [
     "jq_history_reconstruct", "jq_history_reconstruct_bf16", "jq_history_reconstruct_noalloc", "jq_mask_count", "jq_mask_to_ids", "jq_mask_encode", "jq_ids_to_mask", "jq_upload_beliefs",
     "jq_clear_beliefs", "jq_attention_workspace", "jq_attention_forward", "jq_attention_backward", "jq_attention_step",
     "jq_rotary", "jq_layer_norm_forward", "jq_layer_norm_workspace", "jq_layer_norm_backward",
+    "jq_scan_workspace", "jq_scan_saved", "jq_scan_forward", "jq_scan_backward", "jq_scan_step", "jq_conv_workspace",
+    "jq_conv_forward", "jq_conv_backward", "jq_conv_step", "jq_logits_forward", "jq_logits_workspace", "jq_logits_backward",
 ]
 
 
@@ -74,6 +80,40 @@ class Attention(C.Structure):
                 ("d_out", Rows), ("dq", Rows), ("dk", Rows), ("dv", Rows),
                 ("d_final", C.c_void_p), ("d_initial", C.c_void_p),
                 ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64)]
+
+
+class Scan(C.Structure):
+    """jq_scan."""
+    _fields_ = [("dtype", C.c_int32), ("batch", C.c_int32), ("plies", C.c_int32), ("channels", C.c_int32),
+                ("states", C.c_int32), ("groups", C.c_int32), ("softplus", C.c_int32), ("a", C.c_void_p),
+                ("skip", C.c_void_p), ("delta_bias", C.c_void_p), ("starts", C.c_void_p), ("starts_batch", C.c_int64),
+                ("starts_ply", C.c_int64), ("lengths", C.c_void_p), ("initial_state", C.c_void_p),
+                ("final_state", C.c_void_p), ("u", Rows), ("delta", Rows), ("gate", Rows), ("out", Rows), ("b", Rows),
+                ("c", Rows), ("saved", C.c_void_p), ("d_out", Rows), ("du", Rows), ("ddelta", Rows), ("dgate", Rows),
+                ("db", Rows), ("dc", Rows), ("da", C.c_void_p), ("dskip", C.c_void_p), ("ddelta_bias", C.c_void_p),
+                ("d_final", C.c_void_p), ("d_initial", C.c_void_p), ("workspace", C.c_void_p),
+                ("workspace_bytes", C.c_int64)]
+
+
+class Conv(C.Structure):
+    """jq_conv."""
+    _fields_ = [("dtype", C.c_int32), ("weight_dtype", C.c_int32), ("batch", C.c_int32), ("plies", C.c_int32),
+                ("channels", C.c_int32), ("taps", C.c_int32), ("silu", C.c_int32), ("weight", C.c_void_p),
+                ("bias", C.c_void_p), ("starts", C.c_void_p), ("starts_batch", C.c_int64), ("starts_ply", C.c_int64),
+                ("lengths", C.c_void_p), ("initial_state", C.c_void_p), ("final_state", C.c_void_p), ("x", Rows),
+                ("out", Rows), ("d_out", Rows), ("dx", Rows), ("dweight", C.c_void_p), ("dbias", C.c_void_p),
+                ("d_final", C.c_void_p), ("d_initial", C.c_void_p), ("workspace", C.c_void_p),
+                ("workspace_bytes", C.c_int64)]
+
+
+class Logits(C.Structure):
+    """jq_logits."""
+    _fields_ = [("dtype", C.c_int32), ("mask_kind", C.c_int32), ("rows", C.c_int64), ("actions", C.c_int32),
+                ("recent_count", C.c_int32), ("recent64", C.c_int32), ("logits", C.c_void_p),
+                ("logits_stride", C.c_int64), ("bias", C.c_void_p), ("mask", C.c_void_p), ("mask_stride", C.c_int64),
+                ("recent", C.c_void_p), ("recent_stride", C.c_int64), ("recent_lengths", C.c_void_p),
+                ("repetition", C.c_float), ("frequency", C.c_float), ("presence", C.c_float),
+                ("repetitions", C.c_void_p), ("frequencies", C.c_void_p), ("presences", C.c_void_p)]
 
 
 class JunqiError(RuntimeError):
@@ -151,6 +191,16 @@ def bind(L: C.CDLL) -> C.CDLL:
         "jq_layer_norm_workspace": ([I64, I32, C.POINTER(I64)], C.c_int),
         "jq_layer_norm_backward": ([I32, I32, I64, I32, P, I64, P, P, P, P, I64, P, I64, P, P, P, I64, P], C.c_int),
     }
+    S, V, G = C.POINTER(Scan), C.POINTER(Conv), C.POINTER(Logits)
+    sig.update({
+        "jq_scan_workspace": ([S, I32, C.POINTER(I64)], C.c_int), "jq_scan_saved": ([S, C.POINTER(I64)], C.c_int),
+        "jq_scan_forward": ([S, P], C.c_int), "jq_scan_backward": ([S, P], C.c_int),
+        "jq_scan_step": ([S, P, I64, P, P, P], C.c_int),
+        "jq_conv_workspace": ([V, C.POINTER(I64)], C.c_int), "jq_conv_forward": ([V, P], C.c_int),
+        "jq_conv_backward": ([V, P], C.c_int), "jq_conv_step": ([V, P, I64, P, P, P], C.c_int),
+        "jq_logits_forward": ([G, P, I64, P], C.c_int), "jq_logits_workspace": ([G, C.POINTER(I64)], C.c_int),
+        "jq_logits_backward": ([G, P, I64, P, I64, P, P, I64, P], C.c_int),
+    })
     for name, (args, res) in sig.items():
         fn = getattr(L, name)
         fn.argtypes = args

@@ -8,7 +8,7 @@ import sys
 from pathlib import Path
 
 HERE = Path(__file__).resolve().parent
-SOURCES = ["csrc/jq_lib.hip", "csrc/jq_memory.hip", "csrc/jq_topology.cpp"]
+SOURCES = ["csrc/jq_lib.hip", "csrc/jq_memory.hip", "csrc/jq_selective.hip", "csrc/jq_topology.cpp"]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = [
     "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared",

@@ -10,7 +10,7 @@
 #include <utility>
 
 #include "junqi_amd.h"
-#include "jq_error.h"
+#include "jq_entry.h"
 #include "jq_memory.h"
 #include "jq_attention.h"
 #include "jq_rotary.h"
@@ -20,8 +20,6 @@ using namespace jq;
 
 namespace {
 
-hipStream_t strm(void *s) { return reinterpret_cast<hipStream_t>(s); }
-
 // Calls over more bytes than that go past the caches, which would not hold them to
 // their next use; what smaller ones touch is found there. One ply, 4 heads of 64 x 64
 // in bfloat16, through the caches / past them: 1,024 games (67 MB of states) 24.5 /
@@ -29,29 +27,6 @@ hipStream_t strm(void *s) { return reinterpret_cast<hipStream_t>(s); }
 // (5.7 TB/s). Segments of 256 plies, 4 heads of 64, forward, the same rows again: 512
 // games (268 MB) 56 / 64 us, 1,024 135 / 126.
 constexpr int64_t STREAM_BYTES = 400ll << 20;
-
-int check_dtype(int32_t dtype)
-{
-    if (dtype != JQ_F32 && dtype != JQ_BF16) return fail(JQ_E_ARG, "element type %d is neither JQ_F32 nor JQ_BF16", dtype);
-    return JQ_OK;
-}
-
-size_t elem_bytes(int32_t dtype) { return dtype == JQ_F32 ? 4 : 2; }
-
-bool aligned(const void *p, size_t to) { return (uintptr_t)p % to == 0; }
-
-int check_rows(const jq_rows &r, int32_t dtype, const char *name)
-{
-    if (!r.data) return fail(JQ_E_ARG, "null %s", name);
-    if (!aligned(r.data, elem_bytes(dtype))) return fail(JQ_E_ARG, "%s must be aligned to its element size", name);
-    return JQ_OK;
-}
-
-#define TRY(expr)                  \
-    do {                           \
-        const int rc_ = (expr);    \
-        if (rc_) return rc_;       \
-    } while (0)
 
 int check_dims(int32_t batch, int32_t heads, int32_t dk, int32_t dv)
 {

@@ -1,0 +1,543 @@
+// C entry points of a policy's selective memory (state space scan, causal convolution)
+// and of its masked logits. Declarations and contracts live in include/junqi_amd.h.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <climits>
+#include <type_traits>
+
+#include "junqi_amd.h"
+#include "jq_entry.h"
+#include "jq_memory.h"
+#include "jq_scan.h"
+#include "jq_conv.h"
+#include "jq_logits.h"
+
+using namespace jq;
+
+namespace {
+
+constexpr int MOST_CHANNELS = 1 << 20, MOST_PLIES = 1 << 30, MOST_BLOCKS = 1 << 20;
+constexpr int64_t MOST_ELEMENTS = 1ll << 42;   // of a segment's rows: every size below fits 64 bits
+
+template <class F>
+int by_type(int32_t dtype, F &&f)
+{
+    return dtype == JQ_F32 ? f(float()) : f(bf16());
+}
+
+int check_segment(int32_t dtype, int32_t batch, int32_t plies, int32_t channels)
+{
+    TRY(check_dtype(dtype));
+    if (batch < 0 || plies < 0 || plies > MOST_PLIES || channels <= 0 || channels > MOST_CHANNELS)
+        return fail(JQ_E_ARG, "bad shapes (batch %d, plies %d, channels %d)", batch, plies, channels);
+    if ((int64_t)batch * std::max(1, plies) > MOST_ELEMENTS / channels)
+        return fail(JQ_E_ARG, "%d games of %d plies of %d channels are too many", batch, plies, channels);
+    return JQ_OK;
+}
+
+// ------------------------------------------------------------------ scan
+int check_states(int32_t channels, int32_t states, int32_t groups)
+{
+    if (states <= 0 || states > JQ_SCAN_MAX_STATES) return fail(JQ_E_ARG, "states %d not in [1, %d]", states, JQ_SCAN_MAX_STATES);
+    if (groups <= 0 || channels % groups) return fail(JQ_E_ARG, "%d channels do not part into %d groups", channels, groups);
+    return JQ_OK;
+}
+
+int check_scan(const jq_scan *a)
+{
+    if (!a) return fail(JQ_E_ARG, "null arguments");
+    TRY(check_segment(a->dtype, a->batch, a->plies, a->channels));
+    return check_states(a->channels, a->states, a->groups);
+}
+
+int check_scan_inputs(const jq_scan *a)
+{
+    if (!a->a) return fail(JQ_E_ARG, "null a");
+    if (a->plies == 0) return JQ_OK;
+    TRY(check_rows(a->u, a->dtype, "u"));
+    TRY(check_rows(a->delta, a->dtype, "delta"));
+    TRY(check_rows(a->b, a->dtype, "b"));
+    TRY(check_rows(a->c, a->dtype, "c"));
+    if (a->gate.data) TRY(check_rows(a->gate, a->dtype, "gate"));
+    return JQ_OK;
+}
+
+// States of a lane and waves of states.
+struct ScanShape { int ns, sg, waves; bool exact; };
+ScanShape scan_shape(const jq_scan *a)
+{
+    ScanShape s;
+    s.ns = a->states <= 4 ? 4 : a->states <= 8 ? 8 : 16;
+    s.sg = (a->states + s.ns - 1) / s.ns;
+    const int per = a->channels / a->groups;
+    s.waves = (per + 63) / 64;
+    s.exact = s.ns * s.sg == a->states && per % 64 == 0;
+    return s;
+}
+
+// Few games and channels leave most of the card idle unless parts of a long axis run side
+// by side, at the price of its states taken twice.
+constexpr int SPLIT_BELOW = 1024, SPLIT_WAVES = 4096, SPLIT_PLIES = 64;
+struct Split { int segments, seg_plies; };
+Split split_of(const jq_scan *a)
+{
+    const ScanShape s = scan_shape(a);
+    const int64_t waves = std::max<int64_t>(1, (int64_t)a->batch * a->groups * s.waves * s.sg);
+    int64_t want = waves < SPLIT_BELOW ? std::min<int64_t>(SPLIT_WAVES / waves, a->plies / SPLIT_PLIES) : 1;
+    if (want < 4) want = 1;
+    const int64_t each = ((a->plies + want - 1) / want + SCAN_CHUNK - 1) / SCAN_CHUNK * SCAN_CHUNK;
+    if (want == 1 || each == 0) return {1, (int)std::max<int64_t>(each, SCAN_CHUNK)};
+    return {(int)((a->plies + each - 1) / each), (int)each};
+}
+
+// Blocks that share the backward pass's items, each with its own sums of da, dskip and dbias.
+constexpr int BACKWARD_WAVES = 4096;
+int64_t scan_parts(const jq_scan *a)
+{
+    const ScanShape s = scan_shape(a);
+    const int64_t items = (int64_t)a->batch * split_of(a).segments, blocks = (int64_t)s.waves * a->groups;
+    return std::max<int64_t>(1, std::min(items, BACKWARD_WAVES / (blocks * s.sg)));
+}
+
+struct ScanBytes { int64_t state, sum, bc, a; int64_t all() const { return state + sum + bc + a; } };
+ScanBytes scan_bytes(const jq_scan *a, bool backward)
+{
+    const Split split = split_of(a);
+    ScanBytes n{0, 0, 0, 0};
+    if (split.segments > 1) {
+        n.sum = (int64_t)a->batch * split.segments * a->channels * 4;
+        n.state = n.sum * a->states;
+    }
+    if (backward) {
+        if (a->db.data || a->dc.data) n.bc = (int64_t)scan_shape(a).waves * a->batch * a->plies * a->groups * 2 * a->states * 4;
+        if (a->da || a->dskip || a->ddelta_bias) n.a = scan_parts(a) * (a->states + 2) * a->channels * 4;
+    }
+    return n;
+}
+
+int check_scan_workspace(const jq_scan *a, bool backward)
+{
+    const int64_t need = scan_bytes(a, backward).all();
+    if (a->workspace_bytes < need || (need && !a->workspace))
+        return fail(JQ_E_ARG, "workspace of %lld bytes, %lld are needed", (long long)a->workspace_bytes, (long long)need);
+    if (!aligned(a->workspace, 4)) return fail(JQ_E_ARG, "workspace must be 4-byte aligned");
+    return JQ_OK;
+}
+
+SelectArgs select_args(const jq_scan *a, bool backward)
+{
+    SelectArgs s{};
+    const ScanShape shape = scan_shape(a);
+    const Split split = split_of(a);
+    s.u = a->u, s.delta = a->delta, s.gate = a->gate, s.b = a->b, s.c = a->c, s.out = a->out;
+    s.batch = a->batch, s.plies = a->plies, s.channels = a->channels, s.states = a->states, s.groups = a->groups;
+    s.per = a->channels / a->groups, s.waves = shape.waves, s.softplus = a->softplus != 0;
+    s.a = a->a, s.skip = a->skip, s.bias = a->delta_bias;
+    s.starts = a->starts, s.starts_batch = a->starts_batch, s.starts_ply = a->starts_ply;
+    s.lengths = a->lengths;
+    s.s_in = a->initial_state, s.s_out = a->final_state, s.saved = a->saved;
+    s.segments = split.segments, s.seg_plies = split.seg_plies;
+    const ScanBytes n = scan_bytes(a, backward);
+    char *w = static_cast<char *>(a->workspace);
+    s.seg_state = reinterpret_cast<float *>(w);
+    s.seg_sum = reinterpret_cast<float *>(w + n.state);
+    s.part_bc = reinterpret_cast<float *>(w + n.state + n.sum);
+    s.part_a = reinterpret_cast<float *>(w + n.state + n.sum + n.bc);
+    s.want_bc = n.bc, s.want_a = n.a;
+    s.parts = (int)scan_parts(a);
+    return s;
+}
+
+// f(states of a lane, exact)
+template <class F>
+int by_shape(const ScanShape &s, F &&f)
+{
+    auto go = [&](auto ns) { return s.exact ? f(ns, std::true_type()) : f(ns, std::false_type()); };
+    return s.ns == 4 ? go(std::integral_constant<int, 4>()) : s.ns == 8 ? go(std::integral_constant<int, 8>()) : go(std::integral_constant<int, 16>());
+}
+
+int grid_over(int64_t threads) { return (int)std::max<int64_t>(1, std::min<int64_t>((threads + 255) / 256, 1 << 16)); }
+
+template <bool BACK>
+int launch_join(const SelectArgs &s, hipStream_t stream)
+{
+    hipLaunchKernelGGL(k_scan_join<BACK>, dim3(grid_over((int64_t)s.batch * s.states * s.channels)), dim3(256), 0, stream, s);
+    return launch_check("k_scan_join");
+}
+
+int scan_grid(const SelectArgs &s)
+{
+    const int cw = s.waves * s.groups;
+    return cw * (int)std::max<int64_t>(1, std::min<int64_t>((int64_t)s.batch * s.segments, MOST_BLOCKS / cw));
+}
+
+// ------------------------------------------------------------------ convolution
+int check_taps(int32_t dtype, int32_t weight_dtype, int32_t taps)
+{
+    if (weight_dtype != JQ_F32 && weight_dtype != dtype) return fail(JQ_E_ARG, "weights are float32 or of the rows' type");
+    if (taps <= 0 || taps > JQ_CONV_MAX_TAPS) return fail(JQ_E_ARG, "taps %d not in [1, %d]", taps, JQ_CONV_MAX_TAPS);
+    return JQ_OK;
+}
+
+int check_conv(const jq_conv *a)
+{
+    if (!a) return fail(JQ_E_ARG, "null arguments");
+    TRY(check_segment(a->dtype, a->batch, a->plies, a->channels));
+    return check_taps(a->dtype, a->weight_dtype, a->taps);
+}
+
+int check_state_pointer(const void *p, int32_t dtype, const char *name)
+{
+    if (!aligned(p, elem_bytes(dtype))) return fail(JQ_E_ARG, "%s must be aligned to its element size", name);
+    return JQ_OK;
+}
+
+int check_conv_inputs(const jq_conv *a)
+{
+    if (!a->weight) return fail(JQ_E_ARG, "null weight");
+    TRY(check_state_pointer(a->weight, a->weight_dtype, "weight"));
+    TRY(check_state_pointer(a->bias, a->weight_dtype, "bias"));
+    TRY(check_state_pointer(a->initial_state, a->dtype, "initial_state"));
+    if (a->plies) TRY(check_rows(a->x, a->dtype, "x"));
+    return JQ_OK;
+}
+
+int conv_v(int32_t dtype, int taps) { return taps > 4 || dtype == JQ_F32 ? 4 : 8; }
+
+// Threads across channels, and plies of a run: as many runs as keep the card's threads
+// busy, none so short that the taps before it are most of what it reads.
+constexpr int CONV_THREADS = 512 * 1024, CONV_RUN = 16, CONV_BACKWARD_BLOCKS = 1024;
+void conv_shape(ConvArgs &c, int32_t dtype)
+{
+    const int64_t vectors = (c.channels + conv_v(dtype, c.taps) - 1) / conv_v(dtype, c.taps);
+    c.tx = vectors <= 8 ? 8 : vectors <= 16 ? 16 : vectors <= 32 ? 32 : 64;
+    const int64_t across = (vectors + c.tx - 1) / c.tx * c.tx;
+    const int64_t want = std::max<int64_t>(1, CONV_THREADS / across / std::max(1, c.batch));
+    c.run = (int)std::max<int64_t>(CONV_RUN, (c.plies + want - 1) / want);
+    c.runs = std::max(1, (c.plies + c.run - 1) / c.run);
+}
+int conv_blocks_x(const ConvArgs &c, int32_t dtype)
+{
+    const int v = conv_v(dtype, c.taps);
+    return ((c.channels + v - 1) / v + c.tx - 1) / c.tx;
+}
+int64_t conv_parts(const ConvArgs &c, int32_t dtype, int64_t items, int64_t most)
+{
+    const int64_t ty = 256 / c.tx;
+    return std::max<int64_t>(1, std::min((items + ty - 1) / ty, most / conv_blocks_x(c, dtype)));
+}
+
+ConvArgs conv_args(const jq_conv *a)
+{
+    ConvArgs c{};
+    c.x = a->x, c.out = a->out;
+    c.batch = a->batch, c.plies = a->plies, c.channels = a->channels, c.taps = a->taps, c.silu = a->silu != 0;
+    c.weight = a->weight, c.bias = a->bias;
+    c.starts = a->starts, c.starts_batch = a->starts_batch, c.starts_ply = a->starts_ply;
+    c.lengths = a->lengths;
+    c.s_in = a->initial_state, c.s_out = a->final_state;
+    conv_shape(c, a->dtype);
+    return c;
+}
+
+int64_t conv_bytes(const jq_conv *a)
+{
+    const ConvArgs c = conv_args(a);
+    if (!a->dweight && !a->dbias) return 0;
+    return conv_parts(c, a->dtype, (int64_t)c.batch * c.runs, CONV_BACKWARD_BLOCKS) * (c.taps + 1) * c.channels * 4;
+}
+
+// f(rows' type, weights' type, taps)
+template <class F>
+int by_taps(int32_t dtype, int32_t weight_dtype, int taps, F &&f)
+{
+    auto go = [&](auto t, auto w) {
+        using std::integral_constant;
+        return taps <= 2 ? f(t, w, integral_constant<int, 2>()) : taps == 3 ? f(t, w, integral_constant<int, 3>())
+               : taps == 4 ? f(t, w, integral_constant<int, 4>()) : f(t, w, integral_constant<int, 8>());
+    };
+    if (dtype == JQ_F32) return go(float(), float());
+    return weight_dtype == JQ_F32 ? go(bf16(), float()) : go(bf16(), bf16());
+}
+
+// ------------------------------------------------------------------ logits
+int check_logits(const jq_logits *a)
+{
+    if (!a) return fail(JQ_E_ARG, "null arguments");
+    TRY(check_dtype(a->dtype));
+    if (a->rows < 0 || a->rows > INT_MAX || a->actions <= 0 || a->actions > INT_MAX - LOGITS_TILE || a->recent_count < 0 || a->recent_count > INT_MAX - 256)
+        return fail(JQ_E_ARG, "bad shapes (rows %lld, actions %d, recent %d)", (long long)a->rows, a->actions, a->recent_count);
+    if (a->mask && a->mask_kind != JQ_LOGITS_MASK_WORDS && a->mask_kind != JQ_LOGITS_MASK_BYTES) return fail(JQ_E_ARG, "mask kind %d", a->mask_kind);
+    if (a->mask && a->mask_kind == JQ_LOGITS_MASK_WORDS && !aligned(a->mask, 4)) return fail(JQ_E_ARG, "mask words must be 4-byte aligned");
+    if (a->recent_count && !a->recent) return fail(JQ_E_ARG, "null recent");
+    if (!aligned(a->recent, a->recent64 ? 8 : 4)) return fail(JQ_E_ARG, "recent must be aligned to its element size");
+    if (!aligned(a->bias, 4)) return fail(JQ_E_ARG, "bias must be 4-byte aligned");
+    return JQ_OK;
+}
+
+LogitsArgs logits_args(const jq_logits *a)
+{
+    LogitsArgs l{};
+    l.x = a->logits, l.x_stride = a->logits_stride;
+    l.rows = a->rows, l.actions = a->actions, l.tiles = (a->actions + LOGITS_TILE - 1) / LOGITS_TILE;
+    l.bias = a->bias;
+    if (a->mask && a->mask_kind == JQ_LOGITS_MASK_WORDS) l.words = static_cast<const uint32_t *>(a->mask);
+    else l.dense = static_cast<const uint8_t *>(a->mask);
+    l.mask_stride = a->mask_stride;
+    l.recent = a->recent, l.recent_stride = a->recent_stride, l.recent_count = a->recent_count, l.recent64 = a->recent64 != 0;
+    l.recent_lengths = a->recent_lengths;
+    l.repetition = a->repetition, l.frequency = a->frequency, l.presence = a->presence;
+    l.repetitions = a->repetitions, l.frequencies = a->frequencies, l.presences = a->presences;
+    return l;
+}
+
+// Blocks of the backward pass, each with its own sums of dbias.
+constexpr int LOGITS_BLOCKS = 4096;
+int64_t logits_parts(const jq_logits *a)
+{
+    const int64_t tiles = (a->actions + LOGITS_TILE - 1) / LOGITS_TILE;
+    return std::max<int64_t>(1, std::min<int64_t>(a->rows, LOGITS_BLOCKS / tiles));
+}
+
+}  // namespace
+
+extern "C" {
+
+int jq_scan_workspace(const jq_scan *a, int32_t backward, int64_t *bytes)
+{
+    TRY(check_scan(a));
+    if (!bytes) return fail(JQ_E_ARG, "null output");
+    *bytes = scan_bytes(a, backward != 0).all();
+    return JQ_OK;
+}
+
+int jq_scan_saved(const jq_scan *a, int64_t *bytes)
+{
+    TRY(check_scan(a));
+    if (!bytes) return fail(JQ_E_ARG, "null output");
+    *bytes = (int64_t)a->batch * ((a->plies + SCAN_CHUNK - 1) / SCAN_CHUNK) * a->states * a->channels * 4;
+    return JQ_OK;
+}
+
+int jq_scan_forward(const jq_scan *a, void *stream)
+{
+    TRY(check_scan(a));
+    if (a->batch == 0) return JQ_OK;
+    TRY(check_scan_inputs(a));
+    if (a->plies) TRY(check_rows(a->out, a->dtype, "out"));
+    TRY(check_scan_workspace(a, false));
+    const SelectArgs s = select_args(a, false);
+    const ScanShape shape = scan_shape(a);
+    const hipStream_t q = strm(stream);
+    return by_type(a->dtype, [&](auto t) {
+        using T = decltype(t);
+        return by_shape(shape, [&](auto ns, auto exact) {
+            const dim3 grid(scan_grid(s)), block(64 * shape.sg);
+            if (s.segments > 1) {
+                hipLaunchKernelGGL((k_scan_forward<T, ns(), exact(), false>), grid, block, 0, q, s);
+                TRY(launch_check("k_scan_forward (states)"));
+                TRY(launch_join<false>(s, q));
+            }
+            const size_t lds = shape.sg > 1 ? 2 * shape.sg * SCAN_PLIES * 64 * sizeof(float) : 0;
+            hipLaunchKernelGGL((k_scan_forward<T, ns(), exact(), true>), grid, block, lds, q, s);
+            return launch_check("k_scan_forward");
+        });
+    });
+}
+
+int jq_scan_backward(const jq_scan *a, void *stream)
+{
+    TRY(check_scan(a));
+    TRY(check_scan_inputs(a));
+    if (a->plies) TRY(check_rows(a->d_out, a->dtype, "d_out"));
+    if (a->plies && a->batch && !a->saved) return fail(JQ_E_ARG, "null saved");
+    if (a->dgate.data && !a->gate.data) return fail(JQ_E_ARG, "dgate without a gate");
+    for (const jq_rows *r : {&a->du, &a->ddelta, &a->dgate, &a->db, &a->dc})
+        if (r->data) TRY(check_rows(*r, a->dtype, "a gradient"));
+    TRY(check_scan_workspace(a, true));
+    SelectArgs s = select_args(a, true);
+    s.d_out = a->d_out, s.du = a->du, s.ddelta = a->ddelta, s.dgate = a->dgate;
+    s.d_final = a->d_final, s.d_initial = a->d_initial;
+    const ScanShape shape = scan_shape(a);
+    const hipStream_t q = strm(stream);
+    return by_type(a->dtype, [&](auto t) {
+        using T = decltype(t);
+        return by_shape(shape, [&](auto ns, auto exact) {
+            const dim3 block(64 * shape.sg);
+            if (s.segments > 1) {
+                hipLaunchKernelGGL((k_scan_carry<T, ns(), exact()>), dim3(scan_grid(s)), block, 0, q, s);
+                TRY(launch_check("k_scan_carry"));
+                TRY(launch_join<true>(s, q));
+            }
+            const size_t lds = shape.sg > 1 ? 3 * shape.sg * SCAN_CHUNK * 64 * sizeof(float) : 0;
+            hipLaunchKernelGGL((k_scan_backward<T, ns(), exact()>), dim3(s.parts * s.waves * s.groups), block, lds, q, s);
+            TRY(launch_check("k_scan_backward"));
+            if (s.want_bc && s.batch && s.plies) {
+                const int64_t n = (int64_t)s.batch * s.plies * s.groups * 2 * s.states;
+                hipLaunchKernelGGL(k_scan_join_bc<T>, dim3(grid_over(n)), dim3(256), 0, q, s, a->db, a->dc);
+                TRY(launch_check("k_scan_join_bc"));
+            }
+            if (!s.want_a) return JQ_OK;
+            hipLaunchKernelGGL(k_scan_join_a, dim3((int)(((int64_t)(s.states + 2) * s.channels + 15) / 16)), dim3(256), 0, q, s, a->da, a->dskip,
+                               a->ddelta_bias);
+            return launch_check("k_scan_join_a");
+        });
+    });
+}
+
+int jq_scan_step(const jq_scan *a, float *state, int64_t state_rows, const int64_t *rows, const uint8_t *starts, void *stream)
+{
+    TRY(check_scan(a));
+    if (state_rows < 0) return fail(JQ_E_ARG, "negative state_rows");
+    if (a->plies != 1) return fail(JQ_E_ARG, "a step has one ply, not %d", a->plies);
+    if (a->batch == 0) return JQ_OK;
+    TRY(check_scan_inputs(a));
+    TRY(check_rows(a->out, a->dtype, "out"));
+    if (state_rows && !state) return fail(JQ_E_ARG, "null state");
+    if (!aligned(state, 4)) return fail(JQ_E_ARG, "state must be 4-byte aligned");
+    const SelectStepArgs s{a->u, a->delta, a->gate, a->b, a->c, a->out, a->batch, a->channels, a->states, a->groups,
+                           a->channels / a->groups, a->softplus != 0, a->a, a->skip, a->delta_bias, state, state_rows, rows, starts};
+    return by_type(a->dtype, [&](auto t) {
+        using T = decltype(t);
+        auto go = [&](auto l) {
+            const int per = 64 / l(), cw = (a->channels + per - 1) / per;
+            const int at_once = (int)std::max<int64_t>(1, std::min<int64_t>(a->batch, 16384 / cw));
+            hipLaunchKernelGGL((k_scan_step<T, l()>), dim3((int)(((int64_t)cw * at_once + 3) / 4)), dim3(256), 0, strm(stream), s, cw, at_once);
+            return launch_check("k_scan_step");
+        };
+        using std::integral_constant;
+        return a->states <= 4 ? go(integral_constant<int, 1>()) : a->states <= 8 ? go(integral_constant<int, 2>())
+               : a->states <= 16 ? go(integral_constant<int, 4>()) : a->states <= 32 ? go(integral_constant<int, 8>())
+               : go(integral_constant<int, 16>());
+    });
+}
+
+int jq_conv_workspace(const jq_conv *a, int64_t *bytes)
+{
+    TRY(check_conv(a));
+    if (!bytes) return fail(JQ_E_ARG, "null output");
+    *bytes = conv_bytes(a);
+    return JQ_OK;
+}
+
+int jq_conv_forward(const jq_conv *a, void *stream)
+{
+    TRY(check_conv(a));
+    if (a->batch == 0) return JQ_OK;
+    TRY(check_conv_inputs(a));
+    if (a->plies) TRY(check_rows(a->out, a->dtype, "out"));
+    TRY(check_state_pointer(a->final_state, a->dtype, "final_state"));
+    ConvArgs c = conv_args(a);
+    c.parts = (int)conv_parts(c, a->dtype, (int64_t)c.batch * c.runs, MOST_BLOCKS);
+    return by_taps(a->dtype, a->weight_dtype, a->taps, [&](auto t, auto w, auto taps) {
+        hipLaunchKernelGGL((k_conv_forward<decltype(t), decltype(w), taps()>), dim3(c.parts * conv_blocks_x(c, a->dtype)), dim3(256), 0, strm(stream), c);
+        return launch_check("k_conv_forward");
+    });
+}
+
+int jq_conv_backward(const jq_conv *a, void *stream)
+{
+    TRY(check_conv(a));
+    TRY(check_conv_inputs(a));
+    if (a->plies) TRY(check_rows(a->d_out, a->dtype, "d_out"));
+    if (a->dx.data) TRY(check_rows(a->dx, a->dtype, "dx"));
+    TRY(check_state_pointer(a->d_final, a->dtype, "d_final"));
+    TRY(check_state_pointer(a->d_initial, a->dtype, "d_initial"));
+    TRY(check_state_pointer(a->dweight, a->weight_dtype, "dweight"));
+    TRY(check_state_pointer(a->dbias, a->weight_dtype, "dbias"));
+    const int64_t need = conv_bytes(a);
+    if (a->workspace_bytes < need || (need && !a->workspace))
+        return fail(JQ_E_ARG, "workspace of %lld bytes, %lld are needed", (long long)a->workspace_bytes, (long long)need);
+    if (!aligned(a->workspace, 4)) return fail(JQ_E_ARG, "workspace must be 4-byte aligned");
+    ConvArgs c = conv_args(a);
+    c.d_out = a->d_out, c.dx = a->dx, c.d_final = a->d_final, c.d_initial = a->d_initial;
+    c.part = need ? static_cast<float *>(a->workspace) : nullptr;
+    c.parts = (int)conv_parts(c, a->dtype, (int64_t)c.batch * c.runs, CONV_BACKWARD_BLOCKS);
+    return by_taps(a->dtype, a->weight_dtype, a->taps, [&](auto t, auto w, auto taps) {
+        using W = decltype(w);
+        hipLaunchKernelGGL((k_conv_backward<decltype(t), W, taps()>), dim3(c.parts * conv_blocks_x(c, a->dtype)), dim3(256), 0, strm(stream), c);
+        TRY(launch_check("k_conv_backward"));
+        if (!c.part) return JQ_OK;
+        hipLaunchKernelGGL(k_conv_join<W>, dim3((int)(((int64_t)(c.taps + 1) * c.channels + 15) / 16)), dim3(256), 0, strm(stream), c.part, c.parts, c.taps,
+                           c.channels, static_cast<W *>(a->dweight), static_cast<W *>(a->dbias));
+        return launch_check("k_conv_join");
+    });
+}
+
+int jq_conv_step(const jq_conv *a, void *state, int64_t state_rows, const int64_t *rows, const uint8_t *starts, void *stream)
+{
+    TRY(check_conv(a));
+    if (state_rows < 0) return fail(JQ_E_ARG, "negative state_rows");
+    if (a->plies != 1) return fail(JQ_E_ARG, "a step has one ply, not %d", a->plies);
+    if (a->batch == 0) return JQ_OK;
+    TRY(check_conv_inputs(a));
+    TRY(check_rows(a->out, a->dtype, "out"));
+    if (state_rows && !state && a->taps > 1) return fail(JQ_E_ARG, "null state");
+    TRY(check_state_pointer(state, a->dtype, "state"));
+    ConvStepArgs s{conv_args(a), state, state_rows, rows, starts};
+    s.c.parts = (int)conv_parts(s.c, a->dtype, a->batch, 4096);
+    return by_taps(a->dtype, a->weight_dtype, a->taps, [&](auto t, auto w, auto taps) {
+        hipLaunchKernelGGL((k_conv_step<decltype(t), decltype(w), taps()>), dim3(s.c.parts * conv_blocks_x(s.c, a->dtype)), dim3(256), 0, strm(stream), s);
+        return launch_check("k_conv_step");
+    });
+}
+
+int jq_logits_forward(const jq_logits *a, void *out, int64_t out_stride, void *stream)
+{
+    TRY(check_logits(a));
+    if (a->rows == 0) return JQ_OK;
+    if (!a->logits || !out) return fail(JQ_E_ARG, "null device pointer");
+    if (!aligned(a->logits, elem_bytes(a->dtype)) || !aligned(out, elem_bytes(a->dtype)))
+        return fail(JQ_E_ARG, "rows must be aligned to their element size");
+    LogitsArgs l = logits_args(a);
+    l.o = out, l.o_stride = out_stride;
+    const int grid = (int)std::min<int64_t>(l.rows * l.tiles, MOST_BLOCKS);
+    return by_type(a->dtype, [&](auto t) {
+        using T = decltype(t);
+        if (l.recent_count) hipLaunchKernelGGL((k_logits_forward<T, true>), dim3(grid), dim3(256), 0, strm(stream), l);
+        else hipLaunchKernelGGL((k_logits_forward<T, false>), dim3(grid), dim3(256), 0, strm(stream), l);
+        return launch_check("k_logits_forward");
+    });
+}
+
+int jq_logits_workspace(const jq_logits *a, int64_t *bytes)
+{
+    TRY(check_logits(a));
+    if (!bytes) return fail(JQ_E_ARG, "null output");
+    *bytes = logits_parts(a) * a->actions * 4;
+    return JQ_OK;
+}
+
+int jq_logits_backward(const jq_logits *a, const void *d_out, int64_t d_out_stride, void *d_logits, int64_t d_logits_stride,
+                       float *d_bias, void *workspace, int64_t workspace_bytes, void *stream)
+{
+    TRY(check_logits(a));
+    if (a->rows && (!d_out || (a->recent_count && d_logits && !a->logits))) return fail(JQ_E_ARG, "null device pointer");
+    if (!aligned(a->logits, elem_bytes(a->dtype)) || !aligned(d_out, elem_bytes(a->dtype)) || !aligned(d_logits, elem_bytes(a->dtype)))
+        return fail(JQ_E_ARG, "rows must be aligned to their element size");
+    if (!d_logits && !d_bias) return JQ_OK;
+    LogitsArgs l = logits_args(a);
+    l.d = d_out, l.d_stride = d_out_stride, l.o = d_logits, l.o_stride = d_logits_stride;
+    l.parts = (int)logits_parts(a);
+    if (d_bias) {
+        const int64_t need = (int64_t)l.parts * l.actions * 4;
+        if (workspace_bytes < need || !workspace)
+            return fail(JQ_E_ARG, "workspace of %lld bytes, %lld are needed", (long long)workspace_bytes, (long long)need);
+        if (!aligned(workspace, 4)) return fail(JQ_E_ARG, "workspace must be 4-byte aligned");
+        l.part = static_cast<float *>(workspace);
+    }
+    const size_t lds = d_bias ? LOGITS_TILE * sizeof(float) : 0;
+    return by_type(a->dtype, [&](auto t) {
+        using T = decltype(t);
+        const dim3 grid(l.parts * l.tiles);
+        if (l.recent_count && l.o) hipLaunchKernelGGL((k_logits_backward<T, true>), grid, dim3(256), lds, strm(stream), l);
+        else hipLaunchKernelGGL((k_logits_backward<T, false>), grid, dim3(256), lds, strm(stream), l);
+        TRY(launch_check("k_logits_backward"));
+        if (!d_bias) return JQ_OK;
+        hipLaunchKernelGGL(k_logits_join, dim3((l.actions + 15) / 16), dim3(256), 0, strm(stream), l.part, l.parts, l.actions, d_bias);
+        return launch_check("k_logits_join");
+    });
+}
+
+}  // extern "C"

@@ -6,13 +6,23 @@ memory is short).
 Same arguments, shapes, dtypes and ValueError checks as the reference's
 ``_dense_mask_to_csr`` and ``_csr_to_dense_selected``; tensors must be on the
 GPU (there is no host path).
+
+`action_logits` puts such masks, or the packed ones of the environment, on a policy's
+logits, with penalties of repeated actions and biases (the jq_logits_* kernels; no
+counterpart in the reference).
 """
 
 from __future__ import annotations
 
-import torch
+import ctypes as C
+import math
 
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib as L
 from ._lib import check, lib
+from .memory import _DTYPES, _adjacent, _check, _check_rows, _differentiated, _on, _ptr
 
 
 def _stream(t: torch.Tensor) -> int:
@@ -83,3 +93,125 @@ def csr_to_dense_selected(legal_ids: torch.Tensor, legal_counts: torch.Tensor, i
     check(lib.jq_ids_to_mask(ids.data_ptr(), cnt.data_ptr(), int(ids.shape[0]), int(ids.shape[1]), sel.data_ptr(),
                              b, int(flat_action_dim), out.data_ptr(), _stream(ids)))
     return out
+
+
+# ------------------------------------------------------------------ masked logits
+class _Penalties:
+    """Each penalty as one number, or as a float32 tensor of the rows' own."""
+
+    def __init__(self, logits, repetition, frequency, presence):
+        self.numbers, self.tensors = [1.0, 0.0, 0.0], [None, None, None]
+        for i, (name, v) in enumerate((("repetition", repetition), ("frequency", frequency), ("presence", presence))):
+            if isinstance(v, torch.Tensor):
+                _check(name, v, (logits.shape[0],), (torch.float32,), logits)
+                if v.requires_grad and torch.is_grad_enabled():
+                    raise ValueError(f"{name} has no gradient (detach it)")
+                self.tensors[i] = v.contiguous()
+            else:
+                self.numbers[i] = float(v)
+                if not math.isfinite(self.numbers[i]):
+                    raise ValueError(f"{name} must be finite, got {v}")
+        if self.numbers[0] <= 0.0:
+            raise ValueError(f"repetition must be positive, got {repetition}")
+
+
+def _logits_args(logits, bias, legal, recent, lengths, numbers, tensors) -> L.Logits:
+    g = L.Logits(_DTYPES[logits.dtype], L.MASK_BYTES, logits.shape[0], logits.shape[1])
+    g.logits, g.logits_stride, g.bias = logits.data_ptr(), logits.stride(0), _ptr(bias)
+    if legal is not None:
+        g.mask_kind = L.MASK_WORDS_PACKED if legal.dtype == torch.int32 else L.MASK_BYTES
+        g.mask, g.mask_stride = legal.data_ptr(), legal.stride(0)
+    if recent is not None:
+        g.recent_count, g.recent64 = recent.shape[1], recent.dtype == torch.int64
+        g.recent, g.recent_stride, g.recent_lengths = recent.data_ptr(), recent.stride(0), _ptr(lengths)
+    g.repetition, g.frequency, g.presence = numbers
+    g.repetitions, g.frequencies, g.presences = (_ptr(t) for t in tensors)
+    return g
+
+
+def _stream_of(t: torch.Tensor) -> int:
+    return torch._C._cuda_getCurrentRawStream(t.get_device())
+
+
+def _logits_forward(logits, bias, legal, recent, lengths, penalties):
+    out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    g = _logits_args(logits, bias, legal, recent, lengths, penalties.numbers, penalties.tensors)
+    with _on(logits):
+        check(lib.jq_logits_forward(C.byref(g), out.data_ptr(), out.shape[1], _stream_of(logits)))
+    return out
+
+
+class _ActionLogits(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, bias, legal, recent, lengths, penalties):
+        ctx.save_for_backward(logits, bias, legal, recent, lengths, *penalties.tensors)
+        ctx.numbers = penalties.numbers
+        return _logits_forward(logits, bias, legal, recent, lengths, penalties)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, d_out):
+        logits, bias, legal, recent, lengths, *tensors = ctx.saved_tensors
+        d_out = _adjacent(d_out)
+        g = _logits_args(logits, bias, legal, recent, lengths, ctx.numbers, tensors)
+        need = ctx.needs_input_grad
+        d_logits = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device) if need[0] else None
+        d_bias = torch.empty_like(bias) if need[1] else None
+        size, work = C.c_int64(), None
+        if need[1]:
+            check(lib.jq_logits_workspace(C.byref(g), C.byref(size)))
+            work = torch.empty(size.value, dtype=torch.uint8, device=logits.device)
+        with _on(logits):
+            check(lib.jq_logits_backward(C.byref(g), d_out.data_ptr(), d_out.stride(0), _ptr(d_logits), logits.shape[1],
+                                         _ptr(d_bias), _ptr(work), size.value, _stream_of(logits)))
+        return d_logits, d_bias, None, None, None, None
+
+
+def action_logits(logits: torch.Tensor, *, bias: torch.Tensor | None = None, legal: torch.Tensor | None = None,
+                  recent: torch.Tensor | None = None, recent_lengths: torch.Tensor | None = None,
+                  repetition: float | torch.Tensor = 1.0, frequency: float | torch.Tensor = 0.0,
+                  presence: float | torch.Tensor = 0.0) -> torch.Tensor:
+    """A policy's logits with penalties of repeated actions, a bias and the legal mask,
+    ready for a softmax.
+
+    ``logits`` (N, A) float32 or bfloat16. Where ``recent`` (N, L) int32 or int64, the
+    first ``recent_lengths`` (N,) int32 of each row (all if None), names an action count
+    times: x = (x / repetition if x > 0 else x * repetition) - frequency * count -
+    presence; each penalty is a number or an (N,) float32 tensor, and ids outside
+    [0, A) are passed over (padding). Then ``bias`` (A,) float32 is added, and actions
+    that ``legal`` does not have become -infinity: (N, A) bool, or (N, ceil(A / 32))
+    int32 words, bit j of word i for action 32 i + j, as the environment packs them. A
+    row without a legal action is all -infinity. Returns (N, A) of logits' type.
+
+    Differentiable in logits and bias; an illegal action's gradient is 0 whatever comes
+    in. The environment overwrites its masks in place: give a copy of them to a call
+    whose backward pass comes after its next step."""
+    _check_rows("logits", logits)
+    if logits.ndim != 2 or logits.shape[1] < 1:
+        raise ValueError(f"logits must be (N, A) with an action, got {tuple(logits.shape)}")
+    n, a = logits.shape
+    if n > 2 ** 31 - 1 or a > 2 ** 31 - 1 - 4096:
+        raise ValueError(f"{n} rows of {a} actions are too many")
+    if bias is not None:
+        _check("bias", bias, (a,), (torch.float32,), logits)
+        bias = bias.contiguous()
+    if legal is not None:
+        if not isinstance(legal, torch.Tensor) or legal.dtype not in (torch.bool, torch.int32):
+            raise ValueError("legal must be a bool mask or int32 mask words")
+        _check("legal", legal, (n, a if legal.dtype == torch.bool else -(-a // 32)), (legal.dtype,), logits)
+        legal = _adjacent(legal)
+    if recent is None:
+        if recent_lengths is not None:
+            raise ValueError("recent_lengths without recent")
+    else:
+        if not isinstance(recent, torch.Tensor) or recent.ndim != 2 or recent.shape[1] > 2 ** 31 - 257:
+            raise ValueError("recent must be an (N, L) tensor")
+        _check("recent", recent, (n, recent.shape[1]), (torch.int32, torch.int64), logits)
+        recent = _adjacent(recent)
+        if recent_lengths is not None:
+            _check("recent_lengths", recent_lengths, (n,), (torch.int32,), logits)
+            recent_lengths = recent_lengths.contiguous()
+    penalties = _Penalties(logits, repetition, frequency, presence)
+    logits = _adjacent(logits)
+    args = (logits, bias, legal, recent, recent_lengths, penalties)
+    return _ActionLogits.apply(*args) if _differentiated(logits, bias) else _logits_forward(*args)

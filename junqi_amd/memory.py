@@ -1,12 +1,16 @@
 """Operators of a policy's memory over the plies of a game: linear attention with
 a decay for each head (segments of plies with their backward pass, and the step
-of one ply), rotary positions with several axes, and layer norm, through the
-jq_attention_*, jq_rotary and jq_layer_norm_* kernels.
+of one ply), rotary positions with several axes, layer norm, and a selective state
+space scan with its causal convolution (segments with their backward passes, and the
+steps of one ply), through the jq_attention_*, jq_rotary, jq_layer_norm_*, jq_scan_*
+and jq_conv_* kernels.
 
 The opponents' pieces are hidden, so what a policy answers depends on the plies
 before. A state of fixed size for each game and head keeps them: `linear_attention`
 learns it from rollout segments, in which games end and start anew, and
-`linear_attention_step` carries it along with the environment's games.
+`linear_attention_step` carries it along with the environment's games; so do
+`selective_scan` and `causal_conv` with theirs, whose memory forgets as the plies
+tell it to.
 
 Tensors must be on the GPU (there is no host path), in float32 or bfloat16;
 sums, statistics and states are float32. Where linear attention's bfloat16 results
@@ -448,3 +452,378 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     else:
         out = _norm_forward(x2, weight, bias, float(eps), False)[0]
     return out.reshape(x.shape)
+
+
+# ------------------------------------------------------------------ what segments and steps of channels share
+def _plies(t: torch.Tensor) -> L.Rows:
+    """A (batch, plies, channels) tensor with adjacent elements for the C calls."""
+    return L.Rows(t.data_ptr(), t.stride(0), t.stride(1), 0)
+
+
+def _ply(t: torch.Tensor) -> L.Rows:
+    """A (batch, channels) tensor, or (batch, groups, states), with adjacent elements."""
+    return L.Rows(t.data_ptr(), t.stride(0), 0, t.stride(1) if t.ndim == 3 else 0)
+
+
+def _like_plies(t: torch.Tensor) -> torch.Tensor:
+    """`_like` of rows that may be broadcast: no two elements of the result share memory."""
+    return _like(t) if 0 not in t.stride() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+
+
+def _check_sizes(batch: int, plies: int, channels: int) -> None:
+    if channels < 1:
+        raise ValueError("there must be a channel")
+    if batch > _INT_MAX or plies > L.MOST_PLIES or channels > L.MOST_CHANNELS:
+        raise ValueError(f"{batch} games of {plies} plies of {channels} channels are too many")
+
+
+def _check_segments(starts, lengths, b: int, t: int, like: torch.Tensor):
+    """lengths as the C calls take them."""
+    if starts is not None:
+        _check("starts", starts, (b, t), (torch.bool, torch.uint8), like)
+    if lengths is not None:
+        _check("lengths", lengths, (b,), (torch.int32, torch.int64), like)
+        lengths = (lengths if lengths.dtype == torch.int32 else lengths.clamp(0, t).to(torch.int32)).contiguous()
+    return lengths
+
+
+def _set_segments(a, starts, lengths) -> None:
+    if starts is not None:
+        a.starts = starts.data_ptr()
+        a.starts_batch, a.starts_ply = starts.stride()
+    a.lengths = _ptr(lengths)
+
+
+def _give_workspace(a, need: C.c_int64, like: torch.Tensor) -> torch.Tensor | None:
+    if not need.value:
+        return None
+    w = torch.empty(need.value, dtype=torch.uint8, device=like.device)
+    a.workspace, a.workspace_bytes = w.data_ptr(), need.value
+    return w
+
+
+def _check_step(name: str, x: torch.Tensor, state: torch.Tensor, state_shape: tuple[int, ...], dtype: torch.dtype,
+                rows, starts, out, inputs):
+    """rows, starts and out as the C calls take them, and the checks of a step that updates `state` in place."""
+    b = x.shape[0]
+    if not isinstance(state, torch.Tensor) or state.ndim != 3:
+        raise ValueError(f"state must be an (R, {state_shape[0]}, {state_shape[1]}) tensor")
+    _check("state", state, (state.shape[0], *state_shape), (dtype,), x)
+    if not state.is_contiguous():
+        raise ValueError("state must be contiguous: it is updated in place")
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (*inputs, state)):
+        raise ValueError(f"{name}_step has no gradient: use {name}, or torch.no_grad()")
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None
+                                              for t in (*inputs, state)):
+        raise ValueError(f"{name}_step has no forward-mode derivative")
+    if rows is None:
+        if state.shape[0] != b:
+            raise ValueError(f"state must have a row for each of {b} games, got {state.shape[0]} (or rows to be given)")
+    else:
+        _check("rows", rows, (b,), (torch.int64,), x)
+        rows = rows.contiguous()
+    if starts is not None:
+        _check("starts", starts, (b,), (torch.bool, torch.uint8), x)
+        starts = starts.contiguous()
+    if out is None:
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    else:
+        _check("out", out, tuple(x.shape), (x.dtype,), x)
+        if x.shape[1] > 1 and out.stride(1) != 1:
+            raise ValueError("the elements of out's last dimension must be adjacent")
+        if b > 1 and out.stride(0) == 0:
+            raise ValueError("the rows of out must not share memory")
+        if torch.is_grad_enabled() and out.requires_grad:
+            raise ValueError("out must not require a gradient: what is written to it has none")
+    return rows, starts, out
+
+
+# ------------------------------------------------------------------ selective scan
+def _check_scan(u, delta, a, b, c, skip, gate, delta_bias, lead: int):
+    """The checks that segments (lead 2) and steps (lead 1) share; the arguments with one
+    group written out and adjacent elements."""
+    _check_rows("u", u)
+    if u.ndim != lead + 1:
+        raise ValueError(f"u must be {'(B, T, D)' if lead == 2 else '(B, D)'}, got {tuple(u.shape)}")
+    d = u.shape[-1]
+    for name, t in (("delta", delta), ("gate", gate)):
+        if t is not None:
+            _check_rows(name, t, u)
+            if t.shape != u.shape:
+                raise ValueError(f"{name} must have u's shape {tuple(u.shape)}, got {tuple(t.shape)}")
+    _check_rows("b", b, u)
+    _check_rows("c", c, u)
+    if b.shape != c.shape or b.ndim not in (lead + 1, lead + 2) or b.shape[:lead] != u.shape[:lead]:
+        raise ValueError(f"b and c must be u's rows with (N) or (G, N) elements, got {tuple(b.shape)} and {tuple(c.shape)}")
+    if b.ndim == lead + 1:
+        b, c = b.unsqueeze(lead), c.unsqueeze(lead)
+    groups, n = b.shape[lead:]
+    if not 1 <= n <= L.SCAN_MAX_STATES:
+        raise ValueError(f"there must be 1 to {L.SCAN_MAX_STATES} states, got {n}")
+    if d < 1 or groups < 1 or d % groups:
+        raise ValueError(f"{d} channels do not part into {groups} groups")
+    _check_sizes(u.shape[0], u.shape[1] if lead == 2 else 1, d)
+    _check("a", a, (d, n), (torch.float32,), u)
+    for name, t in (("skip", skip), ("delta_bias", delta_bias)):
+        if t is not None:
+            _check(name, t, (d,), (torch.float32,), u)
+    return (_adjacent(u), _adjacent(delta), a.contiguous(), _adjacent(b), _adjacent(c),
+            None if skip is None else skip.contiguous(), None if gate is None else _adjacent(gate),
+            None if delta_bias is None else delta_bias.contiguous())
+
+
+def _scan_args(u, delta, a, b, c, skip, gate, delta_bias, softplus, of=_plies, group_of=_rows) -> L.Scan:
+    s = L.Scan(_DTYPES[u.dtype], u.shape[0], u.shape[1] if u.ndim == 3 else 1, u.shape[-1], b.shape[-1], b.shape[-2],
+               softplus, a.data_ptr(), _ptr(skip), _ptr(delta_bias))
+    s.u, s.delta, s.b, s.c = of(u), of(delta), group_of(b), group_of(c)
+    if gate is not None:
+        s.gate = of(gate)
+    return s
+
+
+def _scan_forward(u, delta, a, b, c, skip, gate, delta_bias, initial, starts, lengths, softplus, with_state, with_saved):
+    s = _scan_args(u, delta, a, b, c, skip, gate, delta_bias, softplus)
+    _set_segments(s, starts, lengths)
+    out = _like_plies(u)
+    final = torch.empty((u.shape[0], *a.shape), dtype=torch.float32, device=u.device) if with_state else None
+    s.out, s.initial_state, s.final_state = _plies(out), _ptr(initial), _ptr(final)
+    saved, need = None, C.c_int64()
+    if with_saved:
+        check(lib.jq_scan_saved(C.byref(s), C.byref(need)))
+        saved = torch.empty(need.value // 4, dtype=torch.float32, device=u.device)
+        s.saved = saved.data_ptr()
+    with _on(u):
+        check(lib.jq_scan_workspace(C.byref(s), 0, C.byref(need)))
+        work = _give_workspace(s, need, u)   # noqa: F841  (kept until the launch)
+        check(lib.jq_scan_forward(C.byref(s), _stream(u)))
+    return out, final, saved
+
+
+class _Scan(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, u, delta, a, b, c, skip, gate, delta_bias, initial, starts, lengths, softplus, with_state):
+        out, final, saved = _scan_forward(u, delta, a, b, c, skip, gate, delta_bias, initial, starts, lengths, softplus,
+                                          with_state, True)
+        ctx.save_for_backward(u, delta, a, b, c, skip, gate, delta_bias, starts, lengths, saved)
+        ctx.softplus = softplus
+        ctx.set_materialize_grads(False)
+        return out, final
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, d_out, d_final):
+        u, delta, a, b, c, skip, gate, delta_bias, starts, lengths, saved = ctx.saved_tensors
+        if d_out is None and d_final is None:
+            return (None,) * 13
+        d_out = torch.zeros_like(u) if d_out is None else _adjacent(d_out)
+        s = _scan_args(u, delta, a, b, c, skip, gate, delta_bias, ctx.softplus)
+        _set_segments(s, starts, lengths)
+        need = ctx.needs_input_grad
+        grads = [None if x is None or not need[i] else
+                 torch.empty_like(x) if i in (2, 5, 7) else _like_plies(x)
+                 for i, x in enumerate((u, delta, a, b, c, skip, gate, delta_bias))]
+        du, ddelta, da, db, dc, dskip, dgate, dbias = grads
+        d_initial = torch.empty((u.shape[0], *a.shape), dtype=torch.float32, device=u.device) if need[8] else None
+        if d_final is not None:
+            d_final = d_final.contiguous()
+        s.saved, s.d_out = saved.data_ptr(), _plies(d_out)
+        for name, t in (("du", du), ("ddelta", ddelta), ("dgate", dgate)):
+            if t is not None:
+                setattr(s, name, _plies(t))
+        for name, t in (("db", db), ("dc", dc)):
+            if t is not None:
+                setattr(s, name, _rows(t))
+        s.da, s.dskip, s.ddelta_bias = _ptr(da), _ptr(dskip), _ptr(dbias)
+        s.d_final, s.d_initial = _ptr(d_final), _ptr(d_initial)
+        size = C.c_int64()
+        with _on(u):
+            check(lib.jq_scan_workspace(C.byref(s), 1, C.byref(size)))
+            work = _give_workspace(s, size, u)   # noqa: F841
+            check(lib.jq_scan_backward(C.byref(s), _stream(u)))
+        return (*grads, d_initial, None, None, None, None)
+
+
+def selective_scan(u: torch.Tensor, delta: torch.Tensor, a: torch.Tensor, b: torch.Tensor, c: torch.Tensor, *,
+                   skip: torch.Tensor | None = None, gate: torch.Tensor | None = None,
+                   delta_bias: torch.Tensor | None = None, softplus: bool = False,
+                   starts: torch.Tensor | None = None, lengths: torch.Tensor | None = None,
+                   initial_state: torch.Tensor | None = None, return_state: bool = False):
+    """A state space scan whose steps depend on the input, over segments of plies.
+
+    For each game, channel d and state n, with ``dt = softplus(delta + delta_bias)``
+    (without the softplus if not ``softplus``) and a state h that begins as
+    ``initial_state`` (zeros if None):
+
+        h = exp(dt[t] * a[d, n]) * (0 if starts[t] else h) + dt[t] * u[t] * b[t, n]
+        out[t] = (sum over n of c[t, n] * h + skip[d] * u[t]) * silu(gate[t])
+
+    ``u``, ``delta``, ``gate`` (B, T, D) and ``b``, ``c`` (B, T, N) or (B, T, G, N),
+    all float32 or all bfloat16, up to 64 states, any strides (time-major rollout
+    buffers go in as transposed views); with G groups, channel d has those of group
+    d // (D / G). ``a`` (D, N), ``skip`` and ``delta_bias`` (D,) float32. ``starts``
+    and ``lengths`` as in `linear_attention`: a game that starts sees nothing of the
+    plies before, plies from a game's length on are padding, their ``out`` and
+    gradients 0. A decay below 2^-126 counts as 0. Returns ``out`` (B, T, D), or with
+    ``return_state`` also the float32 state (B, D, N) after each game's last ply.
+
+    Differentiable in u, delta, a, b, c, skip, gate, delta_bias and initial_state;
+    sums over plies and channels are taken in a fixed order. The backward pass keeps the
+    state before every eighth ply, B * ceil(T / 8) * D * N float32."""
+    u, delta, a, b, c, skip, gate, delta_bias = _check_scan(u, delta, a, b, c, skip, gate, delta_bias, 2)
+    lengths = _check_segments(starts, lengths, u.shape[0], u.shape[1], u)
+    if initial_state is not None:
+        _check("initial_state", initial_state, (u.shape[0], *a.shape), (torch.float32,), u)
+        initial_state = initial_state.contiguous()
+    args = (u, delta, a, b, c, skip, gate, delta_bias, initial_state, starts, lengths, bool(softplus), return_state)
+    if _differentiated(*args[:9]):
+        out, state = _Scan.apply(*args)
+    else:
+        out, state, _ = _scan_forward(*args, False)
+    return (out, state) if return_state else out
+
+
+def selective_scan_step(u: torch.Tensor, delta: torch.Tensor, a: torch.Tensor, b: torch.Tensor, c: torch.Tensor,
+                        state: torch.Tensor, *, skip: torch.Tensor | None = None, gate: torch.Tensor | None = None,
+                        delta_bias: torch.Tensor | None = None, softplus: bool = False,
+                        rows: torch.Tensor | None = None, starts: torch.Tensor | None = None,
+                        out: torch.Tensor | None = None) -> torch.Tensor:
+    """`selective_scan` of one new ply of each game, its state updated in place.
+
+    ``u``, ``delta``, ``gate`` (B, D), ``b``, ``c`` (B, N) or (B, G, N); ``state``
+    (R, D, N) float32, contiguous; ``rows``, ``starts`` and ``out`` as in
+    `linear_attention_step`: a game whose row is outside [0, R) is left out, its output
+    0, and no row may be named twice. Returns (B, D). Not differentiable."""
+    given = (u, delta, a, b, c, skip, gate, delta_bias)
+    u, delta, a, b, c, skip, gate, delta_bias = _check_scan(*given, 1)
+    rows, starts, out = _check_step("selective_scan", u, state, tuple(a.shape), torch.float32, rows, starts, out, given)
+    s = _scan_args(u, delta, a, b, c, skip, gate, delta_bias, bool(softplus), _ply, _ply)
+    s.out = _ply(out)
+    with _on(u):
+        check(lib.jq_scan_step(C.byref(s), state.data_ptr(), state.shape[0], _ptr(rows), _ptr(starts), _stream(u)))
+    increment_version((state, out))   # autograd: what saved them may not use them any more
+    return out
+
+
+# ------------------------------------------------------------------ causal convolution
+def _check_conv(x, weight, bias, lead: int):
+    _check_rows("x", x)
+    if x.ndim != lead + 1:
+        raise ValueError(f"x must be {'(B, T, D)' if lead == 2 else '(B, D)'}, got {tuple(x.shape)}")
+    d = x.shape[-1]
+    _check_sizes(x.shape[0], x.shape[1] if lead == 2 else 1, d)
+    if not isinstance(weight, torch.Tensor) or weight.ndim != 2:
+        raise ValueError("weight must be a (D, taps) tensor")
+    taps = weight.shape[1]
+    if not 1 <= taps <= L.CONV_MAX_TAPS:
+        raise ValueError(f"there must be 1 to {L.CONV_MAX_TAPS} taps, got {taps}")
+    _check("weight", weight, (d, taps), (torch.float32, x.dtype), x)
+    if bias is not None:
+        _check("bias", bias, (d,), (weight.dtype,), x)
+        bias = bias.contiguous()
+    return _adjacent(x), weight.contiguous(), bias
+
+
+def _conv_args(x, weight, bias, silu, of=_plies) -> L.Conv:
+    v = L.Conv(_DTYPES[x.dtype], _DTYPES[weight.dtype], x.shape[0], x.shape[1] if x.ndim == 3 else 1, x.shape[-1],
+               weight.shape[1], silu, weight.data_ptr(), _ptr(bias))
+    v.x = of(x)
+    return v
+
+
+def _conv_forward(x, weight, bias, initial, starts, lengths, silu, with_state):
+    v = _conv_args(x, weight, bias, silu)
+    _set_segments(v, starts, lengths)
+    out = _like_plies(x)
+    final = None
+    if with_state:
+        final = torch.empty((x.shape[0], weight.shape[1] - 1, x.shape[2]), dtype=x.dtype, device=x.device)
+    v.out, v.initial_state, v.final_state = _plies(out), _ptr(initial), _ptr(final)
+    with _on(x):
+        check(lib.jq_conv_forward(C.byref(v), _stream(x)))
+    return out, final
+
+
+class _Conv(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, initial, starts, lengths, silu, with_state):
+        out, final = _conv_forward(x, weight, bias, initial, starts, lengths, silu, with_state)
+        ctx.save_for_backward(x, weight, bias, initial, starts, lengths)
+        ctx.silu = silu
+        ctx.set_materialize_grads(False)
+        return out, final
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, d_out, d_final):
+        x, weight, bias, initial, starts, lengths = ctx.saved_tensors
+        if d_out is None and d_final is None:
+            return (None,) * 8
+        d_out = torch.zeros_like(x) if d_out is None else _adjacent(d_out)
+        v = _conv_args(x, weight, bias, ctx.silu)
+        _set_segments(v, starts, lengths)
+        need = ctx.needs_input_grad
+        dx = _like_plies(x) if need[0] else None
+        dw = torch.empty_like(weight) if need[1] else None
+        db = torch.empty_like(bias) if need[2] else None
+        d_initial = torch.empty_like(initial) if need[3] else None
+        if d_final is not None:
+            d_final = d_final.contiguous()
+        v.initial_state, v.d_out = _ptr(initial), _plies(d_out)
+        if dx is not None:
+            v.dx = _plies(dx)
+        v.dweight, v.dbias, v.d_final, v.d_initial = _ptr(dw), _ptr(db), _ptr(d_final), _ptr(d_initial)
+        size = C.c_int64()
+        with _on(x):
+            check(lib.jq_conv_workspace(C.byref(v), C.byref(size)))
+            work = _give_workspace(v, size, x)   # noqa: F841
+            check(lib.jq_conv_backward(C.byref(v), _stream(x)))
+        return dx, dw, db, d_initial, None, None, None, None
+
+
+def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *, silu: bool = False,
+                starts: torch.Tensor | None = None, lengths: torch.Tensor | None = None,
+                initial_state: torch.Tensor | None = None, return_state: bool = False):
+    """A causal convolution of each channel over its last few plies, as it stands before
+    `selective_scan`.
+
+        out[t] = bias[d] + sum over j < taps of weight[d, j] * x[t - taps + 1 + j],
+
+    then silu(out) if ``silu``. ``x`` (B, T, D) float32 or bfloat16, any strides;
+    ``weight`` (D, taps), up to 8 taps, and ``bias`` (D,) float32 or of x's type, both
+    of one. Inputs before a game's start (``starts``) are 0, those before the first ply
+    are ``initial_state`` (B, taps - 1, D) of x's type, the oldest first (zeros if
+    None); ``lengths`` as in `linear_attention`. Returns ``out`` (B, T, D), or with
+    ``return_state`` also the last taps - 1 inputs of each game, to go on from.
+
+    Differentiable in x, weight, bias and initial_state; the gradients of weight and
+    bias are summed in a fixed order."""
+    x, weight, bias = _check_conv(x, weight, bias, 2)
+    b, t, d = x.shape
+    lengths = _check_segments(starts, lengths, b, t, x)
+    if initial_state is not None:
+        _check("initial_state", initial_state, (b, weight.shape[1] - 1, d), (x.dtype,), x)
+        initial_state = initial_state.contiguous()
+    args = (x, weight, bias, initial_state, starts, lengths, bool(silu), return_state)
+    out, state = (_Conv.apply if _differentiated(*args[:4]) else _conv_forward)(*args)
+    return (out, state) if return_state else out
+
+
+def causal_conv_step(x: torch.Tensor, weight: torch.Tensor, state: torch.Tensor, bias: torch.Tensor | None = None, *,
+                     silu: bool = False, rows: torch.Tensor | None = None, starts: torch.Tensor | None = None,
+                     out: torch.Tensor | None = None) -> torch.Tensor:
+    """`causal_conv` of one new ply of each game, its last inputs updated in place.
+
+    ``x`` (B, D); ``state`` (R, taps - 1, D) of x's type, contiguous; ``rows``,
+    ``starts`` and ``out`` as in `linear_attention_step`: a game whose row is outside
+    [0, R) is left out, its output 0, and no row may be named twice. Returns (B, D).
+    Not differentiable."""
+    given = (x, weight, bias)
+    x, weight, bias = _check_conv(*given, 1)
+    rows, starts, out = _check_step("causal_conv", x, state, (weight.shape[1] - 1, x.shape[1]), x.dtype, rows, starts, out,
+                                    given)
+    v = _conv_args(x, weight, bias, bool(silu), _ply)
+    v.out = _ply(out)
+    with _on(x):
+        check(lib.jq_conv_step(C.byref(v), state.data_ptr(), state.shape[0], _ptr(rows), _ptr(starts), _stream(x)))
+    increment_version((state, out))
+    return out
