@@ -54,7 +54,7 @@ int check_scan(const jq_scan *a)
 int check_scan_inputs(const jq_scan *a)
 {
     if (!a->a) return fail(JQ_E_ARG, "null a");
-    if (a->plies == 0) return JQ_OK;
+    if (a->plies == 0 || a->batch == 0) return JQ_OK;
     TRY(check_rows(a->u, a->dtype, "u"));
     TRY(check_rows(a->delta, a->dtype, "delta"));
     TRY(check_rows(a->b, a->dtype, "b"));
@@ -199,7 +199,7 @@ int check_conv_inputs(const jq_conv *a)
     TRY(check_state_pointer(a->weight, a->weight_dtype, "weight"));
     TRY(check_state_pointer(a->bias, a->weight_dtype, "bias"));
     TRY(check_state_pointer(a->initial_state, a->dtype, "initial_state"));
-    if (a->plies) TRY(check_rows(a->x, a->dtype, "x"));
+    if (a->plies && a->batch) TRY(check_rows(a->x, a->dtype, "x"));
     return JQ_OK;
 }
 
@@ -350,11 +350,11 @@ int jq_scan_backward(const jq_scan *a, void *stream)
 {
     TRY(check_scan(a));
     TRY(check_scan_inputs(a));
-    if (a->plies) TRY(check_rows(a->d_out, a->dtype, "d_out"));
+    if (a->plies && a->batch) TRY(check_rows(a->d_out, a->dtype, "d_out"));
     if (a->plies && a->batch && !a->saved) return fail(JQ_E_ARG, "null saved");
     if (a->dgate.data && !a->gate.data) return fail(JQ_E_ARG, "dgate without a gate");
     for (const jq_rows *r : {&a->du, &a->ddelta, &a->dgate, &a->db, &a->dc})
-        if (r->data) TRY(check_rows(*r, a->dtype, "a gradient"));
+        if (r->data) TRY(check_rows(*r, a->dtype, "a gradient"));   // absent ones are not wanted
     TRY(check_scan_workspace(a, true));
     SelectArgs s = select_args(a, true);
     s.d_out = a->d_out, s.du = a->du, s.ddelta = a->ddelta, s.dgate = a->dgate;
@@ -440,7 +440,7 @@ int jq_conv_backward(const jq_conv *a, void *stream)
 {
     TRY(check_conv(a));
     TRY(check_conv_inputs(a));
-    if (a->plies) TRY(check_rows(a->d_out, a->dtype, "d_out"));
+    if (a->plies && a->batch) TRY(check_rows(a->d_out, a->dtype, "d_out"));
     if (a->dx.data) TRY(check_rows(a->dx, a->dtype, "dx"));
     TRY(check_state_pointer(a->d_final, a->dtype, "d_final"));
     TRY(check_state_pointer(a->d_initial, a->dtype, "d_initial"));
