@@ -510,7 +510,7 @@ int jq_layer_norm_backward(int32_t dtype, int32_t weight_dtype, int64_t rows, in
 /* ---- a policy's selective memory -----------------------------------------------
  * A state space scan whose steps depend on the input, and the short causal
  * convolution before it, beside the operators above and under the same terms.
- * plies stay at or below 2^30, channels at or below 2^20. */
+ * Games and plies stay at or below 2^30, channels at or below 2^20. */
 #define JQ_SCAN_MAX_STATES 64
 #define JQ_CONV_MAX_TAPS 8
 

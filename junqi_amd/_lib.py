@@ -23,7 +23,7 @@ ROTARY_MAX_PAIRS = 4096
 SCAN_MAX_STATES = 64
 CONV_MAX_TAPS = 8
 MASK_WORDS_PACKED, MASK_BYTES = 0, 1
-MOST_CHANNELS, MOST_PLIES = 1 << 20, 1 << 30
+MOST_CHANNELS, MOST_PLIES, MOST_GAMES = 1 << 20, 1 << 30, 1 << 30
 NUM_CELLS = 289
 NUM_ON_BOARD = 129
 NUM_PIDS = 120

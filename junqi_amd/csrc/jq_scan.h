@@ -69,11 +69,60 @@ template <class F, int... I> __device__ __forceinline__ void each_of(F &&f, std:
 }
 template <int N, class F> __device__ __forceinline__ void each_of(F &&f) { each_of(f, std::make_integer_sequence<int, N>()); }
 
-// x of lane I of each row of 16 lanes, as an operand.
+// x of lane I of each row of 16 lanes: an operand of the product that takes it.
 template <int I> __device__ __forceinline__ float row_lane(float x)
 {
     return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), 0x150 + I, 0xF, 0xF, true));
 }
+
+// The compiler folds such an operand into products, not into fused ones, which would take
+// a move for each. In these its two wait states after the operand's write come first.
+#define JQ_ROW_FMAC(d, i, s) "v_fmac_f32_dpp " d ", %[x], " s " row_newbcast:" #i " row_mask:0xf bank_mask:0xf\n"
+
+// y + the sum of row_lane<i>(x) h[i]
+__device__ __forceinline__ float row_dot(float y, float x, const float (&h)[4])
+{
+    asm("s_nop 1\n" JQ_ROW_FMAC("%[y]", 0, "%[a]") JQ_ROW_FMAC("%[y]", 1, "%[b]") JQ_ROW_FMAC("%[y]", 2, "%[c]") JQ_ROW_FMAC("%[y]", 3, "%[d]")
+        : [y] "+v"(y) : [x] "v"(x), [a] "v"(h[0]), [b] "v"(h[1]), [c] "v"(h[2]), [d] "v"(h[3]));
+    return y;
+}
+__device__ __forceinline__ float row_dot(float y, float x, const float (&h)[8])
+{
+    asm("s_nop 1\n" JQ_ROW_FMAC("%[y]", 0, "%[a]") JQ_ROW_FMAC("%[y]", 1, "%[b]") JQ_ROW_FMAC("%[y]", 2, "%[c]") JQ_ROW_FMAC("%[y]", 3, "%[d]")
+        JQ_ROW_FMAC("%[y]", 4, "%[e]") JQ_ROW_FMAC("%[y]", 5, "%[f]") JQ_ROW_FMAC("%[y]", 6, "%[g]") JQ_ROW_FMAC("%[y]", 7, "%[h]")
+        : [y] "+v"(y) : [x] "v"(x), [a] "v"(h[0]), [b] "v"(h[1]), [c] "v"(h[2]), [d] "v"(h[3]), [e] "v"(h[4]), [f] "v"(h[5]),
+          [g] "v"(h[6]), [h] "v"(h[7]));
+    return y;
+}
+__device__ __forceinline__ float row_dot(float y, float x, const float (&h)[16])
+{
+    asm("s_nop 1\n" JQ_ROW_FMAC("%[y]", 0, "%[a]") JQ_ROW_FMAC("%[y]", 1, "%[b]") JQ_ROW_FMAC("%[y]", 2, "%[c]") JQ_ROW_FMAC("%[y]", 3, "%[d]")
+        JQ_ROW_FMAC("%[y]", 4, "%[e]") JQ_ROW_FMAC("%[y]", 5, "%[f]") JQ_ROW_FMAC("%[y]", 6, "%[g]") JQ_ROW_FMAC("%[y]", 7, "%[h]")
+        JQ_ROW_FMAC("%[y]", 8, "%[i]") JQ_ROW_FMAC("%[y]", 9, "%[j]") JQ_ROW_FMAC("%[y]", 10, "%[k]") JQ_ROW_FMAC("%[y]", 11, "%[l]")
+        JQ_ROW_FMAC("%[y]", 12, "%[m]") JQ_ROW_FMAC("%[y]", 13, "%[n]") JQ_ROW_FMAC("%[y]", 14, "%[o]") JQ_ROW_FMAC("%[y]", 15, "%[p]")
+        : [y] "+v"(y) : [x] "v"(x), [a] "v"(h[0]), [b] "v"(h[1]), [c] "v"(h[2]), [d] "v"(h[3]), [e] "v"(h[4]), [f] "v"(h[5]),
+          [g] "v"(h[6]), [h] "v"(h[7]), [i] "v"(h[8]), [j] "v"(h[9]), [k] "v"(h[10]), [l] "v"(h[11]), [m] "v"(h[12]),
+          [n] "v"(h[13]), [o] "v"(h[14]), [p] "v"(h[15]));
+    return y;
+}
+
+// v[i] += row_lane<FIRST + i>(x) y for four i
+template <int FIRST> __device__ __forceinline__ void row_add4(float &a, float &b, float &c, float &d, float x, float y)
+{
+#define JQ_ROW_ADD(i0, i1, i2, i3)                                                                                           \
+    asm("s_nop 1\n" JQ_ROW_FMAC("%[a]", i0, "%[y]") JQ_ROW_FMAC("%[b]", i1, "%[y]") JQ_ROW_FMAC("%[c]", i2, "%[y]")          \
+        JQ_ROW_FMAC("%[d]", i3, "%[y]") : [a] "+v"(a), [b] "+v"(b), [c] "+v"(c), [d] "+v"(d) : [x] "v"(x), [y] "v"(y))
+    if constexpr (FIRST == 0) JQ_ROW_ADD(0, 1, 2, 3);
+    else if constexpr (FIRST == 4) JQ_ROW_ADD(4, 5, 6, 7);
+    else if constexpr (FIRST == 8) JQ_ROW_ADD(8, 9, 10, 11);
+    else JQ_ROW_ADD(12, 13, 14, 15);
+#undef JQ_ROW_ADD
+}
+template <int N> __device__ __forceinline__ void row_add(float (&v)[N], float x, float y)
+{
+    each_of<N / 4>([&](auto q) { row_add4<4 * q>(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3], x, y); });
+}
+#undef JQ_ROW_FMAC
 
 template <int HOW> __device__ __forceinline__ float across(float x)
 {
@@ -117,115 +166,181 @@ __device__ __forceinline__ float lane_sums(float (&v)[N])
     return v[0];
 }
 
-// Where this wave's lanes are: channel, states, rows.
-template <class T, int NS>
-struct Place {
-    int lane, sg, group, ch, n0, row_n;
-    bool on, row_on;
-    __device__ __forceinline__ Place(const SelectArgs &a, int cw)
+// The arguments, read where they are used: held in scalar registers over a pass, those of
+// a dozen tensors would be spilled to vector registers. `hidden` keeps the compiler from
+// moving the reads up to the pass's start.
+typedef const __attribute__((address_space(4))) SelectArgs *SelectArgsPtr;
+typedef const __attribute__((address_space(4))) jq_rows *RowsPtr;
+__device__ __forceinline__ SelectArgsPtr hidden(SelectArgsPtr a)
+{
+    asm volatile("" : "+s"(a));
+    return a;
+}
+__device__ __forceinline__ SelectArgsPtr select_arguments() { return (SelectArgsPtr)__builtin_amdgcn_kernarg_segment_ptr(); }
+
+// Memory behind a wave's own address, at each lane's offset: an offset of NOWHERE reads 0
+// and writes nothing, as all do where `really` is false.
+constexpr uint32_t NOWHERE = 0x80000000u;
+struct Window {
+    char *base;
+    template <class T> __device__ __forceinline__ T get(uint32_t at, uint32_t more = 0, bool really = true) const
     {
-        lane = threadIdx.x % 64;
-        sg = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-        group = cw / a.waves;
-        const int at = (cw % a.waves) * 64 + lane;
-        on = at < a.per;
-        ch = group * a.per + (on ? at : a.per - 1);
-        n0 = sg * NS;
-        row_n = n0 + lane % 16;
-        row_on = lane % 16 < NS && row_n < a.states;
+        const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(base, 0, really ? (int)(NOWHERE - 1) : 0, 0x00020000);
+        if constexpr (sizeof(T) == 2) return __builtin_bit_cast(T, (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(r, at, more, 0));
+        else return __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b32(r, at, more, 0));
     }
-    template <class F> __device__ __forceinline__ void a2(const SelectArgs &a, F &&f) const
+    template <class T> __device__ __forceinline__ void put(uint32_t at, T x, uint32_t more = 0) const
     {
-#pragma unroll
-        for (int i = 0; i < NS; ++i) f(i, n0 + i < a.states ? a.a[(int64_t)ch * a.states + n0 + i] * LOG2E : 0.f);
+        const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(base, 0, (int)(NOWHERE - 1), 0x00020000);
+        if constexpr (sizeof(T) == 2) __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, x), r, at, more, 0);
+        else __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, x), r, at, more, 0);
     }
 };
 
-template <class T> __device__ __forceinline__ const T *at_ply(const jq_rows &r, int64_t b, int64_t t, int64_t h)
+// A tensor's row of ply t, and the bytes from one ply's to the next.
+template <class T> __device__ __forceinline__ Window row_window(RowsPtr r, int64_t b, int64_t t, int64_t h)
 {
-    return row_at<const T>(r, b, t, h);
+    return Window{static_cast<char *>(r->data) + (b * r->batch + t * r->ply + h * r->head) * (int64_t)sizeof(T)};
+}
+template <class T> __device__ __forceinline__ int64_t row_step(RowsPtr r) { return r->ply * (int64_t)sizeof(T); }
+
+// Where this wave's lanes are: channel, states, rows. EXACT: every lane has a channel and
+// each of its states.
+template <class T, int NS, bool EXACT>
+struct Place {
+    int lane, sg, group, ch, n0, states;
+    uint32_t at, row_at, at4;   // bytes into a row of channels, of a group's states, and of channels in float32
+    bool on_;
+    __device__ __forceinline__ Place(SelectArgsPtr a, int cw)
+    {
+        lane = threadIdx.x % 64;
+        sg = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+        group = cw / a->waves;
+        states = a->states;
+        const int c = (cw % a->waves) * 64 + lane;
+        on_ = c < a->per;
+        ch = group * a->per + (on_ ? c : a->per - 1);
+        n0 = sg * NS;
+        const int n = n0 + lane % 16;
+        at = on_ ? (uint32_t)ch * sizeof(T) : NOWHERE;
+        at4 = on_ ? (uint32_t)ch * 4 : NOWHERE;
+        row_at = lane % 16 < NS && n < a->states ? (uint32_t)n * sizeof(T) : NOWHERE;
+    }
+    __device__ __forceinline__ bool on() const { return EXACT || on_; }
+    __device__ __forceinline__ bool has(int i) const { return EXACT || n0 + i < states; }
+    // a, in powers of 2
+    __device__ __forceinline__ void rates(SelectArgsPtr a, float (&A)[NS]) const
+    {
+#pragma unroll
+        for (int i = 0; i < NS; ++i) A[i] = has(i) ? a->a[(int64_t)ch * states + n0 + i] * LOG2E : 0.f;
+    }
+};
+
+// The same for the wave, which a load alone does not say.
+__device__ __forceinline__ int live_plies(const int32_t *lengths, int b, int plies)
+{
+    return lengths ? min(max(__builtin_amdgcn_readfirstlane(lengths[b]), 0), plies) : plies;
 }
 
-__device__ __forceinline__ int live_plies(const SelectArgs &a, int b)
+// Bit k: a game starts at ply t0 + k, k < 8; plies from `end` on are not looked at.
+__device__ __forceinline__ uint32_t starts_of(SelectArgsPtr a, int b, int t0, int end, int lane)
 {
-    return a.lengths ? min(max(a.lengths[b], 0), a.plies) : a.plies;
+    if (!a->starts) return 0;
+    const int k = lane & 7, t = min(t0 + k, end - 1);
+    return __builtin_amdgcn_ballot_w64(a->starts[b * a->starts_batch + t * a->starts_ply] != 0 && t0 + k < end) & 0xFF;
 }
 
-// Bit k: a game starts at ply t0 + k, k < 8.
-__device__ __forceinline__ uint32_t starts_of(const SelectArgs &a, int b, int t0, int end, int lane)
+// The states of this lane in a (.., channels, states) tensor's row, or in a (.., states, channels) one's.
+template <class T, int NS, bool EXACT>
+__device__ __forceinline__ void load_states(const Place<T, NS, EXACT> &p, float (&h)[NS], const float *row)
 {
-    if (!a.starts) return 0;
-    const int t = min(t0 + (lane & 7), end - 1);
-    return __builtin_amdgcn_ballot_w64(a.starts[b * a.starts_batch + t * a.starts_ply] != 0) & 0xFF;
+#pragma unroll
+    for (int i = 0; i < NS; ++i) h[i] = row && p.has(i) ? row[(int64_t)p.ch * p.states + p.n0 + i] : 0.f;
+}
+template <class T, int NS, bool EXACT>
+__device__ __forceinline__ void store_states(const Place<T, NS, EXACT> &p, const float (&h)[NS], float *row)
+{
+    if (p.on())
+#pragma unroll
+        for (int i = 0; i < NS; ++i)
+            if (p.has(i)) row[(int64_t)p.ch * p.states + p.n0 + i] = h[i];
+}
+template <class T, int NS, bool EXACT>
+__device__ __forceinline__ void load_apart(const Place<T, NS, EXACT> &p, float (&h)[NS], const float *row, int channels, bool really = true)
+{
+    const Window from{reinterpret_cast<char *>(const_cast<float *>(row))};
+    uint32_t more = p.n0 * channels * 4;
+#pragma unroll
+    for (int i = 0; i < NS; ++i, more += channels * 4) h[i] = p.has(i) ? from.get<float>(p.at4, more, really) : 0.f;
+}
+template <class T, int NS, bool EXACT>
+__device__ __forceinline__ void store_apart(const Place<T, NS, EXACT> &p, const float (&h)[NS], float *row, int channels)
+{
+    const Window to{reinterpret_cast<char *>(row)};
+    uint32_t more = p.n0 * channels * 4;
+#pragma unroll
+    for (int i = 0; i < NS; ++i, more += channels * 4)
+        if (p.has(i)) to.put(p.at4, h[i], more);
 }
 
 template <class T, int NS, bool EXACT, bool OUT>
-__global__ __launch_bounds__(256) void k_scan_forward(SelectArgs a)
+__global__ __launch_bounds__(256) void k_scan_forward(SelectArgs)
 {
-    extern __shared__ float lds[];   // more than one wave of states: [2][SG][SCAN_PLIES][64] shares of y
-    const int SG = blockDim.x / 64, CW = a.waves * a.groups;
-    const Place<T, NS> p(a, blockIdx.x % CW);
+    constexpr int K = SCAN_PLIES;
+    extern __shared__ float lds[];   // more than one wave of states: [2][SG][K][64] shares of y
+    const SelectArgsPtr a = hidden(select_arguments());
+    const int SG = blockDim.x / 64, CW = a->waves * a->groups;
+    const Place<T, NS, EXACT> p(a, blockIdx.x % CW);
     float A[NS], h[NS];
-    p.a2(a, [&](int i, float x) { A[i] = x; });
-    const float skip = a.skip ? a.skip[p.ch] : 0.f, bias = a.bias ? a.bias[p.ch] : 0.f;
-    const bool gated = OUT && a.gate.data;
-    struct Raw { T u[SCAN_PLIES], delta[SCAN_PLIES], gate[SCAN_PLIES], b[SCAN_PLIES], c[SCAN_PLIES]; };
-    const int64_t items = (int64_t)a.batch * a.segments;
+    p.rates(a, A);
+    const bool skips = a->skip, gated = OUT && a->gate.data, soft = a->softplus, saves = OUT && a->saved;
+    const float skip = skips ? a->skip[p.ch] : 0.f, bias = a->bias ? a->bias[p.ch] : 0.f;
+    struct Raw { T u[K], delta[K], gate[K], b[K], c[K]; };
+    const int items = a->batch * a->segments, channels = a->channels;
+    const int64_t state_bytes = (int64_t)p.states * channels * 4;
     int turn = 0;
-    for (int64_t item = blockIdx.x / CW; item < items; item += gridDim.x / CW) {
-        const int b = item / a.segments, seg = item % a.segments;
-        const int len = live_plies(a, b), begin = seg * a.seg_plies, stop = min(begin + a.seg_plies, a.plies);
-        const int end = min(stop, len);
-#pragma unroll
-        for (int i = 0; i < NS; ++i) {
-            h[i] = 0.f;
-            const int n = p.n0 + i;
-            if (!OUT || n >= a.states) continue;
-            if (seg) h[i] = a.seg_state[((int64_t)(b * (int64_t)a.segments + seg) * a.states + n) * a.channels + p.ch];
-            else if (a.s_in) h[i] = a.s_in[((int64_t)b * a.channels + p.ch) * a.states + n];
-        }
+    for (int item = blockIdx.x / CW; item < items; item += gridDim.x / CW) {
+        SelectArgsPtr q = hidden(a);
+        const int b = item / q->segments, seg = item % q->segments;
+        const int begin = seg * q->seg_plies, stop = min(begin + q->seg_plies, q->plies), end = min(stop, live_plies(q->lengths, b, q->plies));
+        if (OUT && seg) load_apart(p, h, q->seg_state + (int64_t)item * p.states * channels, channels);
+        else load_states(p, h, OUT && q->s_in ? q->s_in + (int64_t)b * channels * p.states : nullptr);
         float total = 0.f;
-        auto fetch = [&](int t0, Raw &r) {
+        Window wu = row_window<T>(&q->u, b, begin, 0), wd = row_window<T>(&q->delta, b, begin, 0), wz = row_window<T>(&q->gate, b, begin, 0),
+               wb = row_window<T>(&q->b, b, begin, p.group), wc = row_window<T>(&q->c, b, begin, p.group), wo = row_window<T>(&q->out, b, begin, 0);
+        Window save{reinterpret_cast<char *>(q->saved) + ((int64_t)b * ((q->plies + SCAN_CHUNK - 1) / SCAN_CHUNK) + begin / SCAN_CHUNK) * state_bytes};
+        auto fetch = [&](int t0, Raw &r, uint32_t &starts) {
+            const SelectArgsPtr q = hidden(a);
+            const int64_t su = row_step<T>(&q->u), sd = row_step<T>(&q->delta), sz = row_step<T>(&q->gate), sb = row_step<T>(&q->b), sc = row_step<T>(&q->c);
 #pragma unroll
-            for (int k = 0; k < SCAN_PLIES; ++k) {
-                const int t = min(t0 + k, end - 1);
-                r.u[k] = at_ply<T>(a.u, b, t, 0)[p.ch];
-                r.delta[k] = at_ply<T>(a.delta, b, t, 0)[p.ch];
-                if (gated) r.gate[k] = at_ply<T>(a.gate, b, t, 0)[p.ch];
-                r.b[k] = r.c[k] = T(0.f);
-                if (p.row_on) {
-                    r.b[k] = at_ply<T>(a.b, b, t, p.group)[p.row_n];
-                    if (OUT) r.c[k] = at_ply<T>(a.c, b, t, p.group)[p.row_n];
-                }
+            for (int k = 0; k < K; ++k) {
+                const bool there = t0 + k < end;
+                r.u[k] = wu.get<T>(p.at, 0, there);
+                r.delta[k] = wd.get<T>(p.at, 0, there);
+                if (gated) r.gate[k] = wz.get<T>(p.at, 0, there);
+                r.b[k] = wb.get<T>(p.row_at, 0, there);
+                if (OUT) r.c[k] = wc.get<T>(p.row_at, 0, there);
+                wu.base += su, wd.base += sd, wz.base += sz, wb.base += sb, wc.base += sc;
             }
+            starts = starts_of(q, b, t0, end, p.lane);
         };
         Raw next;
         uint32_t next_starts = 0;
-        if (begin < end) {
-            fetch(begin, next);
-            next_starts = starts_of(a, b, begin, end, p.lane);
-        }
-        for (int t0 = begin; t0 < end; t0 += SCAN_PLIES) {
+        if (begin < end) fetch(begin, next, next_starts);
+        for (int t0 = begin; t0 < end; t0 += K) {
             const Raw r = next;
             const uint32_t starts = next_starts;
-            if (t0 + SCAN_PLIES < end) {
-                fetch(t0 + SCAN_PLIES, next);
-                next_starts = starts_of(a, b, t0 + SCAN_PLIES, end, p.lane);
+            if (t0 + K < end) fetch(t0 + K, next, next_starts);
+            if (saves && t0 % SCAN_CHUNK == 0) {
+                store_apart(p, h, reinterpret_cast<float *>(save.base), channels);
+                save.base += state_bytes;
             }
-            if (OUT && a.saved && t0 % SCAN_CHUNK == 0 && p.on) {
-                const int chunks = (a.plies + SCAN_CHUNK - 1) / SCAN_CHUNK;
-                float *to = a.saved + ((int64_t)b * chunks + t0 / SCAN_CHUNK) * a.states * a.channels + p.ch;
+            const int64_t step = OUT ? row_step<T>(&hidden(a)->out) : 0;
 #pragma unroll
-                for (int i = 0; i < NS; ++i)
-                    if (p.n0 + i < a.states) to[(int64_t)(p.n0 + i) * a.channels] = h[i];
-            }
-            float y[SCAN_PLIES];
-#pragma unroll
-            for (int k = 0; k < SCAN_PLIES; ++k) {
-                y[k] = 0.f;
-                if (t0 + k >= end) continue;
-                const float u = (float)r.u[k], pre = (float)r.delta[k] + bias, dt = a.softplus ? softplus(pre) : pre;
-                const float push = dt * u, bt = (float)r.b[k], ct = (float)r.c[k];
+            for (int k = 0; k < K; ++k) {
+                if (t0 + k >= end) break;
+                const float u = (float)r.u[k], pre = (float)r.delta[k] + bias, dt = soft ? softplus(pre) : pre;
+                const float push = dt * u, bt = (float)r.b[k];
                 if (starts >> k & 1) {
 #pragma unroll
                     for (int i = 0; i < NS; ++i) h[i] = 0.f;
@@ -233,48 +348,43 @@ __global__ __launch_bounds__(256) void k_scan_forward(SelectArgs a)
                 }
                 if (!OUT) total += dt;
                 each_of<NS>([&](auto i) {
-                    h[i] = fmaf(row_lane<i>(bt), push, exp2_fast(dt * A[i]) * h[i]);
-                    if (!EXACT && p.n0 + i >= a.states) h[i] = 0.f;
-                    if (OUT) y[k] = fmaf(row_lane<i>(ct), h[i], y[k]);
+                    h[i] = fmaf(exp2_fast(dt * A[i]), h[i], row_lane<i>(bt) * push);
+                    if (!p.has(i)) h[i] = 0.f;
                 });
-            }
-            if (!OUT) continue;
-            if (SG > 1) {
-                float *mine = lds + (turn & 1) * SG * SCAN_PLIES * 64;
-#pragma unroll
-                for (int k = 0; k < SCAN_PLIES; ++k) mine[(p.sg * SCAN_PLIES + k) * 64 + p.lane] = y[k];
-                __syncthreads();
-            }
-#pragma unroll
-            for (int k = 0; k < SCAN_PLIES; ++k) {
-                if (t0 + k >= end) continue;
-                if (SG > 1) {
-                    if (k % SG != p.sg) continue;
-                    const float *all = lds + (turn & 1) * SG * SCAN_PLIES * 64 + k * 64 + p.lane;
-                    y[k] = 0.f;
-                    for (int g = 0; g < SG; ++g) y[k] += all[g * SCAN_PLIES * 64];
+                if (!OUT) continue;
+                const float y = row_dot(0.f, (float)r.c[k], h);
+                if (SG > 1) lds[(((turn & 1) * SG + p.sg) * K + k) * 64 + p.lane] = y;
+                else {
+                    float o = skips ? fmaf(skip, u, y) : y;
+                    if (gated) o *= (float)r.gate[k] * sigmoid((float)r.gate[k]);
+                    wo.put<T>(p.at, from_float<T>(o));
+                    wo.base += step;
                 }
-                float o = a.skip ? fmaf(skip, (float)r.u[k], y[k]) : y[k];
-                if (gated) {
-                    const float z = (float)r.gate[k];
-                    o *= z * sigmoid(z);
+            }
+            if (!OUT || SG == 1) continue;
+            __syncthreads();
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                if (t0 + k >= end) break;
+                if (k % SG == p.sg) {
+                    float o = 0.f;
+                    for (int g = 0; g < SG; ++g) o += lds[(((turn & 1) * SG + g) * K + k) * 64 + p.lane];
+                    if (skips) o = fmaf(skip, (float)r.u[k], o);
+                    if (gated) o *= (float)r.gate[k] * sigmoid((float)r.gate[k]);
+                    wo.put<T>(p.at, from_float<T>(o));
                 }
-                if (p.on) row_at<T>(a.out, b, t0 + k, 0)[p.ch] = from_float<T>(o);
+                wo.base += step;
             }
             ++turn;   // the other buffer: the one before is read by then
         }
+        q = hidden(a);
         if (OUT) {
-            for (int t = max(begin, end) + p.sg; t < stop; t += SG)
-                if (p.on) row_at<T>(a.out, b, t, 0)[p.ch] = T(0.f);
-            if (a.s_out && seg == a.segments - 1 && p.on)
-#pragma unroll
-                for (int i = 0; i < NS; ++i)
-                    if (p.n0 + i < a.states) a.s_out[((int64_t)b * a.channels + p.ch) * a.states + p.n0 + i] = h[i];
-        } else if (p.on) {
-#pragma unroll
-            for (int i = 0; i < NS; ++i)
-                if (p.n0 + i < a.states) a.seg_state[(item * a.states + p.n0 + i) * a.channels + p.ch] = h[i];
-            if (p.sg == 0) a.seg_sum[item * a.channels + p.ch] = total;
+            for (int t = max(begin, end); t < stop; ++t)
+                if (t % SG == p.sg) row_window<T>(&q->out, b, t, 0).template put<T>(p.at, T(0.f));
+            if (q->s_out && seg == q->segments - 1) store_states(p, h, q->s_out + (int64_t)b * channels * p.states);
+        } else {
+            store_apart(p, h, q->seg_state + (int64_t)item * p.states * channels, channels);
+            if (p.sg == 0 && p.on()) q->seg_sum[(int64_t)item * channels + p.ch] = total;
         }
     }
 }
@@ -306,44 +416,49 @@ __global__ __launch_bounds__(256) void k_scan_join(SelectArgs a)
 // Backward over a part of the axis: what its gradients of y send to the state before it
 // (seg_state, seg_sum), in reverse.
 template <class T, int NS, bool EXACT>
-__global__ __launch_bounds__(256) void k_scan_carry(SelectArgs a)
+__global__ __launch_bounds__(256) void k_scan_carry(SelectArgs)
 {
-    const int CW = a.waves * a.groups;
-    const Place<T, NS> p(a, blockIdx.x % CW);
+    constexpr int K = SCAN_CHUNK;
+    const SelectArgsPtr a = hidden(select_arguments());
+    const int CW = a->waves * a->groups, items = a->batch * a->segments, channels = a->channels;
+    const Place<T, NS, EXACT> p(a, blockIdx.x % CW);
     float A[NS], dh[NS];
-    p.a2(a, [&](int i, float x) { A[i] = x; });
-    const float bias = a.bias ? a.bias[p.ch] : 0.f;
-    const int64_t items = (int64_t)a.batch * a.segments;
-    for (int64_t item = blockIdx.x / CW; item < items; item += gridDim.x / CW) {
-        const int b = item / a.segments, seg = item % a.segments;
-        const int begin = seg * a.seg_plies, end = min(min(begin + a.seg_plies, a.plies), live_plies(a, b));
+    p.rates(a, A);
+    const bool gated = a->gate.data, soft = a->softplus;
+    const float bias = a->bias ? a->bias[p.ch] : 0.f;
+    for (int item = blockIdx.x / CW; item < items; item += gridDim.x / CW) {
+        SelectArgsPtr q = hidden(a);
+        const int b = item / q->segments, seg = item % q->segments;
+        const int begin = seg * q->seg_plies, end = min(min(begin + q->seg_plies, q->plies), live_plies(q->lengths, b, q->plies));
 #pragma unroll
         for (int i = 0; i < NS; ++i) dh[i] = 0.f;
         float total = 0.f;
-        for (int t0 = begin + (max(end - begin, 1) - 1) / 8 * 8; t0 >= begin && begin < end; t0 -= 8) {
-            const uint32_t starts = starts_of(a, b, t0, end, p.lane);
-            T delta[8], gate[8], d_out[8], c[8];
+        const int top = begin + (max(end - begin, 1) - 1) / K * K;
+        for (int t0 = top; t0 >= begin && begin < end; t0 -= K) {
+            T delta[K], gate[K], d_out[K], c[K];
+            q = hidden(a);
+            const uint32_t starts = starts_of(q, b, t0, end, p.lane);
+            Window wd = row_window<T>(&q->delta, b, t0, 0), wz = row_window<T>(&q->gate, b, t0, 0), wg = row_window<T>(&q->d_out, b, t0, 0),
+                   wc = row_window<T>(&q->c, b, t0, p.group);
+            const int64_t sd = row_step<T>(&q->delta), sz = row_step<T>(&q->gate), sg = row_step<T>(&q->d_out), sc = row_step<T>(&q->c);
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const int t = min(t0 + k, end - 1);
-                delta[k] = at_ply<T>(a.delta, b, t, 0)[p.ch];
-                d_out[k] = at_ply<T>(a.d_out, b, t, 0)[p.ch];
-                if (a.gate.data) gate[k] = at_ply<T>(a.gate, b, t, 0)[p.ch];
-                c[k] = p.row_on ? at_ply<T>(a.c, b, t, p.group)[p.row_n] : T(0.f);
+            for (int k = 0; k < K; ++k) {
+                const bool there = t0 + k < end;
+                delta[k] = wd.get<T>(p.at, 0, there);
+                d_out[k] = wg.get<T>(p.at, 0, there);
+                if (gated) gate[k] = wz.get<T>(p.at, 0, there);
+                c[k] = wc.get<T>(p.row_at, 0, there);
+                wd.base += sd, wz.base += sz, wg.base += sg, wc.base += sc;
             }
 #pragma unroll
-            for (int k = 7; k >= 0; --k) {
+            for (int k = K - 1; k >= 0; --k) {
                 if (t0 + k >= end) continue;
-                const float pre = (float)delta[k] + bias, dt = a.softplus ? softplus(pre) : pre, ct = (float)c[k];
+                const float pre = (float)delta[k] + bias, dt = soft ? softplus(pre) : pre;
                 float dy = (float)d_out[k];
-                if (a.gate.data) {
-                    const float z = (float)gate[k];
-                    dy *= z * sigmoid(z);
-                }
-                each_of<NS>([&](auto i) {
-                    dh[i] = exp2_fast(dt * A[i]) * fmaf(row_lane<i>(ct), dy, dh[i]);
-                    if (!EXACT && p.n0 + i >= a.states) dh[i] = 0.f;
-                });
+                if (gated) dy *= (float)gate[k] * sigmoid((float)gate[k]);
+                row_add(dh, (float)c[k], dy);
+#pragma unroll
+                for (int i = 0; i < NS; ++i) dh[i] = p.has(i) ? dh[i] * exp2_fast(dt * A[i]) : 0.f;
                 total += dt;
                 if (starts >> k & 1) {
 #pragma unroll
@@ -352,11 +467,9 @@ __global__ __launch_bounds__(256) void k_scan_carry(SelectArgs a)
                 }
             }
         }
-        if (!p.on) continue;
-#pragma unroll
-        for (int i = 0; i < NS; ++i)
-            if (p.n0 + i < a.states) a.seg_state[(item * a.states + p.n0 + i) * a.channels + p.ch] = dh[i];
-        if (p.sg == 0) a.seg_sum[item * a.channels + p.ch] = total;
+        q = hidden(a);
+        store_apart(p, dh, q->seg_state + (int64_t)item * p.states * channels, channels);
+        if (p.sg == 0 && p.on()) q->seg_sum[(int64_t)item * channels + p.ch] = total;
     }
 }
 
@@ -366,165 +479,212 @@ __global__ __launch_bounds__(256) void k_scan_carry(SelectArgs a)
 //   dh += c dy;  db = sum over channels of dh dt u;  dc = sum over channels of dy h;
 //   through = sum over n of b dh;  dh = exp(dt a) dh;  w = dh h_{t-1};  da += w dt;
 //   du = dt through + skip dy;  ddt = u through + sum over n of w a
-template <class T, int NS, bool EXACT>
-__global__ __launch_bounds__(256) void k_scan_backward(SelectArgs a)
+// MANY: more than one wave of states, whose shares of y, through and the sum of w a meet in
+// LDS. Registers are what it is short of: two waves a SIMD leave 256, of which 128 hold a
+// chunk's states, so the way back reads its rows again (from the caches), and the next
+// chunk's are asked for when half of the states are done with.
+template <class T, int NS, bool EXACT, bool MANY>
+__global__ __launch_bounds__(MANY ? 256 : 64, 2) void k_scan_backward(SelectArgs)
 {
-    extern __shared__ float lds[];   // more than one wave of states: [3][SG][8][64] shares of y, through and sum of w a
+    extern __shared__ float lds[];   // [3][SG][8][64]
     constexpr int K = SCAN_CHUNK;
-    const int SG = blockDim.x / 64, CW = a.waves * a.groups, cw = blockIdx.x % CW;
-    const Place<T, NS> p(a, cw);
-    const int part = blockIdx.x / CW;
-    float A[NS], dA[NS], dh[NS], h[NS];
-    p.a2(a, [&](int i, float x) { A[i] = x, dA[i] = 0.f; });
-    const float skip = a.skip ? a.skip[p.ch] : 0.f, bias = a.bias ? a.bias[p.ch] : 0.f;
+    const SelectArgsPtr a = hidden(select_arguments());
+    const int SG = MANY ? blockDim.x / 64 : 1, CW = a->waves * a->groups, cw = blockIdx.x % CW, part = blockIdx.x / CW;
+    const Place<T, NS, EXACT> p(a, cw);
+    float A[NS], dA[NS], dh[NS];
+    p.rates(a, A);
+#pragma unroll
+    for (int i = 0; i < NS; ++i) dA[i] = 0.f;
+    const bool skips = a->skip, gated = a->gate.data, soft = a->softplus, want_bc = a->want_bc, want_gate = a->dgate.data, want_u = a->du.data,
+               want_delta = a->ddelta.data;
+    const float skip = skips ? a->skip[p.ch] : 0.f, bias = a->bias ? a->bias[p.ch] : 0.f;
     float dskip = 0.f, dbias = 0.f;
-    const bool gated = a.gate.data;
-    const int chunks = (a.plies + K - 1) / K;
-    const int64_t items = (int64_t)a.batch * a.segments;
-    for (int64_t item = part; item < items; item += a.parts) {
-        const int b = item / a.segments, seg = item % a.segments;
-        const int begin = seg * a.seg_plies, stop = min(begin + a.seg_plies, a.plies), end = min(stop, live_plies(a, b));
-#pragma unroll
-        for (int i = 0; i < NS; ++i) {
-            const int n = p.n0 + i;
-            dh[i] = 0.f;
-            if (n >= a.states) continue;
-            if (a.segments > 1) dh[i] = a.seg_state[(item * a.states + n) * a.channels + p.ch];
-            else if (a.d_final) dh[i] = a.d_final[((int64_t)b * a.channels + p.ch) * a.states + n];
-        }
+    const int items = a->batch * a->segments, channels = a->channels, parts = a->parts;
+    const int sum_n = p.n0 + p.lane / (64 / NS);
+    const uint32_t sum_at = p.lane % (64 / NS) == 0 && (EXACT || sum_n < p.states) ? sum_n * 4 : NOWHERE;
+    struct Raw { T u[K], delta[K], gate[K], d_out[K], b[K], c[K]; };
+    auto share = [&](int j, int g, int k) -> float & { return lds[((j * SG + g) * K + k) * 64 + p.lane]; };
+    for (int item = part; item < items; item += parts) {
+        SelectArgsPtr q = hidden(a);
+        const int b = item / q->segments, seg = item % q->segments;
+        const int begin = seg * q->seg_plies, stop = min(begin + q->seg_plies, q->plies), end = min(stop, live_plies(q->lengths, b, q->plies));
+        if (q->segments > 1) load_apart(p, dh, q->seg_state + (int64_t)item * p.states * channels, channels);
+        else load_states(p, dh, q->d_final ? q->d_final + (int64_t)b * channels * p.states : nullptr);
         for (int t = max(begin, end) + p.sg; t < stop; t += SG) {
-            if (!p.on) continue;
-            if (a.du.data) row_at<T>(a.du, b, t, 0)[p.ch] = T(0.f);
-            if (a.ddelta.data) row_at<T>(a.ddelta, b, t, 0)[p.ch] = T(0.f);
-            if (a.dgate.data) row_at<T>(a.dgate, b, t, 0)[p.ch] = T(0.f);
+            if (want_u) row_window<T>(&q->du, b, t, 0).template put<T>(p.at, T(0.f));
+            if (want_delta) row_window<T>(&q->ddelta, b, t, 0).template put<T>(p.at, T(0.f));
+            if (want_gate) row_window<T>(&q->dgate, b, t, 0).template put<T>(p.at, T(0.f));
         }
-        for (int t0 = begin + (max(end - begin, 1) - 1) / K * K; t0 >= begin && begin < end; t0 -= K) {
-            const uint32_t starts = starts_of(a, b, t0, end, p.lane);
-            T u[K], delta[K], gate[K], d_out[K], bb[K], cc[K];
-            float hist[K][NS], dt[K], dy[K], y[K];
+        const int top = begin + (max(end - begin, 1) - 1) / K * K;
+        auto saved_at = [&](SelectArgsPtr q, int t0) {
+            return q->saved + ((int64_t)b * ((q->plies + K - 1) / K) + t0 / K) * p.states * channels;
+        };
+        auto load = [&](int t0, Raw &r, uint32_t &starts, bool really) {   // nothing is read where not `really`
+            const SelectArgsPtr q = hidden(a);
+            Window wu = row_window<T>(&q->u, b, t0, 0), wd = row_window<T>(&q->delta, b, t0, 0), wz = row_window<T>(&q->gate, b, t0, 0),
+                   wg = row_window<T>(&q->d_out, b, t0, 0), wb = row_window<T>(&q->b, b, t0, p.group), wc = row_window<T>(&q->c, b, t0, p.group);
+            const int64_t su = row_step<T>(&q->u), sd = row_step<T>(&q->delta), sz = row_step<T>(&q->gate), sg = row_step<T>(&q->d_out),
+                          sb = row_step<T>(&q->b), sc = row_step<T>(&q->c);
 #pragma unroll
             for (int k = 0; k < K; ++k) {
-                const int t = min(t0 + k, end - 1);
-                u[k] = at_ply<T>(a.u, b, t, 0)[p.ch];
-                delta[k] = at_ply<T>(a.delta, b, t, 0)[p.ch];
-                d_out[k] = at_ply<T>(a.d_out, b, t, 0)[p.ch];
-                if (gated) gate[k] = at_ply<T>(a.gate, b, t, 0)[p.ch];
-                bb[k] = cc[k] = T(0.f);
-                if (p.row_on) {
-                    bb[k] = at_ply<T>(a.b, b, t, p.group)[p.row_n];
-                    cc[k] = at_ply<T>(a.c, b, t, p.group)[p.row_n];
-                }
+                const bool there = really && t0 + k < end;
+                r.u[k] = wu.get<T>(p.at, 0, there);
+                r.delta[k] = wd.get<T>(p.at, 0, there);
+                r.d_out[k] = wg.get<T>(p.at, 0, there);
+                if (gated) r.gate[k] = wz.get<T>(p.at, 0, there);
+                r.b[k] = wb.get<T>(p.row_at, 0, there);
+                r.c[k] = wc.get<T>(p.row_at, 0, there);
+                wu.base += su, wd.base += sd, wz.base += sz, wg.base += sg, wb.base += sb, wc.base += sc;
             }
-            const float *from = a.saved + ((int64_t)b * chunks + t0 / K) * a.states * a.channels + p.ch;
-#pragma unroll
-            for (int i = 0; i < NS; ++i) h[i] = p.n0 + i < a.states ? from[(int64_t)(p.n0 + i) * a.channels] : 0.f;
-            float *bc = a.part_bc + ((((int64_t)(cw % a.waves) * a.batch + b) * a.plies + t0) * a.groups + p.group) * 2 * a.states;
-            const int64_t bc_ply = (int64_t)a.groups * 2 * a.states;
-            const int sum_n = p.n0 + p.lane / (64 / NS);
-            const bool sum_on = p.lane % (64 / NS) == 0 && sum_n < a.states;
-#pragma unroll
-            for (int k = 0; k < K; ++k) {
-                y[k] = 0.f;
-                if (t0 + k >= end) continue;
-                const float pre = (float)delta[k] + bias, bt = (float)bb[k], ct = (float)cc[k];
-                dt[k] = a.softplus ? softplus(pre) : pre;
-                const float push = dt[k] * (float)u[k];
-                dy[k] = (float)d_out[k];
-                if (gated) dy[k] *= (float)gate[k] * sigmoid((float)gate[k]);
-                if (starts >> k & 1)
-#pragma unroll
-                    for (int i = 0; i < NS; ++i) h[i] = 0.f;
-                float q[NS];
-                each_of<NS>([&](auto i) {
-                    hist[k][i] = h[i];
-                    h[i] = fmaf(row_lane<i>(bt), push, exp2_fast(dt[k] * A[i]) * h[i]);
-                    if (!EXACT && p.n0 + i >= a.states) h[i] = 0.f;
-                    y[k] = fmaf(row_lane<i>(ct), h[i], y[k]);
-                    q[i] = EXACT || p.on ? dy[k] * h[i] : 0.f;
-                });
-                if (a.want_bc) {
-                    const float s = lane_sums<NS>(q);
-                    if (sum_on) bc[k * bc_ply + a.states + sum_n] = s;
-                }
+            starts = really ? starts_of(q, b, t0, end, p.lane) : 0;
+        };
+        // the gradient of a gate and the ones of u and delta, their rows as they lie in memory
+        auto give_gate = [&](const Window &to, T u, T gate, T d_out, float y) {
+            const float z = (float)gate, s = sigmoid(z);
+            to.put<T>(p.at, from_float<T>((float)d_out * (skips ? fmaf(skip, (float)u, y) : y) * s * fmaf(z, 1.f - s, 1.f)));
+        };
+        auto give = [&](const Window &to_u, const Window &to_delta, T u, T delta, float dt, float dy, float s1, float s2) {
+            float d_pre = fmaf(s1, (float)u, s2 * LN2);
+            if (soft) d_pre *= sigmoid((float)delta + bias);
+            if (p.on()) {   // lanes without a channel have read zeros: their sums are not looked at
+                dbias += d_pre;
+                dskip = fmaf(dy, (float)u, dskip);
             }
-            float s1[K], s2[K];
-#pragma unroll
-            for (int k = K - 1; k >= 0; --k) {
-                s1[k] = s2[k] = 0.f;
-                if (t0 + k >= end) continue;
-                const float push = dt[k] * (float)u[k], bt = (float)bb[k], ct = (float)cc[k];
-                const bool start = starts >> k & 1;
-                float q[NS];
-                each_of<NS>([&](auto i) {
-                    dh[i] = fmaf(row_lane<i>(ct), dy[k], dh[i]);
-                    if (!EXACT && p.n0 + i >= a.states) dh[i] = 0.f;
-                    s1[k] = fmaf(row_lane<i>(bt), dh[i], s1[k]);
-                    q[i] = EXACT || p.on ? dh[i] * push : 0.f;
-                });
-                if (a.want_bc) {
-                    const float s = lane_sums<NS>(q);
-                    if (sum_on) bc[k * bc_ply + sum_n] = s;
-                }
-                if (start) {
-#pragma unroll
-                    for (int i = 0; i < NS; ++i) dh[i] = 0.f;
-                } else {
-#pragma unroll
-                    for (int i = 0; i < NS; ++i) {
-                        dh[i] *= exp2_fast(dt[k] * A[i]);
-                        const float w = dh[i] * hist[k][i];
-                        s2[k] = fmaf(w, A[i], s2[k]);
-                        dA[i] = fmaf(w, dt[k], dA[i]);
-                    }
-                }
-            }
-            if (SG > 1) {
-                __syncthreads();   // the shares of the chunk before have been read
+            if (want_u) to_u.put<T>(p.at, from_float<T>(skips ? fmaf(s1, dt, skip * dy) : s1 * dt));
+            if (want_delta) to_delta.put<T>(p.at, from_float<T>(d_pre));
+        };
+        Raw next;
+        float h[NS];
+        uint32_t next_starts = 0;
+        if (begin < end) {
+            load(top, next, next_starts, true);
+            load_apart(p, h, saved_at(q, top), channels);
+        }
+        for (int t0 = top; t0 >= begin && begin < end; t0 -= K) {
+            const uint32_t starts = next_starts;
+            const int count = min(end - t0, K);
+            float hist[K][NS], dt[K], dy[K];
+            {
+                const SelectArgsPtr q = hidden(a);
+                Window to = row_window<T>(&q->dgate, b, t0, 0);
+                const int64_t step = row_step<T>(&q->dgate), sum_step = (int64_t)q->groups * 2 * p.states * 4;
+                Window sums{reinterpret_cast<char *>(q->part_bc) + (((int64_t)(cw % q->waves) * q->batch + b) * q->plies + t0) * sum_step +
+                            (int64_t)(p.group * 2 + 1) * p.states * 4};
 #pragma unroll
                 for (int k = 0; k < K; ++k) {
-                    lds[(p.sg * K + k) * 64 + p.lane] = y[k];
-                    lds[((SG + p.sg) * K + k) * 64 + p.lane] = s1[k];
-                    lds[((2 * SG + p.sg) * K + k) * 64 + p.lane] = s2[k];
-                }
-                __syncthreads();
-            }
+                    if (k >= count) break;
+                    const float pre = (float)next.delta[k] + bias, bt = (float)next.b[k], u = (float)next.u[k];
+                    dt[k] = soft ? softplus(pre) : pre;
+                    dy[k] = (float)next.d_out[k];
+                    if (gated) dy[k] *= (float)next.gate[k] * sigmoid((float)next.gate[k]);
+                    if (starts >> k & 1)
 #pragma unroll
-            for (int k = 0; k < K; ++k) {
-                if (t0 + k >= end || (SG > 1 && k % SG != p.sg)) continue;
-                if (SG > 1) {
-                    y[k] = s1[k] = s2[k] = 0.f;
-                    for (int g = 0; g < SG; ++g) {
-                        y[k] += lds[(g * K + k) * 64 + p.lane];
-                        s1[k] += lds[((SG + g) * K + k) * 64 + p.lane];
-                        s2[k] += lds[((2 * SG + g) * K + k) * 64 + p.lane];
+                        for (int i = 0; i < NS; ++i) h[i] = 0.f;
+                    const float push = dt[k] * u;
+                    float v[NS];
+                    each_of<NS>([&](auto i) {
+                        hist[k][i] = h[i];
+                        h[i] = fmaf(exp2_fast(dt[k] * A[i]), h[i], row_lane<i>(bt) * push);
+                        if (!p.has(i)) h[i] = 0.f;
+                        v[i] = p.on() ? dy[k] * h[i] : 0.f;
+                    });
+                    if (want_gate) {
+                        const float y = row_dot(0.f, (float)next.c[k], h);
+                        if (MANY) share(0, p.sg, k) = y;
+                        else give_gate(to, next.u[k], next.gate[k], next.d_out[k], y);
+                        to.base += step;
+                    }
+                    if (want_bc) {
+                        sums.put(sum_at, lane_sums<NS>(v));
+                        sums.base += sum_step;
                     }
                 }
-                const float uu = (float)u[k], pre = (float)delta[k] + bias;
-                float d_pre = fmaf(s1[k], uu, s2[k] * LN2), d_u = s1[k] * dt[k];
-                if (a.softplus) d_pre *= sigmoid(pre);
-                if (a.skip) {
-                    d_u = fmaf(skip, dy[k], d_u);
-                    y[k] = fmaf(skip, uu, y[k]);
-                    dskip = fmaf(dy[k], uu, dskip);
+            }
+            {
+                const int last = t0 + count - 1;
+                const SelectArgsPtr q = hidden(a);
+                Window wu = row_window<T>(&q->u, b, last, 0), wd = row_window<T>(&q->delta, b, last, 0), wb = row_window<T>(&q->b, b, last, p.group),
+                       wc = row_window<T>(&q->c, b, last, p.group), to_u = row_window<T>(&q->du, b, last, 0), to_delta = row_window<T>(&q->ddelta, b, last, 0);
+                const int64_t su = row_step<T>(&q->u), sd = row_step<T>(&q->delta), sb = row_step<T>(&q->b), sc = row_step<T>(&q->c),
+                              tu = row_step<T>(&q->du), td = row_step<T>(&q->ddelta), sum_step = (int64_t)q->groups * 2 * p.states * 4;
+                Window sums{reinterpret_cast<char *>(q->part_bc) + (((int64_t)(cw % q->waves) * q->batch + b) * q->plies + last) * sum_step +
+                            (int64_t)p.group * 2 * p.states * 4};
+                T u = wu.get<T>(p.at), delta = wd.get<T>(p.at), bb = wb.get<T>(p.row_at), cc = wc.get<T>(p.row_at);
+#pragma unroll
+                for (int k = K - 1; k >= 0; --k) {
+                    if (k == K / 2 - 1) load(t0 - K, next, next_starts, t0 > begin);
+                    if (k >= count) continue;
+                    const T u0 = u, delta0 = delta, b0 = bb, c0 = cc;
+                    if (k) {
+                        wu.base -= su, wd.base -= sd, wb.base -= sb, wc.base -= sc;
+                        u = wu.get<T>(p.at), delta = wd.get<T>(p.at), bb = wb.get<T>(p.row_at), cc = wc.get<T>(p.row_at);
+                    }
+                    asm("" : "+v"(dt[k]));   // the decays once more: kept from the way there they would take 128 registers
+                    const float push = dt[k] * (float)u0;
+                    row_add(dh, (float)c0, dy[k]);
+                    float v[NS];
+#pragma unroll
+                    for (int i = 0; i < NS; ++i) {
+                        if (!p.has(i)) dh[i] = 0.f;
+                        v[i] = p.on() ? dh[i] * push : 0.f;
+                    }
+                    const float s1 = row_dot(0.f, (float)b0, dh);
+                    float s2 = 0.f;
+                    if (want_bc) {
+                        sums.put(sum_at, lane_sums<NS>(v));
+                        sums.base -= sum_step;
+                    }
+                    if (starts >> k & 1) {
+#pragma unroll
+                        for (int i = 0; i < NS; ++i) dh[i] = 0.f;
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < NS; ++i) {
+                            dh[i] *= exp2_fast(dt[k] * A[i]);
+                            const float w = dh[i] * hist[k][i];
+                            s2 = fmaf(w, A[i], s2);
+                            dA[i] = fmaf(w, dt[k], dA[i]);
+                        }
+                    }
+                    if (MANY) share(1, p.sg, k) = s1, share(2, p.sg, k) = s2;
+                    else {
+                        give(to_u, to_delta, u0, delta0, dt[k], dy[k], s1, s2);
+                        to_u.base -= tu, to_delta.base -= td;
+                    }
                 }
-                dbias += d_pre;
-                if (!p.on) continue;
-                if (a.du.data) row_at<T>(a.du, b, t0 + k, 0)[p.ch] = from_float<T>(d_u);
-                if (a.ddelta.data) row_at<T>(a.ddelta, b, t0 + k, 0)[p.ch] = from_float<T>(d_pre);
-                if (a.dgate.data) {
-                    const float z = (float)gate[k], s = sigmoid(z);
-                    row_at<T>(a.dgate, b, t0 + k, 0)[p.ch] = from_float<T>((float)d_out[k] * y[k] * s * fmaf(z, 1.f - s, 1.f));
+                load_apart(p, h, saved_at(hidden(a), t0 - K), channels, t0 > begin);
+            }
+            if constexpr (MANY) {
+                __syncthreads();
+                const SelectArgsPtr q = hidden(a);
+#pragma unroll
+                for (int k = 0; k < K; ++k) {
+                    if (k >= count) break;
+                    if (k % SG != p.sg) continue;
+                    float all[3] = {0.f, 0.f, 0.f};
+                    for (int g = 0; g < SG; ++g) {
+                        if (want_gate) all[0] += share(0, g, k);
+                        all[1] += share(1, g, k);
+                        all[2] += share(2, g, k);
+                    }
+                    const T u = row_window<T>(&q->u, b, t0 + k, 0).template get<T>(p.at);
+                    if (want_gate)
+                        give_gate(row_window<T>(&q->dgate, b, t0 + k, 0), u, row_window<T>(&q->gate, b, t0 + k, 0).template get<T>(p.at),
+                                  row_window<T>(&q->d_out, b, t0 + k, 0).template get<T>(p.at), all[0]);
+                    give(row_window<T>(&q->du, b, t0 + k, 0), row_window<T>(&q->ddelta, b, t0 + k, 0), u,
+                         row_window<T>(&q->delta, b, t0 + k, 0).template get<T>(p.at), dt[k], dy[k], all[1], all[2]);
                 }
+                __syncthreads();   // the next chunk's shares take their place
             }
         }
-        if (a.d_initial && seg == 0 && p.on)
-#pragma unroll
-            for (int i = 0; i < NS; ++i)
-                if (p.n0 + i < a.states) a.d_initial[((int64_t)b * a.channels + p.ch) * a.states + p.n0 + i] = dh[i];
+        if (seg == 0) {
+            float *to = hidden(a)->d_initial;
+            if (to) store_states(p, dh, to + (int64_t)b * channels * p.states);
+        }
     }
-    if (!a.want_a) return;
-    float *to = a.part_a + (int64_t)part * (a.states + 2) * a.channels + p.ch;
-    if (SG > 1) {   // each wave has some plies' share of dskip and dbias
+    const SelectArgsPtr q = hidden(a);
+    if (!q->want_a) return;
+    if constexpr (MANY) {   // each wave has some plies' share of dskip and dbias
         __syncthreads();
         lds[p.sg * 64 + p.lane] = dskip;
         lds[(SG + p.sg) * 64 + p.lane] = dbias;
@@ -535,13 +695,11 @@ __global__ __launch_bounds__(256) void k_scan_backward(SelectArgs a)
             dbias += lds[(SG + g) * 64 + p.lane];
         }
     }
-    if (!p.on) return;
-#pragma unroll
-    for (int i = 0; i < NS; ++i)
-        if (p.n0 + i < a.states) to[(int64_t)(p.n0 + i) * a.channels] = dA[i];
-    if (p.sg == 0) {
-        to[(int64_t)a.states * a.channels] = dskip;
-        to[(int64_t)(a.states + 1) * a.channels] = dbias;
+    float *to = q->part_a + (int64_t)part * (p.states + 2) * channels;
+    store_apart(p, dA, to, channels);
+    if (p.sg == 0 && p.on()) {
+        to[(int64_t)p.states * channels + p.ch] = dskip;
+        to[(int64_t)(p.states + 1) * channels + p.ch] = dbias;
     }
 }
 
@@ -556,7 +714,8 @@ __global__ __launch_bounds__(256) void k_scan_join_bc(SelectArgs a, jq_rows db, 
         const int64_t token = i / n2 / a.groups, b = token / a.plies;
         const int t = token % a.plies;
         float s = 0.f;
-        if (t < live_plies(a, b))
+        const int len = a.lengths ? min(max(a.lengths[b], 0), a.plies) : a.plies;
+        if (t < len)
             for (int w = 0; w < a.waves; ++w) s += a.part_bc[w * all + i];
         const jq_rows &r = j < a.states ? db : dc;
         if (r.data) row_at<T>(r, b, t, g)[j < a.states ? j : j - a.states] = from_float<T>(s);

@@ -19,6 +19,7 @@ namespace {
 
 constexpr int MOST_CHANNELS = 1 << 20, MOST_PLIES = 1 << 30, MOST_BLOCKS = 1 << 20;
 constexpr int64_t MOST_ELEMENTS = 1ll << 42;   // of a segment's rows: every size below fits 64 bits
+constexpr int MOST_GAMES = 1 << 30;            // with the parts of a split axis they fit 32
 
 template <class F>
 int by_type(int32_t dtype, F &&f)
@@ -29,7 +30,7 @@ int by_type(int32_t dtype, F &&f)
 int check_segment(int32_t dtype, int32_t batch, int32_t plies, int32_t channels)
 {
     TRY(check_dtype(dtype));
-    if (batch < 0 || plies < 0 || plies > MOST_PLIES || channels <= 0 || channels > MOST_CHANNELS)
+    if (batch < 0 || batch > MOST_GAMES || plies < 0 || plies > MOST_PLIES || channels <= 0 || channels > MOST_CHANNELS)
         return fail(JQ_E_ARG, "bad shapes (batch %d, plies %d, channels %d)", batch, plies, channels);
     if ((int64_t)batch * std::max(1, plies) > MOST_ELEMENTS / channels)
         return fail(JQ_E_ARG, "%d games of %d plies of %d channels are too many", batch, plies, channels);
@@ -370,8 +371,10 @@ int jq_scan_backward(const jq_scan *a, void *stream)
                 TRY(launch_check("k_scan_carry"));
                 TRY(launch_join<true>(s, q));
             }
-            const size_t lds = shape.sg > 1 ? 3 * shape.sg * SCAN_CHUNK * 64 * sizeof(float) : 0;
-            hipLaunchKernelGGL((k_scan_backward<T, ns(), exact()>), dim3(s.parts * s.waves * s.groups), block, lds, q, s);
+            const dim3 grid(s.parts * s.waves * s.groups);
+            const size_t lds = 3 * shape.sg * SCAN_CHUNK * 64 * sizeof(float);
+            if (shape.sg == 1) hipLaunchKernelGGL((k_scan_backward<T, ns(), exact(), false>), grid, block, 0, q, s);
+            else if constexpr (ns() == 16) hipLaunchKernelGGL((k_scan_backward<T, 16, exact(), true>), grid, block, lds, q, s);
             TRY(launch_check("k_scan_backward"));
             if (s.want_bc && s.batch && s.plies) {
                 const int64_t n = (int64_t)s.batch * s.plies * s.groups * 2 * s.states;

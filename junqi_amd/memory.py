@@ -473,7 +473,7 @@ def _like_plies(t: torch.Tensor) -> torch.Tensor:
 def _check_sizes(batch: int, plies: int, channels: int) -> None:
     if channels < 1:
         raise ValueError("there must be a channel")
-    if batch > _INT_MAX or plies > L.MOST_PLIES or channels > L.MOST_CHANNELS:
+    if batch > L.MOST_GAMES or plies > L.MOST_PLIES or channels > L.MOST_CHANNELS:
         raise ValueError(f"{batch} games of {plies} plies of {channels} channels are too many")
 
 
