@@ -513,6 +513,7 @@ int jq_layer_norm_backward(int32_t dtype, int32_t weight_dtype, int64_t rows, in
  * Games and plies stay at or below 2^30, channels at or below 2^20. */
 #define JQ_SCAN_MAX_STATES 64
 #define JQ_CONV_MAX_TAPS 8
+#define JQ_SCAN_MAX_PLY_STRIDE (1 << 28)   /* bytes between the plies of a scan's rows, at least 0 */
 
 /* The selective scan over segments of plies. For each game, channel d and state n,
  * with dt = softplus(delta + delta_bias) (or without the softplus) and h before the
@@ -541,7 +542,7 @@ typedef struct jq_scan {
     float *da, *dskip, *ddelta_bias;
     const float *d_final;
     float *d_initial;
-    void *workspace;                   /* jq_scan_workspace bytes, 4-byte aligned; NULL if it says 0 */
+    void *workspace;                   /* jq_scan_workspace bytes, 16-byte aligned; NULL if it says 0 */
     int64_t workspace_bytes;
 } jq_scan;
 /* Bytes of workspace that the forward or (backward != 0) backward pass with these outputs takes. */

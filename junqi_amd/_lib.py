@@ -22,6 +22,7 @@ ROTARY_MAX_AXES = 4
 ROTARY_MAX_PAIRS = 4096
 SCAN_MAX_STATES = 64
 CONV_MAX_TAPS = 8
+SCAN_MAX_PLY_STRIDE = 1 << 28
 MASK_WORDS_PACKED, MASK_BYTES = 0, 1
 MOST_CHANNELS, MOST_PLIES, MOST_GAMES = 1 << 20, 1 << 30, 1 << 30
 NUM_CELLS = 289

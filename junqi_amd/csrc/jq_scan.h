@@ -15,6 +15,7 @@ namespace jq {
 constexpr int SCAN_STATES = 64;   // largest states
 constexpr int SCAN_PLIES = 4;     // plies whose rows are on their way while the ones before are computed
 constexpr int SCAN_CHUNK = 8;     // plies of a chunk of the backward pass, which starts from a saved state
+constexpr int scan_far(int ns) { return ns > 8 ? 2 : 0; }   // plies of a chunk whose states wait in LDS: registers would spill
 
 struct SelectArgs {
     jq_rows u, delta, gate, b, c, out;
@@ -45,41 +46,27 @@ constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float sigmoid(float x) { return __builtin_amdgcn_rcpf(1.f + exp2_fast(-LOG2E * x)); }
 
-// log(1 + e^x) = max(x, 0) + 2 atanh(e / (2 + e)), e = e^-|x|: s = e / (2 + e) is at most
-// 1/3, and the series to s^15 is off by less than 2^-26 of the result; small results keep
-// all their digits.
+// log(1 + e^x) = max(x, 0) + 2 atanh(e / (2 + e)), e = e^-|x|, so small results keep all
+// their digits. s = e / (2 + e) is at most 1/3; atanh(s) / s as a polynomial in s^2 of the
+// fourth degree, fitted for the least largest relative error: 4e-9 (the series to s^14
+// takes three terms more).
 __device__ __forceinline__ float softplus(float x)
 {
     const float e = exp2_fast(-LOG2E * fabsf(x)), s = e * __builtin_amdgcn_rcpf(2.f + e), q = s * s;
-    float p = 1.f / 15;
-    p = fmaf(p, q, 1.f / 13);
-    p = fmaf(p, q, 1.f / 11);
-    p = fmaf(p, q, 1.f / 9);
-    p = fmaf(p, q, 1.f / 7);
-    p = fmaf(p, q, 1.f / 5);
-    p = fmaf(p, q, 1.f / 3);
+    float p = 0.14089167f;
+    p = fmaf(p, q, 0.13980301f);
+    p = fmaf(p, q, 0.20012455f);
+    p = fmaf(p, q, 0.33333157f);
     p = fmaf(p, q, 1.f);
-    return fmaxf(x, 0.f) + 2.f * s * p;
+    return fmaf(s + s, p, fmaxf(x, 0.f));
 }
 
-// f(integral_constant<int, 0>()), ..., f(integral_constant<int, N - 1>())
-template <class F, int... I> __device__ __forceinline__ void each_of(F &&f, std::integer_sequence<int, I...>)
-{
-    (f(std::integral_constant<int, I>()), ...);
-}
-template <int N, class F> __device__ __forceinline__ void each_of(F &&f) { each_of(f, std::make_integer_sequence<int, N>()); }
-
-// x of lane I of each row of 16 lanes: an operand of the product that takes it.
-template <int I> __device__ __forceinline__ float row_lane(float x)
-{
-    return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), 0x150 + I, 0xF, 0xF, true));
-}
-
-// The compiler folds such an operand into products, not into fused ones, which would take
-// a move for each. In these its two wait states after the operand's write come first.
+// Products whose one factor is x of lane i of each row of 16 lanes (row_newbcast), as an
+// operand: the compiler folds it into products, not into fused ones, which would take a
+// move for each. The two wait states after x's write come first.
 #define JQ_ROW_FMAC(d, i, s) "v_fmac_f32_dpp " d ", %[x], " s " row_newbcast:" #i " row_mask:0xf bank_mask:0xf\n"
 
-// y + the sum of row_lane<i>(x) h[i]
+// y + the sum of x of lane i times h[i]
 __device__ __forceinline__ float row_dot(float y, float x, const float (&h)[4])
 {
     asm("s_nop 1\n" JQ_ROW_FMAC("%[y]", 0, "%[a]") JQ_ROW_FMAC("%[y]", 1, "%[b]") JQ_ROW_FMAC("%[y]", 2, "%[c]") JQ_ROW_FMAC("%[y]", 3, "%[d]")
@@ -106,23 +93,38 @@ __device__ __forceinline__ float row_dot(float y, float x, const float (&h)[16])
     return y;
 }
 
-// v[i] += row_lane<FIRST + i>(x) y for four i
-template <int FIRST> __device__ __forceinline__ void row_add4(float &a, float &b, float &c, float &d, float x, float y)
+// v[i] += x of lane i times y
+__device__ __forceinline__ void row_add(float (&v)[4], float x, float y)
 {
-#define JQ_ROW_ADD(i0, i1, i2, i3)                                                                                           \
-    asm("s_nop 1\n" JQ_ROW_FMAC("%[a]", i0, "%[y]") JQ_ROW_FMAC("%[b]", i1, "%[y]") JQ_ROW_FMAC("%[c]", i2, "%[y]")          \
-        JQ_ROW_FMAC("%[d]", i3, "%[y]") : [a] "+v"(a), [b] "+v"(b), [c] "+v"(c), [d] "+v"(d) : [x] "v"(x), [y] "v"(y))
-    if constexpr (FIRST == 0) JQ_ROW_ADD(0, 1, 2, 3);
-    else if constexpr (FIRST == 4) JQ_ROW_ADD(4, 5, 6, 7);
-    else if constexpr (FIRST == 8) JQ_ROW_ADD(8, 9, 10, 11);
-    else JQ_ROW_ADD(12, 13, 14, 15);
-#undef JQ_ROW_ADD
+    asm("s_nop 1\n" JQ_ROW_FMAC("%[a]", 0, "%[y]") JQ_ROW_FMAC("%[b]", 1, "%[y]") JQ_ROW_FMAC("%[c]", 2, "%[y]") JQ_ROW_FMAC("%[d]", 3, "%[y]")
+        : [a] "+v"(v[0]), [b] "+v"(v[1]), [c] "+v"(v[2]), [d] "+v"(v[3]) : [x] "v"(x), [y] "v"(y));
 }
-template <int N> __device__ __forceinline__ void row_add(float (&v)[N], float x, float y)
+__device__ __forceinline__ void row_add(float (&v)[8], float x, float y)
 {
-    each_of<N / 4>([&](auto q) { row_add4<4 * q>(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3], x, y); });
+    asm("s_nop 1\n" JQ_ROW_FMAC("%[a]", 0, "%[y]") JQ_ROW_FMAC("%[b]", 1, "%[y]") JQ_ROW_FMAC("%[c]", 2, "%[y]") JQ_ROW_FMAC("%[d]", 3, "%[y]")
+        JQ_ROW_FMAC("%[e]", 4, "%[y]") JQ_ROW_FMAC("%[f]", 5, "%[y]") JQ_ROW_FMAC("%[g]", 6, "%[y]") JQ_ROW_FMAC("%[h]", 7, "%[y]")
+        : [a] "+v"(v[0]), [b] "+v"(v[1]), [c] "+v"(v[2]), [d] "+v"(v[3]), [e] "+v"(v[4]), [f] "+v"(v[5]), [g] "+v"(v[6]),
+          [h] "+v"(v[7]) : [x] "v"(x), [y] "v"(y));
+}
+__device__ __forceinline__ void row_add(float (&v)[16], float x, float y)
+{
+    asm("s_nop 1\n" JQ_ROW_FMAC("%[a]", 0, "%[y]") JQ_ROW_FMAC("%[b]", 1, "%[y]") JQ_ROW_FMAC("%[c]", 2, "%[y]") JQ_ROW_FMAC("%[d]", 3, "%[y]")
+        JQ_ROW_FMAC("%[e]", 4, "%[y]") JQ_ROW_FMAC("%[f]", 5, "%[y]") JQ_ROW_FMAC("%[g]", 6, "%[y]") JQ_ROW_FMAC("%[h]", 7, "%[y]")
+        JQ_ROW_FMAC("%[i]", 8, "%[y]") JQ_ROW_FMAC("%[j]", 9, "%[y]") JQ_ROW_FMAC("%[k]", 10, "%[y]") JQ_ROW_FMAC("%[l]", 11, "%[y]")
+        JQ_ROW_FMAC("%[m]", 12, "%[y]") JQ_ROW_FMAC("%[n]", 13, "%[y]") JQ_ROW_FMAC("%[o]", 14, "%[y]") JQ_ROW_FMAC("%[p]", 15, "%[y]")
+        : [a] "+v"(v[0]), [b] "+v"(v[1]), [c] "+v"(v[2]), [d] "+v"(v[3]), [e] "+v"(v[4]), [f] "+v"(v[5]), [g] "+v"(v[6]),
+          [h] "+v"(v[7]), [i] "+v"(v[8]), [j] "+v"(v[9]), [k] "+v"(v[10]), [l] "+v"(v[11]), [m] "+v"(v[12]), [n] "+v"(v[13]),
+          [o] "+v"(v[14]), [p] "+v"(v[15]) : [x] "v"(x), [y] "v"(y));
 }
 #undef JQ_ROW_FMAC
+
+// A game starts: nothing of the plies before. Rare, so a branch, not a selection in every ply.
+template <int N> __device__ __forceinline__ void forget(float (&v)[N])
+{
+    asm volatile("");
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = 0.f;
+}
 
 template <int HOW> __device__ __forceinline__ float across(float x)
 {
@@ -178,8 +180,8 @@ __device__ __forceinline__ SelectArgsPtr hidden(SelectArgsPtr a)
 }
 __device__ __forceinline__ SelectArgsPtr select_arguments() { return (SelectArgsPtr)__builtin_amdgcn_kernarg_segment_ptr(); }
 
-// Memory behind a wave's own address, at each lane's offset: an offset of NOWHERE reads 0
-// and writes nothing, as all do where `really` is false.
+// Memory behind a wave's own address, at each lane's offset and one for the wave: a lane's
+// offset of NOWHERE reads 0 and writes nothing, as all do where `really` is false.
 constexpr uint32_t NOWHERE = 0x80000000u;
 struct Window {
     char *base;
@@ -197,24 +199,37 @@ struct Window {
     }
 };
 
-// A tensor's row of ply t, and the bytes from one ply's to the next.
-template <class T> __device__ __forceinline__ Window row_window(RowsPtr r, int64_t b, int64_t t, int64_t h)
-{
-    return Window{static_cast<char *>(r->data) + (b * r->batch + t * r->ply + h * r->head) * (int64_t)sizeof(T)};
-}
-template <class T> __device__ __forceinline__ int64_t row_step(RowsPtr r) { return r->ply * (int64_t)sizeof(T); }
+// A tensor's rows from ply t on; `step` bytes part two plies' rows. A chunk's rows are
+// reached by 32-bit offsets: plies are less than SCAN_STEP bytes apart.
+constexpr int64_t SCAN_STEP = 1 << 28;
+struct PlyRows : Window {
+    uint32_t step;
+    template <class T> __device__ __forceinline__ PlyRows(T, RowsPtr r, int64_t b, int64_t t, int64_t h)
+        : Window{static_cast<char *>(r->data) + (b * r->batch + t * r->ply + h * r->head) * (int64_t)sizeof(T)},
+          step((uint32_t)r->ply * (uint32_t)sizeof(T)) {}
+    __device__ __forceinline__ void on(int plies) { base += (uint64_t)step * plies; }
+    __device__ __forceinline__ void back(int plies) { base -= (uint64_t)step * plies; }
+};
 
 // Where this wave's lanes are: channel, states, rows. EXACT: every lane has a channel and
-// each of its states.
-template <class T, int NS, bool EXACT>
+// each of its states. MANY: a block's waves have the states of one wave's channels; else
+// channels of their own, four waves a block so that each SIMD of a CU gets one (blocks of
+// one wave leave some SIMDs with more waves than others).
+template <class T, int NS, bool EXACT, bool MANY>
 struct Place {
-    int lane, sg, group, ch, n0, states;
+    int lane, sg, cw, part, parts,   // parts share the items (game, part of the axis)
+         group, ch, n0, states;
     uint32_t at, row_at, at4;   // bytes into a row of channels, of a group's states, and of channels in float32
     bool on_;
-    __device__ __forceinline__ Place(SelectArgsPtr a, int cw)
+    __device__ __forceinline__ Place(SelectArgsPtr a)
     {
+        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), waves = blockDim.x / 64, CW = a->waves * a->groups;
+        const int w = MANY ? blockIdx.x : blockIdx.x * waves + wave;
         lane = threadIdx.x % 64;
-        sg = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+        sg = MANY ? wave : 0;
+        cw = w % CW;
+        part = w / CW;
+        parts = a->parts;
         group = cw / a->waves;
         states = a->states;
         const int c = (cw % a->waves) * 64 + lane;
@@ -242,55 +257,63 @@ __device__ __forceinline__ int live_plies(const int32_t *lengths, int b, int pli
     return lengths ? min(max(__builtin_amdgcn_readfirstlane(lengths[b]), 0), plies) : plies;
 }
 
-// Bit k: a game starts at ply t0 + k, k < 8; plies from `end` on are not looked at.
-__device__ __forceinline__ uint32_t starts_of(SelectArgsPtr a, int b, int t0, int end, int lane)
-{
-    if (!a->starts) return 0;
-    const int k = lane & 7, t = min(t0 + k, end - 1);
-    return __builtin_amdgcn_ballot_w64(a->starts[b * a->starts_batch + t * a->starts_ply] != 0 && t0 + k < end) & 0xFF;
-}
+// Where a game's plies start games. Bit k: one starts at ply t0 + k, k < 8; plies from
+// `end` on are not looked at.
+struct Starts {
+    const uint8_t *row;
+    int64_t step;
+    __device__ __forceinline__ Starts(SelectArgsPtr a, int b) : row(a->starts ? a->starts + b * a->starts_batch : nullptr), step(a->starts_ply) {}
+    __device__ __forceinline__ uint32_t at(int t0, int end, int lane) const
+    {
+        if (!row) return 0;
+        const int k = lane & 7, t = min(t0 + k, end - 1);
+        return __builtin_amdgcn_ballot_w64(row[t * step] != 0 && t0 + k < end) & 0xFF;
+    }
+};
 
 // The states of this lane in a (.., channels, states) tensor's row, or in a (.., states, channels) one's.
-template <class T, int NS, bool EXACT>
-__device__ __forceinline__ void load_states(const Place<T, NS, EXACT> &p, float (&h)[NS], const float *row)
+template <class T, int NS, bool EXACT, bool MANY>
+__device__ __forceinline__ void load_states(const Place<T, NS, EXACT, MANY> &p, float (&h)[NS], const float *row)
 {
 #pragma unroll
     for (int i = 0; i < NS; ++i) h[i] = row && p.has(i) ? row[(int64_t)p.ch * p.states + p.n0 + i] : 0.f;
 }
-template <class T, int NS, bool EXACT>
-__device__ __forceinline__ void store_states(const Place<T, NS, EXACT> &p, const float (&h)[NS], float *row)
+template <class T, int NS, bool EXACT, bool MANY>
+__device__ __forceinline__ void store_states(const Place<T, NS, EXACT, MANY> &p, const float (&h)[NS], float *row)
 {
     if (p.on())
 #pragma unroll
         for (int i = 0; i < NS; ++i)
             if (p.has(i)) row[(int64_t)p.ch * p.states + p.n0 + i] = h[i];
 }
-template <class T, int NS, bool EXACT>
-__device__ __forceinline__ void load_apart(const Place<T, NS, EXACT> &p, float (&h)[NS], const float *row, int channels, bool really = true)
+template <class T, int NS, bool EXACT, bool MANY>
+__device__ __forceinline__ void load_apart(const Place<T, NS, EXACT, MANY> &p, float (&h)[NS], const float *row, int channels, bool really = true)
 {
     const Window from{reinterpret_cast<char *>(const_cast<float *>(row))};
-    uint32_t more = p.n0 * channels * 4;
+    uint32_t step = channels * 4, more = p.n0 * step;
+    asm volatile("" : "+s"(step));   // its multiples are not worth registers over the pass
 #pragma unroll
-    for (int i = 0; i < NS; ++i, more += channels * 4) h[i] = p.has(i) ? from.get<float>(p.at4, more, really) : 0.f;
+    for (int i = 0; i < NS; ++i, more += step) h[i] = p.has(i) ? from.get<float>(p.at4, more, really) : 0.f;
 }
-template <class T, int NS, bool EXACT>
-__device__ __forceinline__ void store_apart(const Place<T, NS, EXACT> &p, const float (&h)[NS], float *row, int channels)
+template <class T, int NS, bool EXACT, bool MANY>
+__device__ __forceinline__ void store_apart(const Place<T, NS, EXACT, MANY> &p, const float (&h)[NS], float *row, int channels)
 {
     const Window to{reinterpret_cast<char *>(row)};
-    uint32_t more = p.n0 * channels * 4;
+    uint32_t step = channels * 4, more = p.n0 * step;
+    asm volatile("" : "+s"(step));
 #pragma unroll
-    for (int i = 0; i < NS; ++i, more += channels * 4)
+    for (int i = 0; i < NS; ++i, more += step)
         if (p.has(i)) to.put(p.at4, h[i], more);
 }
 
-template <class T, int NS, bool EXACT, bool OUT>
+template <class T, int NS, bool EXACT, bool MANY, bool OUT>
 __global__ __launch_bounds__(256) void k_scan_forward(SelectArgs)
 {
     constexpr int K = SCAN_PLIES;
     extern __shared__ float lds[];   // more than one wave of states: [2][SG][K][64] shares of y
     const SelectArgsPtr a = hidden(select_arguments());
-    const int SG = blockDim.x / 64, CW = a->waves * a->groups;
-    const Place<T, NS, EXACT> p(a, blockIdx.x % CW);
+    const int SG = MANY ? blockDim.x / 64 : 1;
+    const Place<T, NS, EXACT, MANY> p(a);
     float A[NS], h[NS];
     p.rates(a, A);
     const bool skips = a->skip, gated = OUT && a->gate.data, soft = a->softplus, saves = OUT && a->saved;
@@ -299,30 +322,31 @@ __global__ __launch_bounds__(256) void k_scan_forward(SelectArgs)
     const int items = a->batch * a->segments, channels = a->channels;
     const int64_t state_bytes = (int64_t)p.states * channels * 4;
     int turn = 0;
-    for (int item = blockIdx.x / CW; item < items; item += gridDim.x / CW) {
+    if (p.part >= p.parts) return;
+    for (int item = p.part; item < items; item += p.parts) {
         SelectArgsPtr q = hidden(a);
         const int b = item / q->segments, seg = item % q->segments;
         const int begin = seg * q->seg_plies, stop = min(begin + q->seg_plies, q->plies), end = min(stop, live_plies(q->lengths, b, q->plies));
         if (OUT && seg) load_apart(p, h, q->seg_state + (int64_t)item * p.states * channels, channels);
         else load_states(p, h, OUT && q->s_in ? q->s_in + (int64_t)b * channels * p.states : nullptr);
         float total = 0.f;
-        Window wu = row_window<T>(&q->u, b, begin, 0), wd = row_window<T>(&q->delta, b, begin, 0), wz = row_window<T>(&q->gate, b, begin, 0),
-               wb = row_window<T>(&q->b, b, begin, p.group), wc = row_window<T>(&q->c, b, begin, p.group), wo = row_window<T>(&q->out, b, begin, 0);
+        const Starts game(q, b);
+        PlyRows ru(T(), &q->u, b, begin, 0), rd(T(), &q->delta, b, begin, 0), rz(T(), &q->gate, b, begin, 0), rb(T(), &q->b, b, begin, p.group),
+            rc(T(), &q->c, b, begin, p.group), ro(T(), &q->out, b, begin, 0);
         Window save{reinterpret_cast<char *>(q->saved) + ((int64_t)b * ((q->plies + SCAN_CHUNK - 1) / SCAN_CHUNK) + begin / SCAN_CHUNK) * state_bytes};
         auto fetch = [&](int t0, Raw &r, uint32_t &starts) {
-            const SelectArgsPtr q = hidden(a);
-            const int64_t su = row_step<T>(&q->u), sd = row_step<T>(&q->delta), sz = row_step<T>(&q->gate), sb = row_step<T>(&q->b), sc = row_step<T>(&q->c);
+            const int last = end - 1 - t0;
 #pragma unroll
             for (int k = 0; k < K; ++k) {
-                const bool there = t0 + k < end;
-                r.u[k] = wu.get<T>(p.at, 0, there);
-                r.delta[k] = wd.get<T>(p.at, 0, there);
-                if (gated) r.gate[k] = wz.get<T>(p.at, 0, there);
-                r.b[k] = wb.get<T>(p.row_at, 0, there);
-                if (OUT) r.c[k] = wc.get<T>(p.row_at, 0, there);
-                wu.base += su, wd.base += sd, wz.base += sz, wb.base += sb, wc.base += sc;
+                const uint32_t at = min(k, last);   // behind the end the last row again
+                r.u[k] = ru.get<T>(p.at, at * ru.step);
+                r.delta[k] = rd.get<T>(p.at, at * rd.step);
+                if (gated) r.gate[k] = rz.get<T>(p.at, at * rz.step);
+                r.b[k] = rb.get<T>(p.row_at, at * rb.step);
+                if (OUT) r.c[k] = rc.get<T>(p.row_at, at * rc.step);
             }
-            starts = starts_of(q, b, t0, end, p.lane);
+            ru.on(K), rd.on(K), rz.on(K), rb.on(K), rc.on(K);
+            starts = game.at(t0, end, p.lane);
         };
         Raw next;
         uint32_t next_starts = 0;
@@ -335,33 +359,36 @@ __global__ __launch_bounds__(256) void k_scan_forward(SelectArgs)
                 store_apart(p, h, reinterpret_cast<float *>(save.base), channels);
                 save.base += state_bytes;
             }
-            const int64_t step = OUT ? row_step<T>(&hidden(a)->out) : 0;
 #pragma unroll
             for (int k = 0; k < K; ++k) {
                 if (t0 + k >= end) break;
                 const float u = (float)r.u[k], pre = (float)r.delta[k] + bias, dt = soft ? softplus(pre) : pre;
                 const float push = dt * u, bt = (float)r.b[k];
                 if (starts >> k & 1) {
-#pragma unroll
-                    for (int i = 0; i < NS; ++i) h[i] = 0.f;
+                    forget(h);
                     if (!OUT) total = __builtin_nanf("");
                 }
                 if (!OUT) total += dt;
-                each_of<NS>([&](auto i) {
-                    h[i] = fmaf(exp2_fast(dt * A[i]), h[i], row_lane<i>(bt) * push);
+#pragma unroll
+                for (int i = 0; i < NS; ++i) h[i] *= exp2_fast(dt * A[i]);
+                row_add(h, bt, push);
+#pragma unroll
+                for (int i = 0; i < NS; ++i)
                     if (!p.has(i)) h[i] = 0.f;
-                });
                 if (!OUT) continue;
                 const float y = row_dot(0.f, (float)r.c[k], h);
-                if (SG > 1) lds[(((turn & 1) * SG + p.sg) * K + k) * 64 + p.lane] = y;
+                if (MANY) lds[(((turn & 1) * SG + p.sg) * K + k) * 64 + p.lane] = y;
                 else {
                     float o = skips ? fmaf(skip, u, y) : y;
                     if (gated) o *= (float)r.gate[k] * sigmoid((float)r.gate[k]);
-                    wo.put<T>(p.at, from_float<T>(o));
-                    wo.base += step;
+                    ro.put<T>(p.at, from_float<T>(o), k * ro.step);
                 }
             }
-            if (!OUT || SG == 1) continue;
+            if (!OUT) continue;
+            if (!MANY) {
+                ro.on(K);
+                continue;
+            }
             __syncthreads();
 #pragma unroll
             for (int k = 0; k < K; ++k) {
@@ -371,16 +398,16 @@ __global__ __launch_bounds__(256) void k_scan_forward(SelectArgs)
                     for (int g = 0; g < SG; ++g) o += lds[(((turn & 1) * SG + g) * K + k) * 64 + p.lane];
                     if (skips) o = fmaf(skip, (float)r.u[k], o);
                     if (gated) o *= (float)r.gate[k] * sigmoid((float)r.gate[k]);
-                    wo.put<T>(p.at, from_float<T>(o));
+                    ro.put<T>(p.at, from_float<T>(o), k * ro.step);
                 }
-                wo.base += step;
             }
+            ro.on(K);
             ++turn;   // the other buffer: the one before is read by then
         }
         q = hidden(a);
         if (OUT) {
             for (int t = max(begin, end); t < stop; ++t)
-                if (t % SG == p.sg) row_window<T>(&q->out, b, t, 0).template put<T>(p.at, T(0.f));
+                if (t % SG == p.sg) PlyRows(T(), &q->out, b, t, 0).template put<T>(p.at, T(0.f));
             if (q->s_out && seg == q->segments - 1) store_states(p, h, q->s_out + (int64_t)b * channels * p.states);
         } else {
             store_apart(p, h, q->seg_state + (int64_t)item * p.states * channels, channels);
@@ -415,18 +442,19 @@ __global__ __launch_bounds__(256) void k_scan_join(SelectArgs a)
 
 // Backward over a part of the axis: what its gradients of y send to the state before it
 // (seg_state, seg_sum), in reverse.
-template <class T, int NS, bool EXACT>
+template <class T, int NS, bool EXACT, bool MANY>
 __global__ __launch_bounds__(256) void k_scan_carry(SelectArgs)
 {
     constexpr int K = SCAN_CHUNK;
     const SelectArgsPtr a = hidden(select_arguments());
-    const int CW = a->waves * a->groups, items = a->batch * a->segments, channels = a->channels;
-    const Place<T, NS, EXACT> p(a, blockIdx.x % CW);
+    const int items = a->batch * a->segments, channels = a->channels;
+    const Place<T, NS, EXACT, MANY> p(a);
+    if (p.part >= p.parts) return;
     float A[NS], dh[NS];
     p.rates(a, A);
     const bool gated = a->gate.data, soft = a->softplus;
     const float bias = a->bias ? a->bias[p.ch] : 0.f;
-    for (int item = blockIdx.x / CW; item < items; item += gridDim.x / CW) {
+    for (int item = p.part; item < items; item += p.parts) {
         SelectArgsPtr q = hidden(a);
         const int b = item / q->segments, seg = item % q->segments;
         const int begin = seg * q->seg_plies, end = min(min(begin + q->seg_plies, q->plies), live_plies(q->lengths, b, q->plies));
@@ -437,18 +465,15 @@ __global__ __launch_bounds__(256) void k_scan_carry(SelectArgs)
         for (int t0 = top; t0 >= begin && begin < end; t0 -= K) {
             T delta[K], gate[K], d_out[K], c[K];
             q = hidden(a);
-            const uint32_t starts = starts_of(q, b, t0, end, p.lane);
-            Window wd = row_window<T>(&q->delta, b, t0, 0), wz = row_window<T>(&q->gate, b, t0, 0), wg = row_window<T>(&q->d_out, b, t0, 0),
-                   wc = row_window<T>(&q->c, b, t0, p.group);
-            const int64_t sd = row_step<T>(&q->delta), sz = row_step<T>(&q->gate), sg = row_step<T>(&q->d_out), sc = row_step<T>(&q->c);
+            const uint32_t starts = Starts(q, b).at(t0, end, p.lane);
+            const PlyRows rd(T(), &q->delta, b, t0, 0), rz(T(), &q->gate, b, t0, 0), rg(T(), &q->d_out, b, t0, 0), rc(T(), &q->c, b, t0, p.group);
 #pragma unroll
             for (int k = 0; k < K; ++k) {
-                const bool there = t0 + k < end;
-                delta[k] = wd.get<T>(p.at, 0, there);
-                d_out[k] = wg.get<T>(p.at, 0, there);
-                if (gated) gate[k] = wz.get<T>(p.at, 0, there);
-                c[k] = wc.get<T>(p.row_at, 0, there);
-                wd.base += sd, wz.base += sz, wg.base += sg, wc.base += sc;
+                const uint32_t at = min(k, end - 1 - t0);
+                delta[k] = rd.get<T>(p.at, at * rd.step);
+                d_out[k] = rg.get<T>(p.at, at * rg.step);
+                if (gated) gate[k] = rz.get<T>(p.at, at * rz.step);
+                c[k] = rc.get<T>(p.row_at, at * rc.step);
             }
 #pragma unroll
             for (int k = K - 1; k >= 0; --k) {
@@ -461,8 +486,7 @@ __global__ __launch_bounds__(256) void k_scan_carry(SelectArgs)
                 for (int i = 0; i < NS; ++i) dh[i] = p.has(i) ? dh[i] * exp2_fast(dt * A[i]) : 0.f;
                 total += dt;
                 if (starts >> k & 1) {
-#pragma unroll
-                    for (int i = 0; i < NS; ++i) dh[i] = 0.f;
+                    forget(dh);
                     total = __builtin_nanf("");
                 }
             }
@@ -484,13 +508,14 @@ __global__ __launch_bounds__(256) void k_scan_carry(SelectArgs)
 // chunk's states, so the way back reads its rows again (from the caches), and the next
 // chunk's are asked for when half of the states are done with.
 template <class T, int NS, bool EXACT, bool MANY>
-__global__ __launch_bounds__(MANY ? 256 : 64, 2) void k_scan_backward(SelectArgs)
+__global__ __launch_bounds__(256, 2) void k_scan_backward(SelectArgs)
 {
-    extern __shared__ float lds[];   // [3][SG][8][64]
-    constexpr int K = SCAN_CHUNK;
+    extern __shared__ float lds[];   // [waves][FAR][NS / 4][64][4] states, then, of MANY, [3][SG][8][64] shares
+    constexpr int K = SCAN_CHUNK, FAR = scan_far(NS);
     const SelectArgsPtr a = hidden(select_arguments());
-    const int SG = MANY ? blockDim.x / 64 : 1, CW = a->waves * a->groups, cw = blockIdx.x % CW, part = blockIdx.x / CW;
-    const Place<T, NS, EXACT> p(a, cw);
+    const int SG = MANY ? blockDim.x / 64 : 1;
+    const Place<T, NS, EXACT, MANY> p(a);
+    if (p.part >= p.parts) return;   // never of MANY: its waves meet
     float A[NS], dA[NS], dh[NS];
     p.rates(a, A);
 #pragma unroll
@@ -499,77 +524,76 @@ __global__ __launch_bounds__(MANY ? 256 : 64, 2) void k_scan_backward(SelectArgs
                want_delta = a->ddelta.data;
     const float skip = skips ? a->skip[p.ch] : 0.f, bias = a->bias ? a->bias[p.ch] : 0.f;
     float dskip = 0.f, dbias = 0.f;
-    const int items = a->batch * a->segments, channels = a->channels, parts = a->parts;
+    const int items = a->batch * a->segments, channels = a->channels;
     const int sum_n = p.n0 + p.lane / (64 / NS);
     const uint32_t sum_at = p.lane % (64 / NS) == 0 && (EXACT || sum_n < p.states) ? sum_n * 4 : NOWHERE;
     struct Raw { T u[K], delta[K], gate[K], d_out[K], b[K], c[K]; };
-    auto share = [&](int j, int g, int k) -> float & { return lds[((j * SG + g) * K + k) * 64 + p.lane]; };
-    for (int item = part; item < items; item += parts) {
+    float *const far = lds + __builtin_amdgcn_readfirstlane(threadIdx.x / 64) * FAR * NS * 64, *const shares = lds + SG * FAR * NS * 64;
+    auto share = [&](int j, int g, int k) -> float & { return shares[((j * SG + g) * K + k) * 64 + p.lane]; };
+    for (int item = p.part; item < items; item += p.parts) {
         SelectArgsPtr q = hidden(a);
         const int b = item / q->segments, seg = item % q->segments;
         const int begin = seg * q->seg_plies, stop = min(begin + q->seg_plies, q->plies), end = min(stop, live_plies(q->lengths, b, q->plies));
         if (q->segments > 1) load_apart(p, dh, q->seg_state + (int64_t)item * p.states * channels, channels);
         else load_states(p, dh, q->d_final ? q->d_final + (int64_t)b * channels * p.states : nullptr);
         for (int t = max(begin, end) + p.sg; t < stop; t += SG) {
-            if (want_u) row_window<T>(&q->du, b, t, 0).template put<T>(p.at, T(0.f));
-            if (want_delta) row_window<T>(&q->ddelta, b, t, 0).template put<T>(p.at, T(0.f));
-            if (want_gate) row_window<T>(&q->dgate, b, t, 0).template put<T>(p.at, T(0.f));
+            if (want_u) PlyRows(T(), &q->du, b, t, 0).template put<T>(p.at, T(0.f));
+            if (want_delta) PlyRows(T(), &q->ddelta, b, t, 0).template put<T>(p.at, T(0.f));
+            if (want_gate) PlyRows(T(), &q->dgate, b, t, 0).template put<T>(p.at, T(0.f));
         }
         const int top = begin + (max(end - begin, 1) - 1) / K * K;
-        auto saved_at = [&](SelectArgsPtr q, int t0) {
-            return q->saved + ((int64_t)b * ((q->plies + K - 1) / K) + t0 / K) * p.states * channels;
-        };
-        auto load = [&](int t0, Raw &r, uint32_t &starts, bool really) {   // nothing is read where not `really`
-            const SelectArgsPtr q = hidden(a);
-            Window wu = row_window<T>(&q->u, b, t0, 0), wd = row_window<T>(&q->delta, b, t0, 0), wz = row_window<T>(&q->gate, b, t0, 0),
-                   wg = row_window<T>(&q->d_out, b, t0, 0), wb = row_window<T>(&q->b, b, t0, p.group), wc = row_window<T>(&q->c, b, t0, p.group);
-            const int64_t su = row_step<T>(&q->u), sd = row_step<T>(&q->delta), sz = row_step<T>(&q->gate), sg = row_step<T>(&q->d_out),
-                          sb = row_step<T>(&q->b), sc = row_step<T>(&q->c);
+        const Starts game(q, b);
+        PlyRows ru(T(), &q->u, b, top, 0), rd(T(), &q->delta, b, top, 0), rz(T(), &q->gate, b, top, 0), rg(T(), &q->d_out, b, top, 0),
+            rb(T(), &q->b, b, top, p.group), rc(T(), &q->c, b, top, p.group), to_u(T(), &q->du, b, top, 0), to_delta(T(), &q->ddelta, b, top, 0),
+            to_gate(T(), &q->dgate, b, top, 0);
+        const int64_t state_bytes = (int64_t)p.states * channels * 4, sum_step = (int64_t)q->groups * 2 * p.states * 4;
+        const char *saved = reinterpret_cast<const char *>(q->saved) + ((int64_t)b * ((q->plies + K - 1) / K) + top / K) * state_bytes;
+        Window sums{reinterpret_cast<char *>(q->part_bc) + (((int64_t)(p.cw % q->waves) * q->batch + b) * q->plies + top) * sum_step +
+                    (int64_t)p.group * 2 * p.states * 4};
+        // the rows of the chunk `plies` before the one at hand, whose first ply is t0; nothing is read where not `really`
+        auto load = [&](int t0, int plies, Raw &r, uint32_t &starts, bool really) {
+            PlyRows lu = ru, ld = rd, lz = rz, lg = rg, lb = rb, lc = rc;
+            lu.back(plies), ld.back(plies), lz.back(plies), lg.back(plies), lb.back(plies), lc.back(plies);
 #pragma unroll
             for (int k = 0; k < K; ++k) {
-                const bool there = really && t0 + k < end;
-                r.u[k] = wu.get<T>(p.at, 0, there);
-                r.delta[k] = wd.get<T>(p.at, 0, there);
-                r.d_out[k] = wg.get<T>(p.at, 0, there);
-                if (gated) r.gate[k] = wz.get<T>(p.at, 0, there);
-                r.b[k] = wb.get<T>(p.row_at, 0, there);
-                r.c[k] = wc.get<T>(p.row_at, 0, there);
-                wu.base += su, wd.base += sd, wz.base += sz, wg.base += sg, wb.base += sb, wc.base += sc;
+                const uint32_t at = min(k, end - 1 - t0);   // behind the end the last row again
+                r.u[k] = lu.get<T>(p.at, at * lu.step, really);
+                r.delta[k] = ld.get<T>(p.at, at * ld.step, really);
+                r.d_out[k] = lg.get<T>(p.at, at * lg.step, really);
+                if (gated) r.gate[k] = lz.get<T>(p.at, at * lz.step, really);
+                r.b[k] = lb.get<T>(p.row_at, at * lb.step, really);
+                r.c[k] = lc.get<T>(p.row_at, at * lc.step, really);
             }
-            starts = really ? starts_of(q, b, t0, end, p.lane) : 0;
+            starts = really ? game.at(t0, end, p.lane) : 0;
         };
         // the gradient of a gate and the ones of u and delta, their rows as they lie in memory
-        auto give_gate = [&](const Window &to, T u, T gate, T d_out, float y) {
+        auto give_gate = [&](const PlyRows &to, int k, T u, T gate, T d_out, float y) {
             const float z = (float)gate, s = sigmoid(z);
-            to.put<T>(p.at, from_float<T>((float)d_out * (skips ? fmaf(skip, (float)u, y) : y) * s * fmaf(z, 1.f - s, 1.f)));
+            to.put<T>(p.at, from_float<T>((float)d_out * (skips ? fmaf(skip, (float)u, y) : y) * s * fmaf(z, 1.f - s, 1.f)), k * to.step);
         };
-        auto give = [&](const Window &to_u, const Window &to_delta, T u, T delta, float dt, float dy, float s1, float s2) {
+        auto give = [&](const PlyRows &to_u, const PlyRows &to_delta, int k, T u, T delta, float dt, float dy, float s1, float s2) {
             float d_pre = fmaf(s1, (float)u, s2 * LN2);
             if (soft) d_pre *= sigmoid((float)delta + bias);
             if (p.on()) {   // lanes without a channel have read zeros: their sums are not looked at
                 dbias += d_pre;
                 dskip = fmaf(dy, (float)u, dskip);
             }
-            if (want_u) to_u.put<T>(p.at, from_float<T>(skips ? fmaf(s1, dt, skip * dy) : s1 * dt));
-            if (want_delta) to_delta.put<T>(p.at, from_float<T>(d_pre));
+            if (want_u) to_u.put<T>(p.at, from_float<T>(skips ? fmaf(s1, dt, skip * dy) : s1 * dt), k * to_u.step);
+            if (want_delta) to_delta.put<T>(p.at, from_float<T>(d_pre), k * to_delta.step);
         };
         Raw next;
         float h[NS];
         uint32_t next_starts = 0;
         if (begin < end) {
-            load(top, next, next_starts, true);
-            load_apart(p, h, saved_at(q, top), channels);
+            load(top, 0, next, next_starts, true);
+            load_apart(p, h, reinterpret_cast<const float *>(saved), channels);
         }
         for (int t0 = top; t0 >= begin && begin < end; t0 -= K) {
             const uint32_t starts = next_starts;
             const int count = min(end - t0, K);
-            float hist[K][NS], dt[K], dy[K];
+            float hist[K - FAR][NS], dt[K], dy[K];
             {
-                const SelectArgsPtr q = hidden(a);
-                Window to = row_window<T>(&q->dgate, b, t0, 0);
-                const int64_t step = row_step<T>(&q->dgate), sum_step = (int64_t)q->groups * 2 * p.states * 4;
-                Window sums{reinterpret_cast<char *>(q->part_bc) + (((int64_t)(cw % q->waves) * q->batch + b) * q->plies + t0) * sum_step +
-                            (int64_t)(p.group * 2 + 1) * p.states * 4};
+                Window to{sums.base + p.states * 4};
 #pragma unroll
                 for (int k = 0; k < K; ++k) {
                     if (k >= count) break;
@@ -577,47 +601,50 @@ __global__ __launch_bounds__(MANY ? 256 : 64, 2) void k_scan_backward(SelectArgs
                     dt[k] = soft ? softplus(pre) : pre;
                     dy[k] = (float)next.d_out[k];
                     if (gated) dy[k] *= (float)next.gate[k] * sigmoid((float)next.gate[k]);
-                    if (starts >> k & 1)
-#pragma unroll
-                        for (int i = 0; i < NS; ++i) h[i] = 0.f;
+                    if (starts >> k & 1) forget(h);
                     const float push = dt[k] * u;
                     float v[NS];
-                    each_of<NS>([&](auto i) {
-                        hist[k][i] = h[i];
-                        h[i] = fmaf(exp2_fast(dt[k] * A[i]), h[i], row_lane<i>(bt) * push);
+#pragma unroll
+                    for (int i = 0; i < NS; ++i) {
+                        if (k < FAR) far[(k * NS + i / 4 * 4) * 64 + p.lane * 4 + i % 4] = h[i];
+                        else hist[k < FAR ? 0 : k - FAR][i] = h[i];
+                    }
+#pragma unroll
+                    for (int i = 0; i < NS; ++i) h[i] *= exp2_fast(dt[k] * A[i]);
+                    row_add(h, bt, push);
+#pragma unroll
+                    for (int i = 0; i < NS; ++i) {
                         if (!p.has(i)) h[i] = 0.f;
                         v[i] = p.on() ? dy[k] * h[i] : 0.f;
-                    });
+                    }
                     if (want_gate) {
                         const float y = row_dot(0.f, (float)next.c[k], h);
                         if (MANY) share(0, p.sg, k) = y;
-                        else give_gate(to, next.u[k], next.gate[k], next.d_out[k], y);
-                        to.base += step;
+                        else give_gate(to_gate, k, next.u[k], next.gate[k], next.d_out[k], y);
                     }
                     if (want_bc) {
-                        sums.put(sum_at, lane_sums<NS>(v));
-                        sums.base += sum_step;
+                        to.put(sum_at, lane_sums<NS>(v));
+                        to.base += sum_step;
                     }
                 }
             }
             {
-                const int last = t0 + count - 1;
-                const SelectArgsPtr q = hidden(a);
-                Window wu = row_window<T>(&q->u, b, last, 0), wd = row_window<T>(&q->delta, b, last, 0), wb = row_window<T>(&q->b, b, last, p.group),
-                       wc = row_window<T>(&q->c, b, last, p.group), to_u = row_window<T>(&q->du, b, last, 0), to_delta = row_window<T>(&q->ddelta, b, last, 0);
-                const int64_t su = row_step<T>(&q->u), sd = row_step<T>(&q->delta), sb = row_step<T>(&q->b), sc = row_step<T>(&q->c),
-                              tu = row_step<T>(&q->du), td = row_step<T>(&q->ddelta), sum_step = (int64_t)q->groups * 2 * p.states * 4;
-                Window sums{reinterpret_cast<char *>(q->part_bc) + (((int64_t)(cw % q->waves) * q->batch + b) * q->plies + last) * sum_step +
-                            (int64_t)p.group * 2 * p.states * 4};
-                T u = wu.get<T>(p.at), delta = wd.get<T>(p.at), bb = wb.get<T>(p.row_at), cc = wc.get<T>(p.row_at);
+                Window to{sums.base + (count - 1) * sum_step};
+                const uint32_t last = count - 1;
+                T u = ru.get<T>(p.at, last * ru.step), delta = rd.get<T>(p.at, last * rd.step), bb = rb.get<T>(p.row_at, last * rb.step),
+                  cc = rc.get<T>(p.row_at, last * rc.step);
 #pragma unroll
                 for (int k = K - 1; k >= 0; --k) {
-                    if (k == K / 2 - 1) load(t0 - K, next, next_starts, t0 > begin);
+                    if (k == K / 2 - 1) {
+                        load(t0 - K, K, next, next_starts, t0 > begin);
+                        load_apart(p, h, reinterpret_cast<const float *>(saved - state_bytes), channels, t0 > begin);
+                    }
                     if (k >= count) continue;
                     const T u0 = u, delta0 = delta, b0 = bb, c0 = cc;
                     if (k) {
-                        wu.base -= su, wd.base -= sd, wb.base -= sb, wc.base -= sc;
-                        u = wu.get<T>(p.at), delta = wd.get<T>(p.at), bb = wb.get<T>(p.row_at), cc = wc.get<T>(p.row_at);
+                        const uint32_t at = k - 1;
+                        u = ru.get<T>(p.at, at * ru.step), delta = rd.get<T>(p.at, at * rd.step), bb = rb.get<T>(p.row_at, at * rb.step);
+                        cc = rc.get<T>(p.row_at, at * rc.step);
                     }
                     asm("" : "+v"(dt[k]));   // the decays once more: kept from the way there they would take 128 registers
                     const float push = dt[k] * (float)u0;
@@ -631,32 +658,25 @@ __global__ __launch_bounds__(MANY ? 256 : 64, 2) void k_scan_backward(SelectArgs
                     const float s1 = row_dot(0.f, (float)b0, dh);
                     float s2 = 0.f;
                     if (want_bc) {
-                        sums.put(sum_at, lane_sums<NS>(v));
-                        sums.base -= sum_step;
+                        to.put(sum_at, lane_sums<NS>(v));
+                        to.base -= sum_step;
                     }
-                    if (starts >> k & 1) {
-#pragma unroll
-                        for (int i = 0; i < NS; ++i) dh[i] = 0.f;
-                    } else {
+                    if (starts >> k & 1) forget(dh);
+                    else {
 #pragma unroll
                         for (int i = 0; i < NS; ++i) {
                             dh[i] *= exp2_fast(dt[k] * A[i]);
-                            const float w = dh[i] * hist[k][i];
+                            const float w = dh[i] * (k < FAR ? far[(k * NS + i / 4 * 4) * 64 + p.lane * 4 + i % 4] : hist[k < FAR ? 0 : k - FAR][i]);
                             s2 = fmaf(w, A[i], s2);
                             dA[i] = fmaf(w, dt[k], dA[i]);
                         }
                     }
                     if (MANY) share(1, p.sg, k) = s1, share(2, p.sg, k) = s2;
-                    else {
-                        give(to_u, to_delta, u0, delta0, dt[k], dy[k], s1, s2);
-                        to_u.base -= tu, to_delta.base -= td;
-                    }
+                    else give(to_u, to_delta, k, u0, delta0, dt[k], dy[k], s1, s2);
                 }
-                load_apart(p, h, saved_at(hidden(a), t0 - K), channels, t0 > begin);
             }
             if constexpr (MANY) {
                 __syncthreads();
-                const SelectArgsPtr q = hidden(a);
 #pragma unroll
                 for (int k = 0; k < K; ++k) {
                     if (k >= count) break;
@@ -667,15 +687,15 @@ __global__ __launch_bounds__(MANY ? 256 : 64, 2) void k_scan_backward(SelectArgs
                         all[1] += share(1, g, k);
                         all[2] += share(2, g, k);
                     }
-                    const T u = row_window<T>(&q->u, b, t0 + k, 0).template get<T>(p.at);
-                    if (want_gate)
-                        give_gate(row_window<T>(&q->dgate, b, t0 + k, 0), u, row_window<T>(&q->gate, b, t0 + k, 0).template get<T>(p.at),
-                                  row_window<T>(&q->d_out, b, t0 + k, 0).template get<T>(p.at), all[0]);
-                    give(row_window<T>(&q->du, b, t0 + k, 0), row_window<T>(&q->ddelta, b, t0 + k, 0), u,
-                         row_window<T>(&q->delta, b, t0 + k, 0).template get<T>(p.at), dt[k], dy[k], all[1], all[2]);
+                    const T u = ru.get<T>(p.at, k * ru.step);
+                    if (want_gate) give_gate(to_gate, k, u, rz.get<T>(p.at, k * rz.step), rg.get<T>(p.at, k * rg.step), all[0]);
+                    give(to_u, to_delta, k, u, rd.get<T>(p.at, k * rd.step), dt[k], dy[k], all[1], all[2]);
                 }
                 __syncthreads();   // the next chunk's shares take their place
             }
+            ru.back(K), rd.back(K), rz.back(K), rg.back(K), rb.back(K), rc.back(K), to_u.back(K), to_delta.back(K), to_gate.back(K);
+            saved -= state_bytes;
+            sums.base -= K * sum_step;
         }
         if (seg == 0) {
             float *to = hidden(a)->d_initial;
@@ -686,16 +706,16 @@ __global__ __launch_bounds__(MANY ? 256 : 64, 2) void k_scan_backward(SelectArgs
     if (!q->want_a) return;
     if constexpr (MANY) {   // each wave has some plies' share of dskip and dbias
         __syncthreads();
-        lds[p.sg * 64 + p.lane] = dskip;
-        lds[(SG + p.sg) * 64 + p.lane] = dbias;
+        share(0, p.sg, 0) = dskip;
+        share(1, p.sg, 0) = dbias;
         __syncthreads();
         dskip = dbias = 0.f;
         for (int g = 0; g < SG; ++g) {
-            dskip += lds[g * 64 + p.lane];
-            dbias += lds[(SG + g) * 64 + p.lane];
+            dskip += share(0, g, 0);
+            dbias += share(1, g, 0);
         }
     }
-    float *to = q->part_a + (int64_t)part * (p.states + 2) * channels;
+    float *to = q->part_a + (int64_t)p.part * (p.states + 2) * channels;
     store_apart(p, dA, to, channels);
     if (p.sg == 0 && p.on()) {
         to[(int64_t)p.states * channels + p.ch] = dskip;
@@ -703,22 +723,27 @@ __global__ __launch_bounds__(MANY ? 256 : 64, 2) void k_scan_backward(SelectArgs
     }
 }
 
-// db and dc: the waves' shares summed in a fixed order; 0 from a game's length on.
-template <class T>
+// db and dc: the waves' shares summed in a fixed order; 0 from a game's length on. N values
+// a thread, which lie together: states is a multiple of N.
+template <class T, int N>
 __global__ __launch_bounds__(256) void k_scan_join_bc(SelectArgs a, jq_rows db, jq_rows dc)
 {
-    const int n2 = 2 * a.states;
+    typedef float V __attribute__((ext_vector_type(N)));
+    const int n2 = 2 * a.states / N;
     const int64_t tokens = (int64_t)a.batch * a.plies, all = tokens * a.groups * n2;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
-        const int j = i % n2, g = i / n2 % a.groups;
-        const int64_t token = i / n2 / a.groups, b = token / a.plies;
-        const int t = token % a.plies;
-        float s = 0.f;
+        const int64_t of = i / n2, token = of / a.groups, b = token / a.plies;
+        const int j = (int)(i - of * n2) * N, g = (int)(of - token * a.groups), t = (int)(token - b * a.plies);
         const int len = a.lengths ? min(max(a.lengths[b], 0), a.plies) : a.plies;
+        V s{};
         if (t < len)
-            for (int w = 0; w < a.waves; ++w) s += a.part_bc[w * all + i];
+#pragma unroll 4
+            for (int w = 0; w < a.waves; ++w) s += reinterpret_cast<const V *>(a.part_bc)[w * all + i];
         const jq_rows &r = j < a.states ? db : dc;
-        if (r.data) row_at<T>(r, b, t, g)[j < a.states ? j : j - a.states] = from_float<T>(s);
+        if (!r.data) continue;
+        T *to = row_at<T>(r, b, t, g) + (j < a.states ? j : j - a.states);
+#pragma unroll
+        for (int e = 0; e < N; ++e) to[e] = from_float<T>(s[e]);
     }
 }
 

@@ -18,6 +18,7 @@ using namespace jq;
 namespace {
 
 constexpr int MOST_CHANNELS = 1 << 20, MOST_PLIES = 1 << 30, MOST_BLOCKS = 1 << 20;
+static_assert(SCAN_STEP == JQ_SCAN_MAX_PLY_STRIDE, "the header's limit");
 constexpr int64_t MOST_ELEMENTS = 1ll << 42;   // of a segment's rows: every size below fits 64 bits
 constexpr int MOST_GAMES = 1 << 30;            // with the parts of a split axis they fit 32
 
@@ -52,15 +53,24 @@ int check_scan(const jq_scan *a)
     return check_states(a->channels, a->states, a->groups);
 }
 
+// Rows of a segment whose plies a chunk's 32-bit offsets reach.
+int check_ply_rows(const jq_scan *a, const jq_rows &r, const char *name)
+{
+    TRY(check_rows(r, a->dtype, name));
+    if (a->plies > 1 && (r.ply < 0 || r.ply > JQ_SCAN_MAX_PLY_STRIDE / (int64_t)elem_bytes(a->dtype)))
+        return fail(JQ_E_ARG, "the plies of %s are %lld elements apart", name, (long long)r.ply);
+    return JQ_OK;
+}
+
 int check_scan_inputs(const jq_scan *a)
 {
     if (!a->a) return fail(JQ_E_ARG, "null a");
     if (a->plies == 0 || a->batch == 0) return JQ_OK;
-    TRY(check_rows(a->u, a->dtype, "u"));
-    TRY(check_rows(a->delta, a->dtype, "delta"));
-    TRY(check_rows(a->b, a->dtype, "b"));
-    TRY(check_rows(a->c, a->dtype, "c"));
-    if (a->gate.data) TRY(check_rows(a->gate, a->dtype, "gate"));
+    TRY(check_ply_rows(a, a->u, "u"));
+    TRY(check_ply_rows(a, a->delta, "delta"));
+    TRY(check_ply_rows(a, a->b, "b"));
+    TRY(check_ply_rows(a, a->c, "c"));
+    if (a->gate.data) TRY(check_ply_rows(a, a->gate, "gate"));
     return JQ_OK;
 }
 
@@ -93,7 +103,7 @@ Split split_of(const jq_scan *a)
 }
 
 // Blocks that share the backward pass's items, each with its own sums of da, dskip and dbias.
-constexpr int BACKWARD_WAVES = 4096;
+constexpr int BACKWARD_WAVES = 2048;
 int64_t scan_parts(const jq_scan *a)
 {
     const ScanShape s = scan_shape(a);
@@ -122,7 +132,7 @@ int check_scan_workspace(const jq_scan *a, bool backward)
     const int64_t need = scan_bytes(a, backward).all();
     if (a->workspace_bytes < need || (need && !a->workspace))
         return fail(JQ_E_ARG, "workspace of %lld bytes, %lld are needed", (long long)a->workspace_bytes, (long long)need);
-    if (!aligned(a->workspace, 4)) return fail(JQ_E_ARG, "workspace must be 4-byte aligned");
+    if (!aligned(a->workspace, 16)) return fail(JQ_E_ARG, "workspace must be 16-byte aligned");
     return JQ_OK;
 }
 
@@ -141,21 +151,23 @@ SelectArgs select_args(const jq_scan *a, bool backward)
     s.segments = split.segments, s.seg_plies = split.seg_plies;
     const ScanBytes n = scan_bytes(a, backward);
     char *w = static_cast<char *>(a->workspace);
-    s.seg_state = reinterpret_cast<float *>(w);
-    s.seg_sum = reinterpret_cast<float *>(w + n.state);
-    s.part_bc = reinterpret_cast<float *>(w + n.state + n.sum);
-    s.part_a = reinterpret_cast<float *>(w + n.state + n.sum + n.bc);
+    s.part_bc = reinterpret_cast<float *>(w);   // first: read in vectors
+    s.seg_state = reinterpret_cast<float *>(w + n.bc);
+    s.seg_sum = reinterpret_cast<float *>(w + n.bc + n.state);
+    s.part_a = reinterpret_cast<float *>(w + n.bc + n.state + n.sum);
     s.want_bc = n.bc, s.want_a = n.a;
-    s.parts = (int)scan_parts(a);
     return s;
 }
 
-// f(states of a lane, exact)
+// f(states of a lane, exact, more than one wave of states)
 template <class F>
 int by_shape(const ScanShape &s, F &&f)
 {
-    auto go = [&](auto ns) { return s.exact ? f(ns, std::true_type()) : f(ns, std::false_type()); };
-    return s.ns == 4 ? go(std::integral_constant<int, 4>()) : s.ns == 8 ? go(std::integral_constant<int, 8>()) : go(std::integral_constant<int, 16>());
+    using std::integral_constant;
+    auto go = [&](auto ns, auto many) { return s.exact ? f(ns, std::true_type(), many) : f(ns, std::false_type(), many); };
+    if (s.sg > 1) return go(integral_constant<int, 16>(), std::true_type());
+    return s.ns == 4 ? go(integral_constant<int, 4>(), std::false_type())
+           : s.ns == 8 ? go(integral_constant<int, 8>(), std::false_type()) : go(integral_constant<int, 16>(), std::false_type());
 }
 
 int grid_over(int64_t threads) { return (int)std::max<int64_t>(1, std::min<int64_t>((threads + 255) / 256, 1 << 16)); }
@@ -167,10 +179,16 @@ int launch_join(const SelectArgs &s, hipStream_t stream)
     return launch_check("k_scan_join");
 }
 
-int scan_grid(const SelectArgs &s)
+// Blocks and threads of a pass in which `parts` share the items, and s.parts set to them.
+constexpr int SCAN_BLOCK_WAVES = 4;
+struct ScanGrid { dim3 grid, block; };
+ScanGrid scan_grid(SelectArgs &s, const ScanShape &shape, int64_t parts)
 {
     const int cw = s.waves * s.groups;
-    return cw * (int)std::max<int64_t>(1, std::min<int64_t>((int64_t)s.batch * s.segments, MOST_BLOCKS / cw));
+    s.parts = (int)std::max<int64_t>(1, std::min<int64_t>(parts, MOST_BLOCKS / cw));
+    const int64_t waves = (int64_t)cw * s.parts;
+    if (shape.sg > 1) return {dim3((int)waves), dim3(64 * shape.sg)};
+    return {dim3((int)((waves + SCAN_BLOCK_WAVES - 1) / SCAN_BLOCK_WAVES)), dim3(64 * SCAN_BLOCK_WAVES)};
 }
 
 // ------------------------------------------------------------------ convolution
@@ -326,22 +344,22 @@ int jq_scan_forward(const jq_scan *a, void *stream)
     TRY(check_scan(a));
     if (a->batch == 0) return JQ_OK;
     TRY(check_scan_inputs(a));
-    if (a->plies) TRY(check_rows(a->out, a->dtype, "out"));
+    if (a->plies) TRY(check_ply_rows(a, a->out, "out"));
     TRY(check_scan_workspace(a, false));
-    const SelectArgs s = select_args(a, false);
+    SelectArgs s = select_args(a, false);
     const ScanShape shape = scan_shape(a);
     const hipStream_t q = strm(stream);
+    const ScanGrid g = scan_grid(s, shape, (int64_t)s.batch * s.segments);
     return by_type(a->dtype, [&](auto t) {
         using T = decltype(t);
-        return by_shape(shape, [&](auto ns, auto exact) {
-            const dim3 grid(scan_grid(s)), block(64 * shape.sg);
+        return by_shape(shape, [&](auto ns, auto exact, auto many) {
             if (s.segments > 1) {
-                hipLaunchKernelGGL((k_scan_forward<T, ns(), exact(), false>), grid, block, 0, q, s);
+                hipLaunchKernelGGL((k_scan_forward<T, ns(), exact(), many(), false>), g.grid, g.block, 0, q, s);
                 TRY(launch_check("k_scan_forward (states)"));
                 TRY(launch_join<false>(s, q));
             }
-            const size_t lds = shape.sg > 1 ? 2 * shape.sg * SCAN_PLIES * 64 * sizeof(float) : 0;
-            hipLaunchKernelGGL((k_scan_forward<T, ns(), exact(), true>), grid, block, lds, q, s);
+            const size_t lds = many() ? 2 * shape.sg * SCAN_PLIES * 64 * sizeof(float) : 0;
+            hipLaunchKernelGGL((k_scan_forward<T, ns(), exact(), many(), true>), g.grid, g.block, lds, q, s);
             return launch_check("k_scan_forward");
         });
     });
@@ -351,34 +369,36 @@ int jq_scan_backward(const jq_scan *a, void *stream)
 {
     TRY(check_scan(a));
     TRY(check_scan_inputs(a));
-    if (a->plies && a->batch) TRY(check_rows(a->d_out, a->dtype, "d_out"));
+    if (a->plies && a->batch) TRY(check_ply_rows(a, a->d_out, "d_out"));
     if (a->plies && a->batch && !a->saved) return fail(JQ_E_ARG, "null saved");
     if (a->dgate.data && !a->gate.data) return fail(JQ_E_ARG, "dgate without a gate");
     for (const jq_rows *r : {&a->du, &a->ddelta, &a->dgate, &a->db, &a->dc})
-        if (r->data) TRY(check_rows(*r, a->dtype, "a gradient"));   // absent ones are not wanted
+        if (r->data) TRY(check_ply_rows(a, *r, "a gradient"));   // absent ones are not wanted
     TRY(check_scan_workspace(a, true));
     SelectArgs s = select_args(a, true);
     s.d_out = a->d_out, s.du = a->du, s.ddelta = a->ddelta, s.dgate = a->dgate;
     s.d_final = a->d_final, s.d_initial = a->d_initial;
     const ScanShape shape = scan_shape(a);
     const hipStream_t q = strm(stream);
+    const int64_t parts = scan_parts(a);
     return by_type(a->dtype, [&](auto t) {
         using T = decltype(t);
-        return by_shape(shape, [&](auto ns, auto exact) {
-            const dim3 block(64 * shape.sg);
+        return by_shape(shape, [&](auto ns, auto exact, auto many) {
             if (s.segments > 1) {
-                hipLaunchKernelGGL((k_scan_carry<T, ns(), exact()>), dim3(scan_grid(s)), block, 0, q, s);
+                const ScanGrid g = scan_grid(s, shape, (int64_t)s.batch * s.segments);
+                hipLaunchKernelGGL((k_scan_carry<T, ns(), exact(), many()>), g.grid, g.block, 0, q, s);
                 TRY(launch_check("k_scan_carry"));
                 TRY(launch_join<true>(s, q));
             }
-            const dim3 grid(s.parts * s.waves * s.groups);
-            const size_t lds = 3 * shape.sg * SCAN_CHUNK * 64 * sizeof(float);
-            if (shape.sg == 1) hipLaunchKernelGGL((k_scan_backward<T, ns(), exact(), false>), grid, block, 0, q, s);
-            else if constexpr (ns() == 16) hipLaunchKernelGGL((k_scan_backward<T, 16, exact(), true>), grid, block, lds, q, s);
+            const ScanGrid g = scan_grid(s, shape, parts);
+            const size_t far = (size_t)g.block.x * scan_far(ns()) * ns() * sizeof(float);
+            const size_t shares = many() ? 3 * shape.sg * SCAN_CHUNK * 64 * sizeof(float) : 0;
+            hipLaunchKernelGGL((k_scan_backward<T, ns(), exact(), many()>), g.grid, g.block, far + shares, q, s);
             TRY(launch_check("k_scan_backward"));
             if (s.want_bc && s.batch && s.plies) {
                 const int64_t n = (int64_t)s.batch * s.plies * s.groups * 2 * s.states;
-                hipLaunchKernelGGL(k_scan_join_bc<T>, dim3(grid_over(n)), dim3(256), 0, q, s, a->db, a->dc);
+                if (s.states % 4 == 0) hipLaunchKernelGGL((k_scan_join_bc<T, 4>), dim3(grid_over(n / 4)), dim3(256), 0, q, s, a->db, a->dc);
+                else hipLaunchKernelGGL((k_scan_join_bc<T, 1>), dim3(grid_over(n)), dim3(256), 0, q, s, a->db, a->dc);
                 TRY(launch_check("k_scan_join_bc"));
             }
             if (!s.want_a) return JQ_OK;

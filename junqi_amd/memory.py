@@ -539,6 +539,13 @@ def _check_step(name: str, x: torch.Tensor, state: torch.Tensor, state_shape: tu
 
 
 # ------------------------------------------------------------------ selective scan
+def _near(t: torch.Tensor) -> torch.Tensor:
+    """`t` with adjacent elements and plies that the scan's 32-bit offsets reach, or a copy that has them."""
+    t = _adjacent(t)
+    far = t.shape[1] > 1 and t.stride(1) * t.element_size() > L.SCAN_MAX_PLY_STRIDE
+    return t.contiguous() if far else t
+
+
 def _check_scan(u, delta, a, b, c, skip, gate, delta_bias, lead: int):
     """The checks that segments (lead 2) and steps (lead 1) share; the arguments with one
     group written out and adjacent elements."""
@@ -567,8 +574,9 @@ def _check_scan(u, delta, a, b, c, skip, gate, delta_bias, lead: int):
     for name, t in (("skip", skip), ("delta_bias", delta_bias)):
         if t is not None:
             _check(name, t, (d,), (torch.float32,), u)
-    return (_adjacent(u), _adjacent(delta), a.contiguous(), _adjacent(b), _adjacent(c),
-            None if skip is None else skip.contiguous(), None if gate is None else _adjacent(gate),
+    near = _near if lead == 2 else _adjacent
+    return (near(u), near(delta), a.contiguous(), near(b), near(c),
+            None if skip is None else skip.contiguous(), None if gate is None else near(gate),
             None if delta_bias is None else delta_bias.contiguous())
 
 
@@ -615,7 +623,7 @@ class _Scan(torch.autograd.Function):
         u, delta, a, b, c, skip, gate, delta_bias, starts, lengths, saved = ctx.saved_tensors
         if d_out is None and d_final is None:
             return (None,) * 13
-        d_out = torch.zeros_like(u) if d_out is None else _adjacent(d_out)
+        d_out = torch.zeros_like(u) if d_out is None else _near(d_out)
         s = _scan_args(u, delta, a, b, c, skip, gate, delta_bias, ctx.softplus)
         _set_segments(s, starts, lengths)
         need = ctx.needs_input_grad
