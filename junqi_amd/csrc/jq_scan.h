@@ -588,9 +588,10 @@ __global__ __launch_bounds__(256, 2) void k_scan_backward(SelectArgs)
             load(top, 0, next, next_starts, true);
             load_apart(p, h, reinterpret_cast<const float *>(saved), channels);
         }
-        for (int t0 = top; t0 >= begin && begin < end; t0 -= K) {
+        // the chunk from ply t0 on; whole: K plies
+        auto chunk = [&](int t0, auto whole) {
             const uint32_t starts = next_starts;
-            const int count = min(end - t0, K);
+            const int count = whole ? K : min(end - t0, K);
             float hist[K - FAR][NS], dt[K], dy[K];
             {
                 Window to{sums.base + p.states * 4};
@@ -696,6 +697,12 @@ __global__ __launch_bounds__(256, 2) void k_scan_backward(SelectArgs)
             ru.back(K), rd.back(K), rz.back(K), rg.back(K), rb.back(K), rc.back(K), to_u.back(K), to_delta.back(K), to_gate.back(K);
             saved -= state_bytes;
             sums.base -= K * sum_step;
+        };
+        if (begin < end) {
+            // only the last chunk may have fewer plies: the others take code without a way round each
+            int t0 = top;
+            if (end - top < K) chunk(t0, std::false_type()), t0 -= K;
+            for (; t0 >= begin; t0 -= K) chunk(t0, std::true_type());
         }
         if (seg == 0) {
             float *to = hidden(a)->d_initial;
