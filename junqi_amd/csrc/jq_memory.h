@@ -32,6 +32,43 @@ template <class T> struct Vec;
 template <> struct Vec<float> { typedef f32x4 type; static constexpr int N = 4; };
 template <> struct Vec<bf16> { typedef bf16x8 type; static constexpr int N = 8; };
 
+template <class T, int V> struct Pack { typedef T type __attribute__((ext_vector_type(V))); };
+
+// V elements at any element alignment, zeros from n on (n >= 1).
+template <class T, int V>
+__device__ __forceinline__ typename Pack<T, V>::type load_some(const T *p, int n)
+{
+    typedef typename Pack<T, V>::type R;
+    typedef R At __attribute__((aligned(sizeof(T))));
+    if (n >= V) return *reinterpret_cast<const At *>(p);
+    R r;
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+        const T y = p[e < n ? e : n - 1];
+        r[e] = e < n ? y : T(0.f);
+    }
+    return r;
+}
+template <class T, int V>
+__device__ __forceinline__ void store_some(T *p, int n, typename Pack<T, V>::type r)
+{
+    typedef typename Pack<T, V>::type R;
+    typedef R At __attribute__((aligned(sizeof(T))));
+    if (n >= V) *reinterpret_cast<At *>(p) = r;
+    else
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+            if (e < n) p[e] = r[e];
+}
+template <class T, int V>
+__device__ __forceinline__ void store_floats(T *p, int n, const float *x)
+{
+    typename Pack<T, V>::type r;
+#pragma unroll
+    for (int e = 0; e < V; ++e) r[e] = from_float<T>(x[e]);
+    store_some<T, V>(p, n, r);
+}
+
 // x + x of the lane O lanes across (l ^ O), O a power of two, where the lanes of each
 // aligned group of O hold one sum: then a mirrored row stands for O = 4 and 8, and no
 // step goes through LDS.

@@ -790,69 +790,87 @@ struct SelectStepArgs {
     const uint8_t *starts;
 };
 
-// L lanes a channel, four states each: a wave walks games with its channels' a in
-// registers, so what it moves is the states.
-template <class T, int L>
+// L lanes a channel, four states each. Bound by the states, read and written once: a wave
+// walks games with its channels' a in registers and the next game's state, rows and flags
+// on their way; the states of calls that the caches would not hold to the next ply go past
+// them.
+template <class T, int L, bool STREAM>
 __global__ __launch_bounds__(256) void k_scan_step(SelectStepArgs a, int channel_waves, int at_once)
 {
     constexpr int PER = 64 / L;
     typedef f32x4 At __attribute__((aligned(4)));
     const int lane = threadIdx.x % 64;
-    const int64_t wave = (int64_t)blockIdx.x * 4 + threadIdx.x / 64;
-    if (wave >= (int64_t)channel_waves * at_once) return;
+    const int wave = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    if (wave >= channel_waves * at_once) return;
     const int cw = wave % channel_waves;
     const int ch = cw * PER + lane / L, n = lane % L * 4, left = min(a.states - n, 4);
     const bool on = ch < a.channels, mine = on && left > 0;
-    const int at = on ? ch : 0, group = at / a.per;
+    const int at = on ? ch : a.channels - 1, group = at / a.per;
     float A[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) A[e] = mine && e < left ? a.a[(int64_t)at * a.states + n + e] * LOG2E : 0.f;
     const float skip = a.skip ? a.skip[at] : 0.f, bias = a.bias ? a.bias[at] : 0.f;
-    for (int64_t game = wave / channel_waves; game < a.batch; game += at_once) {
-        const int64_t row = a.rows ? a.rows[game] : game;
-        if (row < 0 || row >= a.state_rows) {
-            if (on && n == 0) row_at<T>(a.out, game, 0, 0)[ch] = T(0.f);
-            continue;
-        }
-        float *s = a.state + (row * a.channels + at) * a.states + n;
-        const bool start = a.starts && a.starts[game];
-        float h[4], bt[4], ct[4];
+    struct Game { int64_t row; f32x4 h; T b[4], c[4], u, delta, gate; bool start, there; };
+    auto load = [&](int game, Game &g) {
+        g.row = a.rows ? a.rows[game] : game;
+        g.there = g.row >= 0 && g.row < a.state_rows;
+        g.start = a.starts && a.starts[game];
+        g.u = row_at<const T>(a.u, game, 0, 0)[at];
+        g.delta = row_at<const T>(a.delta, game, 0, 0)[at];
+        if (a.gate.data) g.gate = row_at<const T>(a.gate, game, 0, 0)[at];
         const T *pb = row_at<const T>(a.b, game, 0, group) + n, *pc = row_at<const T>(a.c, game, 0, group) + n;
-        if (left >= 4) {
-            const f32x4 v = *reinterpret_cast<const At *>(s);
+        g.h = f32x4{};
 #pragma unroll
-            for (int e = 0; e < 4; ++e) h[e] = v[e], bt[e] = (float)pb[e], ct[e] = (float)pc[e];
+        for (int e = 0; e < 4; ++e) g.b[e] = g.c[e] = T(0.f);
+        if (!mine) return;
+        const float *s = a.state + (g.row * a.channels + at) * a.states + n;
+        if (left >= 4) {
+            if (g.there) g.h = STREAM ? __builtin_nontemporal_load(reinterpret_cast<const At *>(s)) : *reinterpret_cast<const At *>(s);
+            const typename Pack<T, 4>::type vb = load_some<T, 4>(pb, 4), vc = load_some<T, 4>(pc, 4);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) g.b[e] = vb[e], g.c[e] = vc[e];
         } else
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const bool there = e < left;
-                h[e] = there ? s[e] : 0.f;
-                bt[e] = there ? (float)pb[e] : 0.f;
-                ct[e] = there ? (float)pc[e] : 0.f;
-            }
-        const float u = (float)row_at<const T>(a.u, game, 0, 0)[at], pre = (float)row_at<const T>(a.delta, game, 0, 0)[at] + bias;
-        const float dt = a.softplus ? softplus(pre) : pre, push = dt * u;
+            for (int e = 0; e < 4; ++e)
+                if (e < left) {
+                    if (g.there) g.h[e] = s[e];
+                    g.b[e] = pb[e], g.c[e] = pc[e];
+                }
+    };
+    int game = wave / channel_waves;
+    Game next;
+    if (game < a.batch) load(game, next);
+    for (; game < a.batch; game += at_once) {
+        const Game g = next;
+        if (game + at_once < a.batch) load(game + at_once, next);
+        T *out = row_at<T>(a.out, game, 0, 0) + at;
+        if (!g.there) {
+            if (on && n == 0) *out = T(0.f);
+            continue;
+        }
+        const float u = (float)g.u, pre = (float)g.delta + bias, dt = a.softplus ? softplus(pre) : pre, push = dt * u;
+        f32x4 h;
         float y = 0.f;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const float old = start ? 0.f : exp2_fast(dt * A[e]) * h[e];
-            h[e] = fmaf(bt[e], push, old);
-            if (e < left) y = fmaf(ct[e], h[e], y);
+            const float old = g.start ? 0.f : exp2_fast(dt * A[e]) * g.h[e];
+            h[e] = fmaf((float)g.b[e], push, old);
+            if (e < left) y = fmaf((float)g.c[e], h[e], y);
         }
         if (mine) {
-            if (left >= 4) *reinterpret_cast<At *>(s) = At{h[0], h[1], h[2], h[3]};
-            else
+            float *s = a.state + (g.row * a.channels + at) * a.states + n;
+            if (left >= 4) {
+                if (STREAM) __builtin_nontemporal_store(h, reinterpret_cast<At *>(s));
+                else *reinterpret_cast<At *>(s) = h;
+            } else
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
                     if (e < left) s[e] = h[e];
         }
         y = group_total<L>(y);
         if (a.skip) y = fmaf(skip, u, y);
-        if (a.gate.data) {
-            const float z = (float)row_at<const T>(a.gate, game, 0, 0)[at];
-            y *= z * sigmoid(z);
-        }
-        if (on && n == 0) row_at<T>(a.out, game, 0, 0)[ch] = from_float<T>(y);
+        if (a.gate.data) y *= (float)g.gate * sigmoid((float)g.gate);
+        if (on && n == 0) *out = from_float<T>(y);
     }
 }
 

@@ -111,6 +111,11 @@ int64_t scan_parts(const jq_scan *a)
     return std::max<int64_t>(1, std::min(items, BACKWARD_WAVES / (blocks * s.sg)));
 }
 
+// One ply: waves that walk the games, and the bytes of states past which they would not be
+// found in the caches at the next ply.
+constexpr int STEP_GAME_WAVES = 16384;
+constexpr int64_t STEP_STREAM_BYTES = 400ll << 20;
+
 struct ScanBytes { int64_t state, sum, bc, a; int64_t all() const { return state + sum + bc + a; } };
 ScanBytes scan_bytes(const jq_scan *a, bool backward)
 {
@@ -281,11 +286,12 @@ int by_taps(int32_t dtype, int32_t weight_dtype, int taps, F &&f)
 }
 
 // ------------------------------------------------------------------ logits
+constexpr int LOGITS_MOST_ACTIONS = INT_MAX - 4096;   // a lane's columns are walked that far past the last
 int check_logits(const jq_logits *a)
 {
     if (!a) return fail(JQ_E_ARG, "null arguments");
     TRY(check_dtype(a->dtype));
-    if (a->rows < 0 || a->rows > INT_MAX || a->actions <= 0 || a->actions > INT_MAX - LOGITS_TILE || a->recent_count < 0 || a->recent_count > INT_MAX - 256)
+    if (a->rows < 0 || a->rows > INT_MAX || a->actions <= 0 || a->actions > LOGITS_MOST_ACTIONS || a->recent_count < 0 || a->recent_count > INT_MAX - 256)
         return fail(JQ_E_ARG, "bad shapes (rows %lld, actions %d, recent %d)", (long long)a->rows, a->actions, a->recent_count);
     if (a->mask && a->mask_kind != JQ_LOGITS_MASK_WORDS && a->mask_kind != JQ_LOGITS_MASK_BYTES) return fail(JQ_E_ARG, "mask kind %d", a->mask_kind);
     if (a->mask && a->mask_kind == JQ_LOGITS_MASK_WORDS && !aligned(a->mask, 4)) return fail(JQ_E_ARG, "mask words must be 4-byte aligned");
@@ -299,7 +305,7 @@ LogitsArgs logits_args(const jq_logits *a)
 {
     LogitsArgs l{};
     l.x = a->logits, l.x_stride = a->logits_stride;
-    l.rows = a->rows, l.actions = a->actions, l.tiles = (a->actions + LOGITS_TILE - 1) / LOGITS_TILE;
+    l.rows = a->rows, l.actions = a->actions;
     l.bias = a->bias;
     if (a->mask && a->mask_kind == JQ_LOGITS_MASK_WORDS) l.words = static_cast<const uint32_t *>(a->mask);
     else l.dense = static_cast<const uint8_t *>(a->mask);
@@ -311,12 +317,41 @@ LogitsArgs logits_args(const jq_logits *a)
     return l;
 }
 
-// Blocks of the backward pass, each with its own sums of dbias.
-constexpr int LOGITS_BLOCKS = 4096;
+// Columns of a wave: whole rows where there are enough for the card's waves, else parts of
+// them, and no more than LDS has a mask for. Blocks of as many waves as LDS has tables for
+// (a wave gets at most as many actions as it has columns).
+constexpr int LOGITS_WAVES = 4096, LOGITS_TABLE_TILE = 2048;
+constexpr size_t LOGITS_LDS = 64 << 10;
+struct LogitsGrid { dim3 grid, block; size_t lds; };
+template <class T>
+LogitsGrid logits_grid(LogitsArgs &l)
+{
+    constexpr int64_t STEP = 64 * Vec<T>::N;   // a vector for each lane
+    const int64_t want = std::max<int64_t>(1, LOGITS_WAVES / std::max<int64_t>(1, l.rows));
+    int64_t tile = std::min<int64_t>((l.actions / want + STEP) / STEP * STEP, LOGITS_TILE);
+    if (l.recent_count > LOGITS_TABLE_TILE) tile = std::min<int64_t>(tile, LOGITS_TABLE_TILE);
+    l.tile = (int)tile;
+    l.tiles = (int)((l.actions + tile - 1) / tile);
+    l.mask_words = (int)((std::min<int64_t>(tile, l.actions) + 31) / 32);
+    l.slots = 0;
+    if (l.recent_count)
+        for (l.slots = 64; l.slots < 2 * std::min(l.recent_count, l.tile); l.slots *= 2) {}
+    const size_t each = 4 * ((size_t)l.mask_words + 2 * l.slots);
+    int waves = 4;
+    while (waves > 1 && waves * each > LOGITS_LDS) waves /= 2;
+    return {dim3((unsigned)std::min<int64_t>((l.rows * l.tiles + waves - 1) / waves, 1 << 23)), dim3(64 * waves), waves * each};
+}
+
+// Blocks along the rows that sum dbias.
+constexpr int LOGITS_BIAS_BLOCKS = 2048;
+int bias_tiles(const jq_logits *a)
+{
+    const int64_t columns = 256 * (a->dtype == JQ_F32 ? 4 : 8);
+    return (int)((a->actions + columns - 1) / columns);
+}
 int64_t logits_parts(const jq_logits *a)
 {
-    const int64_t tiles = (a->actions + LOGITS_TILE - 1) / LOGITS_TILE;
-    return std::max<int64_t>(1, std::min<int64_t>(a->rows, LOGITS_BLOCKS / tiles));
+    return std::max<int64_t>(1, std::min<int64_t>((a->rows + 3) / 4, LOGITS_BIAS_BLOCKS / bias_tiles(a)));
 }
 
 }  // namespace
@@ -425,8 +460,11 @@ int jq_scan_step(const jq_scan *a, float *state, int64_t state_rows, const int64
         using T = decltype(t);
         auto go = [&](auto l) {
             const int per = 64 / l(), cw = (a->channels + per - 1) / per;
-            const int at_once = (int)std::max<int64_t>(1, std::min<int64_t>(a->batch, 16384 / cw));
-            hipLaunchKernelGGL((k_scan_step<T, l()>), dim3((int)(((int64_t)cw * at_once + 3) / 4)), dim3(256), 0, strm(stream), s, cw, at_once);
+            const int at_once = (int)std::max<int64_t>(1, std::min<int64_t>(a->batch, STEP_GAME_WAVES / cw));
+            const dim3 grid((int)(((int64_t)cw * at_once + 3) / 4));
+            if ((int64_t)a->batch * a->channels * a->states * 4 > STEP_STREAM_BYTES)
+                hipLaunchKernelGGL((k_scan_step<T, l(), true>), grid, dim3(256), 0, strm(stream), s, cw, at_once);
+            else hipLaunchKernelGGL((k_scan_step<T, l(), false>), grid, dim3(256), 0, strm(stream), s, cw, at_once);
             return launch_check("k_scan_step");
         };
         using std::integral_constant;
@@ -515,12 +553,11 @@ int jq_logits_forward(const jq_logits *a, void *out, int64_t out_stride, void *s
         return fail(JQ_E_ARG, "rows must be aligned to their element size");
     LogitsArgs l = logits_args(a);
     l.o = out, l.o_stride = out_stride;
-    const int grid = (int)std::min<int64_t>(l.rows * l.tiles, MOST_BLOCKS);
     return by_type(a->dtype, [&](auto t) {
         using T = decltype(t);
-        if (l.recent_count) hipLaunchKernelGGL((k_logits_forward<T, true>), dim3(grid), dim3(256), 0, strm(stream), l);
-        else hipLaunchKernelGGL((k_logits_forward<T, false>), dim3(grid), dim3(256), 0, strm(stream), l);
-        return launch_check("k_logits_forward");
+        const LogitsGrid g = logits_grid<T>(l);
+        hipLaunchKernelGGL((k_logits<T, false>), g.grid, g.block, g.lds, strm(stream), l);
+        return launch_check("k_logits");
     });
 }
 
@@ -542,22 +579,26 @@ int jq_logits_backward(const jq_logits *a, const void *d_out, int64_t d_out_stri
     if (!d_logits && !d_bias) return JQ_OK;
     LogitsArgs l = logits_args(a);
     l.d = d_out, l.d_stride = d_out_stride, l.o = d_logits, l.o_stride = d_logits_stride;
-    l.parts = (int)logits_parts(a);
     if (d_bias) {
+        l.parts = (int)logits_parts(a);
         const int64_t need = (int64_t)l.parts * l.actions * 4;
         if (workspace_bytes < need || !workspace)
             return fail(JQ_E_ARG, "workspace of %lld bytes, %lld are needed", (long long)workspace_bytes, (long long)need);
         if (!aligned(workspace, 4)) return fail(JQ_E_ARG, "workspace must be 4-byte aligned");
         l.part = static_cast<float *>(workspace);
     }
-    const size_t lds = d_bias ? LOGITS_TILE * sizeof(float) : 0;
     return by_type(a->dtype, [&](auto t) {
         using T = decltype(t);
-        const dim3 grid(l.parts * l.tiles);
-        if (l.recent_count && l.o) hipLaunchKernelGGL((k_logits_backward<T, true>), grid, dim3(256), lds, strm(stream), l);
-        else hipLaunchKernelGGL((k_logits_backward<T, false>), grid, dim3(256), lds, strm(stream), l);
-        TRY(launch_check("k_logits_backward"));
+        if (d_logits && l.rows) {
+            const LogitsGrid g = logits_grid<T>(l);
+            hipLaunchKernelGGL((k_logits<T, true>), g.grid, g.block, g.lds, strm(stream), l);
+            TRY(launch_check("k_logits (gradient)"));
+        }
         if (!d_bias) return JQ_OK;
+        LogitsArgs sums = l;
+        sums.tiles = bias_tiles(a);
+        hipLaunchKernelGGL((k_logits_bias<T>), dim3(sums.tiles * sums.parts), dim3(256), 0, strm(stream), sums);
+        TRY(launch_check("k_logits_bias"));
         hipLaunchKernelGGL(k_logits_join, dim3((l.actions + 15) / 16), dim3(256), 0, strm(stream), l.part, l.parts, l.actions, d_bias);
         return launch_check("k_logits_join");
     });
