@@ -113,7 +113,7 @@ int64_t scan_parts(const jq_scan *a)
 
 // One ply: waves that walk the games, and the bytes of states past which they would not be
 // found in the caches at the next ply.
-constexpr int STEP_GAME_WAVES = 16384;
+constexpr int STEP_GAME_WAVES = 65536;
 constexpr int64_t STEP_STREAM_BYTES = 400ll << 20;
 
 struct ScanBytes { int64_t state, sum, bc, a; int64_t all() const { return state + sum + bc + a; } };
@@ -227,29 +227,27 @@ int check_conv_inputs(const jq_conv *a)
     return JQ_OK;
 }
 
-int conv_v(int32_t dtype, int taps) { return taps > 4 || dtype == JQ_F32 ? 4 : 8; }
+int conv_v(int32_t dtype, int taps, bool backward) { return taps > 4 || dtype == JQ_F32 || (backward && CONV_BACK_VEC == 4) ? 4 : 8; }
 
 // Threads across channels, and plies of a run: as many runs as keep the card's threads
 // busy, none so short that the taps before it are most of what it reads.
-constexpr int CONV_THREADS = 512 * 1024, CONV_RUN = 16, CONV_BACKWARD_BLOCKS = 1024;
-void conv_shape(ConvArgs &c, int32_t dtype)
+constexpr int CONV_THREADS = 512 * 1024, CONV_RUN = 16, CONV_BACKWARD_BLOCKS = 1024, CONV_STEP_BLOCKS = 4096;
+struct ConvShape { int blocks_x, v; };
+ConvShape conv_shape(ConvArgs &c, int32_t dtype, bool backward)
 {
-    const int64_t vectors = (c.channels + conv_v(dtype, c.taps) - 1) / conv_v(dtype, c.taps);
+    const int v = conv_v(dtype, c.taps, backward);
+    const int64_t vectors = (c.channels + v - 1) / v;
     c.tx = vectors <= 8 ? 8 : vectors <= 16 ? 16 : vectors <= 32 ? 32 : 64;
     const int64_t across = (vectors + c.tx - 1) / c.tx * c.tx;
     const int64_t want = std::max<int64_t>(1, CONV_THREADS / across / std::max(1, c.batch));
     c.run = (int)std::max<int64_t>(CONV_RUN, (c.plies + want - 1) / want);
     c.runs = std::max(1, (c.plies + c.run - 1) / c.run);
+    return {(int)(across / c.tx), v};
 }
-int conv_blocks_x(const ConvArgs &c, int32_t dtype)
+int64_t conv_parts(const ConvArgs &c, const ConvShape &s, int64_t items, int64_t most)
 {
-    const int v = conv_v(dtype, c.taps);
-    return ((c.channels + v - 1) / v + c.tx - 1) / c.tx;
-}
-int64_t conv_parts(const ConvArgs &c, int32_t dtype, int64_t items, int64_t most)
-{
-    const int64_t ty = 256 / c.tx;
-    return std::max<int64_t>(1, std::min((items + ty - 1) / ty, most / conv_blocks_x(c, dtype)));
+    const int64_t rows = 256 / c.tx;
+    return std::max<int64_t>(1, std::min((items + rows - 1) / rows, most / s.blocks_x));
 }
 
 ConvArgs conv_args(const jq_conv *a)
@@ -261,15 +259,15 @@ ConvArgs conv_args(const jq_conv *a)
     c.starts = a->starts, c.starts_batch = a->starts_batch, c.starts_ply = a->starts_ply;
     c.lengths = a->lengths;
     c.s_in = a->initial_state, c.s_out = a->final_state;
-    conv_shape(c, a->dtype);
     return c;
 }
 
 int64_t conv_bytes(const jq_conv *a)
 {
-    const ConvArgs c = conv_args(a);
+    ConvArgs c = conv_args(a);
     if (!a->dweight && !a->dbias) return 0;
-    return conv_parts(c, a->dtype, (int64_t)c.batch * c.runs, CONV_BACKWARD_BLOCKS) * (c.taps + 1) * c.channels * 4;
+    const ConvShape s = conv_shape(c, a->dtype, true);
+    return conv_parts(c, s, (int64_t)c.batch * c.runs, CONV_BACKWARD_BLOCKS) * (c.taps + 1) * c.channels * 4;
 }
 
 // f(rows' type, weights' type, taps)
@@ -490,9 +488,10 @@ int jq_conv_forward(const jq_conv *a, void *stream)
     if (a->plies) TRY(check_rows(a->out, a->dtype, "out"));
     TRY(check_state_pointer(a->final_state, a->dtype, "final_state"));
     ConvArgs c = conv_args(a);
-    c.parts = (int)conv_parts(c, a->dtype, (int64_t)c.batch * c.runs, MOST_BLOCKS);
+    const ConvShape s = conv_shape(c, a->dtype, false);
+    c.parts = (int)conv_parts(c, s, (int64_t)c.batch * c.runs, MOST_BLOCKS);
     return by_taps(a->dtype, a->weight_dtype, a->taps, [&](auto t, auto w, auto taps) {
-        hipLaunchKernelGGL((k_conv_forward<decltype(t), decltype(w), taps()>), dim3(c.parts * conv_blocks_x(c, a->dtype)), dim3(256), 0, strm(stream), c);
+        hipLaunchKernelGGL((k_conv_forward<decltype(t), decltype(w), taps()>), dim3(c.parts * s.blocks_x), dim3(256), 0, strm(stream), c);
         return launch_check("k_conv_forward");
     });
 }
@@ -514,10 +513,11 @@ int jq_conv_backward(const jq_conv *a, void *stream)
     ConvArgs c = conv_args(a);
     c.d_out = a->d_out, c.dx = a->dx, c.d_final = a->d_final, c.d_initial = a->d_initial;
     c.part = need ? static_cast<float *>(a->workspace) : nullptr;
-    c.parts = (int)conv_parts(c, a->dtype, (int64_t)c.batch * c.runs, CONV_BACKWARD_BLOCKS);
+    const ConvShape s = conv_shape(c, a->dtype, true);
+    c.parts = (int)conv_parts(c, s, (int64_t)c.batch * c.runs, CONV_BACKWARD_BLOCKS);
     return by_taps(a->dtype, a->weight_dtype, a->taps, [&](auto t, auto w, auto taps) {
         using W = decltype(w);
-        hipLaunchKernelGGL((k_conv_backward<decltype(t), W, taps()>), dim3(c.parts * conv_blocks_x(c, a->dtype)), dim3(256), 0, strm(stream), c);
+        hipLaunchKernelGGL((k_conv_backward<decltype(t), W, taps()>), dim3(c.parts * s.blocks_x), dim3(256), 0, strm(stream), c);
         TRY(launch_check("k_conv_backward"));
         if (!c.part) return JQ_OK;
         hipLaunchKernelGGL(k_conv_join<W>, dim3((int)(((int64_t)(c.taps + 1) * c.channels + 15) / 16)), dim3(256), 0, strm(stream), c.part, c.parts, c.taps,
@@ -537,9 +537,10 @@ int jq_conv_step(const jq_conv *a, void *state, int64_t state_rows, const int64_
     if (state_rows && !state && a->taps > 1) return fail(JQ_E_ARG, "null state");
     TRY(check_state_pointer(state, a->dtype, "state"));
     ConvStepArgs s{conv_args(a), state, state_rows, rows, starts};
-    s.c.parts = (int)conv_parts(s.c, a->dtype, a->batch, 4096);
+    const ConvShape shape = conv_shape(s.c, a->dtype, false);
+    s.c.parts = (int)conv_parts(s.c, shape, a->batch, CONV_STEP_BLOCKS);
     return by_taps(a->dtype, a->weight_dtype, a->taps, [&](auto t, auto w, auto taps) {
-        hipLaunchKernelGGL((k_conv_step<decltype(t), decltype(w), taps()>), dim3(s.c.parts * conv_blocks_x(s.c, a->dtype)), dim3(256), 0, strm(stream), s);
+        hipLaunchKernelGGL((k_conv_step<decltype(t), decltype(w), taps()>), dim3(s.c.parts * shape.blocks_x), dim3(256), 0, strm(stream), s);
         return launch_check("k_conv_step");
     });
 }
