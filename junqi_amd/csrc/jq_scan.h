@@ -199,6 +199,24 @@ struct Window {
     }
 };
 
+// What a call has and wants, in one scalar register: a truth value of each would take two.
+enum : uint32_t { HAS_SKIP = 1, HAS_GATE = 2, SOFTPLUS = 4, SAVES = 8, WANT_BC = 16, WANT_GATE = 32, WANT_U = 64, WANT_DELTA = 128 };
+struct Has {
+    uint32_t bits;
+    __device__ __forceinline__ explicit Has(SelectArgsPtr a)
+        : bits((a->skip ? HAS_SKIP : 0) | (a->gate.data ? HAS_GATE : 0) | (a->softplus ? SOFTPLUS : 0) | (a->saved ? SAVES : 0) |
+               (a->want_bc ? WANT_BC : 0) | (a->dgate.data ? WANT_GATE : 0) | (a->du.data ? WANT_U : 0) | (a->ddelta.data ? WANT_DELTA : 0))
+    {
+        asm volatile("" : "+s"(bits));
+    }
+    __device__ __forceinline__ bool operator()(uint32_t what) const
+    {
+        uint32_t b = bits;
+        asm volatile("" : "+s"(b));   // looked at anew each time
+        return b & what;
+    }
+};
+
 // A tensor's rows from ply t on; `step` bytes part two plies' rows. A chunk's rows are
 // reached by 32-bit offsets: plies are less than SCAN_STEP bytes apart.
 constexpr int64_t SCAN_STEP = 1 << 28;
@@ -316,8 +334,8 @@ __global__ __launch_bounds__(256) void k_scan_forward(SelectArgs)
     const Place<T, NS, EXACT, MANY> p(a);
     float A[NS], h[NS];
     p.rates(a, A);
-    const bool skips = a->skip, gated = OUT && a->gate.data, soft = a->softplus, saves = OUT && a->saved;
-    const float skip = skips ? a->skip[p.ch] : 0.f, bias = a->bias ? a->bias[p.ch] : 0.f;
+    const Has has(a);
+    const float skip = a->skip ? a->skip[p.ch] : 0.f, bias = a->bias ? a->bias[p.ch] : 0.f;
     struct Raw { T u[K], delta[K], gate[K], b[K], c[K]; };
     const int items = a->batch * a->segments, channels = a->channels;
     const int64_t state_bytes = (int64_t)p.states * channels * 4;
@@ -341,7 +359,7 @@ __global__ __launch_bounds__(256) void k_scan_forward(SelectArgs)
                 const uint32_t at = min(k, last);   // behind the end the last row again
                 r.u[k] = ru.get<T>(p.at, at * ru.step);
                 r.delta[k] = rd.get<T>(p.at, at * rd.step);
-                if (gated) r.gate[k] = rz.get<T>(p.at, at * rz.step);
+                if (OUT && has(HAS_GATE)) r.gate[k] = rz.get<T>(p.at, at * rz.step);
                 r.b[k] = rb.get<T>(p.row_at, at * rb.step);
                 if (OUT) r.c[k] = rc.get<T>(p.row_at, at * rc.step);
             }
@@ -355,14 +373,14 @@ __global__ __launch_bounds__(256) void k_scan_forward(SelectArgs)
             const Raw r = next;
             const uint32_t starts = next_starts;
             if (t0 + K < end) fetch(t0 + K, next, next_starts);
-            if (saves && t0 % SCAN_CHUNK == 0) {
+            if (OUT && has(SAVES) && t0 % SCAN_CHUNK == 0) {
                 store_apart(p, h, reinterpret_cast<float *>(save.base), channels);
                 save.base += state_bytes;
             }
 #pragma unroll
             for (int k = 0; k < K; ++k) {
                 if (t0 + k >= end) break;
-                const float u = (float)r.u[k], pre = (float)r.delta[k] + bias, dt = soft ? softplus(pre) : pre;
+                const float u = (float)r.u[k], pre = (float)r.delta[k] + bias, dt = has(SOFTPLUS) ? softplus(pre) : pre;
                 const float push = dt * u, bt = (float)r.b[k];
                 if (starts >> k & 1) {
                     forget(h);
@@ -379,8 +397,8 @@ __global__ __launch_bounds__(256) void k_scan_forward(SelectArgs)
                 const float y = row_dot(0.f, (float)r.c[k], h);
                 if (MANY) lds[(((turn & 1) * SG + p.sg) * K + k) * 64 + p.lane] = y;
                 else {
-                    float o = skips ? fmaf(skip, u, y) : y;
-                    if (gated) o *= (float)r.gate[k] * sigmoid((float)r.gate[k]);
+                    float o = has(HAS_SKIP) ? fmaf(skip, u, y) : y;
+                    if (OUT && has(HAS_GATE)) o *= (float)r.gate[k] * sigmoid((float)r.gate[k]);
                     ro.put<T>(p.at, from_float<T>(o), k * ro.step);
                 }
             }
@@ -396,8 +414,8 @@ __global__ __launch_bounds__(256) void k_scan_forward(SelectArgs)
                 if (k % SG == p.sg) {
                     float o = 0.f;
                     for (int g = 0; g < SG; ++g) o += lds[(((turn & 1) * SG + g) * K + k) * 64 + p.lane];
-                    if (skips) o = fmaf(skip, (float)r.u[k], o);
-                    if (gated) o *= (float)r.gate[k] * sigmoid((float)r.gate[k]);
+                    if (has(HAS_SKIP)) o = fmaf(skip, (float)r.u[k], o);
+                    if (OUT && has(HAS_GATE)) o *= (float)r.gate[k] * sigmoid((float)r.gate[k]);
                     ro.put<T>(p.at, from_float<T>(o), k * ro.step);
                 }
             }
@@ -429,13 +447,25 @@ __global__ __launch_bounds__(256) void k_scan_join(SelectArgs a)
         const float *in = BACK ? a.d_final : a.s_in;
         float h = in ? in[home] : 0.f;
         const float A = a.a[(int64_t)ch * a.states + n] * LOG2E;
-        for (int s = 0; s < a.segments; ++s) {
-            const int64_t seg = b * a.segments + (BACK ? a.segments - 1 - s : s);
-            float *at = a.seg_state + seg * step + (int64_t)n * a.channels + ch;
-            const float add = *at, sum = a.seg_sum[seg * a.channels + ch];
-            *at = h;
-            // an infinity stays one over any number of plies: no power is 0
-            h = sum != sum ? add : fmaf(fmaxf(exp2_fast(sum * A), 0x1p-126f), h, add);
+        // parts are asked for AHEAD at a time: one after the other, each waits for the last
+        constexpr int AHEAD = 16;
+        float *first = a.seg_state + (b * a.segments + (BACK ? a.segments - 1 : 0)) * step + (int64_t)n * a.channels + ch;
+        const float *sums = a.seg_sum + (b * a.segments + (BACK ? a.segments - 1 : 0)) * a.channels + ch;
+        const int64_t by = BACK ? -step : step, sum_by = BACK ? -a.channels : a.channels;
+        for (int s0 = 0; s0 < a.segments; s0 += AHEAD) {
+            float add[AHEAD], keep[AHEAD];
+#pragma unroll
+            for (int k = 0; k < AHEAD; ++k) {
+                const int s = min(s0 + k, a.segments - 1);
+                add[k] = first[s * by], keep[k] = sums[s * sum_by];
+            }
+#pragma unroll
+            for (int k = 0; k < AHEAD; ++k) {
+                if (s0 + k >= a.segments) break;
+                first[(s0 + k) * by] = h;
+                // an infinity stays one over any number of plies: no power is 0
+                h = keep[k] != keep[k] ? add[k] : fmaf(fmaxf(exp2_fast(keep[k] * A), 0x1p-126f), h, add[k]);
+            }
         }
     }
 }
@@ -452,7 +482,7 @@ __global__ __launch_bounds__(256) void k_scan_carry(SelectArgs)
     if (p.part >= p.parts) return;
     float A[NS], dh[NS];
     p.rates(a, A);
-    const bool gated = a->gate.data, soft = a->softplus;
+    const Has has(a);
     const float bias = a->bias ? a->bias[p.ch] : 0.f;
     for (int item = p.part; item < items; item += p.parts) {
         SelectArgsPtr q = hidden(a);
@@ -472,15 +502,15 @@ __global__ __launch_bounds__(256) void k_scan_carry(SelectArgs)
                 const uint32_t at = min(k, end - 1 - t0);
                 delta[k] = rd.get<T>(p.at, at * rd.step);
                 d_out[k] = rg.get<T>(p.at, at * rg.step);
-                if (gated) gate[k] = rz.get<T>(p.at, at * rz.step);
+                if (has(HAS_GATE)) gate[k] = rz.get<T>(p.at, at * rz.step);
                 c[k] = rc.get<T>(p.row_at, at * rc.step);
             }
 #pragma unroll
             for (int k = K - 1; k >= 0; --k) {
                 if (t0 + k >= end) continue;
-                const float pre = (float)delta[k] + bias, dt = soft ? softplus(pre) : pre;
+                const float pre = (float)delta[k] + bias, dt = has(SOFTPLUS) ? softplus(pre) : pre;
                 float dy = (float)d_out[k];
-                if (gated) dy *= (float)gate[k] * sigmoid((float)gate[k]);
+                if (has(HAS_GATE)) dy *= (float)gate[k] * sigmoid((float)gate[k]);
                 row_add(dh, (float)c[k], dy);
 #pragma unroll
                 for (int i = 0; i < NS; ++i) dh[i] = p.has(i) ? dh[i] * exp2_fast(dt * A[i]) : 0.f;
@@ -520,9 +550,8 @@ __global__ __launch_bounds__(256, 2) void k_scan_backward(SelectArgs)
     p.rates(a, A);
 #pragma unroll
     for (int i = 0; i < NS; ++i) dA[i] = 0.f;
-    const bool skips = a->skip, gated = a->gate.data, soft = a->softplus, want_bc = a->want_bc, want_gate = a->dgate.data, want_u = a->du.data,
-               want_delta = a->ddelta.data;
-    const float skip = skips ? a->skip[p.ch] : 0.f, bias = a->bias ? a->bias[p.ch] : 0.f;
+    const Has has(a);
+    const float skip = a->skip ? a->skip[p.ch] : 0.f, bias = a->bias ? a->bias[p.ch] : 0.f;
     float dskip = 0.f, dbias = 0.f;
     const int items = a->batch * a->segments, channels = a->channels;
     const int sum_n = p.n0 + p.lane / (64 / NS);
@@ -537,9 +566,9 @@ __global__ __launch_bounds__(256, 2) void k_scan_backward(SelectArgs)
         if (q->segments > 1) load_apart(p, dh, q->seg_state + (int64_t)item * p.states * channels, channels);
         else load_states(p, dh, q->d_final ? q->d_final + (int64_t)b * channels * p.states : nullptr);
         for (int t = max(begin, end) + p.sg; t < stop; t += SG) {
-            if (want_u) PlyRows(T(), &q->du, b, t, 0).template put<T>(p.at, T(0.f));
-            if (want_delta) PlyRows(T(), &q->ddelta, b, t, 0).template put<T>(p.at, T(0.f));
-            if (want_gate) PlyRows(T(), &q->dgate, b, t, 0).template put<T>(p.at, T(0.f));
+            if (has(WANT_U)) PlyRows(T(), &q->du, b, t, 0).template put<T>(p.at, T(0.f));
+            if (has(WANT_DELTA)) PlyRows(T(), &q->ddelta, b, t, 0).template put<T>(p.at, T(0.f));
+            if (has(WANT_GATE)) PlyRows(T(), &q->dgate, b, t, 0).template put<T>(p.at, T(0.f));
         }
         const int top = begin + (max(end - begin, 1) - 1) / K * K;
         const Starts game(q, b);
@@ -560,7 +589,7 @@ __global__ __launch_bounds__(256, 2) void k_scan_backward(SelectArgs)
                 r.u[k] = lu.get<T>(p.at, at * lu.step, really);
                 r.delta[k] = ld.get<T>(p.at, at * ld.step, really);
                 r.d_out[k] = lg.get<T>(p.at, at * lg.step, really);
-                if (gated) r.gate[k] = lz.get<T>(p.at, at * lz.step, really);
+                if (has(HAS_GATE)) r.gate[k] = lz.get<T>(p.at, at * lz.step, really);
                 r.b[k] = lb.get<T>(p.row_at, at * lb.step, really);
                 r.c[k] = lc.get<T>(p.row_at, at * lc.step, really);
             }
@@ -569,17 +598,17 @@ __global__ __launch_bounds__(256, 2) void k_scan_backward(SelectArgs)
         // the gradient of a gate and the ones of u and delta, their rows as they lie in memory
         auto give_gate = [&](const PlyRows &to, int k, T u, T gate, T d_out, float y) {
             const float z = (float)gate, s = sigmoid(z);
-            to.put<T>(p.at, from_float<T>((float)d_out * (skips ? fmaf(skip, (float)u, y) : y) * s * fmaf(z, 1.f - s, 1.f)), k * to.step);
+            to.put<T>(p.at, from_float<T>((float)d_out * (has(HAS_SKIP) ? fmaf(skip, (float)u, y) : y) * s * fmaf(z, 1.f - s, 1.f)), k * to.step);
         };
         auto give = [&](const PlyRows &to_u, const PlyRows &to_delta, int k, T u, T delta, float dt, float dy, float s1, float s2) {
             float d_pre = fmaf(s1, (float)u, s2 * LN2);
-            if (soft) d_pre *= sigmoid((float)delta + bias);
+            if (has(SOFTPLUS)) d_pre *= sigmoid((float)delta + bias);
             if (p.on()) {   // lanes without a channel have read zeros: their sums are not looked at
                 dbias += d_pre;
                 dskip = fmaf(dy, (float)u, dskip);
             }
-            if (want_u) to_u.put<T>(p.at, from_float<T>(skips ? fmaf(s1, dt, skip * dy) : s1 * dt), k * to_u.step);
-            if (want_delta) to_delta.put<T>(p.at, from_float<T>(d_pre), k * to_delta.step);
+            if (has(WANT_U)) to_u.put<T>(p.at, from_float<T>(has(HAS_SKIP) ? fmaf(s1, dt, skip * dy) : s1 * dt), k * to_u.step);
+            if (has(WANT_DELTA)) to_delta.put<T>(p.at, from_float<T>(d_pre), k * to_delta.step);
         };
         Raw next;
         float h[NS];
@@ -599,9 +628,9 @@ __global__ __launch_bounds__(256, 2) void k_scan_backward(SelectArgs)
                 for (int k = 0; k < K; ++k) {
                     if (k >= count) break;
                     const float pre = (float)next.delta[k] + bias, bt = (float)next.b[k], u = (float)next.u[k];
-                    dt[k] = soft ? softplus(pre) : pre;
+                    dt[k] = has(SOFTPLUS) ? softplus(pre) : pre;
                     dy[k] = (float)next.d_out[k];
-                    if (gated) dy[k] *= (float)next.gate[k] * sigmoid((float)next.gate[k]);
+                    if (has(HAS_GATE)) dy[k] *= (float)next.gate[k] * sigmoid((float)next.gate[k]);
                     if (starts >> k & 1) forget(h);
                     const float push = dt[k] * u;
                     float v[NS];
@@ -618,12 +647,12 @@ __global__ __launch_bounds__(256, 2) void k_scan_backward(SelectArgs)
                         if (!p.has(i)) h[i] = 0.f;
                         v[i] = p.on() ? dy[k] * h[i] : 0.f;
                     }
-                    if (want_gate) {
+                    if (has(WANT_GATE)) {
                         const float y = row_dot(0.f, (float)next.c[k], h);
                         if (MANY) share(0, p.sg, k) = y;
                         else give_gate(to_gate, k, next.u[k], next.gate[k], next.d_out[k], y);
                     }
-                    if (want_bc) {
+                    if (has(WANT_BC)) {
                         to.put(sum_at, lane_sums<NS>(v));
                         to.base += sum_step;
                     }
@@ -658,7 +687,7 @@ __global__ __launch_bounds__(256, 2) void k_scan_backward(SelectArgs)
                     }
                     const float s1 = row_dot(0.f, (float)b0, dh);
                     float s2 = 0.f;
-                    if (want_bc) {
+                    if (has(WANT_BC)) {
                         to.put(sum_at, lane_sums<NS>(v));
                         to.base -= sum_step;
                     }
@@ -684,12 +713,12 @@ __global__ __launch_bounds__(256, 2) void k_scan_backward(SelectArgs)
                     if (k % SG != p.sg) continue;
                     float all[3] = {0.f, 0.f, 0.f};
                     for (int g = 0; g < SG; ++g) {
-                        if (want_gate) all[0] += share(0, g, k);
+                        if (has(WANT_GATE)) all[0] += share(0, g, k);
                         all[1] += share(1, g, k);
                         all[2] += share(2, g, k);
                     }
                     const T u = ru.get<T>(p.at, k * ru.step);
-                    if (want_gate) give_gate(to_gate, k, u, rz.get<T>(p.at, k * rz.step), rg.get<T>(p.at, k * rg.step), all[0]);
+                    if (has(WANT_GATE)) give_gate(to_gate, k, u, rz.get<T>(p.at, k * rz.step), rg.get<T>(p.at, k * rg.step), all[0]);
                     give(to_u, to_delta, k, u, rd.get<T>(p.at, k * rd.step), dt[k], dy[k], all[1], all[2]);
                 }
                 __syncthreads();   // the next chunk's shares take their place

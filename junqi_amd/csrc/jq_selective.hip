@@ -74,32 +74,27 @@ int check_scan_inputs(const jq_scan *a)
     return JQ_OK;
 }
 
-// States of a lane and waves of states.
-struct ScanShape { int ns, sg, waves; bool exact; };
-ScanShape scan_shape(const jq_scan *a)
-{
-    ScanShape s;
-    s.ns = a->states <= 4 ? 4 : a->states <= 8 ? 8 : 16;
-    s.sg = (a->states + s.ns - 1) / s.ns;
-    const int per = a->channels / a->groups;
-    s.waves = (per + 63) / 64;
-    s.exact = s.ns * s.sg == a->states && per % 64 == 0;
-    return s;
-}
+// States of a lane and waves of states, and the parts of a split axis.
+struct ScanShape { int ns, sg, waves, segments, seg_plies; bool exact; };
 
 // Few games and channels leave most of the card idle unless parts of a long axis run side
 // by side, at the price of its states taken twice.
 constexpr int SPLIT_BELOW = 1024, SPLIT_WAVES = 4096, SPLIT_PLIES = 64;
-struct Split { int segments, seg_plies; };
-Split split_of(const jq_scan *a)
+ScanShape scan_shape(const jq_scan *a)
 {
-    const ScanShape s = scan_shape(a);
-    const int64_t waves = std::max<int64_t>(1, (int64_t)a->batch * a->groups * s.waves * s.sg);
-    int64_t want = waves < SPLIT_BELOW ? std::min<int64_t>(SPLIT_WAVES / waves, a->plies / SPLIT_PLIES) : 1;
+    ScanShape s;
+    const int per = a->channels / a->groups;
+    s.waves = (per + 63) / 64;
+    s.ns = a->states <= 4 ? 4 : a->states <= 8 ? 8 : 16;
+    s.sg = (a->states + s.ns - 1) / s.ns;
+    const int64_t waves = std::max<int64_t>(1, (int64_t)a->batch * a->groups * s.waves);
+    int64_t want = waves * s.sg < SPLIT_BELOW ? std::min<int64_t>(SPLIT_WAVES / (waves * s.sg), a->plies / SPLIT_PLIES) : 1;
     if (want < 4) want = 1;
     const int64_t each = ((a->plies + want - 1) / want + SCAN_CHUNK - 1) / SCAN_CHUNK * SCAN_CHUNK;
-    if (want == 1 || each == 0) return {1, (int)std::max<int64_t>(each, SCAN_CHUNK)};
-    return {(int)((a->plies + each - 1) / each), (int)each};
+    s.seg_plies = (int)std::max<int64_t>(each, SCAN_CHUNK);
+    s.segments = want == 1 ? 1 : (int)((a->plies + each - 1) / each);
+    s.exact = s.ns * s.sg == a->states && per % 64 == 0;
+    return s;
 }
 
 // Blocks that share the backward pass's items, each with its own sums of da, dskip and dbias.
@@ -107,26 +102,26 @@ constexpr int BACKWARD_WAVES = 2048;
 int64_t scan_parts(const jq_scan *a)
 {
     const ScanShape s = scan_shape(a);
-    const int64_t items = (int64_t)a->batch * split_of(a).segments, blocks = (int64_t)s.waves * a->groups;
+    const int64_t items = (int64_t)a->batch * s.segments, blocks = (int64_t)s.waves * a->groups;
     return std::max<int64_t>(1, std::min(items, BACKWARD_WAVES / (blocks * s.sg)));
 }
 
 // One ply: waves that walk the games, and the bytes of states past which they would not be
 // found in the caches at the next ply.
-constexpr int STEP_GAME_WAVES = 65536;
+constexpr int STEP_GAME_WAVES = 32768;
 constexpr int64_t STEP_STREAM_BYTES = 400ll << 20;
 
 struct ScanBytes { int64_t state, sum, bc, a; int64_t all() const { return state + sum + bc + a; } };
 ScanBytes scan_bytes(const jq_scan *a, bool backward)
 {
-    const Split split = split_of(a);
+    const ScanShape s = scan_shape(a);
     ScanBytes n{0, 0, 0, 0};
-    if (split.segments > 1) {
-        n.sum = (int64_t)a->batch * split.segments * a->channels * 4;
+    if (s.segments > 1) {
+        n.sum = (int64_t)a->batch * s.segments * a->channels * 4;
         n.state = n.sum * a->states;
     }
     if (backward) {
-        if (a->db.data || a->dc.data) n.bc = (int64_t)scan_shape(a).waves * a->batch * a->plies * a->groups * 2 * a->states * 4;
+        if (a->db.data || a->dc.data) n.bc = (int64_t)s.waves * a->batch * a->plies * a->groups * 2 * a->states * 4;
         if (a->da || a->dskip || a->ddelta_bias) n.a = scan_parts(a) * (a->states + 2) * a->channels * 4;
     }
     return n;
@@ -145,7 +140,6 @@ SelectArgs select_args(const jq_scan *a, bool backward)
 {
     SelectArgs s{};
     const ScanShape shape = scan_shape(a);
-    const Split split = split_of(a);
     s.u = a->u, s.delta = a->delta, s.gate = a->gate, s.b = a->b, s.c = a->c, s.out = a->out;
     s.batch = a->batch, s.plies = a->plies, s.channels = a->channels, s.states = a->states, s.groups = a->groups;
     s.per = a->channels / a->groups, s.waves = shape.waves, s.softplus = a->softplus != 0;
@@ -153,7 +147,7 @@ SelectArgs select_args(const jq_scan *a, bool backward)
     s.starts = a->starts, s.starts_batch = a->starts_batch, s.starts_ply = a->starts_ply;
     s.lengths = a->lengths;
     s.s_in = a->initial_state, s.s_out = a->final_state, s.saved = a->saved;
-    s.segments = split.segments, s.seg_plies = split.seg_plies;
+    s.segments = shape.segments, s.seg_plies = shape.seg_plies;
     const ScanBytes n = scan_bytes(a, backward);
     char *w = static_cast<char *>(a->workspace);
     s.part_bc = reinterpret_cast<float *>(w);   // first: read in vectors
@@ -231,7 +225,7 @@ int conv_v(int32_t dtype, int taps, bool backward) { return taps > 4 || dtype ==
 
 // Threads across channels, and plies of a run: as many runs as keep the card's threads
 // busy, none so short that the taps before it are most of what it reads.
-constexpr int CONV_THREADS = 512 * 1024, CONV_RUN = 16, CONV_BACKWARD_BLOCKS = 1024, CONV_STEP_BLOCKS = 4096;
+constexpr int CONV_THREADS = 128 * 1024, CONV_RUN = 16, CONV_BACKWARD_BLOCKS = 1024, CONV_STEP_BLOCKS = 2048;
 struct ConvShape { int blocks_x, v; };
 ConvShape conv_shape(ConvArgs &c, int32_t dtype, bool backward)
 {
