@@ -457,12 +457,14 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
 # ------------------------------------------------------------------ what segments and steps of channels share
 def _plies(t: torch.Tensor) -> L.Rows:
     """A (batch, plies, channels) tensor with adjacent elements for the C calls."""
-    return L.Rows(t.data_ptr(), t.stride(0), t.stride(1), 0)
+    s = t.stride()
+    return L.Rows(t.data_ptr(), s[0], s[1], 0)
 
 
 def _ply(t: torch.Tensor) -> L.Rows:
     """A (batch, channels) tensor, or (batch, groups, states), with adjacent elements."""
-    return L.Rows(t.data_ptr(), t.stride(0), 0, t.stride(1) if t.ndim == 3 else 0)
+    s = t.stride()
+    return L.Rows(t.data_ptr(), s[0], 0, s[1] if len(s) == 3 else 0)
 
 
 def _like_plies(t: torch.Tensor) -> torch.Tensor:
@@ -511,8 +513,11 @@ def _check_step(name: str, x: torch.Tensor, state: torch.Tensor, state_shape: tu
     _check("state", state, (state.shape[0], *state_shape), (dtype,), x)
     if not state.is_contiguous():
         raise ValueError("state must be contiguous: it is updated in place")
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (*inputs, state)):
-        raise ValueError(f"{name}_step has no gradient: use {name}, or torch.no_grad()")
+    grads = torch.is_grad_enabled()
+    if grads:
+        for t in (state, *inputs):
+            if t is not None and t.requires_grad:
+                raise ValueError(f"{name}_step has no gradient: use {name}, or torch.no_grad()")
     if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None
                                               for t in (*inputs, state)):
         raise ValueError(f"{name}_step has no forward-mode derivative")
@@ -526,14 +531,14 @@ def _check_step(name: str, x: torch.Tensor, state: torch.Tensor, state_shape: tu
         _check("starts", starts, (b,), (torch.bool, torch.uint8), x)
         starts = starts.contiguous()
     if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        out = x.new_empty(x.shape)
     else:
         _check("out", out, tuple(x.shape), (x.dtype,), x)
         if x.shape[1] > 1 and out.stride(1) != 1:
             raise ValueError("the elements of out's last dimension must be adjacent")
         if b > 1 and out.stride(0) == 0:
             raise ValueError("the rows of out must not share memory")
-        if torch.is_grad_enabled() and out.requires_grad:
+        if grads and out.requires_grad:
             raise ValueError("out must not require a gradient: what is written to it has none")
     return rows, starts, out
 
