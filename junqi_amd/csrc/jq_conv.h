@@ -6,20 +6,27 @@
 namespace jq {
 
 // out_t = bias + sum over j of weight[j] x_{t - taps + 1 + j}, then x sigmoid(x) where
-// `silu`; inputs before a game's start are not there. A thread has V channels of 16 bytes
-// together and walks a run of plies with the last inputs in registers, so a row is read
-// once but for the taps - 1 before a run.
-constexpr int CONV_TAPS = 8;   // largest taps
-constexpr int CONV_BACK_VEC = 4;
+// `silu`; inputs before a game's start are not there. A thread has V channels together and
+// walks a run of plies with the last inputs in a ring of registers, so a row is read once but
+// for the taps - 1 before a run, and the next step's rows are asked for before this one's
+// results are stored: loads behind stores are seen only after these. Bound by the rows'
+// traffic forward (1,024 games x 256 plies of 512 channels, four taps, bfloat16, 537 MB: 97
+// us, 5.5 TB/s), by that and its products backward (805 MB: 225 us, 3.6 TB/s, VALU busy 57 %).
+// With an address worked out for every access, and a step's loads behind the last one's
+// stores, 164 and 332 us.
 // Plies of a step, whose rows are on their way while the step before is computed: a
 // multiple of the taps, so that the last inputs stay where they are in registers.
 constexpr int conv_step(int taps) { return taps == 2 ? 4 : taps; }
 
-// Channels of a thread: 16 bytes, 8 where 8 taps of 8 channels would not fit the registers.
+// Channels of a thread, V: 4 of float32 and behind four taps, whose registers would not
+// hold more. Of bfloat16 8 or 4, 1e8 elements of four taps, us with 8 / with 4:
+//                            512 channels   500 (rows 8-byte aligned)   501 (2-byte aligned)
+//   forward                     98 / 121           183 / 120                187 / 263
+//   one ply, 32,768 games       46 / 40             59 / 50                  62 / 62
+//   backward                   246 / 205           646 / 220                653 / 452
+// (the backward pass holds four times the taps' registers). So: forward 8, unless rows lie
+// at 8 bytes and not at 16; the others 4.
 template <class T, int TAPS> constexpr int conv_vec() { return TAPS > 4 ? 4 : 16 / (int)sizeof(T); }
-
-// Of the backward pass, which holds four times the taps' registers.
-template <class T, int TAPS> constexpr int conv_back_vec() { return CONV_BACK_VEC > 0 && conv_vec<T, TAPS>() > CONV_BACK_VEC ? CONV_BACK_VEC : conv_vec<T, TAPS>(); }
 
 struct ConvArgs {
     jq_rows x, out;
@@ -139,10 +146,10 @@ template <class T> struct PlyPointer {
     __device__ __forceinline__ PlyPointer(const jq_rows &r, int64_t b, int64_t t, int c) : at(row_at<T>(r, b, t, 0) + c), step(r.ply) {}
 };
 
-template <class T, class W, int TAPS>
+template <class T, class W, int TAPS, int V>
 __global__ __launch_bounds__(256) void k_conv_forward(ConvArgs a)
 {
-    constexpr int V = conv_vec<T, TAPS>(), U = conv_step(TAPS);
+    constexpr int U = conv_step(TAPS);
     typedef typename Pack<T, V>::type Raw;
     const ConvPlace p(a, V);
     if (p.n <= 0) return;
@@ -214,7 +221,7 @@ __global__ __launch_bounds__(256) void k_conv_forward(ConvArgs a)
 template <class T, class W, int TAPS>
 __global__ __launch_bounds__(256) void k_conv_backward(ConvArgs a)
 {
-    constexpr int V = conv_back_vec<T, TAPS>(), U = conv_step(TAPS);
+    constexpr int V = 4, U = conv_step(TAPS);
     typedef typename Pack<T, V>::type Raw;
     __shared__ float red[256 * V];
     const ConvPlace p(a, V);
@@ -382,7 +389,7 @@ struct ConvStepArgs {
 template <class T, class W, int TAPS>
 __global__ __launch_bounds__(256) void k_conv_step(ConvStepArgs s)
 {
-    constexpr int V = conv_vec<T, TAPS>();
+    constexpr int V = 4;
     typedef typename Pack<T, V>::type Raw;
     const ConvArgs &a = s.c;
     const ConvPlace p(a, V);

@@ -9,10 +9,16 @@ namespace jq {
 // For each game, channel d and state n, with dt = softplus(delta + bias):
 //   h_t = exp(dt_t a) h_{t-1} + dt_t u_t b_t;   y_t = sum over n of c_t h_t, + skip u_t;   out = y silu(gate)
 // A lane has a channel and NS of its states in registers; a wave has 64 channels of one
-// group, and the SG waves of a block the states of these. b_t and c_t, the same for all
-// channels of a group, lie in lanes 0 .. NS - 1 of each row of 16 and reach the products
-// as their row-broadcast operands, without an instruction of their own.
-constexpr int SCAN_STATES = 64;   // largest states
+// group, and more than 16 states are parted among the waves of a block. b_t and c_t, the
+// same for all channels of a group, lie in lanes 0 .. NS - 1 of each row of 16 and reach
+// the products as their row-broadcast operands, without an instruction of their own.
+// Bound by the vector units: a state of a ply takes five instructions (of which the
+// exponential as long as two) forward and thirteen backward, with the sums of db and dc
+// over channels 17.5. 512 games x 256 plies of 512 channels of 16 states in bfloat16:
+// forward 327 us (126 instructions a ply and wave, of which 80 the states', the units busy
+// three quarters of the time; the rows and saved states are 1.1 GB), backward 1,095 us (392
+// a ply and wave, busy 80 %). Without these operands, with 64-bit addresses in vector
+// registers and the arguments of a dozen tensors held over the pass: 3,160 us in all.
 constexpr int SCAN_PLIES = 4;     // plies whose rows are on their way while the ones before are computed
 constexpr int SCAN_CHUNK = 8;     // plies of a chunk of the backward pass, which starts from a saved state
 constexpr int scan_far(int ns) { return ns > 8 ? 2 : 0; }   // plies of a chunk whose states wait in LDS: registers would spill

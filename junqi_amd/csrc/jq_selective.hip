@@ -77,8 +77,16 @@ int check_scan_inputs(const jq_scan *a)
 // States of a lane and waves of states, and the parts of a split axis.
 struct ScanShape { int ns, sg, waves, segments, seg_plies; bool exact; };
 
-// Few games and channels leave most of the card idle unless parts of a long axis run side
-// by side, at the price of its states taken twice.
+// Few games and channels leave most of the card's 1,024 SIMDs idle unless parts of a long
+// axis run side by side, at the price of its states taken twice. Split / in one piece, us,
+// 16 states in bfloat16:
+//                    forward, plies            with the gradients
+//   waves          512          2,048          512           2,048
+//      64        55 / 213      79 / 832      221 / 941      288 / 3,629
+//     256        78 / 212     242 / 872      287 / 943      961 / 3,788
+//     512       129 / 213     468 / 901      513 / 977    1,853 / 3,859
+//   1,024       247 / 215     919 / 910      974 / 1,017  3,625 / 4,033
+// So: below 1,024 waves, from four parts of 64 plies on.
 constexpr int SPLIT_BELOW = 1024, SPLIT_WAVES = 4096, SPLIT_PLIES = 64;
 ScanShape scan_shape(const jq_scan *a)
 {
@@ -106,8 +114,10 @@ int64_t scan_parts(const jq_scan *a)
     return std::max<int64_t>(1, std::min(items, BACKWARD_WAVES / (blocks * s.sg)));
 }
 
-// One ply: waves that walk the games, and the bytes of states past which they would not be
-// found in the caches at the next ply.
+// One ply: waves that walk the games (32,768 games of 512 channels of 16 states, us at 8,192 /
+// 16,384 / 32,768 / 131,072 waves and one game each: 563 / 491 / 459 / 468 / 832), and the
+// bytes of states past which they would not be found in the caches at the next ply (that call
+// through them 550).
 constexpr int STEP_GAME_WAVES = 32768;
 constexpr int64_t STEP_STREAM_BYTES = 400ll << 20;
 
@@ -221,15 +231,27 @@ int check_conv_inputs(const jq_conv *a)
     return JQ_OK;
 }
 
-int conv_v(int32_t dtype, int taps, bool backward) { return taps > 4 || dtype == JQ_F32 || (backward && CONV_BACK_VEC == 4) ? 4 : 8; }
+// Whether r's rows lie at multiples of `bytes`.
+bool rows_at(const jq_rows &r, int32_t dtype, int64_t bytes)
+{
+    const int64_t n = bytes / (int64_t)elem_bytes(dtype);
+    return aligned(r.data, bytes) && r.batch % n == 0 && r.ply % n == 0;
+}
+int conv_forward_vec(const jq_conv *a)
+{
+    if (a->dtype == JQ_F32 || a->taps > 4) return 4;
+    const bool eight = rows_at(a->x, a->dtype, 8) && rows_at(a->out, a->dtype, 8), sixteen = rows_at(a->x, a->dtype, 16) && rows_at(a->out, a->dtype, 16);
+    return eight && !sixteen ? 4 : 8;
+}
 
 // Threads across channels, and plies of a run: as many runs as keep the card's threads
-// busy, none so short that the taps before it are most of what it reads.
-constexpr int CONV_THREADS = 128 * 1024, CONV_RUN = 16, CONV_BACKWARD_BLOCKS = 1024, CONV_STEP_BLOCKS = 2048;
+// busy, none so short that the taps before it are most of what it reads (1,024 games of 256
+// plies of 512 channels, training, us at 64 K / 128 K / 256 K / 512 K threads: 361 / 318 /
+// 356 / 378). Blocks of the backward pass, each with its own sums, and of one ply.
+constexpr int CONV_THREADS = 128 * 1024, CONV_RUN = 16, CONV_BACKWARD_BLOCKS = 1024, CONV_STEP_BLOCKS = 4096;
 struct ConvShape { int blocks_x, v; };
-ConvShape conv_shape(ConvArgs &c, int32_t dtype, bool backward)
+ConvShape conv_shape(ConvArgs &c, int v)
 {
-    const int v = conv_v(dtype, c.taps, backward);
     const int64_t vectors = (c.channels + v - 1) / v;
     c.tx = vectors <= 8 ? 8 : vectors <= 16 ? 16 : vectors <= 32 ? 32 : 64;
     const int64_t across = (vectors + c.tx - 1) / c.tx * c.tx;
@@ -260,7 +282,7 @@ int64_t conv_bytes(const jq_conv *a)
 {
     ConvArgs c = conv_args(a);
     if (!a->dweight && !a->dbias) return 0;
-    const ConvShape s = conv_shape(c, a->dtype, true);
+    const ConvShape s = conv_shape(c, 4);
     return conv_parts(c, s, (int64_t)c.batch * c.runs, CONV_BACKWARD_BLOCKS) * (c.taps + 1) * c.channels * 4;
 }
 
@@ -482,10 +504,18 @@ int jq_conv_forward(const jq_conv *a, void *stream)
     if (a->plies) TRY(check_rows(a->out, a->dtype, "out"));
     TRY(check_state_pointer(a->final_state, a->dtype, "final_state"));
     ConvArgs c = conv_args(a);
-    const ConvShape s = conv_shape(c, a->dtype, false);
+    const ConvShape s = conv_shape(c, conv_forward_vec(a));
     c.parts = (int)conv_parts(c, s, (int64_t)c.batch * c.runs, MOST_BLOCKS);
     return by_taps(a->dtype, a->weight_dtype, a->taps, [&](auto t, auto w, auto taps) {
-        hipLaunchKernelGGL((k_conv_forward<decltype(t), decltype(w), taps()>), dim3(c.parts * s.blocks_x), dim3(256), 0, strm(stream), c);
+        using T = decltype(t);
+        using W = decltype(w);
+        const dim3 grid(c.parts * s.blocks_x);
+        if constexpr (conv_vec<T, taps()>() == 8)
+            if (s.v == 8) {
+                hipLaunchKernelGGL((k_conv_forward<T, W, taps(), 8>), grid, dim3(256), 0, strm(stream), c);
+                return launch_check("k_conv_forward");
+            }
+        hipLaunchKernelGGL((k_conv_forward<T, W, taps(), 4>), grid, dim3(256), 0, strm(stream), c);
         return launch_check("k_conv_forward");
     });
 }
@@ -507,7 +537,7 @@ int jq_conv_backward(const jq_conv *a, void *stream)
     ConvArgs c = conv_args(a);
     c.d_out = a->d_out, c.dx = a->dx, c.d_final = a->d_final, c.d_initial = a->d_initial;
     c.part = need ? static_cast<float *>(a->workspace) : nullptr;
-    const ConvShape s = conv_shape(c, a->dtype, true);
+    const ConvShape s = conv_shape(c, 4);
     c.parts = (int)conv_parts(c, s, (int64_t)c.batch * c.runs, CONV_BACKWARD_BLOCKS);
     return by_taps(a->dtype, a->weight_dtype, a->taps, [&](auto t, auto w, auto taps) {
         using W = decltype(w);
@@ -531,7 +561,7 @@ int jq_conv_step(const jq_conv *a, void *state, int64_t state_rows, const int64_
     if (state_rows && !state && a->taps > 1) return fail(JQ_E_ARG, "null state");
     TRY(check_state_pointer(state, a->dtype, "state"));
     ConvStepArgs s{conv_args(a), state, state_rows, rows, starts};
-    const ConvShape shape = conv_shape(s.c, a->dtype, false);
+    const ConvShape shape = conv_shape(s.c, 4);
     s.c.parts = (int)conv_parts(s.c, shape, a->batch, CONV_STEP_BLOCKS);
     return by_taps(a->dtype, a->weight_dtype, a->taps, [&](auto t, auto w, auto taps) {
         hipLaunchKernelGGL((k_conv_step<decltype(t), decltype(w), taps()>), dim3(s.c.parts * shape.blocks_x), dim3(256), 0, strm(stream), s);
