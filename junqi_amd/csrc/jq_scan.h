@@ -15,10 +15,11 @@ namespace jq {
 // Bound by the vector units: a state of a ply takes five instructions (of which the
 // exponential as long as two) forward and thirteen backward, with the sums of db and dc
 // over channels 17.5. 512 games x 256 plies of 512 channels of 16 states in bfloat16:
-// forward 327 us (126 instructions a ply and wave, of which 80 the states', the units busy
-// three quarters of the time; the rows and saved states are 1.1 GB), backward 1,095 us (392
-// a ply and wave, busy 80 %). Without these operands, with 64-bit addresses in vector
-// registers and the arguments of a dozen tensors held over the pass: 3,160 us in all.
+// forward 331 us (120 instructions a ply and wave, of which 80 the states', the units busy
+// 78 % of the time; the rows and saved states are 1.1 GB), backward 1,110 us (392 a ply
+// and wave, busy 74 %, 86 while its waves live). Without these operands, with 64-bit
+// addresses in vector registers and the arguments of a dozen tensors held over the pass:
+// 3,160 us in all.
 constexpr int SCAN_PLIES = 4;     // plies whose rows are on their way while the ones before are computed
 constexpr int SCAN_CHUNK = 8;     // plies of a chunk of the backward pass, which starts from a saved state
 constexpr int scan_far(int ns) { return ns > 8 ? 2 : 0; }   // plies of a chunk whose states wait in LDS: registers would spill

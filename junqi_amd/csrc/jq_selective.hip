@@ -86,7 +86,9 @@ struct ScanShape { int ns, sg, waves, segments, seg_plies; bool exact; };
 //     256        78 / 212     242 / 872      287 / 943      961 / 3,788
 //     512       129 / 213     468 / 901      513 / 977    1,853 / 3,859
 //   1,024       247 / 215     919 / 910      974 / 1,017  3,625 / 4,033
-// So: below 1,024 waves, from four parts of 64 plies on.
+// So: below 1,024 waves, from four parts of 64 plies on. Waves of all parts (two records of
+// 65,537 plies, us at 2,048 / 4,096 / 8,192): 605 / 520 / 509; the middle one, for the third
+// doubles the states kept between them.
 constexpr int SPLIT_BELOW = 1024, SPLIT_WAVES = 4096, SPLIT_PLIES = 64;
 ScanShape scan_shape(const jq_scan *a)
 {
@@ -105,7 +107,9 @@ ScanShape scan_shape(const jq_scan *a)
     return s;
 }
 
-// Blocks that share the backward pass's items, each with its own sums of da, dskip and dbias.
+// Waves that share the backward pass's items, each with its own sums of da, dskip and dbias:
+// as many as its registers let live (training, us at 1,024 / 2,048 / 4,096: 1,852 / 1,416 /
+// 1,402, the last with twice the sums to keep and join).
 constexpr int BACKWARD_WAVES = 2048;
 int64_t scan_parts(const jq_scan *a)
 {
@@ -356,7 +360,8 @@ LogitsGrid logits_grid(LogitsArgs &l)
     return {dim3((unsigned)std::min<int64_t>((l.rows * l.tiles + waves - 1) / waves, 1 << 23)), dim3(64 * waves), waves * each};
 }
 
-// Blocks along the rows that sum dbias.
+// Blocks along the rows that sum dbias (4,096 rows of 16,641, training, us at 1,024 / 2,048 /
+// 4,096: 272 / 248 / 252).
 constexpr int LOGITS_BIAS_BLOCKS = 2048;
 int bias_tiles(const jq_logits *a)
 {
