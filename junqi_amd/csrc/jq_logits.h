@@ -92,7 +92,7 @@ struct Tile {
     {
         row = item / a.tiles;
         c0 = (int)(item - row * a.tiles) * a.tile;
-        c1 = min(c0 + a.tile, a.actions);
+        c1 = c0 + min(a.tile, a.actions - c0);   // c0 + a.tile may not fit 32 bits
         count = !a.recent_count ? 0 : a.recent_lengths ? min(max(a.recent_lengths[row], 0), a.recent_count) : a.recent_count;
         mask = reinterpret_cast<uint32_t *>(lds) + __builtin_amdgcn_readfirstlane(threadIdx.x / 64) * (a.mask_words + 2 * a.slots);
         table = reinterpret_cast<int *>(mask + a.mask_words);

@@ -115,3 +115,23 @@ def test_far_plies():
     out = memory.selective_scan(u, u, a, b, b, softplus=True)
     few = memory.selective_scan(u[-3:].contiguous(), u[-3:].contiguous(), a, b[-3:], b[-3:], softplus=True)
     assert torch.equal(out[-3:], few)
+
+
+def test_the_widest_row():
+    """As many actions as a call may have: the last columns' ends pass 32 bits."""
+    from junqi_amd import masks
+    acts, tail = 2 ** 31 - 1 - 4096, 70001
+    x = _rows(1, acts)
+    recent = torch.tensor([[acts - 1, 3, acts]], device="cuda")
+    leaf = x.requires_grad_()
+    out = masks.action_logits(leaf, recent=recent, presence=1.0, repetition=2.0)
+    d, = torch.autograd.grad(out, leaf, x.detach())
+    out = out.detach()
+    for at in (slice(0, tail), slice(acts - tail, acts)):
+        k = 3 if at.start == 0 else tail - 1
+        few = x.detach()[:, at].clone()
+        want, grad = few.clone(), few.clone()
+        y = few[0, k].float()
+        want[0, k] = ((y / 2 if y > 0 else y * 2) - 1).to(BF16)
+        grad[0, k] = (y * (0.5 if y > 0 else 2.0)).to(BF16)
+        assert torch.equal(out[:, at], want) and torch.equal(d[:, at], grad)
