@@ -1,7 +1,5 @@
 // The selective state space scan, forward and backward, and its step of one ply.
 #pragma once
-#include <utility>
-
 #include "jq_memory.h"
 
 namespace jq {

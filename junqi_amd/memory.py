@@ -16,7 +16,10 @@ Tensors must be on the GPU (there is no host path), in float32 or bfloat16;
 sums, statistics and states are float32. Where linear attention's bfloat16 results
 are products with float32 operands (a state, the weights of the plies), these are
 taken with 16 bits, so that the result's own rounding is what it is off by. Calls run
-on torch's current stream and do not synchronise. Wrong arguments raise ValueError.
+on torch's current stream and do not synchronise, and may be captured in graphs; a
+backward pass is captured with leaves that no eager autograd graph still holds (detached
+ones of its own), because autograd would wait for the eager graph's stream within the
+capture. Wrong arguments raise ValueError.
 """
 
 from __future__ import annotations
