@@ -439,6 +439,19 @@ __global__ __launch_bounds__(256) void k_scan_forward(SelectArgs)
     }
 }
 
+// h 2^x as the product of what is returned, h times a whole power, and frac, in [1, 2). The
+// power of a whole part, 64 plies or more, may be past either end of float32 where each
+// ply's is a common number: so it is never taken by itself. 0 stays 0 and an infinity one
+// behind any power, a tiny h grows, and a large one decays to 0. Past 2^+-1024 nothing
+// but 0 and the infinities is left of any h.
+__device__ __forceinline__ float times_power(float h, float x, float &frac)
+{
+    x = fminf(fmaxf(x, -1024.f), 1024.f);
+    const float whole = floorf(x);
+    frac = exp2_fast(x - whole);
+    return ldexpf(h, (int)whole);
+}
+
 // What each part of a split axis adds becomes the state before it (BACK: the gradient
 // behind it): one thread for each game, state and channel.
 template <bool BACK>
@@ -467,9 +480,9 @@ __global__ __launch_bounds__(256) void k_scan_join(SelectArgs a)
 #pragma unroll
             for (int k = 0; k < AHEAD; ++k) {
                 if (s0 + k >= a.segments) break;
+                float frac;
                 first[(s0 + k) * by] = h;
-                // an infinity stays one over any number of plies: no power is 0
-                h = keep[k] != keep[k] ? add[k] : fmaf(fmaxf(exp2_fast(keep[k] * A), 0x1p-126f), h, add[k]);
+                h = keep[k] != keep[k] ? add[k] : fmaf(times_power(h, keep[k] * A, frac), frac, add[k]);
             }
         }
     }

@@ -679,7 +679,8 @@ def selective_scan(u: torch.Tensor, delta: torch.Tensor, a: torch.Tensor, b: tor
     d // (D / G). ``a`` (D, N), ``skip`` and ``delta_bias`` (D,) float32. ``starts``
     and ``lengths`` as in `linear_attention`: a game that starts sees nothing of the
     plies before, plies from a game's length on are padding, their ``out`` and
-    gradients 0. A decay below 2^-126 counts as 0. Returns ``out`` (B, T, D), or with
+    gradients 0. A ply's decay below 2^-126 counts as 0, one past float32's end as
+    infinite (it makes NaN of a state of 0). Returns ``out`` (B, T, D), or with
     ``return_state`` also the float32 state (B, D, N) after each game's last ply.
 
     Differentiable in u, delta, a, b, c, skip, gate, delta_bias and initial_state;

@@ -1,0 +1,44 @@
+"""What action_logits tells autograd, keeps and refuses, and its penalties at float32's ends, on
+an MI355X."""
+
+from __future__ import annotations
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+pytestmark = pytest.mark.gpu
+
+BF16, F32 = torch.bfloat16, torch.float32
+
+
+@pytest.fixture(scope="module")
+def masks():
+    if not torch.cuda.is_available():
+        pytest.fail("GPU test collected on a machine without a visible GPU")
+    from junqi_amd import masks as M
+    return M
+
+
+def test_forward_mode_is_refused(masks):
+    """An input with a tangent is refused, whether it requires a gradient or not, and never taken
+    as a constant: the logits and the bias, and each penalty of the rows' own."""
+    import torch.autograd.forward_ad as fw
+    recent = torch.tensor([[1, 1, 3]] * 4, device="cuda")
+    args = {"logits": torch.randn(4, 9, device="cuda"), "bias": torch.randn(9, device="cuda"),
+            "repetition": torch.full((4,), 1.5, device="cuda"), "frequency": torch.rand(4, device="cuda"),
+            "presence": torch.rand(4, device="cuda")}
+
+    def call(logits, **kw):
+        return masks.action_logits(logits, recent=recent, **kw)
+    plain = call(**args)
+    for name in args:
+        for grad in (False, True):
+            with fw.dual_level():
+                given = {k: v.detach() for k, v in args.items()}
+                given[name] = fw.make_dual(given[name].clone().requires_grad_(grad), torch.ones_like(given[name]))
+                for mode in (torch.enable_grad(), torch.no_grad()):
+                    with mode, pytest.raises((NotImplementedError, ValueError, RuntimeError)):
+                        call(**given)
+    with fw.dual_level():     # inside a level, inputs without tangents are as anywhere else
+        assert torch.equal(call(**args), plain)
