@@ -259,21 +259,27 @@ __global__ __launch_bounds__(256) void k_logits_bias(LogitsArgs a)
         if (e < n) a.part[(int64_t)part * a.actions + c + e] = sum[e];
 }
 
-// dbias: the blocks' shares summed in a fixed order.
+// dbias: the blocks' shares summed in a fixed order, 16 columns a block at a time: a block for
+// each 16 would be 2^32 threads, more than a launch may have, from 2^28 actions on.
+constexpr int LOGITS_JOIN_BLOCKS = 1 << 20;
 __global__ __launch_bounds__(256) void k_logits_join(const float *part, int parts, int actions, float *dbias)
 {
     __shared__ float red[16][17];
-    const int64_t col = (int64_t)blockIdx.x * 16 + threadIdx.x % 16;
-    const int slice = threadIdx.x / 16;
-    float s = 0.f;
-    if (col < actions)
-        for (int q = slice; q < parts; q += 16) s += part[(int64_t)q * actions + col];
-    red[slice][threadIdx.x % 16] = s;
-    __syncthreads();
-    if (slice || col >= actions) return;
-    s = 0.f;
-    for (int q = 0; q < 16; ++q) s += red[q][threadIdx.x];
-    dbias[col] = s;
+    const int lane = threadIdx.x % 16, slice = threadIdx.x / 16;
+    for (int64_t c0 = (int64_t)blockIdx.x * 16; c0 < actions; c0 += (int64_t)gridDim.x * 16) {
+        const int64_t col = c0 + lane;
+        float s = 0.f;
+        if (col < actions)
+            for (int q = slice; q < parts; q += 16) s += part[(int64_t)q * actions + col];
+        red[slice][lane] = s;
+        __syncthreads();
+        if (!slice && col < actions) {
+            s = 0.f;
+            for (int q = 0; q < 16; ++q) s += red[q][lane];
+            dbias[col] = s;
+        }
+        __syncthreads();   // red is written anew
+    }
 }
 
 }  // namespace jq

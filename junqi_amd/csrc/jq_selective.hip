@@ -629,7 +629,7 @@ int jq_logits_backward(const jq_logits *a, const void *d_out, int64_t d_out_stri
         sums.tiles = bias_tiles(a);
         hipLaunchKernelGGL((k_logits_bias<T>), dim3(sums.tiles * sums.parts), dim3(256), 0, strm(stream), sums);
         TRY(launch_check("k_logits_bias"));
-        hipLaunchKernelGGL(k_logits_join, dim3((l.actions + 15) / 16), dim3(256), 0, strm(stream), l.part, l.parts, l.actions, d_bias);
+        hipLaunchKernelGGL(k_logits_join, dim3(std::min((l.actions + 15) / 16, LOGITS_JOIN_BLOCKS)), dim3(256), 0, strm(stream), l.part, l.parts, l.actions, d_bias);
         return launch_check("k_logits_join");
     });
 }
