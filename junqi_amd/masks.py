@@ -18,6 +18,7 @@ import ctypes as C
 import math
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib as L
@@ -106,6 +107,8 @@ class _Penalties:
                 _check(name, v, (logits.shape[0],), (torch.float32,), logits)
                 if v.requires_grad and torch.is_grad_enabled():
                     raise ValueError(f"{name} has no gradient (detach it)")
+                if forward_ad._current_level >= 0 and forward_ad.unpack_dual(v).tangent is not None:
+                    raise ValueError(f"{name} has no forward-mode derivative")
                 self.tensors[i] = v.contiguous()
             else:
                 self.numbers[i] = float(v)

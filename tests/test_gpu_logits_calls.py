@@ -42,3 +42,15 @@ def test_forward_mode_is_refused(masks):
                         call(**given)
     with fw.dual_level():     # inside a level, inputs without tangents are as anywhere else
         assert torch.equal(call(**args), plain)
+
+
+def test_a_second_derivative_is_refused(masks):
+    x, bias = torch.randn(4, 9, device="cuda", requires_grad=True), torch.randn(9, device="cuda", requires_grad=True)
+    out = masks.action_logits(x, bias=bias, recent=torch.tensor([[1, 3]] * 4, device="cuda"), repetition=1.5)
+    weight = torch.randn(4, 9, device="cuda", requires_grad=True)
+    g = torch.autograd.grad((out * weight).sum(), [x, bias], create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(g[0].sum() + g[1].sum(), weight)
+    for name in ("repetition", "frequency", "presence"):
+        with pytest.raises(ValueError, match="no gradient"):
+            masks.action_logits(x, recent=torch.tensor([[1]] * 4, device="cuda"), **{name: torch.ones(4, device="cuda", requires_grad=True)})
