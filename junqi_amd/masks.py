@@ -111,11 +111,11 @@ class _Penalties:
                     raise ValueError(f"{name} has no forward-mode derivative")
                 self.tensors[i] = v.contiguous()
             else:
-                self.numbers[i] = float(v)
+                self.numbers[i] = C.c_float(float(v)).value   # as the kernel has it
                 if not math.isfinite(self.numbers[i]):
-                    raise ValueError(f"{name} must be finite, got {v}")
+                    raise ValueError(f"{name} must be finite in float32, got {v}")
         if self.numbers[0] <= 0.0:
-            raise ValueError(f"repetition must be positive, got {repetition}")
+            raise ValueError(f"repetition must be positive in float32, got {repetition}")
 
 
 def _logits_args(logits, bias, legal, recent, lengths, numbers, tensors) -> L.Logits:
@@ -180,8 +180,9 @@ def action_logits(logits: torch.Tensor, *, bias: torch.Tensor | None = None, leg
     ``logits`` (N, A) float32 or bfloat16. Where ``recent`` (N, L) int32 or int64, the
     first ``recent_lengths`` (N,) int32 of each row (all if None), names an action count
     times: x = (x / repetition if x > 0 else x * repetition) - frequency * count -
-    presence; each penalty is a number or an (N,) float32 tensor, and ids outside
-    [0, A) are passed over (padding). Then ``bias`` (A,) float32 is added, and actions
+    presence; each penalty is a finite number, a repetition above 0, or an (N,) float32
+    tensor, whose values are not looked at (that would wait for the GPU): the formula is
+    taken with them as they are. Ids outside [0, A) are passed over (padding). Then ``bias`` (A,) float32 is added, and actions
     that ``legal`` does not have become -infinity: (N, A) bool, or (N, ceil(A / 32))
     int32 words, bit j of word i for action 32 i + j, as the environment packs them. A
     row without a legal action is all -infinity. Returns (N, A) of logits' type.
