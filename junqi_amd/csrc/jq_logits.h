@@ -72,14 +72,15 @@ __device__ __forceinline__ uint32_t legal_bits(const LogitsArgs &a, int64_t row,
     return all;
 }
 
+// The few named columns of a row are divided, not multiplied by a reciprocal: one rounding,
+// and no infinity where the repetition is below 2^-128.
 struct Penalty {
-    float repetition, inverse, frequency, presence;
+    float repetition, frequency, presence;
     __device__ __forceinline__ Penalty(const LogitsArgs &a, int64_t row)
     {
         repetition = a.repetitions ? a.repetitions[row] : a.repetition;
         frequency = a.frequencies ? a.frequencies[row] : a.frequency;
         presence = a.presences ? a.presences[row] : a.presence;
-        inverse = 1.f / repetition;
     }
 };
 
@@ -212,9 +213,8 @@ __global__ __launch_bounds__(256) void k_logits(LogitsArgs a)
         __builtin_amdgcn_s_waitcnt(0);   // the row is written before its named columns are written again
         const Penalty p(a, t.row);
         t.each_recent(a, [&](int c, int count) {
-            const float y = (float)x[c];
-            if (BACK) o[c] = from_float<T>((float)d[c] * (y > 0.f ? p.inverse : p.repetition));
-            else o[c] = from_float<T>((y > 0.f ? y * p.inverse : y * p.repetition) - fmaf(p.frequency, (float)count, p.presence) + (biased ? a.bias[c] : 0.f));
+            const float y = (float)x[c], v = BACK ? (float)d[c] : y, held = y > 0.f ? v / p.repetition : v * p.repetition;
+            o[c] = from_float<T>(BACK ? held : held - fmaf(p.frequency, (float)count, p.presence) + (biased ? a.bias[c] : 0.f));
         });
     }
 }

@@ -54,3 +54,29 @@ def test_a_second_derivative_is_refused(masks):
     for name in ("repetition", "frequency", "presence"):
         with pytest.raises(ValueError, match="no gradient"):
             masks.action_logits(x, recent=torch.tensor([[1]] * 4, device="cuda"), **{name: torch.ones(4, device="cuda", requires_grad=True)})
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_a_repetition_divides(masks, dtype):
+    """x / repetition is one rounding, and so is its gradient: a product with a rounded
+    reciprocal is two, and an infinity for a repetition below 2^-128."""
+    g = torch.Generator().manual_seed(3)
+    n, acts = 64, 257
+    x = (2 * torch.randn(n, acts, generator=g)).to(dtype)
+    d = torch.randn(n, acts, generator=g).to(dtype)
+    rep = 0.5 + torch.rand(n, generator=g)
+    rep[:3] = torch.tensor([1e-39, 2.5e-39, 3e38])       # the first two: float32's reciprocal is an infinity
+    x[:2], d[:2] = (1e-10 * x[:2].float()).to(dtype), (1e-10 * d[:2].float()).to(dtype)
+    x[2], d[2] = (1e30 * x[2].float().abs()).to(dtype), (1e30 * d[2].float()).to(dtype)
+    recent = torch.arange(0, acts, 2).repeat(n, 1)
+    named = torch.zeros(acts, dtype=torch.bool)
+    named[::2] = True
+    v, r = x.float(), rep[:, None]
+    want = torch.where(named, torch.where(v > 0, v / r, v * r), v).to(dtype)
+    want_d = torch.where(named, torch.where(v > 0, d.float() / r, d.float() * r), d.float()).to(dtype)
+    leaf = x.cuda().requires_grad_()
+    out = masks.action_logits(leaf, recent=recent.cuda(), repetition=rep.cuda())
+    got, = torch.autograd.grad(out, leaf, d.cuda())
+    assert want.isfinite().all() and want_d.isfinite().all()
+    assert torch.equal(out.detach().cpu(), want)
+    assert torch.equal(got.cpu(), want_d)
