@@ -21,6 +21,13 @@ inline size_t elem_bytes(int32_t dtype) { return dtype == JQ_F32 ? 4 : 2; }
 
 inline bool aligned(const void *p, size_t to) { return (uintptr_t)p % to == 0; }
 
+// A pointer to elements of `bytes`, or NULL.
+inline int check_pointer(const void *p, size_t bytes, const char *name)
+{
+    if (!aligned(p, bytes)) return fail(JQ_E_ARG, "%s must be aligned to its element size", name);
+    return JQ_OK;
+}
+
 inline int check_rows(const jq_rows &r, int32_t dtype, const char *name)
 {
     if (!r.data) return fail(JQ_E_ARG, "null %s", name);

@@ -65,6 +65,9 @@ int check_ply_rows(const jq_scan *a, const jq_rows &r, const char *name)
 int check_scan_inputs(const jq_scan *a)
 {
     if (!a->a) return fail(JQ_E_ARG, "null a");
+    TRY(check_pointer(a->a, 4, "a"));
+    TRY(check_pointer(a->skip, 4, "skip"));
+    TRY(check_pointer(a->delta_bias, 4, "delta_bias"));
     if (a->plies == 0 || a->batch == 0) return JQ_OK;
     TRY(check_ply_rows(a, a->u, "u"));
     TRY(check_ply_rows(a, a->delta, "delta"));
@@ -219,18 +222,13 @@ int check_conv(const jq_conv *a)
     return check_taps(a->dtype, a->weight_dtype, a->taps);
 }
 
-int check_state_pointer(const void *p, int32_t dtype, const char *name)
-{
-    if (!aligned(p, elem_bytes(dtype))) return fail(JQ_E_ARG, "%s must be aligned to its element size", name);
-    return JQ_OK;
-}
-
 int check_conv_inputs(const jq_conv *a)
 {
     if (!a->weight) return fail(JQ_E_ARG, "null weight");
-    TRY(check_state_pointer(a->weight, a->weight_dtype, "weight"));
-    TRY(check_state_pointer(a->bias, a->weight_dtype, "bias"));
-    TRY(check_state_pointer(a->initial_state, a->dtype, "initial_state"));
+    TRY(check_pointer(a->weight, elem_bytes(a->weight_dtype), "weight"));
+    TRY(check_pointer(a->bias, elem_bytes(a->weight_dtype), "bias"));
+    TRY(check_pointer(a->initial_state, elem_bytes(a->dtype), "initial_state"));
+    TRY(check_pointer(a->lengths, 4, "lengths"));
     if (a->plies && a->batch) TRY(check_rows(a->x, a->dtype, "x"));
     return JQ_OK;
 }
@@ -316,7 +314,10 @@ int check_logits(const jq_logits *a)
     if (a->recent_count && !a->recent) return fail(JQ_E_ARG, "null recent");
     if (!aligned(a->recent, a->recent64 ? 8 : 4)) return fail(JQ_E_ARG, "recent must be aligned to its element size");
     if (!aligned(a->bias, 4)) return fail(JQ_E_ARG, "bias must be 4-byte aligned");
-    return JQ_OK;
+    TRY(check_pointer(a->recent_lengths, 4, "recent_lengths"));
+    TRY(check_pointer(a->repetitions, 4, "repetitions"));
+    TRY(check_pointer(a->frequencies, 4, "frequencies"));
+    return check_pointer(a->presences, 4, "presences");
 }
 
 LogitsArgs logits_args(const jq_logits *a)
@@ -399,6 +400,10 @@ int jq_scan_forward(const jq_scan *a, void *stream)
     if (a->batch == 0) return JQ_OK;
     TRY(check_scan_inputs(a));
     if (a->plies) TRY(check_ply_rows(a, a->out, "out"));
+    TRY(check_pointer(a->lengths, 4, "lengths"));
+    TRY(check_pointer(a->initial_state, 4, "initial_state"));
+    TRY(check_pointer(a->final_state, 4, "final_state"));
+    TRY(check_pointer(a->saved, 4, "saved"));
     TRY(check_scan_workspace(a, false));
     SelectArgs s = select_args(a, false);
     const ScanShape shape = scan_shape(a);
@@ -428,6 +433,13 @@ int jq_scan_backward(const jq_scan *a, void *stream)
     if (a->dgate.data && !a->gate.data) return fail(JQ_E_ARG, "dgate without a gate");
     for (const jq_rows *r : {&a->du, &a->ddelta, &a->dgate, &a->db, &a->dc})
         if (r->data) TRY(check_ply_rows(a, *r, "a gradient"));   // absent ones are not wanted
+    TRY(check_pointer(a->lengths, 4, "lengths"));
+    TRY(check_pointer(a->saved, 4, "saved"));
+    TRY(check_pointer(a->da, 4, "da"));
+    TRY(check_pointer(a->dskip, 4, "dskip"));
+    TRY(check_pointer(a->ddelta_bias, 4, "ddelta_bias"));
+    TRY(check_pointer(a->d_final, 4, "d_final"));
+    TRY(check_pointer(a->d_initial, 4, "d_initial"));
     TRY(check_scan_workspace(a, true));
     SelectArgs s = select_args(a, true);
     s.d_out = a->d_out, s.du = a->du, s.ddelta = a->ddelta, s.dgate = a->dgate;
@@ -472,6 +484,7 @@ int jq_scan_step(const jq_scan *a, float *state, int64_t state_rows, const int64
     TRY(check_scan_inputs(a));
     TRY(check_rows(a->out, a->dtype, "out"));
     if (state_rows && !state) return fail(JQ_E_ARG, "null state");
+    TRY(check_pointer(rows, 8, "rows"));
     if (!aligned(state, 4)) return fail(JQ_E_ARG, "state must be 4-byte aligned");
     const SelectStepArgs s{a->u, a->delta, a->gate, a->b, a->c, a->out, a->batch, a->channels, a->states, a->groups,
                            a->channels / a->groups, a->softplus != 0, a->a, a->skip, a->delta_bias, state, state_rows, rows, starts};
@@ -507,7 +520,7 @@ int jq_conv_forward(const jq_conv *a, void *stream)
     if (a->batch == 0) return JQ_OK;
     TRY(check_conv_inputs(a));
     if (a->plies) TRY(check_rows(a->out, a->dtype, "out"));
-    TRY(check_state_pointer(a->final_state, a->dtype, "final_state"));
+    TRY(check_pointer(a->final_state, elem_bytes(a->dtype), "final_state"));
     ConvArgs c = conv_args(a);
     const ConvShape s = conv_shape(c, conv_forward_vec(a));
     c.parts = (int)conv_parts(c, s, (int64_t)c.batch * c.runs, MOST_BLOCKS);
@@ -531,10 +544,10 @@ int jq_conv_backward(const jq_conv *a, void *stream)
     TRY(check_conv_inputs(a));
     if (a->plies && a->batch) TRY(check_rows(a->d_out, a->dtype, "d_out"));
     if (a->dx.data) TRY(check_rows(a->dx, a->dtype, "dx"));
-    TRY(check_state_pointer(a->d_final, a->dtype, "d_final"));
-    TRY(check_state_pointer(a->d_initial, a->dtype, "d_initial"));
-    TRY(check_state_pointer(a->dweight, a->weight_dtype, "dweight"));
-    TRY(check_state_pointer(a->dbias, a->weight_dtype, "dbias"));
+    TRY(check_pointer(a->d_final, elem_bytes(a->dtype), "d_final"));
+    TRY(check_pointer(a->d_initial, elem_bytes(a->dtype), "d_initial"));
+    TRY(check_pointer(a->dweight, elem_bytes(a->weight_dtype), "dweight"));
+    TRY(check_pointer(a->dbias, elem_bytes(a->weight_dtype), "dbias"));
     const int64_t need = conv_bytes(a);
     if (a->workspace_bytes < need || (need && !a->workspace))
         return fail(JQ_E_ARG, "workspace of %lld bytes, %lld are needed", (long long)a->workspace_bytes, (long long)need);
@@ -564,7 +577,8 @@ int jq_conv_step(const jq_conv *a, void *state, int64_t state_rows, const int64_
     TRY(check_conv_inputs(a));
     TRY(check_rows(a->out, a->dtype, "out"));
     if (state_rows && !state && a->taps > 1) return fail(JQ_E_ARG, "null state");
-    TRY(check_state_pointer(state, a->dtype, "state"));
+    TRY(check_pointer(rows, 8, "rows"));
+    TRY(check_pointer(state, elem_bytes(a->dtype), "state"));
     ConvStepArgs s{conv_args(a), state, state_rows, rows, starts};
     const ConvShape shape = conv_shape(s.c, 4);
     s.c.parts = (int)conv_parts(s.c, shape, a->batch, CONV_STEP_BLOCKS);
@@ -615,6 +629,7 @@ int jq_logits_backward(const jq_logits *a, const void *d_out, int64_t d_out_stri
         if (workspace_bytes < need || !workspace)
             return fail(JQ_E_ARG, "workspace of %lld bytes, %lld are needed", (long long)workspace_bytes, (long long)need);
         if (!aligned(workspace, 4)) return fail(JQ_E_ARG, "workspace must be 4-byte aligned");
+        TRY(check_pointer(d_bias, 4, "d_bias"));
         l.part = static_cast<float *>(workspace);
     }
     return by_type(a->dtype, [&](auto t) {
