@@ -510,7 +510,8 @@ int jq_layer_norm_backward(int32_t dtype, int32_t weight_dtype, int64_t rows, in
 /* ---- a policy's selective memory -----------------------------------------------
  * A state space scan whose steps depend on the input, and the short causal
  * convolution before it, beside the operators above and under the same terms.
- * Games and plies stay at or below 2^30, channels at or below 2^20. */
+ * Games and plies stay at or below 2^30, channels at or below 2^20. What a call writes
+ * shares no memory with anything else that it reads or writes, nor rows with each other. */
 #define JQ_SCAN_MAX_STATES 64
 #define JQ_CONV_MAX_TAPS 8
 #define JQ_SCAN_MAX_PLY_STRIDE (1 << 28)   /* bytes between the plies of a scan's rows, at least 0 */
@@ -589,7 +590,8 @@ int jq_conv_step(const jq_conv *a, void *state, int64_t state_rows, const int64_
 /* ---- what a policy answers with -------------------------------------------------
  * Logits of the actions, with count how often the row's recent actions name one:
  *   x = logit; where count > 0: x = (x > 0 ? x / repetition : x * repetition) - frequency * count - presence;
- *   out = x + bias where the mask has the action, else -infinity. */
+ *   out = x + bias where the mask has the action, else -infinity.
+ * What a call writes shares no memory with anything else that it reads or writes. */
 #define JQ_LOGITS_MASK_WORDS 0   /* (rows, ceil(actions / 32)) uint32, bit j of word i is action 32 i + j */
 #define JQ_LOGITS_MASK_BYTES 1   /* (rows, actions) uint8 */
 typedef struct jq_logits {

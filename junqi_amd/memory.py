@@ -539,7 +539,7 @@ def _check_step(name: str, x: torch.Tensor, state: torch.Tensor, state_shape: tu
         _check("out", out, tuple(x.shape), (x.dtype,), x)
         if x.shape[1] > 1 and out.stride(1) != 1:
             raise ValueError("the elements of out's last dimension must be adjacent")
-        if b > 1 and out.stride(0) == 0:
+        if b > 1 and out.stride(0) < x.shape[1]:
             raise ValueError("the rows of out must not share memory")
         if grads and out.requires_grad:
             raise ValueError("out must not require a gradient: what is written to it has none")
@@ -709,7 +709,8 @@ def selective_scan_step(u: torch.Tensor, delta: torch.Tensor, a: torch.Tensor, b
     ``u``, ``delta``, ``gate`` (B, D), ``b``, ``c`` (B, N) or (B, G, N); ``state``
     (R, D, N) float32, contiguous; ``rows``, ``starts`` and ``out`` as in
     `linear_attention_step`: a game whose row is outside [0, R) is left out, its output
-    0, and no row may be named twice. Returns (B, D). Not differentiable."""
+    0, and no row may be named twice; the rows of ``out`` share no memory, and none with
+    the other arguments. Returns (B, D). Not differentiable."""
     given = (u, delta, a, b, c, skip, gate, delta_bias)
     u, delta, a, b, c, skip, gate, delta_bias = _check_scan(*given, 1)
     rows, starts, out = _check_step("selective_scan", u, state, tuple(a.shape), torch.float32, rows, starts, out, given)
@@ -832,8 +833,9 @@ def causal_conv_step(x: torch.Tensor, weight: torch.Tensor, state: torch.Tensor,
 
     ``x`` (B, D); ``state`` (R, taps - 1, D) of x's type, contiguous; ``rows``,
     ``starts`` and ``out`` as in `linear_attention_step`: a game whose row is outside
-    [0, R) is left out, its output 0, and no row may be named twice. Returns (B, D).
-    Not differentiable."""
+    [0, R) is left out, its output 0, and no row may be named twice; the rows of ``out``
+    share no memory, and none with the other arguments. Returns (B, D). Not
+    differentiable."""
     given = (x, weight, bias)
     x, weight, bias = _check_conv(*given, 1)
     rows, starts, out = _check_step("causal_conv", x, state, (weight.shape[1] - 1, x.shape[1]), x.dtype, rows, starts, out,

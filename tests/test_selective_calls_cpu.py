@@ -86,3 +86,21 @@ def test_logits_bias_gradient_alignment(jl):
     g.repetition = 1.0
     assert jl.lib.jq_logits_backward(C.byref(g), 64, 8, 64, 8, 66, 64, 1 << 20, None) == jl.JQ_E_ARG
     assert b"d_bias" in jl.lib.jq_last_error()
+
+
+@pytest.mark.parametrize("stride,good", [(0, False), (1, False), (7, False), (8, True), (9, True)])
+def test_rows_of_out_that_share_memory(stride, good):
+    """Games that write the same elements would race; rows apart, or one game, go on to the call."""
+    from torch._subclasses import FakeTensorMode
+
+    from junqi_amd import memory
+    with FakeTensorMode():
+        def z(*shape):
+            return torch.empty(shape, device="cuda")
+        out = z(64).as_strided((5, 8), (stride, 1))
+        for call in (lambda o, b: memory.selective_scan_step(z(b, 8), z(b, 8), z(8, 4), z(b, 4), z(b, 4), z(b, 8, 4), out=o),
+                     lambda o, b: memory.causal_conv_step(z(b, 8), z(8, 4), z(b, 3, 8), out=o)):
+            for o, b, ok in ((out, 5, good), (out[:1], 1, True)):
+                with pytest.raises(Exception) as e:     # without a GPU every call ends somewhere
+                    call(o, b)
+                assert ("share memory" in str(e.value)) != ok
