@@ -600,7 +600,7 @@ typedef struct jq_logits {
     int64_t rows;
     int32_t actions;
     int32_t recent_count, recent64;    /* recent: int32 or (recent64 != 0) int64 */
-    const void *logits;
+    const void *logits;                /* a backward pass without recent actions does not read them: NULL will do */
     int64_t logits_stride;             /* strides between rows, in elements */
     const float *bias;                 /* float32 (actions); NULL: 0 */
     const void *mask;                  /* NULL: every action */

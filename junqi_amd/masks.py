@@ -118,9 +118,12 @@ class _Penalties:
             raise ValueError(f"repetition must be positive in float32, got {repetition}")
 
 
-def _logits_args(logits, bias, legal, recent, lengths, numbers, tensors) -> L.Logits:
-    g = L.Logits(_DTYPES[logits.dtype], L.MASK_BYTES, logits.shape[0], logits.shape[1])
-    g.logits, g.logits_stride, g.bias = logits.data_ptr(), logits.stride(0), _ptr(bias)
+def _logits_args(like, logits, bias, legal, recent, lengths, numbers, tensors) -> L.Logits:
+    """`like` has the logits' type and shape, where a backward pass has no use for them."""
+    g = L.Logits(_DTYPES[like.dtype], L.MASK_BYTES, like.shape[0], like.shape[1])
+    g.bias = _ptr(bias)
+    if logits is not None:
+        g.logits, g.logits_stride = logits.data_ptr(), logits.stride(0)
     if legal is not None:
         g.mask_kind = L.MASK_WORDS_PACKED if legal.dtype == torch.int32 else L.MASK_BYTES
         g.mask, g.mask_stride = legal.data_ptr(), legal.stride(0)
@@ -138,7 +141,7 @@ def _stream_of(t: torch.Tensor) -> int:
 
 def _logits_forward(logits, bias, legal, recent, lengths, penalties):
     out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-    g = _logits_args(logits, bias, legal, recent, lengths, penalties.numbers, penalties.tensors)
+    g = _logits_args(logits, logits, bias, legal, recent, lengths, penalties.numbers, penalties.tensors)
     with _on(logits):
         check(lib.jq_logits_forward(C.byref(g), out.data_ptr(), out.shape[1], _stream_of(logits)))
     return out
@@ -147,7 +150,8 @@ def _logits_forward(logits, bias, legal, recent, lengths, penalties):
 class _ActionLogits(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, bias, legal, recent, lengths, penalties):
-        ctx.save_for_backward(logits, bias, legal, recent, lengths, *penalties.tensors)
+        # only a repetition's gradient looks at the logits
+        ctx.save_for_backward(None if recent is None else logits, bias, legal, recent, lengths, *penalties.tensors)
         ctx.numbers = penalties.numbers
         return _logits_forward(logits, bias, legal, recent, lengths, penalties)
 
@@ -156,17 +160,17 @@ class _ActionLogits(torch.autograd.Function):
     def backward(ctx, d_out):
         logits, bias, legal, recent, lengths, *tensors = ctx.saved_tensors
         d_out = _adjacent(d_out)
-        g = _logits_args(logits, bias, legal, recent, lengths, ctx.numbers, tensors)
+        g = _logits_args(d_out, logits, bias, legal, recent, lengths, ctx.numbers, tensors)
         need = ctx.needs_input_grad
-        d_logits = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device) if need[0] else None
+        d_logits = torch.empty(d_out.shape, dtype=d_out.dtype, device=d_out.device) if need[0] else None
         d_bias = torch.empty_like(bias) if need[1] else None
         size, work = C.c_int64(), None
         if need[1]:
             check(lib.jq_logits_workspace(C.byref(g), C.byref(size)))
-            work = torch.empty(size.value, dtype=torch.uint8, device=logits.device)
-        with _on(logits):
-            check(lib.jq_logits_backward(C.byref(g), d_out.data_ptr(), d_out.stride(0), _ptr(d_logits), logits.shape[1],
-                                         _ptr(d_bias), _ptr(work), size.value, _stream_of(logits)))
+            work = torch.empty(size.value, dtype=torch.uint8, device=d_out.device)
+        with _on(d_out):
+            check(lib.jq_logits_backward(C.byref(g), d_out.data_ptr(), d_out.stride(0), _ptr(d_logits), d_out.shape[1],
+                                         _ptr(d_bias), _ptr(work), size.value, _stream_of(d_out)))
         return d_logits, d_bias, None, None, None, None
 
 

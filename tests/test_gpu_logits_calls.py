@@ -80,3 +80,29 @@ def test_a_repetition_divides(masks, dtype):
     assert want.isfinite().all() and want_d.isfinite().all()
     assert torch.equal(out.detach().cpu(), want)
     assert torch.equal(got.cpu(), want_d)
+
+
+def test_what_the_backward_pass_keeps(masks):
+    """The logits only where recent actions are held against them: else they are free to go, or
+    to be changed in place, after the call."""
+    legal = torch.rand(40, 16641, device="cuda") < 0.01
+    d = torch.randn(40, 16641, device="cuda")
+    x = torch.randn(40, 16641, device="cuda").requires_grad_()
+    bias = torch.randn(16641, device="cuda").requires_grad_()
+    for recent in (None, torch.randint(0, 16641, (40, 8), device="cuda")):
+        held = []
+        y = x * 1.0
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: held.append(t.data_ptr()) or t, lambda t: t):
+            masks.action_logits(y, bias=bias, legal=legal, recent=recent, repetition=1.5)
+        assert (y.data_ptr() in held) == (recent is not None)
+        out = masks.action_logits(y, bias=bias, legal=legal, recent=recent, repetition=1.5)   # autograd's own check: without hooks
+        with torch.no_grad():
+            y.mul_(2.0)
+        if recent is None:
+            g = torch.autograd.grad(out, [x, bias], d)
+            assert torch.equal(g[0], torch.where(legal, d, 0.0))
+            want = torch.where(legal, d, 0.0).double().sum(0)
+            assert ((g[1] - want).abs() <= 40 * 2.0 ** -24 * torch.where(legal, d, 0.0).abs().double().sum(0)).all()
+        else:
+            with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                torch.autograd.grad(out, [x, bias], d)
