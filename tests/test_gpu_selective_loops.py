@@ -94,8 +94,8 @@ def test_sums_of_several_games(memory, shape, dtype):
     S._check_scan(memory, x)
 
 
-@pytest.mark.parametrize("types", [(F32, F32), (BF16, F32), (BF16, BF16)])
-@pytest.mark.parametrize("shape", [(1500, 4, 520, 4), (1400, 3, 516, 7)])
+@pytest.mark.parametrize("shape,types", [((1500, 4, 520, 4), (F32, F32)), ((1500, 4, 520, 4), (BF16, F32)), ((1500, 4, 520, 4), (BF16, BF16)),
+                                         ((1400, 3, 516, 7), (BF16, F32))])
 def test_sums_of_several_games_of_the_convolution(memory, shape, types):
     S._check_conv(memory, S._conv_inputs(sum(shape), *shape, dtype=types[0], wdtype=types[1]))
 
