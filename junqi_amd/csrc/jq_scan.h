@@ -130,6 +130,9 @@ template <int N> __device__ __forceinline__ void forget(float (&v)[N])
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = 0.f;
 }
+// The step that such a ply's decays are taken with: so small that no rate makes an infinity of
+// them, which would make NaN of the zeros; of dt's sign, so that a rate of -infinity is none either.
+__device__ __forceinline__ float no_step(float dt) { return copysignf(0x1p-126f, dt); }
 
 template <int HOW> __device__ __forceinline__ float across(float x)
 {
@@ -385,13 +388,15 @@ __global__ __launch_bounds__(256) void k_scan_forward(SelectArgs)
 #pragma unroll
             for (int k = 0; k < K; ++k) {
                 if (t0 + k >= end) break;
-                const float u = (float)r.u[k], pre = (float)r.delta[k] + bias, dt = has(SOFTPLUS) ? softplus(pre) : pre;
+                const float u = (float)r.u[k], pre = (float)r.delta[k] + bias;
+                float dt = has(SOFTPLUS) ? softplus(pre) : pre;
                 const float push = dt * u, bt = (float)r.b[k];
+                if (!OUT) total += dt;
                 if (starts >> k & 1) {
                     forget(h);
+                    dt = no_step(dt);
                     if (!OUT) total = __builtin_nanf("");
                 }
-                if (!OUT) total += dt;
 #pragma unroll
                 for (int i = 0; i < NS; ++i) h[i] *= exp2_fast(dt * A[i]);
                 row_add(h, bt, push);
@@ -649,7 +654,11 @@ __global__ __launch_bounds__(256, 2) void k_scan_backward(SelectArgs)
                     dt[k] = has(SOFTPLUS) ? softplus(pre) : pre;
                     dy[k] = (float)next.d_out[k];
                     if (has(HAS_GATE)) dy[k] *= (float)next.gate[k] * sigmoid((float)next.gate[k]);
-                    if (starts >> k & 1) forget(h);
+                    float step = dt[k];
+                    if (starts >> k & 1) {
+                        forget(h);
+                        step = no_step(step);
+                    }
                     const float push = dt[k] * u;
                     float v[NS];
 #pragma unroll
@@ -658,7 +667,7 @@ __global__ __launch_bounds__(256, 2) void k_scan_backward(SelectArgs)
                         else hist[k < FAR ? 0 : k - FAR][i] = h[i];
                     }
 #pragma unroll
-                    for (int i = 0; i < NS; ++i) h[i] *= exp2_fast(dt[k] * A[i]);
+                    for (int i = 0; i < NS; ++i) h[i] *= exp2_fast(step * A[i]);
                     row_add(h, bt, push);
 #pragma unroll
                     for (int i = 0; i < NS; ++i) {

@@ -133,3 +133,25 @@ def test_infinities_stay(memory):
             assert got[0][0, t, 6].isfinite() or rate > 0
         assert bool(got[1][0, 5].isinf().all()) == (rate < 0)
         assert got[1][0, 6].isfinite().all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("plies", [20, 320])
+@pytest.mark.parametrize("size", SIZES)
+def test_a_start_has_no_decay(memory, size, plies, dtype):
+    """The ply that starts a game, also with a decay past float32's end, sees its input alone:
+    in segments, whole and split, as one ply by itself."""
+    at = (0, 7, plies - 5)
+    x = _inputs(2, plies, *size, dtype, 1.0, 0.01, starts=at)
+    x["delta"][:, list(at)] = 9984.0     # e^99.8 to e^100.8; a number of bfloat16 too
+    g = torch.Generator().manual_seed(5)
+    x["state"] = torch.randn(2, *size, generator=g)
+    got, _ = _check(memory, x, 0.0101 * plies, plies)
+    y = {k: v.cuda() if isinstance(v, torch.Tensor) else v for k, v in x.items()}
+    state = y["state"].clone()
+    for t in range(8):
+        out = memory.selective_scan_step(y["u"][:, t], y["delta"][:, t], y["a"], y["b"][:, t], y["c"][:, t], state, starts=y["starts"][:, t])
+        assert out.isfinite().all() and got["out"][:, t].isfinite().all()
+        if t in at:
+            assert (state - (y["delta"][:, t, :, None].float() * y["u"][:, t, :, None].float()) * y["b"][:, t].float()).abs().max() <= \
+                2.0 ** -23 * state.abs().max()
