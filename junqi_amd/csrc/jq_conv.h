@@ -11,7 +11,10 @@ namespace jq {
 // for the taps - 1 before a run, and the next step's rows are asked for before this one's
 // results are stored: loads behind stores are seen only after these. Bound by the rows'
 // traffic forward (1,024 games x 256 plies of 512 channels, four taps, bfloat16, 537 MB: 97
-// us, 5.5 TB/s), by that and its products backward (805 MB: 225 us, 3.6 TB/s, VALU busy 57 %).
+// us, 5.5 TB/s), by that and its products backward (805 MB: 228 us, 3.6 TB/s, VALU busy 56 %,
+// 177 registers: two waves a SIMD, and one of 256 behind five to eight taps, 435 us).
+// A row that ends inside a thread's channels takes that thread, and so its wave, element by
+// element there: 501 channels 186 us forward and 639 with gradients, 512 97 and 301.
 // With an address worked out for every access, and a step's loads behind the last one's
 // stores, 164 and 332 us.
 // Plies of a step, whose rows are on their way while the step before is computed: a

@@ -15,8 +15,8 @@ namespace jq {
 // loads behind stores are seen only after these. Where none of a lane's columns is legal it
 // reads no logits: a policy's masks leave a few dozen of 16,641. The columns are written
 // without the penalties; where a recent action is legal, the wave counts these in a table
-// of its own in LDS and writes their columns again. 32,768 rows of 16,641 in bfloat16: 386 us
-// (1.09 GB written, 0.28 GB read); 705 with the counts of a tile's actions in LDS and
+// of its own in LDS and writes their columns again. 32,768 rows of 16,641 in bfloat16: 385 us
+// (1.09 GB written, 0.28 GB read; waves wait three quarters of the time); 705 with the counts of a tile's actions in LDS and
 // barriers around them, 611 with a wave for four vectors a lane, 513 with loads behind
 // stores. Vectors that straddle 16 bytes, as odd rows' do, cost nothing here (stores of
 // nothing but -infinity 228 us, aligned 251).

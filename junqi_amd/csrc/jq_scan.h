@@ -13,11 +13,11 @@ namespace jq {
 // Bound by the vector units: a state of a ply takes five instructions (of which the
 // exponential as long as two) forward and thirteen backward, with the sums of db and dc
 // over channels 17.5. 512 games x 256 plies of 512 channels of 16 states in bfloat16:
-// forward 331 us (120 instructions a ply and wave, of which 80 the states', the units busy
-// 78 % of the time; the rows and saved states are 1.1 GB), backward 1,110 us (392 a ply
-// and wave, busy 74 %, 86 while its waves live). Without these operands, with 64-bit
-// addresses in vector registers and the arguments of a dozen tensors held over the pass:
-// 3,160 us in all.
+// forward 334 us (121 instructions a ply and wave, of which 80 the states', the units busy
+// 77 % of the time; the rows and saved states are 1.1 GB), backward 1,115 us (393 a ply
+// and wave, busy 74 %, 86 while its waves live), times under the profiler; 1,419 us in all
+// without it. Without these operands, with 64-bit addresses in vector registers and the
+// arguments of a dozen tensors held over the pass: 3,160 us in all.
 constexpr int SCAN_PLIES = 4;     // plies whose rows are on their way while the ones before are computed
 constexpr int SCAN_CHUNK = 8;     // plies of a chunk of the backward pass, which starts from a saved state
 constexpr int scan_far(int ns) { return ns > 8 ? 2 : 0; }   // plies of a chunk whose states wait in LDS: registers would spill
@@ -53,8 +53,8 @@ __device__ __forceinline__ float sigmoid(float x) { return __builtin_amdgcn_rcpf
 
 // log(1 + e^x) = max(x, 0) + 2 atanh(e / (2 + e)), e = e^-|x|, so small results keep all
 // their digits. s = e / (2 + e) is at most 1/3; atanh(s) / s as a polynomial in s^2 of the
-// fourth degree, fitted for the least largest relative error: 4e-9 (the series to s^14
-// takes three terms more).
+// fourth degree, fitted for the least largest relative error: below 1e-8 with these
+// coefficients (the series to s^14 takes three terms more).
 __device__ __forceinline__ float softplus(float x)
 {
     const float e = exp2_fast(-LOG2E * fabsf(x)), s = e * __builtin_amdgcn_rcpf(2.f + e), q = s * s;
@@ -178,7 +178,10 @@ __device__ __forceinline__ float lane_sums(float (&v)[N])
 
 // The arguments, read where they are used: held in scalar registers over a pass, those of
 // a dozen tensors would be spilled to vector registers. `hidden` keeps the compiler from
-// moving the reads up to the pass's start.
+// moving the reads up to the pass's start. The backward pass spills all the same (nine rows'
+// cursors and steps, its flags): 202 scalars of bfloat16 and 16 states whose lanes all have
+// a channel, 11 % of its vector instructions; 632 and 30 % where some have none, for then
+// each state's check is a condition to keep, too.
 typedef const __attribute__((address_space(4))) SelectArgs *SelectArgsPtr;
 typedef const __attribute__((address_space(4))) jq_rows *RowsPtr;
 __device__ __forceinline__ SelectArgsPtr hidden(SelectArgsPtr a)
@@ -238,7 +241,8 @@ struct PlyRows : Window {
 };
 
 // Where this wave's lanes are: channel, states, rows. EXACT: every lane has a channel and
-// each of its states. MANY: a block's waves have the states of one wave's channels; else
+// each of its states (one flag for both: 500 channels of 16 states take the states' checks
+// as well, 160 against 134 us forward and 872 against 694 with gradients). MANY: a block's waves have the states of one wave's channels; else
 // channels of their own, four waves a block so that each SIMD of a CU gets one (blocks of
 // one wave leave some SIMDs with more waves than others).
 template <class T, int NS, bool EXACT, bool MANY>
@@ -557,9 +561,10 @@ __global__ __launch_bounds__(256) void k_scan_carry(SelectArgs)
 //   through = sum over n of b dh;  dh = exp(dt a) dh;  w = dh h_{t-1};  da += w dt;
 //   du = dt through + skip dy;  ddt = u through + sum over n of w a
 // MANY: more than one wave of states, whose shares of y, through and the sum of w a meet in
-// LDS. Registers are what it is short of: two waves a SIMD leave 256, of which 128 hold a
-// chunk's states, so the way back reads its rows again (from the caches), and the next
-// chunk's are asked for when half of the states are done with.
+// LDS. Registers are what it is short of: two waves a SIMD leave 256, of which 96 hold six
+// plies' states of 16 (the first two plies' wait in LDS), so the way back reads its rows
+// again (from the caches), and the next chunk's are asked for when half of the states are
+// done with.
 template <class T, int NS, bool EXACT, bool MANY>
 __global__ __launch_bounds__(256, 2) void k_scan_backward(SelectArgs)
 {
