@@ -106,3 +106,13 @@ def test_what_the_backward_pass_keeps(masks):
         else:
             with pytest.raises(RuntimeError, match="modified by an inplace operation"):
                 torch.autograd.grad(out, [x, bias], d)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("shape,recent", [((5, 700), 3000), ((3, 40000), 5000), ((2, 70001), 2049), ((4, 2048), 2048), ((60, 33), 2100)])
+def test_long_lists_of_recent_actions(masks, shape, recent, dtype):
+    """More of them than a wave's table has room for at once: the rows go in narrower parts."""
+    from tests import test_gpu_logits as T
+    for packed in (False, True):
+        T._check(masks, T._inputs(sum(shape), *shape, dtype=dtype, density=0.3, recent=recent), packed=packed, int64=packed)
+    T._check(masks, T._inputs(sum(shape) + 1, *shape, dtype=dtype, density=None, recent=recent, each=True), lengths=False)
